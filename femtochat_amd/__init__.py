@@ -6,7 +6,8 @@ host-side mirror of the reference's ``Kernels`` attention API, and
 ``femtochat_amd.prologue`` the rotary embedding + RMS norm that
 ``CausalSelfAttention`` applies to Q and K before it, and
 ``femtochat_amd.loss`` the cross-entropy and token-embedding kernels either
-side of the model (include/femtochat_loss.h), ``femtochat_amd.optim`` the
+side of the model (include/femtochat_loss.h), ``femtochat_amd.answer_loss`` the
+policy and preference losses over its answers, ``femtochat_amd.optim`` the
 optimizer kernels (include/femtochat_optim.h).
 """
 from .kernels import (  # noqa: F401
@@ -46,6 +47,17 @@ from .loss import (  # noqa: F401
     embedding_,
     embedding_gradient_,
     valid_target_count,
+)
+from .answer_loss import (  # noqa: F401
+    PolicyLossFunction,
+    PreferenceLossFunction,
+    policy_loss,
+    policy_loss_,
+    policy_loss_fused_,
+    policy_loss_gradient_,
+    preference_loss,
+    preference_loss_,
+    preference_loss_gradient_,
 )
 from .optim import (  # noqa: F401
     AdamW,

@@ -84,6 +84,36 @@ class XentDesc(ctypes.Structure):
     ]
 
 
+class AnswerDesc(ctypes.Structure):
+    _fields_ = [
+        ("V", ctypes.c_int32),
+        ("answers", ctypes.c_int32),
+        ("T", ctypes.c_int32),
+        ("index_base", ctypes.c_int32),
+        ("ignore_index", ctypes.c_int64),
+        ("index_type", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("reduction", ctypes.c_int32),
+        ("flags", ctypes.c_uint32),
+    ]
+
+
+class PolicyOptions(ctypes.Structure):
+    _fields_ = [
+        ("clip_low", ctypes.c_double),
+        ("clip_high", ctypes.c_double),
+        ("kl", ctypes.c_double),
+        ("advantage_per_answer", ctypes.c_int32),
+    ]
+
+
+class PreferenceOptions(ctypes.Structure):
+    _fields_ = [
+        ("beta", ctypes.c_double),
+        ("label_smoothing", ctypes.c_double),
+    ]
+
+
 class EmbedDesc(ctypes.Structure):
     _fields_ = [
         ("D", ctypes.c_int32),
@@ -182,6 +212,14 @@ _SIGNATURES = {
     "fc_cross_entropy_bwd": (ctypes.c_int, [ctypes.POINTER(XentDesc), _P, _P, _P, _P, _P, _P, _P]),
     "fc_cross_entropy_bwd_full": (ctypes.c_int, [ctypes.POINTER(XentDesc), _P, _P, _P, _P, _P, _P, _P]),
     "fc_cross_entropy_fused": (ctypes.c_int, [ctypes.POINTER(XentDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "fc_policy_loss_fwd": (ctypes.c_int, [ctypes.POINTER(AnswerDesc), ctypes.POINTER(PolicyOptions)] + [_P] * 12),
+    "fc_policy_loss_bwd": (ctypes.c_int, [ctypes.POINTER(AnswerDesc)] + [_P] * 8),
+    "fc_policy_loss_fused": (ctypes.c_int, [ctypes.POINTER(AnswerDesc), ctypes.POINTER(PolicyOptions)] + [_P] * 14),
+    "fc_preference_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(AnswerDesc), ctypes.POINTER(ctypes.c_size_t)]),
+    "fc_preference_loss_fwd": (ctypes.c_int, [ctypes.POINTER(AnswerDesc), ctypes.POINTER(PreferenceOptions)] + [_P] * 10
+                               + [ctypes.c_size_t, _P]),
+    "fc_preference_loss_bwd": (ctypes.c_int, [ctypes.POINTER(AnswerDesc)] + [_P] * 7),
+    "fc_scale_gradient": (ctypes.c_int, [_P, ctypes.c_int32, ctypes.c_int64, _P, _P]),
     "fc_embedding_fwd": (ctypes.c_int, [ctypes.POINTER(EmbedDesc), _P, _P, _P, _P]),
     "fc_embedding_bwd": (ctypes.c_int, [ctypes.POINTER(EmbedDesc), _P, _P, _P, _P]),
     "fc_embedding_bwd_full": (ctypes.c_int, [ctypes.POINTER(EmbedDesc), _P, _P, _P, _P]),

@@ -131,6 +131,91 @@ fc_status fc_embedding_bwd_workspace_bytes(const fc_embed_desc* desc, size_t* by
 fc_status fc_embedding_bwd_sorted(const fc_embed_desc* desc, float* dweights, const void* dy, const void* tokens,
                                   void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Losses over the answers of a chat model --------------------------------
+ * Fine-tuning by sampled answers (a clipped policy loss with a KL term) and by
+ * pairs of answers (a preference loss).  No reference counterpart.
+ *
+ *   logits, dlogits (V, T, answers) : x[(b*T + t)*V + v], float32 or bfloat16
+ *   tokens          (T, answers)    : the answers' tokens; ignore_index marks the
+ *                                     prompt and the padding, whose logits are
+ *                                     neither read nor given a gradient (zeros,
+ *                                     or left alone when adding)
+ * A token's log-probability is lp = x[y] - max - log(sum(exp(x - max))) over its
+ * column; a token outside the vocabulary that is not ignore_index makes its loss,
+ * and its column of the gradient, NaN.  logits and dlogits must lie alike against
+ * 16 bytes. */
+typedef struct {
+  int32_t V;            /* vocabulary size */
+  int32_t answers, T;   /* answers and tokens of each */
+  int32_t index_base;   /* 1: Julia indices, 0: zero-based */
+  int64_t ignore_index;
+  int32_t index_type;   /* fc_index_type of tokens */
+  int32_t dtype;        /* FC_F32 or FC_BF16: logits and dlogits */
+  int32_t reduction;    /* fc_reduction: over the answers' tokens (policy) or the pairs (preference) */
+  uint32_t flags;       /* FC_FLAG_OVERWRITE: the backward writes dlogits instead of adding */
+} fc_answer_desc;
+
+typedef struct {
+  double clip_low, clip_high;    /* the ratio is clipped to [1 - clip_low, 1 + clip_high] */
+  double kl;                     /* factor of the KL term, 0: none */
+  int32_t advantage_per_answer;  /* 0: advantages per token (T, answers); 1: one per answer */
+} fc_policy_options;
+
+typedef struct {
+  double beta;             /* scale of the log ratios, above 0 */
+  double label_smoothing;  /* share of pairs taken as labelled the wrong way round */
+} fc_preference_options;
+
+/* With r = exp(lp - old) and d = ref - lp:
+     loss = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl (exp(d) - d - 1)
+   per token (losses, 0 where ignored).  Optional: logprobs (lp), and for the
+   backward stats (two floats per token: the column's max and sum(exp(x - max)))
+   and weights (d loss / d lp), reduced (1 float: the sum, or the mean over the
+   answers' tokens) and count (1 float: those tokens). */
+fc_status fc_policy_loss_fwd(const fc_answer_desc* desc, const fc_policy_options* options, const void* logits,
+                             const void* tokens, const float* old_logprobs, const float* advantages,
+                             const float* ref_logprobs, float* losses, float* logprobs, float* stats,
+                             float* weights, float* reduced, float* count, void* stream);
+
+/* dlogits += (or, with FC_FLAG_OVERWRITE, =) dy w (onehot - softmax(x)) from the
+   forward's stats and weights, divided by count[0] for the mean.  dy may be null
+   (1): 1 float (sum, mean) or one per token (none). */
+fc_status fc_policy_loss_bwd(const fc_answer_desc* desc, void* dlogits, const void* logits, const void* tokens,
+                             const float* stats, const float* weights, const float* dy, const float* count,
+                             void* stream);
+
+/* Both in one pass: the logits are read once and dlogits is written once
+   (whatever desc->flags says).  count is written too, and required for the mean.
+   Columns of up to 256 KB less 16 bytes (FC_ERR_UNSUPPORTED above). */
+fc_status fc_policy_loss_fused(const fc_answer_desc* desc, const fc_policy_options* options, const void* logits,
+                               const void* tokens, const float* old_logprobs, const float* advantages,
+                               const float* ref_logprobs, float* losses, float* logprobs, float* stats,
+                               float* weights, float* reduced, float* count, void* dlogits, const float* dy,
+                               void* stream);
+
+/* Pairs of answers: the first answers/2 were chosen over the others, in order.
+   With rewards beta (sum of lp over the answer - ref) and h the chosen reward
+   less the rejected one,
+     loss = -(1 - e) log(sigmoid(h)) - e log(sigmoid(-h)),  e = label_smoothing
+   per pair (losses).  ref_logprobs: the reference model's sums, one per answer.
+   Optional: rewards (one per answer), logprobs (per token), reduced (1 float),
+   and for the backward stats (as above) and weights (one per answer: d loss / d lp).
+   workspace: fc_preference_workspace_bytes, 8-byte aligned. */
+fc_status fc_preference_workspace_bytes(const fc_answer_desc* desc, size_t* bytes);
+fc_status fc_preference_loss_fwd(const fc_answer_desc* desc, const fc_preference_options* options,
+                                 const void* logits, const void* tokens, const float* ref_logprobs, float* losses,
+                                 float* rewards, float* logprobs, float* stats, float* weights, float* reduced,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* As fc_policy_loss_bwd; dy: 1 float, or one per pair (none). */
+fc_status fc_preference_loss_bwd(const fc_answer_desc* desc, void* dlogits, const void* logits, const void* tokens,
+                                 const float* stats, const float* weights, const float* dy, void* stream);
+
+/* x[i] *= dy[0] for 0 <= i < n (float32 or bfloat16, the product rounded once);
+   where dy[0] is 1, x is not touched.  For a gradient that was formed beside its
+   loss and is scaled once the loss's own gradient is known. */
+fc_status fc_scale_gradient(void* x, int32_t dtype, int64_t n, const float* dy, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
