@@ -60,6 +60,15 @@ class AttnDesc(ctypes.Structure):
     ]
 
 
+class AttnScore(ctypes.Structure):
+    _fields_ = [
+        ("softcap", ctypes.c_float),
+        ("prefix_per_token", ctypes.c_int32),
+        ("slopes", ctypes.c_void_p),
+        ("prefix", ctypes.c_void_p),
+    ]
+
+
 class RopeNormDesc(ctypes.Structure):
     _fields_ = [
         ("D", ctypes.c_int32),
@@ -200,6 +209,20 @@ _SIGNATURES = {
     "fc_attn_bwd": (
         ctypes.c_int,
         [ctypes.POINTER(AttnDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P],
+    ),
+    "fc_attn_score_workspace_bytes": (
+        ctypes.c_int,
+        [ctypes.POINTER(AttnDesc), ctypes.POINTER(AttnScore), ctypes.c_int32, ctypes.c_int32,
+         ctypes.POINTER(ctypes.c_size_t)],
+    ),
+    "fc_attn_score_fwd": (
+        ctypes.c_int,
+        [ctypes.POINTER(AttnDesc), ctypes.POINTER(AttnScore), _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P],
+    ),
+    "fc_attn_score_bwd": (
+        ctypes.c_int,
+        [ctypes.POINTER(AttnDesc), ctypes.POINTER(AttnScore), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
+         ctypes.c_size_t, _P],
     ),
     "fc_attn_bwd_noalloc": (
         ctypes.c_int,

@@ -23,7 +23,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .kernels import _check_tensor, _dtype_code, _ptr, _stream_ptr
+from .kernels import _call, _check_tensor, _dtype_code, _ptr
 from .loss import _INDEX, _REDUCTIONS, valid_target_count
 
 __all__ = [
@@ -41,15 +41,6 @@ __all__ = [
 _LOGITS = (torch.float32, torch.bfloat16)
 _F32 = (torch.float32,)
 _FUSED_BYTES = (1 << 18) - 16  # the longest column that fc_policy_loss_fused holds
-
-
-def _call(dev: torch.device, entry, *args) -> None:
-    """The library's call on the tensors' device, whichever is current."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        _lib.check(entry(*args, _stream_ptr(dev)))
-        return
-    with torch.cuda.device(dev):
-        _lib.check(entry(*args, _stream_ptr(dev)))
 
 
 def _desc(logits, tokens, ignore_index, reduction, index_base, overwrite=False) -> _lib.AnswerDesc:

@@ -35,7 +35,13 @@ HIPCC_FLAGS = [
 # exact-mode backward (dK/dV at D = 128 spills 115 registers without it: 1336
 # against 696 us for 8 x 2048 tokens, H6).
 _VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
-EXTRA_FLAGS = {"attn_bwd_dkdv_vgpr.hip": _VGPR_FORM, "attn_bwd.hip": _VGPR_FORM}
+EXTRA_FLAGS = {"attn_bwd_dkdv_vgpr.hip": _VGPR_FORM, "attn_bwd.hip": _VGPR_FORM, "attn_score_dkdv_vgpr.hip": _VGPR_FORM}
+
+# Sources compiled once for each kind of score (csrc/attn_score.hpp: a prefix, and
+# with it a cap, a bias, or both).
+# (the longest to compile first)
+SCORE_SOURCES = ["attn_score_dkdv.hip", "attn_score_dkdv_vgpr.hip", "attn_score_dq.hip", "attn_score_fwd.hip"]
+SCORES = (1, 3, 5, 7)
 
 
 def hipcc() -> str:
@@ -57,10 +63,12 @@ def _run(cmd):
 def build(verbose: bool = False) -> Path:
     cc = hipcc()
     BUILD.mkdir(exist_ok=True)
-    objs = [BUILD / (Path(s).stem + ".o") for s in SOURCES]
-    cmds = [[cc, *HIPCC_FLAGS, *EXTRA_FLAGS.get(s, []), "-c", str(CSRC / s), "-o", str(o)]
-            for s, o in zip(SOURCES, objs)]
-    with ThreadPoolExecutor(max_workers=len(cmds)) as ex:
+    units = [(s, f"{Path(s).stem}{n}.o", [f"-DFC_SCORE={n}"]) for s in SCORE_SOURCES for n in SCORES]
+    units += [(s, Path(s).stem + ".o", []) for s in SOURCES]
+    objs = [BUILD / o for _, o, _ in units]
+    cmds = [[cc, *HIPCC_FLAGS, *EXTRA_FLAGS.get(s, []), *define, "-c", str(CSRC / s), "-o", str(BUILD / o)]
+            for s, o, define in units]
+    with ThreadPoolExecutor(max_workers=max(1, os.cpu_count() or 1)) as ex:
         for err in ex.map(_run, cmds):
             if verbose and err.strip():
                 print(err)

@@ -161,11 +161,57 @@ uint32_t fc_attn_supported_head_dims(void) {
   return mask;
 }
 
-fc_status fc_attn_workspace_bytes(const fc_attn_desc* desc, int32_t pass, int32_t positions_given, size_t* bytes) {
+}  // extern "C"
+
+namespace {
+
+// The scores' part of the problem; a score without a cap, slopes and a prefix is a plain one.
+fc_status score_problem(const fc_attn_score* score, fc::Problem* p) {
+  if (score == nullptr) return FC_OK;
+  if (!(score->softcap >= 0.0f && score->softcap < INFINITY))
+    return fail(FC_ERR_INVALID_ARGUMENT, "softcap must be finite and at least 0 (0: none)");
+  if (((reinterpret_cast<uintptr_t>(score->slopes) | reinterpret_cast<uintptr_t>(score->prefix)) & 3) != 0)
+    return fail(FC_ERR_INVALID_ARGUMENT, "slopes and prefix must be 4-byte aligned");
+  p->prefix = score->prefix != nullptr;
+  const bool cap = score->softcap > 0.0f, bias = score->slopes != nullptr;
+  if (!cap && !bias && !p->prefix) return FC_OK;
+  if (!p->bf16) return fail(FC_ERR_UNSUPPORTED, "capped, biased and prefix-masked scores need fast mode (bf16 Q, K and V)");
+  p->score = 1 + (cap ? 2 : 0) + (bias ? 4 : 0);
+  return FC_OK;
+}
+
+fc::ScoreArgs score_args(const fc::Problem& p, const fc_attn_score* score) {
+  fc::ScoreArgs a{};
+  if (p.score == 0) return a;
+  if (score->softcap > 0.0f) {
+    a.cap_in = (float)(2.0 * 1.4426950408889634 / ((double)score->softcap * std::sqrt((double)p.D)));
+    a.cap_out = (float)(1.4426950408889634 * score->softcap);
+  }
+  a.slopes = score->slopes;
+  a.prefix = score->prefix;
+  a.prefix_per_token = score->prefix_per_token != 0;
+  return a;
+}
+
+fc::BoundsArgs bounds_args(const fc::Problem& p, const int32_t* positions, const fc_attn_score* score, int32_t* chunk_lb,
+                           int32_t* chunk_ub) {
+  fc::BoundsArgs a{positions, chunk_lb, p.T, p.B, p.left, nullptr, nullptr, 0, 0};
+  if (p.prefix) {
+    a.chunk_ub = chunk_ub;
+    a.prefix = score->prefix;
+    a.prefix_per_token = score->prefix_per_token != 0;
+    a.right = p.right;
+  }
+  return a;
+}
+
+fc_status workspace_bytes(const fc_attn_desc* desc, const fc_attn_score* score, int32_t pass, int32_t positions_given,
+                          size_t* bytes) {
   fc::Problem p;
-  const fc_status st = make_problem(desc, &p);
+  fc_status st = make_problem(desc, &p);
   if (st != FC_OK) return st;
   if (bytes == nullptr) return fail(FC_ERR_INVALID_ARGUMENT, "bytes is null");
+  if ((st = score_problem(score, &p)) != FC_OK) return st;
   p.positions = positions_given != 0;
   if (pass == FC_PASS_FORWARD) {
     *bytes = fc::fwd_workspace(p).total;
@@ -177,14 +223,15 @@ fc_status fc_attn_workspace_bytes(const fc_attn_desc* desc, int32_t pass, int32_
   return ok();
 }
 
-fc_status fc_attn_fwd(const fc_attn_desc* desc, const void* Q, const void* K, const void* V,
-                      const int32_t* positions, void* O, float* l, float* m, void* workspace,
-                      size_t workspace_bytes, void* stream) {
+fc_status fwd_run(const char* who, const fc_attn_desc* desc, const fc_attn_score* score, const void* Q, const void* K,
+                  const void* V, const int32_t* positions, void* O, float* l, float* m, void* workspace,
+                  size_t workspace_bytes, void* stream) {
   fc::Problem p;
   fc_status st = make_problem(desc, &p);
   if (st != FC_OK) return st;
   if (Q == nullptr || K == nullptr || V == nullptr || O == nullptr || l == nullptr || m == nullptr)
-    return fail(FC_ERR_INVALID_ARGUMENT, "fc_attn_fwd: a required pointer is null");
+    return fail(FC_ERR_INVALID_ARGUMENT, "%s: a required pointer is null", who);
+  if ((st = score_problem(score, &p)) != FC_OK) return st;
   p.positions = positions != nullptr;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   // The workspace is optional (with one, fast mode with positions takes the
@@ -212,9 +259,10 @@ fc_status fc_attn_fwd(const fc_attn_desc* desc, const void* Q, const void* K, co
   if (fc::ordered(p) && w != nullptr) {
     int32_t* chunk_lb = reinterpret_cast<int32_t*>(w + ws.chunk_lb);
     order = reinterpret_cast<int32_t*>(w + ws.qorder);
-    e = fc::launch_bounds(p, fc::BoundsArgs{positions, chunk_lb, p.T, p.B, p.left}, s);
+    int32_t* chunk_ub = p.prefix ? reinterpret_cast<int32_t*>(w + ws.chunk_ub) : nullptr;
+    e = fc::launch_bounds(p, bounds_args(p, positions, score, chunk_lb, chunk_ub), s);
     if (e != hipSuccess) return fail(FC_ERR_HIP, "bounds launch failed: %s", hipGetErrorString(e));
-    e = fc::launch_order(p, fc::OrderArgs{chunk_lb, order, nullptr, p.T, p.B, p.left, p.right}, s);
+    e = fc::launch_order(p, fc::OrderArgs{chunk_lb, order, nullptr, p.T, p.B, p.left, p.right, chunk_ub}, s);
     if (e != hipSuccess) return fail(FC_ERR_HIP, "order launch failed: %s", hipGetErrorString(e));
   }
   fc::FwdArgs a{};
@@ -238,10 +286,36 @@ fc_status fc_attn_fwd(const fc_attn_desc* desc, const void* Q, const void* K, co
   e = fc::device_cus(&a.cus);
   if (e != hipSuccess) return fail(FC_ERR_HIP, "forward: %s", hipGetErrorString(e));
   a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)p.D));
+  a.score = score_args(p, score);
   e = fc::launch_fwd(p, a, s);
   if (e != hipSuccess) return fail(FC_ERR_HIP, "forward launch failed: %s", hipGetErrorString(e));
   if (out != O && (st = copy_values(out, O, p.out_bf16, nq, s)) != FC_OK) return st;
   return ok();
+}
+
+}  // namespace
+
+extern "C" {
+
+fc_status fc_attn_workspace_bytes(const fc_attn_desc* desc, int32_t pass, int32_t positions_given, size_t* bytes) {
+  return workspace_bytes(desc, nullptr, pass, positions_given, bytes);
+}
+
+fc_status fc_attn_score_workspace_bytes(const fc_attn_desc* desc, const fc_attn_score* score, int32_t pass,
+                                        int32_t positions_given, size_t* bytes) {
+  return workspace_bytes(desc, score, pass, positions_given, bytes);
+}
+
+fc_status fc_attn_fwd(const fc_attn_desc* desc, const void* Q, const void* K, const void* V,
+                      const int32_t* positions, void* O, float* l, float* m, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  return fwd_run("fc_attn_fwd", desc, nullptr, Q, K, V, positions, O, l, m, workspace, workspace_bytes, stream);
+}
+
+fc_status fc_attn_score_fwd(const fc_attn_desc* desc, const fc_attn_score* score, const void* Q, const void* K,
+                            const void* V, const int32_t* positions, void* O, float* l, float* m, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  return fwd_run("fc_attn_score_fwd", desc, score, Q, K, V, positions, O, l, m, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"
@@ -249,14 +323,15 @@ fc_status fc_attn_fwd(const fc_attn_desc* desc, const void* Q, const void* K, co
 namespace {
 
 // Validation the two backward entry points share: the problem, the pointers.
-fc_status bwd_problem(const char* who, const fc_attn_desc* desc, const void* dO, const void* Q, const void* K,
+fc_status bwd_problem(const char* who, const fc_attn_desc* desc, const fc_attn_score* score, const void* dO, const void* Q, const void* K,
                       const void* V, const void* O, const float* l, const float* m, const int32_t* positions,
                       const void* dQ, const void* dK, const void* dV, fc::Problem* p) {
-  const fc_status st = make_problem(desc, p);
+  fc_status st = make_problem(desc, p);
   if (st != FC_OK) return st;
   if (dO == nullptr || Q == nullptr || K == nullptr || V == nullptr || O == nullptr || l == nullptr ||
       m == nullptr || dQ == nullptr || dK == nullptr || dV == nullptr)
     return fail(FC_ERR_INVALID_ARGUMENT, "%s: a required pointer is null", who);
+  if ((st = score_problem(score, p)) != FC_OK) return st;
   p->positions = positions != nullptr;
   return FC_OK;
 }
@@ -265,7 +340,7 @@ fc_status bwd_problem(const char* who, const fc_attn_desc* desc, const void* dO,
 // (bwd_workspace(p).total bytes, 256-byte aligned).  Every workspace byte the
 // kernels read is written earlier in the same sequence, so the workspace
 // needs no clearing.
-fc_status bwd_launch(const fc::Problem& p, const void* dO, const void* Q, const void* K, const void* V,
+fc_status bwd_launch(const fc::Problem& p, const fc_attn_score* score, const void* dO, const void* Q, const void* K, const void* V,
                      const void* O, const float* l, const float* m, const int32_t* positions, void* dQ, void* dK,
                      void* dV, char* w, hipStream_t s) {
   const fc::BwdWorkspace ws = fc::bwd_workspace(p);
@@ -296,10 +371,11 @@ fc_status bwd_launch(const fc::Problem& p, const void* dO, const void* Q, const 
   }
 
   int32_t* chunk_lb = nullptr;
-  if (p.positions) {
+  int32_t* chunk_ub = nullptr;
+  if (p.positions || p.prefix) {
     chunk_lb = reinterpret_cast<int32_t*>(w + ws.chunk_lb);
-    fc::BoundsArgs ba{positions, chunk_lb, p.T, p.B, p.left};
-    e = fc::launch_bounds(p, ba, s);
+    if (p.prefix) chunk_ub = reinterpret_cast<int32_t*>(w + ws.chunk_ub);
+    e = fc::launch_bounds(p, bounds_args(p, positions, score, chunk_lb, chunk_ub), s);
     if (e != hipSuccess) return fail(FC_ERR_HIP, "bounds launch failed: %s", hipGetErrorString(e));
   }
   int32_t* qorder = nullptr;
@@ -307,7 +383,7 @@ fc_status bwd_launch(const fc::Problem& p, const void* dO, const void* Q, const 
   if (fc::ordered(p)) {
     qorder = reinterpret_cast<int32_t*>(w + ws.qorder);
     korder = reinterpret_cast<int32_t*>(w + ws.korder);
-    e = fc::launch_order(p, fc::OrderArgs{chunk_lb, qorder, korder, p.T, p.B, p.left, p.right}, s);
+    e = fc::launch_order(p, fc::OrderArgs{chunk_lb, qorder, korder, p.T, p.B, p.left, p.right, chunk_ub}, s);
     if (e != hipSuccess) return fail(FC_ERR_HIP, "order launch failed: %s", hipGetErrorString(e));
   }
 
@@ -338,7 +414,10 @@ fc_status bwd_launch(const fc::Problem& p, const void* dO, const void* Q, const 
   a.accumulate = p.accumulate ? 1 : 0;
   e = fc::device_cus(&a.cus);
   if (e != hipSuccess) return fail(FC_ERR_HIP, "backward: %s", hipGetErrorString(e));
-  a.scale = (float)(1.0 / std::sqrt((double)p.D));
+  // (the factor 4 of a cap's derivative, attn_score.hpp)
+  a.scale = (float)((p.score & 2 ? 4.0 : 1.0) / std::sqrt((double)p.D));
+  a.score = score_args(p, score);
+  a.chunk_ub = chunk_ub;
   a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)p.D));
   if (fused_stats) {
     a.stats = 1;
@@ -361,7 +440,7 @@ fc_status bwd_launch(const fc::Problem& p, const void* dO, const void* Q, const 
 }
 
 // bwd_launch, with the tensors that needs_room names moved through the workspace.
-fc_status bwd_run(const fc::Problem& p, const void* dO, const void* Q, const void* K, const void* V, const void* O,
+fc_status bwd_run(const fc::Problem& p, const fc_attn_score* score, const void* dO, const void* Q, const void* K, const void* V, const void* O,
                   const float* l, const float* m, const int32_t* positions, void* dQ, void* dK, void* dV, char* w,
                   hipStream_t s) {
   const fc::PadWorkspace pw = fc::pad_workspace(p, true);
@@ -379,7 +458,7 @@ fc_status bwd_run(const fc::Problem& p, const void* dO, const void* Q, const voi
     if (!needs_room(p, grads[i])) at[i] = grads[i];
     else if (p.accumulate && (st = copy_values(grads[i], at[i], p.grad_bf16, counts[i], s)) != FC_OK) return st;
   }
-  st = bwd_launch(p, dO, Q, K, V, O, l, m, positions, at[0], at[1], at[2], w, s);
+  st = bwd_launch(p, score, dO, Q, K, V, O, l, m, positions, at[0], at[1], at[2], w, s);
   for (int i = 0; i < 3 && st == FC_OK; ++i)
     if (at[i] != grads[i]) st = copy_values(at[i], grads[i], p.grad_bf16, counts[i], s);
   return st;
@@ -389,11 +468,12 @@ fc_status bwd_run(const fc::Problem& p, const void* dO, const void* Q, const voi
 
 extern "C" {
 
-fc_status fc_attn_bwd(const fc_attn_desc* desc, const void* dO, const void* Q, const void* K, const void* V,
-                      const void* O, const float* l, const float* m, const int32_t* positions, void* dQ,
-                      void* dK, void* dV, void* workspace, size_t workspace_bytes, void* stream) {
+static fc_status bwd_entry(const char* who, const fc_attn_desc* desc, const fc_attn_score* score, const void* dO,
+                           const void* Q, const void* K, const void* V, const void* O, const float* l, const float* m,
+                           const int32_t* positions, void* dQ, void* dK, void* dV, void* workspace,
+                           size_t workspace_bytes, void* stream) {
   fc::Problem p;
-  const fc_status st = bwd_problem("fc_attn_bwd", desc, dO, Q, K, V, O, l, m, positions, dQ, dK, dV, &p);
+  const fc_status st = bwd_problem(who, desc, score, dO, Q, K, V, O, l, m, positions, dQ, dK, dV, &p);
   if (st != FC_OK) return st;
   const fc::BwdWorkspace ws = fc::bwd_workspace(p);
   if (workspace == nullptr || workspace_bytes < ws.total)
@@ -401,8 +481,23 @@ fc_status fc_attn_bwd(const fc_attn_desc* desc, const void* dO, const void* Q, c
                 workspace == nullptr ? " (null)" : "");
   if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
     return fail(FC_ERR_WORKSPACE, "workspace must be 256-byte aligned");
-  return bwd_run(p, dO, Q, K, V, O, l, m, positions, dQ, dK, dV, static_cast<char*>(workspace),
+  return bwd_run(p, score, dO, Q, K, V, O, l, m, positions, dQ, dK, dV, static_cast<char*>(workspace),
                  static_cast<hipStream_t>(stream));
+}
+
+fc_status fc_attn_bwd(const fc_attn_desc* desc, const void* dO, const void* Q, const void* K, const void* V,
+                      const void* O, const float* l, const float* m, const int32_t* positions, void* dQ,
+                      void* dK, void* dV, void* workspace, size_t workspace_bytes, void* stream) {
+  return bwd_entry("fc_attn_bwd", desc, nullptr, dO, Q, K, V, O, l, m, positions, dQ, dK, dV, workspace, workspace_bytes,
+                   stream);
+}
+
+fc_status fc_attn_score_bwd(const fc_attn_desc* desc, const fc_attn_score* score, const void* dO, const void* Q,
+                            const void* K, const void* V, const void* O, const float* l, const float* m,
+                            const int32_t* positions, void* dQ, void* dK, void* dV, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  return bwd_entry("fc_attn_score_bwd", desc, score, dO, Q, K, V, O, l, m, positions, dQ, dK, dV, workspace,
+                   workspace_bytes, stream);
 }
 
 }  // extern "C"
@@ -450,7 +545,7 @@ fc_status fc_attn_bwd_noalloc(const fc_attn_desc* desc, const void* dO, const vo
                               const void* O, const float* l, const float* m, const int32_t* positions, void* dQ,
                               void* dK, void* dV, void* stream) {
   fc::Problem p;
-  fc_status st = bwd_problem("fc_attn_bwd_noalloc", desc, dO, Q, K, V, O, l, m, positions, dQ, dK, dV, &p);
+  fc_status st = bwd_problem("fc_attn_bwd_noalloc", desc, nullptr, dO, Q, K, V, O, l, m, positions, dQ, dK, dV, &p);
   if (st != FC_OK) return st;
   const size_t need = fc::bwd_workspace(p).total;
   if (need > (size_t)FC_ATTN_NOALLOC_SCRATCH_BYTES)
@@ -461,7 +556,7 @@ fc_status fc_attn_bwd_noalloc(const fc_attn_desc* desc, const void* dO, const vo
   char* w = nullptr;
   st = current_scratch(&w);
   if (st != FC_OK) return st;
-  return bwd_run(p, dO, Q, K, V, O, l, m, positions, dQ, dK, dV, w, static_cast<hipStream_t>(stream));
+  return bwd_run(p, nullptr, dO, Q, K, V, O, l, m, positions, dQ, dK, dV, w, static_cast<hipStream_t>(stream));
 }
 
 // ---- attention prologue (rope_norm.hip) -----------------------------------

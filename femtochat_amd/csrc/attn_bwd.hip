@@ -22,6 +22,7 @@
 //                    so dS^T is directly the B operand of dQ^T += K^T dS^T.
 #include "attn_exact.hpp"
 #include "attn_launch.hpp"
+#include "attn_score.hpp"
 
 #include <type_traits>
 
@@ -84,14 +85,38 @@ __global__ __launch_bounds__(kThreads) void attn_bounds_kernel(BoundsArgs a) {
   }
 }
 
+// The same with a prefix, and per chunk the (min, max) last visible key beside it (a
+// query at or beyond T counts as -1).
+__global__ __launch_bounds__(kThreads) void attn_prefix_bounds_kernel(BoundsArgs a) {
+  const int nc = (a.T + 31) / 32;
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t chunk = i >> 5;
+  const bool live = chunk < (int64_t)nc * a.B;  // uniform over each half-wave
+  const int b = live ? (int)(chunk / nc) : 0;
+  const int q = live ? 32 * (int)(chunk - (int64_t)b * nc) + (int)(i & 31) : a.T;
+  const int32_t* pos = a.pos != nullptr ? a.pos + (int64_t)b * a.T : nullptr;
+  const int32_t* prefix = a.prefix + (int64_t)b * (a.prefix_per_token ? a.T : 1);
+  const int lb = key_lb(q, a.T, a.left, pos);
+  const int ub = score_ub(q, a.T, a.right, pos, prefix, a.prefix_per_token != 0);
+  const int lo = wave_min32(lb), hi = wave_max32(lb), ulo = wave_min32(ub), uhi = wave_max32(ub);
+  if (live && (i & 31) == 0) {
+    a.chunk_lb[2 * chunk] = lo;
+    a.chunk_lb[2 * chunk + 1] = hi;
+    a.chunk_ub[2 * chunk] = ulo;
+    a.chunk_ub[2 * chunk + 1] = uhi;
+  }
+}
+
 // Work order of the fast kernels' tiles with positions, in one workgroup.
 // The smallest key lower bound of every 128-query tile (from the chunk
 // bounds) goes to LDS; then the work of each item of 128 rows, in steps:
 //  * query tile [q0, q1] (forward and dQ): the 64-key tiles from the one
-//    holding its smallest lower bound up to the one holding key_ub(q1);
+//    holding its smallest lower bound up to the one holding key_ub(q1), or with
+//    a prefix its largest upper bound;
 //  * key tile [k0, k1] (dK/dV): the 128-query tiles between k0 - right and
 //    k1 + left whose smallest lower bound is at most k1, which are the
-//    tiles the dK/dV kernel visits;
+//    tiles the dK/dV kernel visits (with a prefix, from tile 0 on those that
+//    also reach k0);
 // and finally each item's rank: the items of more work, plus the items of
 // equal work and lower index.  order[rank] = item.  The inner loops read
 // LDS in runs of 8 with no exit inside a run, so the reads of a run are in
@@ -102,6 +127,7 @@ constexpr int kOrderRun = 8;
 __global__ __launch_bounds__(kOrderThreads) void attn_order_kernel(OrderArgs a) {
   static_assert(kOrderKStep == kOrderRows, "a dK/dV step is one tabulated query tile");
   __shared__ int s_lb[kOrderMaxItems + kOrderRun];
+  __shared__ int s_ub[kOrderMaxItems + kOrderRun];  // with a prefix: a query tile's largest upper bound
   __shared__ __attribute__((aligned(16))) int s_work[kOrderMaxItems + kOrderRun];
   const int tid = threadIdx.x, T = a.T;
   const int nc = (T + 31) / 32, n128 = (T + kOrderRows - 1) / kOrderRows;
@@ -114,6 +140,13 @@ __global__ __launch_bounds__(kOrderThreads) void attn_order_kernel(OrderArgs a) 
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) lo = min(lo, cb[2 * min(kChunks * t + c, nc - 1)]);  // loads without a branch
     s_lb[i] = lo;
+    if (a.chunk_ub != nullptr) {
+      const int32_t* ub = a.chunk_ub + (int64_t)b * nc * 2;
+      int hi = -1;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) hi = max(hi, ub[2 * min(kChunks * t + c, nc - 1) + 1]);
+      s_ub[i] = hi;
+    }
   }
   // Padding after the last item: never counted (ranks) or masked (key steps).
   if (tid < kOrderRun) s_work[items + tid] = INT_MIN;
@@ -146,7 +179,8 @@ __global__ __launch_bounds__(kOrderThreads) void attn_order_kernel(OrderArgs a) 
     for (int i = tid; i < items; i += kOrderThreads) {
       const int t = i % n128;
       const int kmin = s_lb[i];
-      const int kmax = key_ub(min(t * kOrderRows + kOrderRows - 1, T - 1), T, a.right);
+      int kmax = key_ub(min(t * kOrderRows + kOrderRows - 1, T - 1), T, a.right);
+      if (a.chunk_ub != nullptr) kmax = s_ub[i];
       s_work[i] = kmax >= kmin ? (kmax - (kmin / kOrderTile) * kOrderTile) / kOrderTile + 1 : 0;
     }
     __syncthreads();
@@ -157,9 +191,11 @@ __global__ __launch_bounds__(kOrderThreads) void attn_order_kernel(OrderArgs a) 
     for (int i = tid; i < items; i += kOrderThreads) {
       const int b = i / n128, t = i - b * n128;
       const int k0 = t * kOrderRows, k1 = min(k0 + kOrderRows, T) - 1;
-      const int qlo = max(0, k0 - a.right), qhi = min(T - 1, k1 + a.left);
+      const int qlo = a.chunk_ub != nullptr ? 0 : max(0, k0 - a.right), qhi = min(T - 1, k1 + a.left);
       int n = 0;
-      if (qhi >= qlo) {
+      if (a.chunk_ub != nullptr) {
+        for (int u = 0; u <= qhi / kOrderKStep; ++u) n += (s_lb[b * n128 + u] <= k1 && s_ub[b * n128 + u] >= k0) ? 1 : 0;
+      } else if (qhi >= qlo) {
         const int* row = s_lb + b * n128;
         const int ulast = qhi / kOrderKStep;
         for (int u0 = qlo / kOrderKStep; u0 <= ulast; u0 += kOrderRun) {
@@ -681,7 +717,8 @@ hipError_t launch_bounds(const Problem& p, const BoundsArgs& a, hipStream_t s) {
   const int64_t n = (int64_t)((p.T + 31) / 32) * p.B * 32;  // one lane per query slot
   const dim3 grid((unsigned)((n + kThreads - 1) / kThreads)), block(kThreads);
   const ProfileMark mk = profile_begin(s);
-  hipLaunchKernelGGL(attn_bounds_kernel, grid, block, 0, s, a);
+  if (a.prefix != nullptr) hipLaunchKernelGGL(attn_prefix_bounds_kernel, grid, block, 0, s, a);
+  else hipLaunchKernelGGL(attn_bounds_kernel, grid, block, 0, s, a);
   const hipError_t e = hipGetLastError();
   profile_end(mk, "attn_bounds", s);
   return e;

@@ -8,6 +8,7 @@
 
 #include "attn_fast.hpp"
 #include "attn_launch.hpp"
+#include "attn_score.hpp"
 
 #include <type_traits>
 
@@ -34,7 +35,12 @@ struct DkdvFastCfg {
 // wave's own instruction stream, and sched_group_barrier interleaves them
 // (plus the LDS reads) within each phase.  LDS fragments are requested a
 // phase, or a few products, before their use.
-template <int D>
+// What a step's scores need beyond c2 (attn_score.hpp); with a cap, lse holds
+// lse2 - cap_out.
+struct StepScore {
+  float cap_in, cap_out, slope2;
+};
+template <int D, int kScore>
 struct DkdvStep {
   using C = DkdvFastCfg<D>;
   using M = Mma<bf16>;
@@ -42,6 +48,8 @@ struct DkdvStep {
   static constexpr int NPH = NQB + 2;            // phases of the body
   static constexpr int NTR = 2 * DB;             // transposed fragments per operand and block
   static constexpr int NPRE = NTR < 2 ? NTR : 2;  // of them requested one phase early
+  static constexpr int kNoUpper = -2;            // in place of chunk upper bounds: the window's own
+  static constexpr int kMoreValu = ((kScore & kCap) ? 4 : 0) + ((kScore & kBias) ? 2 : 0);  // per score
   static constexpr int kSchedVALU = 0x2, kSchedMFMA = 0x8, kSchedDSRead = 0x100;
 
   // dma(k), k = 0..NPH-1, issues a share of the next tile's loads; the body
@@ -51,7 +59,7 @@ struct DkdvStep {
   __device__ __attribute__((always_inline)) static inline void run(const Dma& dma, const char* Qs, const char* Os, const float* lse,
                                     const float* delta, const int* lbs, const int* lbc, const bf16x8* kf,
                                     const bf16x8* vf, f32x16* dk, f32x16* dv, const FragOffsets<DkdvFastCfg<D>::kW>& fo, int q0,
-                                    int key, int kw0, int kw1, int g, int T, int right, float c2) {
+                                    int key, int kw0, int kw1, int g, int T, int right, float c2, const StepScore& sc) {
     // Smallest and largest key lower bound over the tile's queries, from the
     // per-chunk bounds published with the tile (no cross-lane reduction).
     int lbmin = lbc[0], lbmax = lbc[NQB];
@@ -63,8 +71,19 @@ struct DkdvStep {
     // LDS broadcasts, the same on every lane: scalar branches below.
     lbmin = __builtin_amdgcn_readfirstlane(lbmin);
     lbmax = __builtin_amdgcn_readfirstlane(lbmax);
-    const int ubmin = q0 + BQ - 1 >= T ? -1 : key_ub(q0, T, right);  // ub is monotone in q
-    const int ubmax = key_ub(min(q0 + BQ - 1, T - 1), T, right);
+    int ubmin = q0 + BQ - 1 >= T ? -1 : key_ub(q0, T, right);  // ub is monotone in q
+    int ubmax = key_ub(min(q0 + BQ - 1, T - 1), T, right);
+    if (kScore && lbc[2 * NQB] != kNoUpper) {  // a prefix's upper bounds, published like the lower ones
+      ubmin = lbc[2 * NQB];
+      ubmax = lbc[3 * NQB];
+#pragma unroll
+      for (int c = 1; c < NQB; ++c) {
+        ubmin = min(ubmin, lbc[2 * NQB + c]);
+        ubmax = max(ubmax, lbc[3 * NQB + c]);
+      }
+      ubmin = __builtin_amdgcn_readfirstlane(ubmin);
+      ubmax = __builtin_amdgcn_readfirstlane(ubmax);
+    }
     if (lbmin > kw1 || ubmax < kw0) {
 #pragma unroll
       for (int k = 0; k < NPH; ++k) dma(k);
@@ -74,13 +93,13 @@ struct DkdvStep {
     // steps cut by only one side of it test only that side.
     const bool lower = lbmax > kw0, upper = kw1 > ubmin;
     if (!lower && !upper)
-      body<0>(dma, Qs, Os, lse, delta, lbs, kf, vf, dk, dv, fo, q0, key, g, T, right, c2);
+      body<0>(dma, Qs, Os, lse, delta, lbs, kf, vf, dk, dv, fo, q0, key, g, T, right, c2, sc);
     else if (!lower)
-      body<kUpper>(dma, Qs, Os, lse, delta, lbs, kf, vf, dk, dv, fo, q0, key, g, T, right, c2);
+      body<kUpper>(dma, Qs, Os, lse, delta, lbs, kf, vf, dk, dv, fo, q0, key, g, T, right, c2, sc);
     else if (!upper)
-      body<kLower>(dma, Qs, Os, lse, delta, lbs, kf, vf, dk, dv, fo, q0, key, g, T, right, c2);
+      body<kLower>(dma, Qs, Os, lse, delta, lbs, kf, vf, dk, dv, fo, q0, key, g, T, right, c2, sc);
     else
-      body<kBoth>(dma, Qs, Os, lse, delta, lbs, kf, vf, dk, dv, fo, q0, key, g, T, right, c2);
+      body<kBoth>(dma, Qs, Os, lse, delta, lbs, kf, vf, dk, dv, fo, q0, key, g, T, right, c2, sc);
   }
 
   __device__ static inline void stats(const float* lse, const float* delta, int qb, int g, f32x4* L, f32x4* Dl) {
@@ -93,12 +112,13 @@ struct DkdvStep {
   }
   // Key lower bounds of the block's rows, and a factor 0 on rows with a
   // single visible key (whose dS is zero), else 1.
-  __device__ static inline void bounds(const int* lbs, int qb, int g, i32x4* LB, f32x4* Z) {
+  __device__ static inline void bounds(const int* lbs, int qb, int g, i32x4* LB, f32x4* Z, i32x4* UB) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int i0 = 32 * qb + 8 * j + 4 * g;
       LB[j] = *reinterpret_cast<const i32x4*>(&lbs[i0]);
       Z[j] = *reinterpret_cast<const f32x4*>(&lbs[BQ + i0]);
+      if (kScore) UB[j] = *reinterpret_cast<const i32x4*>(&lbs[2 * BQ + i0]);  // and upper bounds
     }
   }
 
@@ -111,21 +131,31 @@ struct DkdvStep {
   // only occurs in steps that test the upper side.
   template <int kSides>
   __device__ __attribute__((always_inline)) static inline void softmax(f32x16& s, f32x16& dp, const f32x4* L, const f32x4* Dl, const i32x4* LB,
-                                        const f32x4* Z, int qb, int q0, int key, int g, int T, int right, float c2,
-                                        bf16x8* pf, bf16x8* sf) {
+                                        const f32x4* Z, const i32x4* UB, int qb, int q0, int key, int g, int T, int right, float c2,
+                                        const StepScore& sc, bf16x8* pf, bf16x8* sf) {
     // key - q <= right  <=>  x >= -(8j + t) for row 4g + 8j + t; a key at or
     // past T (the last key tile's padding) fails it for every row, so that
     // P and dS stay zero there even for a row whose lse2 is -inf.
     const int x = key < T ? q0 + 32 * qb + 4 * g - key + right : -(1 << 30);
+    const float d = (float)(q0 + 32 * qb + 4 * g - key);  // the distance of row 4g
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const int r = 4 * j + t;
-        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -L[j][t]));
-        if (kSides & kUpper) p = x >= -(8 * j + t) ? p : 0.0f;
+        float e, u = 0.0f;
+        if constexpr ((kScore & kCap) != 0) {
+          u = cap_part(s[r], sc.cap_in);
+          e = __builtin_fmaf(-2.0f * sc.cap_out, u, -L[j][t]);
+        } else {
+          e = __builtin_fmaf(s[r], c2, -L[j][t]);
+        }
+        if constexpr ((kScore & kBias) != 0) e = __builtin_fmaf(-sc.slope2, __builtin_fabsf(d + (float)(8 * j + t)), e);
+        float p = __builtin_amdgcn_exp2f(e);
+        if (kSides & kUpper) p = (kScore ? key <= UB[j][t] : x >= -(8 * j + t)) ? p : 0.0f;
         if (kSides & kLower) p = key >= LB[j][t] ? p : 0.0f;
         float ds = p * (dp[r] - Dl[j][t]);
+        if constexpr ((kScore & kCap) != 0) ds *= __builtin_fmaf(-u, u, u);
         if (kSides) ds *= Z[j][t];
         s[r] = p;
         dp[r] = ds;
@@ -146,13 +176,14 @@ struct DkdvStep {
   __device__ __attribute__((always_inline)) static inline void body(const Dma& dma, const char* Qs, const char* Os, const float* lse,
                                      const float* delta, const int* lbs, const bf16x8* kf, const bf16x8* vf,
                                      f32x16* dk, f32x16* dv, const FragOffsets<DkdvFastCfg<D>::kW>& fo, int q0, int key, int g,
-                                     int T, int right, float c2) {
+                                     int T, int right, float c2, const StepScore& sc) {
     constexpr int M1 = 2 * KC;   // MFMAs of S, dP per block
     constexpr int M2 = 2 * NTR;  // MFMAs of dV, dK per block
     f32x16 s[NQB], dp[NQB];
     f32x4 L[NQB][4], Dl[NQB][4];
     i32x4 LB[NQB][4];
     f32x4 Z[NQB][4];
+    i32x4 UB[NQB][4];
     bf16x8 pf[NQB][2], sf[NQB][2];
     bf16x8 ofr[NQB][NTR], qfr[NQB][NTR];  // index h * DB + db
 #pragma unroll
@@ -170,7 +201,7 @@ struct DkdvStep {
           oa[c] = as_bf16x8(lds_load16(ot, fo.nat(c)));
         }
         stats(lse, delta, b1, g, L[b1], Dl[b1]);
-        if (kSides) bounds(lbs, b1, g, LB[b1], Z[b1]);
+        if (kSides) bounds(lbs, b1, g, LB[b1], Z[b1], UB[b1]);
         s[b1] = zero16();
         dp[b1] = zero16();
 #pragma unroll
@@ -193,7 +224,7 @@ struct DkdvStep {
         }
       }
       if (bs >= 0 && bs < NQB) {
-        softmax<kSides>(s[bs], dp[bs], L[bs], Dl[bs], LB[bs], Z[bs], bs, q0, key, g, T, right, c2, pf[bs],
+        softmax<kSides>(s[bs], dp[bs], L[bs], Dl[bs], LB[bs], Z[bs], UB[bs], bs, q0, key, g, T, right, c2, sc, pf[bs],
                            sf[bs]);
         // First transposed fragments of the block, for the next phase.
 #pragma unroll
@@ -212,8 +243,8 @@ struct DkdvStep {
         if (i < nmf) {
           __builtin_amdgcn_sched_group_barrier(kSchedMFMA, 1, 0);
           __builtin_amdgcn_sched_group_barrier(kSchedDSRead, 2, 0);
-          if (valu && nmf > 16) __builtin_amdgcn_sched_group_barrier(kSchedVALU, 4, 0);
-          if (valu && nmf <= 16) __builtin_amdgcn_sched_group_barrier(kSchedVALU, 8, 0);
+          if (valu && nmf > 16) __builtin_amdgcn_sched_group_barrier(kSchedVALU, 4 + kMoreValu / 2, 0);
+          if (valu && nmf <= 16) __builtin_amdgcn_sched_group_barrier(kSchedVALU, 8 + kMoreValu, 0);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -221,7 +252,7 @@ struct DkdvStep {
   }
 };
 
-template <int D>
+template <int D, int kScore>
 __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs a) {
   using C = DkdvFastCfg<D>;
   constexpr int BQ = C::kBQ, KC = C::kKC, DB = C::kDB;
@@ -231,8 +262,9 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
   __shared__ __attribute__((aligned(1024))) char bufB[C::kStageBytes];
   __shared__ __attribute__((aligned(16))) float s_lse[2][BQ];
   __shared__ __attribute__((aligned(16))) float s_delta[2][BQ];
-  __shared__ __attribute__((aligned(16))) int s_lb[2][2 * BQ];  // per slot: lb, then z as float (see softmax)
-  __shared__ __attribute__((aligned(16))) int s_lbc[2][2][BQ / 32];  // per slot: chunk min, max of s_lb
+  constexpr int kKinds = kScore ? 3 : 2;
+  __shared__ __attribute__((aligned(16))) int s_lb[2][kKinds * BQ];  // per slot: lb, then z as float (see softmax), then ub
+  __shared__ __attribute__((aligned(16))) int s_lbc[2][kScore ? 4 : 2][BQ / 32];  // per slot: chunk min, max of lb, then of ub
   constexpr int kVisTiles = 256;  // query tiles whose visibility is tabulated in LDS
   __shared__ unsigned char s_vis[kVisTiles];
 
@@ -308,6 +340,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
   int b = 0, kvh = 0, k0 = 0, k1 = 0, kw0 = 0, kw1 = 0, key = 0;
   const int32_t* pos = nullptr;
   const int32_t* clb = nullptr;
+  const int32_t* cub = nullptr;     // with a prefix
+  const int32_t* prefix = nullptr;
   int qt_begin = 0, n_qt_tiles = 0, t_first = 0, G = 0;
   bool vis_table = false;
   f32x16 dk[DB], dv[DB];  // the item's dK (unscaled) and dV
@@ -323,6 +357,12 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
     int lo = clb[2 * c0];
 #pragma unroll
     for (int c = 1; c < BQ / 32; ++c) lo = min(lo, clb[2 * min(c0 + c, nchunks - 1)]);
+    if (kScore && cub != nullptr) {  // and none that ends before k0
+      int hi = cub[2 * c0 + 1];
+#pragma unroll
+      for (int c = 1; c < BQ / 32; ++c) hi = max(hi, cub[2 * min(c0 + c, nchunks - 1) + 1]);
+      return (lo <= k1) & (hi >= k0);
+    }
     return lo <= k1;
   };
   auto tile_visible = [&](int qt) -> bool {
@@ -353,8 +393,14 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
     key = kw0 + l32;
     pos = a.pos ? a.pos + (int64_t)b * T : nullptr;
     clb = a.chunk_lb ? a.chunk_lb + (int64_t)b * nchunks * 2 : nullptr;
-    // Query tiles that can see [k0, k1]: q in [k0 - right, k1 + left].
-    const int qlo = max(0, k0 - a.right);
+    // Query tiles that can see [k0, k1]: q in [k0 - right, k1 + left], from the
+    // first on where a prefix shows later keys to earlier queries.
+    int qlo = max(0, k0 - a.right);
+    if constexpr (kScore != 0) {
+      cub = a.chunk_ub ? a.chunk_ub + (int64_t)b * nchunks * 2 : nullptr;
+      prefix = a.score.prefix ? a.score.prefix + (int64_t)b * (a.score.prefix_per_token ? T : 1) : nullptr;
+      if (cub != nullptr) qlo = 0;
+    }
     const int qhi = min(T - 1, k1 + a.left);
     qt_begin = qlo / BQ;
     n_qt_tiles = qhi >= qlo ? qhi / BQ - qt_begin + 1 : 0;
@@ -372,6 +418,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
   plan.init(wave, lane, qpitch);
   float st_lse = 0.0f, st_delta = 0.0f;
   int st_q = 0, st_pos = 0, st_cmin = 0, st_cmax = 0;
+  int st_pre = 0, st_umin = 0, st_umax = 0;  // with a prefix
   const float c2 = a.scale_log2;
 
   // issue() starts loading step st: the row statistics, positions and chunk
@@ -386,7 +433,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
   uint32_t nx_at = 0;
   // Phases 0..3 of a step issue the loads, so they have the rest of the step
   // to land; later phases issue none.
-  constexpr int NPH = DkdvStep<D>::NPH, NDMA = NPH < 4 ? NPH : 4;
+  constexpr int NPH = DkdvStep<D, kScore>::NPH, NDMA = NPH < 4 ? NPH : 4;
   constexpr int kPer = (DmaPlan<D, BQ>::kPerWave + NDMA - 1) / NDMA;
   auto dma_part = [&](int k) {
 #pragma unroll
@@ -416,6 +463,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
       st_lse = a.lse2[srow + qc];
       st_delta = a.delta[srow + qc];
       st_pos = (pos != nullptr ? pos : stand_in)[qc];
+      if (kScore) st_pre = (prefix != nullptr ? prefix : stand_in)[a.score.prefix_per_token ? qc : 0];
     }
     if (tid < BQ / 32) {
       // The bounds kernel's per-chunk (min, max) key lower bound.
@@ -423,17 +471,27 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
       const int32_t* cb = clb != nullptr ? clb + 2 * c : stand_in;
       st_cmin = cb[0];
       st_cmax = cb[clb != nullptr ? 1 : 0];
+      if (kScore) {
+        const int32_t* ub = cub != nullptr ? cub + 2 * c : stand_in;
+        st_umin = ub[0];
+        st_umax = ub[cub != nullptr ? 1 : 0];
+      }
     }
   };
   auto publish = [&](int slot) {
     if (tid < BQ) {
       const bool in = st_q < T;
-      s_lse[slot][tid] = in ? st_lse : INFINITY;
+      s_lse[slot][tid] = in ? ((kScore & kCap) ? st_lse - a.score.cap_out : st_lse) : INFINITY;
       s_delta[slot][tid] = in ? st_delta : 0.0f;
       int lb = T;
       if (in) lb = max(0, max(st_q - a.left, pos != nullptr ? st_q - st_pos : 0));
       s_lb[slot][tid] = lb;
-      s_lb[slot][BQ + tid] = __builtin_bit_cast(int, key_ub(st_q, T, a.right) > lb ? 1.0f : 0.0f);
+      int ub = key_ub(st_q, T, a.right);
+      if constexpr (kScore != 0) {
+        if (prefix != nullptr) ub = prefix_ub(st_q, T, a.right, st_pos, pos != nullptr, st_pre);
+        s_lb[slot][2 * BQ + tid] = ub;
+      }
+      s_lb[slot][BQ + tid] = __builtin_bit_cast(int, ub > lb ? 1.0f : 0.0f);
     }
     if (tid < BQ / 32) {
       // Key lower bounds of chunk tid of the tile (queries at or beyond T
@@ -447,14 +505,25 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
       }
       s_lbc[slot][0][tid] = lo;
       s_lbc[slot][1][tid] = hi;
+      if constexpr (kScore != 0) {
+        // (a chunk the sequence's end cuts has queries without keys)
+        s_lbc[slot][2][tid] = cub == nullptr ? DkdvStep<D, kScore>::kNoUpper : qc0 + 31 < T ? st_umin : -1;
+        s_lbc[slot][3][tid] = qc0 < T ? st_umax : -1;
+      }
     }
   };
   // Inlined by force: with four step bodies per buffer the compiler would
   // otherwise make this a call (all live registers saved around it).
   auto compute = [&](Step st, const char* buf, int slot) __attribute__((always_inline)) {
     const int q0 = (qt_begin + st.t) * BQ;
-    DkdvStep<D>::run(dma_part, buf, buf + C::kTileBytes, s_lse[slot], s_delta[slot], s_lb[slot], s_lbc[slot][0], kf, vf, dk, dv,
-                     fo, q0, key, kw0, kw1, g, T, a.right, c2);
+    StepScore sc{0.0f, 0.0f, 0.0f};
+    if constexpr ((kScore & kCap) != 0) {
+      sc.cap_in = a.score.cap_in;
+      sc.cap_out = a.score.cap_out;
+    }
+    if constexpr ((kScore & kBias) != 0) sc.slope2 = a.score.slopes[kvh * a.group + st.h] * kLog2e;
+    DkdvStep<D, kScore>::run(dma_part, buf, buf + C::kTileBytes, s_lse[slot], s_delta[slot], s_lb[slot], s_lbc[slot][0], kf, vf, dk, dv,
+                             fo, q0, key, kw0, kw1, g, T, a.right, c2, sc);
   };
 
   // The first step of the item set up last: its tile into bufA and its row
@@ -688,7 +757,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
   }
 }
 
-template <int D>
+template <int D, int kScore = 0>
 static hipError_t launch_dkdv_fast_t(const Problem& p, const BwdArgs& a, hipStream_t s) {
   const int n_kt = (p.T + DkdvFastCfg<D>::kBK - 1) / DkdvFastCfg<D>::kBK;
   const int n_items = n_kt * p.Hkv * p.B;
@@ -699,9 +768,9 @@ static hipError_t launch_dkdv_fast_t(const Problem& p, const BwdArgs& a, hipStre
   const int slots = cus >= kXcds && cus < n_items ? cus : n_items;
   const dim3 grid(slots), block(kThreads);
   const ProfileMark mk = profile_begin(s);
-  hipLaunchKernelGGL((attn_bwd_dkdv_fast_kernel<D>), grid, block, 0, s, a);
+  hipLaunchKernelGGL((attn_bwd_dkdv_fast_kernel<D, kScore>), grid, block, 0, s, a);
   const hipError_t e = hipGetLastError();
-  profile_end(mk, "attn_bwd_dkdv_bf16", s);
+  profile_end(mk, kScore ? "attn_bwd_dkdv_score_bf16" : "attn_bwd_dkdv_bf16", s);
   return e;
 }
 

@@ -11,6 +11,14 @@
 
 namespace fc {
 
+// Scores beyond q.k / sqrt(D) (attn_score.hpp), unused by the plain kernels.
+struct ScoreArgs {
+  float cap_in, cap_out;  // 2 log2(e) / (c sqrt(D)) and c log2(e)
+  const float* slopes;    // H, or null
+  const int32_t* prefix;  // (B, T) or (B), or null
+  int prefix_per_token;
+};
+
 struct FwdArgs {
   const void* Q;
   const void* K;
@@ -25,6 +33,7 @@ struct FwdArgs {
   int out_bf16;
   int cus;  // compute units (paired_position)
   float scale_log2;
+  ScoreArgs score;
 };
 
 struct PreArgs {
@@ -44,6 +53,10 @@ struct BoundsArgs {
   const int32_t* pos;
   int32_t* chunk_lb;  // [B][ceil(T/32)][2] = (min, max) of key_lb
   int T, B, left;
+  // with a prefix: the same of the last visible key
+  int32_t* chunk_ub;
+  const int32_t* prefix;
+  int prefix_per_token, right;
 };
 
 // Work order of the fast kernels with positions: attn_problem.hpp.
@@ -52,6 +65,7 @@ struct OrderArgs {
   int32_t* qorder;          // query tiles by decreasing key tiles, or null
   int32_t* korder;          // key tiles by decreasing query steps, or null
   int T, B, left, right;
+  const int32_t* chunk_ub;  // with a prefix, or null
 };
 
 struct BwdArgs {
@@ -85,8 +99,10 @@ struct BwdArgs {
   int H, Hkv, T, B, group, left, right;
   int grad_bf16, accumulate;
   int cus;  // compute units (paired_position)
-  float scale;       // 1/sqrt(D)
+  float scale;       // 1/sqrt(D) (capped scores: 4/sqrt(D))
   float scale_log2;  // log2(e)/sqrt(D)
+  ScoreArgs score;
+  const int32_t* chunk_ub;  // with a prefix: per 32 queries the (min, max) last visible key, or null
 };
 
 // Attention prologue (rope_norm.hip): rotary embedding then RMS norm x 1.2
@@ -191,6 +207,11 @@ hipError_t launch_bwd_dq(const Problem& p, const BwdArgs& a, hipStream_t s);
 hipError_t launch_fwd_fast(const Problem& p, const FwdArgs& a, hipStream_t s);
 hipError_t launch_bwd_dkdv_fast(const Problem& p, const BwdArgs& a, hipStream_t s);
 hipError_t launch_bwd_dq_fast(const Problem& p, const BwdArgs& a, hipStream_t s);
+// The same with the scores of p.score (attn_score_*.hip), one unit per variant.
+template <int kScore> hipError_t launch_score_fwd(const Problem& p, const FwdArgs& a, hipStream_t s);
+template <int kScore> hipError_t launch_score_dq(const Problem& p, const BwdArgs& a, hipStream_t s);
+template <int kScore> hipError_t launch_score_dkdv(const Problem& p, const BwdArgs& a, hipStream_t s);
+template <int kScore> hipError_t launch_score_dkdv_vgpr(const Problem& p, const BwdArgs& a, hipStream_t s);
 // The dK/dV kernel at head dims 16, 32 and 64 (attn_bwd_dkdv_vgpr.hip).
 hipError_t launch_bwd_dkdv_fast_vgpr(const Problem& p, const BwdArgs& a, hipStream_t s);
 

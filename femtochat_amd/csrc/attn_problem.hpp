@@ -26,6 +26,8 @@ struct Problem {
   bool grad_bf16;   // dQ/dK/dV storage
   bool accumulate;  // backward adds into dQ/dK/dV
   bool positions;
+  int score;        // 0, or the kinds of attn_score.hpp (a prefix, a cap, a bias)
+  bool prefix;
 };
 
 // XCDs of an MI355X: the hardware sends workgroup id to XCD id % kXcds.
@@ -141,6 +143,8 @@ inline fc_status make_problem(const fc_attn_desc* d, Problem* p, char* msg, size
   p->grad_bf16 = d->grad_dtype == FC_BF16;
   p->accumulate = (d->flags & FC_FLAG_OVERWRITE) == 0;
   p->positions = false;
+  p->score = 0;
+  p->prefix = false;
   return FC_OK;
 }
 
@@ -153,7 +157,7 @@ inline size_t order_bytes(const Problem& p) { return (size_t)p.B * ((p.T + kOrde
 // per-32-query key bounds and the query tiles' order (optional: without a
 // workspace the forward runs in the default order).
 struct FwdWorkspace {
-  size_t chunk_lb, qorder, total;
+  size_t chunk_lb, qorder, chunk_ub, total;
 };
 
 // What the workspace of head dims 48, 80, 96 and 112 begins with (byte
@@ -199,6 +203,8 @@ inline FwdWorkspace fwd_workspace(const Problem& p) {
     off = align256(off + chunk_bounds_bytes(p));
     w.qorder = off;
     off = align256(off + order_bytes(p));
+    w.chunk_ub = off;
+    if (p.prefix) off = align256(off + chunk_bounds_bytes(p));
   }
   w.total = off;
   return w;
@@ -207,11 +213,11 @@ inline FwdWorkspace fwd_workspace(const Problem& p) {
 // Workspace layout of the backward pass (byte offsets, 256-aligned):
 // PadWorkspace, then Delta and the base-2
 // log-sum-exp per query, per-32-query key bounds with
-// positions, a bf16 copy of an fp32 dO in fast mode, in fast mode the
+// positions (or a prefix, which also has upper ones), a bf16 copy of an fp32 dO in fast mode, in fast mode the
 // dK/dV kernel's work counters, and the dQ and dK/dV orders when the work
 // order applies.
 struct BwdWorkspace {
-  size_t delta, lse2, chunk_lb, dO16, queue, qorder, korder, total;
+  size_t delta, lse2, chunk_lb, dO16, queue, qorder, korder, chunk_ub, total;
 };
 
 inline BwdWorkspace bwd_workspace(const Problem& p) {
@@ -223,7 +229,7 @@ inline BwdWorkspace bwd_workspace(const Problem& p) {
   w.lse2 = off;
   off = align256(off + nq * sizeof(float));
   w.chunk_lb = off;
-  if (p.positions) off = align256(off + chunk_bounds_bytes(p));
+  if (p.positions || p.prefix) off = align256(off + chunk_bounds_bytes(p));
   w.dO16 = off;
   if (p.bf16 && !p.dout_bf16) off = align256(off + nq * p.Dk * sizeof(uint16_t));
   w.queue = off;  // the fast dK/dV kernel's work counters, one per XCD
@@ -232,6 +238,8 @@ inline BwdWorkspace bwd_workspace(const Problem& p) {
   if (ordered(p)) off = align256(off + order_bytes(p));
   w.korder = off;
   if (ordered(p)) off = align256(off + order_bytes(p));
+  w.chunk_ub = off;
+  if (p.prefix) off = align256(off + chunk_bounds_bytes(p));
   w.total = off;
   return w;
 }

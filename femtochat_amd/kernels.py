@@ -31,7 +31,12 @@ tuple with (-1, 0) meaning causal.
 
 New relative to the reference: ``positions=`` enables a document mask (key k
 is visible to query q only if k >= q - positions[q]); ``positions=None`` is the
-reference's behaviour exactly.
+reference's behaviour exactly.  So do ``softcap=`` (scores S become
+c tanh(S / c)), ``slopes=`` ((H,) float32: slopes[h] |q - k| is subtracted, after
+the cap) and ``prefix=`` (int32, (B,) or (B, T): each query also sees the keys up
+to the end of its prefix, the first ``prefix`` tokens of its row, or with
+positions of its document), in ``MFMAFast`` only; a backward takes what its
+forward took.
 """
 from __future__ import annotations
 
@@ -259,12 +264,35 @@ def _desc(A, Q, K, window, out_dtype, dout_dtype, grad_dtype, overwrite=False) -
 
 
 @lru_cache(maxsize=256)
-def _workspace_bytes(fields: bytes, which: int, with_positions: bool) -> int:
+def _workspace_bytes(fields: bytes, which: int, with_positions: bool, with_prefix: bool = False) -> int:
     """fc_attn_workspace_bytes of a descriptor (its bytes: sizes and options only)."""
     n = ctypes.c_size_t(0)
     d = _lib.AttnDesc.from_buffer_copy(fields)
-    _lib.check(_lib.lib().fc_attn_workspace_bytes(ctypes.byref(d), which, int(with_positions), ctypes.byref(n)))
+    score = _lib.AttnScore(0.0, 0, None, 4 if with_prefix else None)  # only whether there is a prefix counts
+    _lib.check(_lib.lib().fc_attn_score_workspace_bytes(ctypes.byref(d), ctypes.byref(score), which,
+                                                        int(with_positions), ctypes.byref(n)))
     return n.value
+
+
+def _score(softcap, slopes, prefix, device, B: int, T: int, H: int) -> Optional[_lib.AttnScore]:
+    """The scores' options as the library takes them, or None for plain scores."""
+    if not softcap and slopes is None and prefix is None:
+        return None
+    if slopes is not None:
+        _check_tensor("slopes", slopes, (H,), (torch.float32,), device)
+    per_token = prefix is not None and isinstance(prefix, torch.Tensor) and prefix.dim() != 1
+    if prefix is not None:
+        _check_tensor("prefix", prefix, (B, T) if per_token else (B,), (torch.int32,), device)
+    return _lib.AttnScore(float(softcap), int(per_token), _ptr(slopes), _ptr(prefix))
+
+
+def _call(device: torch.device, entry, *args) -> None:
+    """A library call on the tensors' device, whichever is current."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        _lib.check(entry(*args, _stream_ptr(device)))
+        return
+    with torch.cuda.device(device):
+        _lib.check(entry(*args, _stream_ptr(device)))
 
 
 def _check_common(A, Q, K, V, positions):
@@ -291,28 +319,30 @@ def _check_common(A, Q, K, V, positions):
 
 
 def attention_(A, O, l, m, Q, K, V, window: Tuple[int, int], *, positions=None,
-               workspace: Optional[torch.Tensor] = None, **options) -> None:
+               workspace: Optional[torch.Tensor] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None,
+               prefix: Optional[torch.Tensor] = None, **options) -> None:
     """Forward into caller buffers: ``attention!(𝒜, O, ℓ, m, Q, K, V, window)``
     (src/kernels.jl:419; ext/FemtoChatCUDAExt.jl:1242-1260).  O is bfloat16 or
     float32 (fast) / float32 (exact); ℓ and m are float32 (B,H,T).  With
     positions in fast mode the library orders the query tiles by their work
     in a small workspace (allocated here unless ``workspace`` is given, of
-    ``forward_workspace_bytes`` bytes); other problems need none."""
+    ``forward_workspace_bytes`` bytes); other problems need none.  ``softcap``,
+    ``slopes`` and ``prefix`` change the scores (module documentation)."""
     _reject_unknown(options)
     device, B, T, H, Hkv, D = _check_common(A, Q, K, V, positions)
     out_dtypes = (torch.bfloat16, torch.float32) if isinstance(A, MFMAFast) else (torch.float32,)
     _check_tensor("O", O, (B, T, H, D), out_dtypes, device)
     _check_tensor("l", l, _stats_shape(l, B, H, T), (torch.float32,), device)
     _check_tensor("m", m, _stats_shape(m, B, H, T), (torch.float32,), device)
-    _forward(A, O, l, m, Q, K, V, window, positions, workspace)
+    _forward(A, O, l, m, Q, K, V, window, positions, workspace, _score(softcap, slopes, prefix, device, B, T, H))
 
 
-def _forward(A, O, l, m, Q, K, V, window, positions, workspace=None) -> None:
+def _forward(A, O, l, m, Q, K, V, window, positions, workspace=None, score=None) -> None:
     """attention_ on checked tensors."""
     device = Q.device
     oc = _dtype_code(O.dtype)
     d = _desc(A, Q, K, window, oc, oc, oc)
-    nbytes = _workspace_bytes(bytes(d), _lib.FC_PASS_FORWARD, positions is not None)
+    nbytes = _workspace_bytes(bytes(d), _lib.FC_PASS_FORWARD, positions is not None, score is not None and bool(score.prefix))
     aligned = None
     if nbytes > 0:
         if workspace is None:
@@ -320,18 +350,20 @@ def _forward(A, O, l, m, Q, K, V, window, positions, workspace=None) -> None:
         elif workspace.device != device or workspace.numel() * workspace.element_size() < nbytes + 256:
             raise ValueError(f"workspace must be a {nbytes + 256}-byte tensor on {device}")
         aligned = (workspace.data_ptr() + 255) & ~255
-    _lib.check(_lib.lib().fc_attn_fwd(ctypes.byref(d), Q.data_ptr(), K.data_ptr(), V.data_ptr(), _ptr(positions),
-                                      O.data_ptr(), l.data_ptr(), m.data_ptr(), aligned, nbytes, _stream_ptr(device)))
+    _call(device, _lib.lib().fc_attn_score_fwd, ctypes.byref(d), score, Q.data_ptr(), K.data_ptr(), V.data_ptr(),
+          _ptr(positions), O.data_ptr(), l.data_ptr(), m.data_ptr(), aligned, nbytes)
 
 
 def delta_attention_(
     A, dQ, dK, dV, dO, Q, K, V, O, l, m, window: Tuple[int, int], *, positions=None, accumulate: bool = True,
-    workspace: Optional[torch.Tensor] = None, **options,
+    workspace: Optional[torch.Tensor] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None,
+    prefix: Optional[torch.Tensor] = None, **options,
 ) -> None:
     """Backward into caller buffers: ``Δattention!(𝒜, dQ, dK, dV, dO, Q, K, V, O,
     ℓ, m, window; accumulate=true)`` (src/kernels.jl:420;
     ext/FemtoChatCUDAExt.jl:1747-1790).  Adds into dQ/dK/dV unless
-    ``accumulate=False``.  Gradients may be bfloat16 or float32 (fast mode)."""
+    ``accumulate=False``.  Gradients may be bfloat16 or float32 (fast mode).
+    ``softcap``, ``slopes`` and ``prefix`` as the forward's."""
     _reject_unknown(options)
     device, B, T, H, Hkv, D = _check_common(A, Q, K, V, positions)
     fast = isinstance(A, MFMAFast)
@@ -343,40 +375,40 @@ def delta_attention_(
     _check_tensor("dQ", dQ, (B, T, H, D), io_dtypes, device)
     _check_tensor("dK", dK, (B, T, Hkv, D), (dQ.dtype,), device)
     _check_tensor("dV", dV, (B, T, Hkv, D), (dQ.dtype,), device)
-    _backward(A, dQ, dK, dV, dO, Q, K, V, O, l, m, window, positions, accumulate, workspace)
+    _backward(A, dQ, dK, dV, dO, Q, K, V, O, l, m, window, positions, accumulate, workspace,
+              _score(softcap, slopes, prefix, device, B, T, H))
 
 
-def _backward(A, dQ, dK, dV, dO, Q, K, V, O, l, m, window, positions, accumulate, workspace=None) -> None:
+def _backward(A, dQ, dK, dV, dO, Q, K, V, O, l, m, window, positions, accumulate, workspace=None, score=None) -> None:
     """delta_attention_ on checked tensors."""
     device = Q.device
     d = _desc(A, Q, K, window, _dtype_code(O.dtype), _dtype_code(dO.dtype), _dtype_code(dQ.dtype),
               overwrite=not accumulate)
-    nbytes = _workspace_bytes(bytes(d), _lib.FC_PASS_BACKWARD, positions is not None)
+    nbytes = _workspace_bytes(bytes(d), _lib.FC_PASS_BACKWARD, positions is not None, score is not None and bool(score.prefix))
     if workspace is None:  # freed to this stream's pool on return, so later work on the stream comes after the kernels
         workspace = torch.empty(max(nbytes, 256) + 256, dtype=torch.uint8, device=device)
     elif workspace.device != device or workspace.numel() * workspace.element_size() < nbytes + 256:
         raise ValueError(f"workspace must be a {nbytes + 256}-byte tensor on {device}")
-    _lib.check(_lib.lib().fc_attn_bwd(
-        ctypes.byref(d), dO.data_ptr(), Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), l.data_ptr(),
-        m.data_ptr(), _ptr(positions), dQ.data_ptr(), dK.data_ptr(), dV.data_ptr(),
-        (workspace.data_ptr() + 255) & ~255, nbytes, _stream_ptr(device)))
+    _call(device, _lib.lib().fc_attn_score_bwd, ctypes.byref(d), score, dO.data_ptr(), Q.data_ptr(), K.data_ptr(),
+          V.data_ptr(), O.data_ptr(), l.data_ptr(), m.data_ptr(), _ptr(positions), dQ.data_ptr(), dK.data_ptr(),
+          dV.data_ptr(), (workspace.data_ptr() + 255) & ~255, nbytes)
 
 
-def forward_workspace_bytes(A, Q, K, *, positions=None) -> int:
+def forward_workspace_bytes(A, Q, K, *, positions=None, prefix=None) -> int:
     """Bytes of the caller-owned workspace ``attention_(…, workspace=)``
     accepts (the library's requirement plus 256 bytes of alignment slack; 0
     when the problem needs none)."""
     d = _desc(A, Q, K, (-1, 0), _dtype_code(Q.dtype), _dtype_code(Q.dtype), _dtype_code(Q.dtype))
-    n = _workspace_bytes(bytes(d), _lib.FC_PASS_FORWARD, positions is not None)
+    n = _workspace_bytes(bytes(d), _lib.FC_PASS_FORWARD, positions is not None, prefix is not None)
     return n + 256 if n > 0 else 0
 
 
-def backward_workspace_bytes(A, Q, K, *, positions=None, dout_dtype=None) -> int:
+def backward_workspace_bytes(A, Q, K, *, positions=None, dout_dtype=None, prefix=None) -> int:
     """Bytes of the caller-owned workspace ``delta_attention_(…, workspace=)``
     accepts (the library's requirement plus 256 bytes of alignment slack)."""
     dd = _dtype_code(dout_dtype or Q.dtype)
     d = _desc(A, Q, K, (-1, 0), dd, dd, dd)
-    return _workspace_bytes(bytes(d), _lib.FC_PASS_BACKWARD, positions is not None) + 256
+    return _workspace_bytes(bytes(d), _lib.FC_PASS_BACKWARD, positions is not None, prefix is not None) + 256
 
 
 def _reject_unknown(options: dict) -> None:
@@ -387,7 +419,8 @@ def _reject_unknown(options: dict) -> None:
         raise TypeError(f"unexpected keyword(s) {sorted(unknown)}")
 
 
-def attention_state(A, Q, K, V, window, *, positions=None, **options) -> AttentionState:
+def attention_state(A, Q, K, V, window, *, positions=None, softcap: float = 0.0, slopes=None, prefix=None,
+                    **options) -> AttentionState:
     """Allocate O, ℓ, m, convert inputs, run the forward and return the saved
     state (src/kernels.jl:425-433).  ``A`` may be the ``attention`` function
     itself, which selects the default instruction like
@@ -405,10 +438,11 @@ def attention_state(A, Q, K, V, window, *, positions=None, **options) -> Attenti
     l = torch.empty((B, H, T), dtype=F, device=Q.device)
     m = torch.empty((B, H, T), dtype=F, device=Q.device)
     if options:
-        attention_(A, O, l, m, Qc, Kc, Vc, window, positions=positions, **options)
+        attention_(A, O, l, m, Qc, Kc, Vc, window, positions=positions, softcap=softcap, slopes=slopes, prefix=prefix,
+                   **options)
     else:  # O, l and m need no checks
         _check_common(A, Qc, Kc, Vc, positions)
-        _forward(A, O, l, m, Qc, Kc, Vc, window, positions)
+        _forward(A, O, l, m, Qc, Kc, Vc, window, positions, None, _score(softcap, slopes, prefix, Q.device, B, T, H))
     return AttentionState(A, Qc, Kc, Vc, O, l, m)
 
 
@@ -430,22 +464,23 @@ def attention(*args, positions=None, forward=None, backward=None, **options) -> 
 
 
 class AttentionFunction(torch.autograd.Function):
-    """Differentiable attention, the role of the reference's Enzyme rule
+    """``AttentionFunction.apply(Q, K, V, window, A, positions, softcap, slopes,
+    prefix)``: differentiable attention, the role of the reference's Enzyme rule
     (ext/FemtoChatEnzymeExt.jl:221-278): forward = ``attention_state``; reverse =
     ``Δattention!`` overwriting fresh gradient buffers."""
 
     @staticmethod
-    def forward(ctx, Q, K, V, window, A=None, positions=None):
+    def forward(ctx, Q, K, V, window, A=None, positions=None, softcap=0.0, slopes=None, prefix=None):
         A = A if A is not None else instruction(Q.dtype, Q.device, Q.shape[-1])
-        st = attention_state(A, Q, K, V, window, positions=positions)
-        ctx.save_for_backward(st.Q, st.K, st.V, st.O, st.l, st.m, positions)
-        ctx.A, ctx.window = A, window
+        st = attention_state(A, Q, K, V, window, positions=positions, softcap=softcap, slopes=slopes, prefix=prefix)
+        ctx.save_for_backward(st.Q, st.K, st.V, st.O, st.l, st.m, positions, slopes, prefix)
+        ctx.A, ctx.window, ctx.softcap = A, window, softcap
         ctx.dtypes = (Q.dtype, K.dtype, V.dtype)
         return st.O
 
     @staticmethod
     def backward(ctx, dO):
-        Q, K, V, O, l, m, positions = ctx.saved_tensors
+        Q, K, V, O, l, m, positions, slopes, prefix = ctx.saved_tensors
         dO = dO.contiguous()
         if dO.dtype != O.dtype:
             dO = dO.to(O.dtype)
@@ -457,9 +492,10 @@ class AttentionFunction(torch.autograd.Function):
         if isinstance(ctx.A, MFMAFast) and all(dt == torch.bfloat16 for dt in ctx.dtypes):
             gdtype = torch.bfloat16
         dQ, dK, dV = (torch.empty(x.shape, dtype=gdtype, device=Q.device) for x in (Q, K, V))
-        delta_attention_(ctx.A, dQ, dK, dV, dO, Q, K, V, O, l, m, ctx.window, positions=positions, accumulate=False)
+        delta_attention_(ctx.A, dQ, dK, dV, dO, Q, K, V, O, l, m, ctx.window, positions=positions, accumulate=False,
+                         softcap=ctx.softcap, slopes=slopes, prefix=prefix)
         out = [g.to(dt) if g.dtype != dt else g for g, dt in zip((dQ, dK, dV), ctx.dtypes)]
-        return out[0], out[1], out[2], None, None, None
+        return (out[0], out[1], out[2]) + (None,) * 6
 
 
 def capabilities(device: int = 0) -> dict:

@@ -130,6 +130,43 @@ fc_status fc_attn_bwd_noalloc(const fc_attn_desc* desc, const void* dO,
                               const int32_t* positions, void* dQ, void* dK,
                               void* dV, void* stream);
 
+/* ---- Capped, biased and prefix-masked scores --------------------------------
+ * The forward and the backward with scores beyond q.k/sqrt(D).  No reference
+ * counterpart.
+ *   softcap c > 0 : S <- c tanh(S / c)                       (S = q.k/sqrt(D))
+ *   slopes  (H)   : S <- S - slopes[h] |q - k|, after the cap; any finite values
+ *   prefix        : a query also sees the keys up to the end of its prefix,
+ *                   k <= max(q + right, start + n - 1), where start is the
+ *                   query's document's first token (q - positions[q], 0 without
+ *                   positions); the window's left side and the document still
+ *                   bound it from below.  n is prefix[b*T + q] (per token) or
+ *                   prefix[b] (one value per row), taken as 0 below 0 and T
+ *                   above T.
+ * Everything else is as above: rows with no visible key, the statistics (of the
+ * finished scores), the document mask, GQA, the workspace, the gradients (dS = 0
+ * for a query with a single visible key).  slopes and prefix have no gradient.
+ * Fast mode only (FC_ERR_UNSUPPORTED otherwise); a score with softcap 0 and null
+ * slopes and prefix is the plain one in either mode.  A capped score is off by at
+ * most c 2^-21. */
+typedef struct {
+  float softcap;             /* 0: none */
+  int32_t prefix_per_token;  /* prefix is (T,B), one value per token; else (B) */
+  const float* slopes;       /* device, H values, or NULL */
+  const int32_t* prefix;     /* device, or NULL */
+} fc_attn_score;
+
+fc_status fc_attn_score_workspace_bytes(const fc_attn_desc* desc, const fc_attn_score* score, int32_t pass,
+                                        int32_t positions_given, size_t* bytes);
+fc_status fc_attn_score_fwd(const fc_attn_desc* desc, const fc_attn_score* score, const void* Q,
+                            const void* K, const void* V, const int32_t* positions, void* O,
+                            float* l, float* m, void* workspace, size_t workspace_bytes,
+                            void* stream);
+fc_status fc_attn_score_bwd(const fc_attn_desc* desc, const fc_attn_score* score, const void* dO,
+                            const void* Q, const void* K, const void* V, const void* O,
+                            const float* l, const float* m, const int32_t* positions, void* dQ,
+                            void* dK, void* dV, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
 /* ---- Attention prologue ---------------------------------------------------
  * Rotary embedding followed by the RMS norm over the head dimension scaled by
  * 1.2, applied to Q or K as CausalSelfAttention does before calling
