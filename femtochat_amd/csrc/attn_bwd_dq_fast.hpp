@@ -171,6 +171,61 @@ __global__ __launch_bounds__(kThreads, 2) void attn_bwd_dq_fast_kernel(BwdArgs a
   const float c2 = a.scale_log2;
   const float slope2 = (kScore & kBias) ? a.score.slopes[h] * kLog2e : 0.0f;
   const float base = (kScore & kCap) ? neg_lse + a.score.cap_out : neg_lse;
+  // P of key k0 + acc_row(r, g), and the cap's r (attn_score.hpp) in u.
+  auto prob = [&](float x, int k0, int r, float& u) __attribute__((always_inline)) -> float {
+    float e;
+    if constexpr ((kScore & kCap) != 0) {
+      u = cap_part(x, a.score.cap_in);
+      e = __builtin_fmaf(-2.0f * a.score.cap_out, u, base);
+    } else {
+      e = __builtin_fmaf(x, c2, neg_lse);
+    }
+    if constexpr ((kScore & kBias) != 0)
+      e = __builtin_fmaf(-slope2, __builtin_fabsf((float)(q - k0 - 4 * g) - (float)acc_row(r, 0)), e);
+    return __builtin_amdgcn_exp2f(e);
+  };
+  if constexpr (kScore != 0) {
+    // Delta from a bf16 O carries O's rounding into every dS of its row, as large an
+    // error as the rounding of dS itself.  Over many rows it stays under 4e-3 of dQ
+    // and dK; over few it does not (up to 9e-3 at 32 rows, 5e-3 at 129, against 3e-3
+    // without it), so short sequences, whose kernels are bound by latency, sum
+    // Delta = P dP over their keys first.
+    constexpr int kShort = 256;
+    if (a.stats && T <= kShort) {
+      float sum = 0.0f;
+      dma_wait_barrier();
+      for (int it = 0; it < ntiles; ++it) {
+        const int kt = kt0 + it * BN;
+        const char* Ks = it & 1 ? bufB : bufA;
+        issue(it + 1, it & 1 ? bufA : bufB);
+#pragma unroll
+        for (int k = 0; k < NPH; ++k) dma_part(k);
+#pragma unroll
+        for (int blk = 0; blk < NKB; ++blk) {
+          f32x16 sv = zero16(), dv = zero16();
+#pragma unroll
+          for (int c = 0; c < KC; ++c) {
+            sv = M::mma(as_bf16x8(lds_load16(Ks + 32 * blk * 2 * C::kW, fo.nat(c))), qf[c], sv);
+            dv = M::mma(as_bf16x8(lds_load16(Ks + C::kTileBytes + 32 * blk * 2 * C::kW, fo.nat(c))), of[c], dv);
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int kk = kt + 32 * blk + acc_row(r, g);
+            float u = 0.0f;
+            const float p = prob(sv[r], kt + 32 * blk, r, u);
+            sum += ((kk >= lb) & (kk <= ub)) ? p * dv[r] : 0.0f;
+          }
+        }
+        dma_wait_barrier();
+      }
+      dlt = q < T ? sum + __shfl_xor(sum, 32) : 0.0f;
+      if (ntiles > 0) {  // the first tile again
+        issue(0, bufA);
+#pragma unroll
+        for (int k = 0; k < NPH; ++k) dma_part(k);
+      }
+    }
+  }
 
   // Tile body: a pipeline over the tile's two 32-key blocks, phase i holding
   // S^T, dP^T of block i, the softmax of block i-1 and dQ^T += K^T dS^T of
@@ -217,16 +272,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_bwd_dq_fast_kernel(BwdArgs a
       if (bs >= 0 && bs < NKB) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          float e, u = 0.0f;  // the exponent of P, and the cap's r (attn_score.hpp)
-          if constexpr ((kScore & kCap) != 0) {
-            u = cap_part(s[bs][r], a.score.cap_in);
-            e = __builtin_fmaf(-2.0f * a.score.cap_out, u, base);
-          } else {
-            e = __builtin_fmaf(s[bs][r], c2, neg_lse);
-          }
-          if constexpr ((kScore & kBias) != 0)
-            e = __builtin_fmaf(-slope2, __builtin_fabsf((float)(q - kt - 32 * bs - 4 * g) - (float)acc_row(r, 0)), e);
-          const float p = __builtin_amdgcn_exp2f(e);
+          float u = 0.0f;
+          const float p = prob(s[bs][r], kt + 32 * bs, r, u);
           float ds = p * (dp[bs][r] - dlt);
           if constexpr ((kScore & kCap) != 0) ds *= __builtin_fmaf(-u, u, u);
           if (need_mask) {
