@@ -20,7 +20,6 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .kernels import _call, _check_tensor, _dtype_code, _ptr
@@ -193,42 +192,57 @@ class PolicyLossFunction(torch.autograd.Function):
     def forward(ctx, logits, tokens, old_logprobs, advantages, ref_logprobs=None, clip=(0.2, 0.2), kl=0.0,
                 ignore_index=-1, reduction="mean"):
         logits = logits.contiguous()
-        dev, shape = logits.device, tuple(tokens.shape)
-        new = lambda *s: torch.empty(s, dtype=torch.float32, device=dev)  # noqa: E731
-        losses, stats, weights = new(*shape), new(*shape, 2), new(*shape)
-        reduced = None if reduction == "none" else new(1)
-        count = new(1) if reduction == "mean" else None
-        how = dict(ref_logprobs=ref_logprobs, clip=clip, kl=kl, ignore_index=ignore_index, reduction=reduction,
-                   stats=stats, weights=weights, reduced=reduced)
+        d = _desc(logits, tokens, ignore_index, reduction, 0, overwrite=True)
+        o = _options(logits, tokens, old_logprobs, advantages, ref_logprobs, clip, kl)
+        dev, n = logits.device, tokens.numel()
+        # One allocation for what the backward needs and for the losses (a small step
+        # is host time): stats (2 n), weights (n), losses (n), the count.
+        room = torch.empty(4 * n + 1, dtype=torch.float32, device=dev)
+        out = torch.empty(tokens.shape if reduction == "none" else (), dtype=torch.float32, device=dev)
+        at = room.data_ptr()
+        stats, weights, losses, count = at, at + 8 * n, at + 12 * n, at + 16 * n
+        reduced = out.data_ptr()
+        if reduction == "none":
+            losses, reduced = reduced, None
+        inputs = (logits.data_ptr(), tokens.data_ptr(), old_logprobs.data_ptr(), advantages.data_ptr(), _ptr(ref_logprobs),
+                  losses, None, stats, weights)
         ctx.delta = None
-        if (ctx.needs_input_grad[0] and reduction != "none" and logits.dim() == 3
+        if (ctx.needs_input_grad[0] and reduction != "none"
                 and logits.shape[-1] * logits.element_size() <= _FUSED_BYTES):
             ctx.delta = _gradient_like(logits)
-            policy_loss_fused_(losses, ctx.delta, logits, tokens, old_logprobs, advantages, count=count, **how)
+            _call(dev, _lib.lib().fc_policy_loss_fused, ctypes.byref(d), ctypes.byref(o), *inputs, reduced, count,
+                  ctx.delta.data_ptr(), None)
         else:
-            policy_loss_(losses, logits, tokens, old_logprobs, advantages, count=count, **how)
-        ctx.save_for_backward(logits, tokens, stats, weights, count)
-        ctx.ignore_index, ctx.reduction = ignore_index, reduction
-        return losses if reduction == "none" else reduced[0]
+            _call(dev, _lib.lib().fc_policy_loss_fwd, ctypes.byref(d), ctypes.byref(o), *inputs, reduced, count)
+        ctx.save_for_backward(logits, tokens, room)
+        ctx.desc, ctx.count = d, n
+        return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        logits, tokens, stats, weights, count = ctx.saved_tensors
         delta, ctx.delta = ctx.delta, None
-        if delta is None:
-            delta = _gradient_like(logits)
-            policy_loss_gradient_(delta, logits, tokens, dout, stats, weights, ignore_index=ctx.ignore_index,
-                                  reduction=ctx.reduction, count=count, accumulate=False)
+        logits, tokens, room = ctx.saved_tensors
+        dout = _as_floats(dout)
+        if delta is not None:
+            _call(delta.device, _lib.lib().fc_scale_gradient, delta.data_ptr(), ctx.desc.dtype, delta.numel(),
+                  dout.data_ptr())
         else:
-            _scale(delta, dout)
+            delta = _gradient_like(logits)
+            at, n = room.data_ptr(), ctx.count
+            _call(delta.device, _lib.lib().fc_policy_loss_bwd, ctypes.byref(ctx.desc), delta.data_ptr(),
+                  logits.data_ptr(), tokens.data_ptr(), at, at + 8 * n, dout.data_ptr(), at + 16 * n)
         return (delta,) + (None,) * 8
+
+
+def _as_floats(dy: torch.Tensor) -> torch.Tensor:
+    if dy.dtype != torch.float32:
+        dy = dy.float()
+    return dy if dy.is_contiguous() else dy.contiguous()
 
 
 def _scale(x: torch.Tensor, dy: torch.Tensor) -> None:
     """x *= dy (one value, on the device), in place; not touched where dy is 1."""
-    dy = dy.to(device=x.device, dtype=torch.float32).contiguous()
-    _call(x.device, _lib.lib().fc_scale_gradient, _ptr(x), _dtype_code(x.dtype), x.numel(), _ptr(dy))
+    _call(x.device, _lib.lib().fc_scale_gradient, _ptr(x), _dtype_code(x.dtype), x.numel(), _ptr(_as_floats(dy)))
 
 
 # ---- the preference loss --------------------------------------------------------
@@ -304,24 +318,35 @@ class PreferenceLossFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, ref_logprobs, beta=0.1, label_smoothing=0.0, ignore_index=-1, reduction="mean"):
         logits = logits.contiguous()
-        dev, shape = logits.device, tuple(tokens.shape)
-        new = lambda *s: torch.empty(s, dtype=torch.float32, device=dev)  # noqa: E731
-        losses, rewards, weights = new(shape[0] // 2), new(shape[0]), new(shape[0])
-        stats = new(*shape, 2)
-        reduced = None if reduction == "none" else new(1)
-        preference_loss_(losses, logits, tokens, ref_logprobs, beta=beta, label_smoothing=label_smoothing,
-                         ignore_index=ignore_index, reduction=reduction, rewards=rewards, stats=stats, weights=weights,
-                         reduced=reduced)
-        ctx.save_for_backward(logits, tokens, stats, weights)
-        ctx.ignore_index, ctx.reduction = ignore_index, reduction
+        d = _desc(logits, tokens, ignore_index, reduction, 0, overwrite=True)
+        dev, n, B = logits.device, tokens.numel(), tokens.shape[0]
+        if B % 2 != 0:
+            raise ValueError(f"answers come in pairs, got {B}")
+        _check_tensor("ref_logprobs", ref_logprobs, (B,), _F32, dev)
+        o = _lib.PreferenceOptions(float(beta), float(label_smoothing))
+        # One allocation: the workspace (n float64), stats (2 n), weights (B), losses (B/2).
+        room = torch.empty(4 * n + B + B // 2, dtype=torch.float32, device=dev)
+        out = torch.empty((B // 2,) if reduction == "none" else (), dtype=torch.float32, device=dev)
+        rewards = torch.empty((B,), dtype=torch.float32, device=dev)
+        at = room.data_ptr()
+        stats, weights = at + 8 * n, at + 16 * n
+        losses, reduced = weights + 4 * B, out.data_ptr()
+        if reduction == "none":
+            losses, reduced = reduced, None
+        _call(dev, _lib.lib().fc_preference_loss_fwd, ctypes.byref(d), ctypes.byref(o), logits.data_ptr(),
+              tokens.data_ptr(), ref_logprobs.data_ptr(), losses, rewards.data_ptr(), None, stats, weights, reduced, at,
+              8 * n)
+        ctx.save_for_backward(logits, tokens, room)
+        ctx.desc, ctx.count = d, n
         ctx.mark_non_differentiable(rewards)
-        return (losses if reduction == "none" else reduced[0]), rewards
+        return out, rewards
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout, _):
-        logits, tokens, stats, weights = ctx.saved_tensors
+        logits, tokens, room = ctx.saved_tensors
+        dout = _as_floats(dout)
         delta = _gradient_like(logits)
-        preference_loss_gradient_(delta, logits, tokens, dout, stats, weights, ignore_index=ctx.ignore_index,
-                                  reduction=ctx.reduction, accumulate=False)
+        at, n = room.data_ptr(), ctx.count
+        _call(delta.device, _lib.lib().fc_preference_loss_bwd, ctypes.byref(ctx.desc), delta.data_ptr(), logits.data_ptr(),
+              tokens.data_ptr(), at + 8 * n, at + 16 * n, dout.data_ptr())
         return (delta,) + (None,) * 6

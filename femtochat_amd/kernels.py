@@ -146,6 +146,11 @@ def _dtype_code(dtype: torch.dtype) -> int:
     return code
 
 
+@lru_cache(maxsize=1)
+def _head_dims() -> int:
+    return _lib.lib().fc_attn_supported_head_dims()
+
+
 def instruction(dtype: torch.dtype, device=None, D: Optional[int] = None):
     """Default implementation for a dtype and head dim, like the reference's
     ``instruction(F, dev, Val(D))`` (ext/FemtoChatCUDAExt.jl:214-223): the
@@ -155,8 +160,7 @@ def instruction(dtype: torch.dtype, device=None, D: Optional[int] = None):
     if dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise TypeError(f"no HIP attention for dtype {dtype}")
     if D is not None:
-        mask = _lib.lib().fc_attn_supported_head_dims()
-        if not (0 < D <= 128 and D % 16 == 0 and (mask >> (D // 16 - 1)) & 1):
+        if not (0 < D <= 128 and D % 16 == 0 and (_head_dims() >> (D // 16 - 1)) & 1):
             raise _lib.AttentionError(_lib.FC_ERR_UNSUPPORTED, f"head_dim {D} is not supported")
     return MFMAFast()
 
@@ -194,6 +198,8 @@ def attention_inputs(A, Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor):
     the fast path stores Q/K/V in bfloat16, the exact path in float32.  GPU
     tensors are converted by the library (``fc_convert``)."""
     if isinstance(A, MFMAFast):
+        if Q.dtype == K.dtype == V.dtype == torch.bfloat16:
+            return Q, K, V
         target = torch.bfloat16
     elif isinstance(A, MFMAExact):
         target = torch.float32
@@ -274,6 +280,16 @@ def _workspace_bytes(fields: bytes, which: int, with_positions: bool, with_prefi
     return n.value
 
 
+@lru_cache(maxsize=256)
+def _plan(D: int, H: int, Hkv: int, T: int, B: int, left: int, right: int, mode: int, in_dtype, out_dtype, dout_dtype,
+          grad_dtype, overwrite: bool, which: int, with_positions: bool, with_prefix: bool):
+    """(descriptor, its workspace bytes) of a call: sizes and options only, so the
+    same call again finds them here."""
+    d = _lib.AttnDesc(D, H, Hkv, T, B, left, right, mode, _dtype_code(in_dtype), _dtype_code(out_dtype),
+                      _dtype_code(dout_dtype), _dtype_code(grad_dtype), _lib.FC_FLAG_OVERWRITE if overwrite else 0)
+    return d, _workspace_bytes(bytes(d), which, with_positions, with_prefix)
+
+
 def _score(softcap, slopes, prefix, device, B: int, T: int, H: int) -> Optional[_lib.AttnScore]:
     """The scores' options as the library takes them, or None for plain scores."""
     if not softcap and slopes is None and prefix is None:
@@ -339,10 +355,10 @@ def attention_(A, O, l, m, Q, K, V, window: Tuple[int, int], *, positions=None,
 
 def _forward(A, O, l, m, Q, K, V, window, positions, workspace=None, score=None) -> None:
     """attention_ on checked tensors."""
-    device = Q.device
-    oc = _dtype_code(O.dtype)
-    d = _desc(A, Q, K, window, oc, oc, oc)
-    nbytes = _workspace_bytes(bytes(d), _lib.FC_PASS_FORWARD, positions is not None, score is not None and bool(score.prefix))
+    device, dt = Q.device, O.dtype
+    B, T, H, D = Q.shape
+    d, nbytes = _plan(D, H, K.shape[2], T, B, int(window[0]), int(window[1]), A.mode, Q.dtype, dt, dt, dt, False,
+                      _lib.FC_PASS_FORWARD, positions is not None, score is not None and score.prefix is not None)
     aligned = None
     if nbytes > 0:
         if workspace is None:
@@ -382,9 +398,10 @@ def delta_attention_(
 def _backward(A, dQ, dK, dV, dO, Q, K, V, O, l, m, window, positions, accumulate, workspace=None, score=None) -> None:
     """delta_attention_ on checked tensors."""
     device = Q.device
-    d = _desc(A, Q, K, window, _dtype_code(O.dtype), _dtype_code(dO.dtype), _dtype_code(dQ.dtype),
-              overwrite=not accumulate)
-    nbytes = _workspace_bytes(bytes(d), _lib.FC_PASS_BACKWARD, positions is not None, score is not None and bool(score.prefix))
+    B, T, H, D = Q.shape
+    d, nbytes = _plan(D, H, K.shape[2], T, B, int(window[0]), int(window[1]), A.mode, Q.dtype, O.dtype, dO.dtype, dQ.dtype,
+                      not accumulate, _lib.FC_PASS_BACKWARD, positions is not None,
+                      score is not None and score.prefix is not None)
     if workspace is None:  # freed to this stream's pool on return, so later work on the stream comes after the kernels
         workspace = torch.empty(max(nbytes, 256) + 256, dtype=torch.uint8, device=device)
     elif workspace.device != device or workspace.numel() * workspace.element_size() < nbytes + 256:
@@ -481,7 +498,8 @@ class AttentionFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dO):
         Q, K, V, O, l, m, positions, slopes, prefix = ctx.saved_tensors
-        dO = dO.contiguous()
+        if not dO.is_contiguous():
+            dO = dO.contiguous()
         if dO.dtype != O.dtype:
             dO = dO.to(O.dtype)
         # The fast kernels sum in float32 and round once on the way out, so
@@ -491,9 +509,13 @@ class AttentionFunction(torch.autograd.Function):
         gdtype = torch.float32
         if isinstance(ctx.A, MFMAFast) and all(dt == torch.bfloat16 for dt in ctx.dtypes):
             gdtype = torch.bfloat16
-        dQ, dK, dV = (torch.empty(x.shape, dtype=gdtype, device=Q.device) for x in (Q, K, V))
-        delta_attention_(ctx.A, dQ, dK, dV, dO, Q, K, V, O, l, m, ctx.window, positions=positions, accumulate=False,
-                         softcap=ctx.softcap, slopes=slopes, prefix=prefix)
+        device = Q.device
+        dQ, dK, dV = (torch.empty(x.shape, dtype=gdtype, device=device) for x in (Q, K, V))
+        # The forward checked what it saved (a toy layer's step is all host time: 149
+        # us with delta_attention_'s checks again, 135 without).
+        B, T, H, _ = Q.shape
+        _backward(ctx.A, dQ, dK, dV, dO, Q, K, V, O, l, m, ctx.window, positions, False, None,
+                  _score(ctx.softcap, slopes, prefix, device, B, T, H))
         out = [g.to(dt) if g.dtype != dt else g for g, dt in zip((dQ, dK, dV), ctx.dtypes)]
         return (out[0], out[1], out[2]) + (None,) * 6
 
