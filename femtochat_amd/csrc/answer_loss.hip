@@ -396,11 +396,11 @@ __device__ inline int target_from(int64_t y, int V, int64_t j) {
   return y >= 0 && y < V ? (int)max((int64_t)-1, min(y - j, (int64_t)INT_MAX)) : -1;
 }
 
-// The whole (token, vocabulary) array in address order, one 16-byte chunk per
-// thread, whatever V is; a chunk across two columns goes value by value, and so
-// do the values in front of the array's first 16-byte boundary and behind its
-// last one (chunk 0 starts at `head` values).  Columns outside the answers are
-// written as zeros (overwriting) or left alone, and not read.
+// The whole (token, vocabulary) array in one sweep, a 16-byte chunk per thread,
+// whatever V is; a chunk across two columns goes value by value, and so do the
+// values in front of the array's first 16-byte boundary and behind its last one
+// (chunk 0 starts at `head` values).  Columns outside the answers are written as
+// zeros (overwriting) or left alone, and not read.
 template <typename E, bool kOverwrite>
 __global__ __launch_bounds__(256) void answer_grad_kernel(AnswerArgs a, int head) {
   constexpr int kPer = Chunk<E>::kPer;
@@ -420,7 +420,9 @@ __global__ __launch_bounds__(256) void answer_grad_kernel(AnswerArgs a, int head
     grad_values<1>(&v, st.x, f / st.y, f, j == raw - a.index_base ? 0 : -1);
     out[e] = from_f32<E>(kOverwrite ? v : v + to_f32(out[e]));
   };
-  const int64_t b0 = head + (int64_t)blockIdx.x * (256 * kPer);  // the block's first value
+  // From the array's end: the forward's last reads are still in the Infinity Cache
+  // (8192 x 32768 bf16, forward and gradient: 278 -> 271 us; 2262 x 50257 fp32: 240 -> 232).
+  const int64_t b0 = head + (int64_t)(gridDim.x - 1 - blockIdx.x) * (256 * kPer);  // the block's first value
   const int64_t e = b0 + (int64_t)threadIdx.x * kPer;
   if (blockIdx.x == 0 && (int)threadIdx.x < head) value(threadIdx.x);
   // A block inside one column has its token and what belongs to it in scalar registers.

@@ -418,6 +418,26 @@ fc_status bwd_launch(const fc::Problem& p, const fc_attn_score* score, const voi
   a.scale = (float)((p.score & 2 ? 4.0 : 1.0) / std::sqrt((double)p.D));
   a.score = score_args(p, score);
   a.chunk_ub = chunk_ub;
+  const fc::DkdvSplit split = fc::dkdv_split(p);
+  a.split_heads = split.heads;
+  a.split_tiles = split.tiles;
+  // dK/dV, whole or in parts that are then joined.
+  auto run_dkdv = [&]() -> fc_status {
+    fc::BwdArgs k = a;
+    if (split.parts() > 1) {
+      k.dK = w + ws.part_k;
+      k.dV = w + ws.part_v;
+      k.grad_bf16 = k.accumulate = 0;
+    }
+    hipError_t e = fc::launch_bwd_dkdv(p, k, s);
+    if (e == hipSuccess && split.parts() > 1) {
+      const fc::JoinArgs j{static_cast<const float*>(k.dK), static_cast<const float*>(k.dV), dK, dV,
+                           (int64_t)p.B * p.T * p.Hkv * p.D, split.parts(), a.grad_bf16, a.accumulate};
+      e = fc::launch_join(j, s);
+    }
+    if (e != hipSuccess) return fail(FC_ERR_HIP, "dK/dV launch failed: %s", hipGetErrorString(e));
+    return FC_OK;
+  };
   a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)p.D));
   if (fused_stats) {
     a.stats = 1;
@@ -428,12 +448,11 @@ fc_status bwd_launch(const fc::Problem& p, const fc_attn_score* score, const voi
     a.lse2_out = pa.lse2;
     e = fc::launch_bwd_dq(p, a, s);
     if (e != hipSuccess) return fail(FC_ERR_HIP, "dQ launch failed: %s", hipGetErrorString(e));
-    e = fc::launch_bwd_dkdv(p, a, s);
-    if (e != hipSuccess) return fail(FC_ERR_HIP, "dK/dV launch failed: %s", hipGetErrorString(e));
-    return ok();
+    const fc_status st = run_dkdv();
+    return st != FC_OK ? st : ok();
   }
-  e = fc::launch_bwd_dkdv(p, a, s);
-  if (e != hipSuccess) return fail(FC_ERR_HIP, "dK/dV launch failed: %s", hipGetErrorString(e));
+  const fc_status st = run_dkdv();
+  if (st != FC_OK) return st;
   e = fc::launch_bwd_dq(p, a, s);
   if (e != hipSuccess) return fail(FC_ERR_HIP, "dQ launch failed: %s", hipGetErrorString(e));
   return ok();

@@ -289,7 +289,9 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
   // its Q and dO tiles to all its key tiles.
   const int rows = a.Hkv * a.B;
   const int n_kt = (T + C::kBK - 1) / C::kBK;
-  const int n_items = n_kt * rows;
+  // Scored kernels may split an item (DkdvSplit), its parts adjacent.
+  const int n_split = kScore ? a.split_heads * a.split_tiles : 1;
+  const int n_whole = n_kt * rows, n_items = n_whole * n_split;
   const int xcd = (int)blockIdx.x % kXcds;
   static_assert(C::kBK == kOrderRows && C::kBQ == kOrderKStep, "the work order counts this tiling");
   // (batch, KV head, key tile) of an item: in the work order (korder[k] =
@@ -298,6 +300,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
   // KV head) one after another on one XCD, as for the query tiles), else
   // key tiles outer and rows inner.
   auto decode = [&](int item, int& ib, int& ikvh, int& ikt) {
+    if (kScore) item /= n_split;
     if (a.korder != nullptr) {
       const int k = item / a.Hkv;
       ikvh = item - k * a.Hkv;
@@ -305,7 +308,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
       ib = e / n_kt;
       ikt = e - ib * n_kt;
     } else if (a.local_order) {
-      const int e = xcd_chunk_entry(item, n_items);
+      const int e = xcd_chunk_entry(item, n_whole);
       ikt = e % n_kt;
       const int bk = e / n_kt;
       ib = bk / a.Hkv;
@@ -343,6 +346,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
   const int32_t* cub = nullptr;     // with a prefix
   const int32_t* prefix = nullptr;
   int qt_begin = 0, n_qt_tiles = 0, t_first = 0, G = 0;
+  int h_first = 0, tile_part = 0, part = 0;  // of a split item
   bool vis_table = false;
   f32x16 dk[DB], dv[DB];  // the item's dK (unscaled) and dV
 
@@ -375,6 +379,12 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
     int h, t;
   };
   auto first_tile = [&](int t) -> int {
+    if constexpr (kScore != 0) {
+      if (a.split_tiles > 1) {  // (a power of two)
+        while (t < n_qt_tiles && (((qt_begin + t) & (a.split_tiles - 1)) != tile_part || !tile_visible(qt_begin + t))) ++t;
+        return t;
+      }
+    }
     while (t < n_qt_tiles && !tile_visible(qt_begin + t)) ++t;
     return t;
   };
@@ -386,6 +396,11 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
   auto setup = [&](int it) {
     int kt;
     decode(it, b, kvh, kt);
+    if constexpr (kScore != 0) {
+      part = it % n_split;
+      h_first = (part % a.split_heads) * (a.group / a.split_heads);
+      tile_part = part / a.split_heads;
+    }
     k0 = kt * C::kBK;
     k1 = min(k0 + C::kBK, T) - 1;
     kw0 = k0 + 32 * wave;
@@ -410,7 +425,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
     }
     __syncthreads();
     t_first = first_tile(0);
-    G = t_first < n_qt_tiles ? a.group : 0;  // no visible tile: no step
+    G = t_first < n_qt_tiles ? (kScore ? a.group / a.split_heads : a.group) : 0;  // no visible tile: no step
   };
   FragOffsets<DkdvFastCfg<D>::kW> fo;
   fo.init(lane);
@@ -448,7 +463,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
     nx_o = buffer_words(a.dO, 0);
   };
   auto issue = [&](Step st, char* buf) {
-    const int h = kvh * a.group + st.h;
+    const int h = kvh * a.group + (kScore ? h_first : 0) + st.h;
     const int q0 = (qt_begin + st.t) * BQ;
     const int64_t hoff = (((int64_t)b * T * a.H + h) * D) * 2;
     nx_at = lds_addr(buf);
@@ -521,7 +536,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
       sc.cap_in = a.score.cap_in;
       sc.cap_out = a.score.cap_out;
     }
-    if constexpr ((kScore & kBias) != 0) sc.slope2 = a.score.slopes[kvh * a.group + st.h] * kLog2e;
+    if constexpr ((kScore & kBias) != 0) sc.slope2 = a.score.slopes[kvh * a.group + h_first + st.h] * kLog2e;
     DkdvStep<D, kScore>::run(dma_part, buf, buf + C::kTileBytes, s_lse[slot], s_delta[slot], s_lb[slot], s_lbc[slot][0], kf, vf, dk, dv,
                              fo, q0, key, kw0, kw1, g, T, a.right, c2, sc);
   };
@@ -577,7 +592,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
   const int next = s_next;
   // This item's stores need its row and keys; the next item's K, V, first
   // tile and row statistics load meanwhile.
-  const int eb = b, ekvh = kvh, ekw0 = kw0;
+  const int eb = b, ekvh = kvh, ekw0 = kw0, epart = part;
   if (next < n_items) {
     load_kv(next);
     setup(next);
@@ -590,7 +605,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
   // the hardware drops them, so no store needs a branch or 64-bit address
   // arithmetic.  (A slice of 2^31 bytes or more takes the plain loop below.)
   const int64_t row_elems = (int64_t)a.Hkv * D;  // elements between consecutive keys
-  const int64_t slice0 = (int64_t)eb * T * row_elems + (int64_t)ekvh * D;
+  const int64_t part0 = kScore ? (int64_t)epart * a.B * T * row_elems : 0;  // parts lie one after another
+  const int64_t slice0 = part0 + (int64_t)eb * T * row_elems + (int64_t)ekvh * D;
   const int esz = a.grad_bf16 ? 2 : 4;
   const int64_t slice_bytes = ((int64_t)(T - 1) * row_elems + D) * esz;
   if (slice_bytes < ((int64_t)1 << 31)) {
@@ -726,7 +742,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
       for (int r = 0; r < 16; ++r) {
         const int kk = ekw0 + acc_row(r, g);
         if (kk < T) {
-          const int64_t off = ((int64_t)eb * T + kk) * a.Hkv * D + (int64_t)ekvh * D + d;
+          const int64_t off = part0 + ((int64_t)eb * T + kk) * a.Hkv * D + (int64_t)ekvh * D + d;
           float vk = dk[db][r] * a.scale, vv = dv[db][r];
           if (a.grad_bf16) {
             bf16* pk = static_cast<bf16*>(a.dK) + off;
@@ -760,7 +776,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
 template <int D, int kScore = 0>
 static hipError_t launch_dkdv_fast_t(const Problem& p, const BwdArgs& a, hipStream_t s) {
   const int n_kt = (p.T + DkdvFastCfg<D>::kBK - 1) / DkdvFastCfg<D>::kBK;
-  const int n_items = n_kt * p.Hkv * p.B;
+  const int n_items = n_kt * p.Hkv * p.B * (kScore ? a.split_heads * a.split_tiles : 1);
   int cus = 0;
   const hipError_t ec = device_cus(&cus);
   if (ec != hipSuccess) return ec;

@@ -23,16 +23,27 @@ struct DqFastCfg {
   static constexpr int kStageBytes = 2 * kTileBytes;  // K, V
 };
 
-template <int D, int kScore>
-__global__ __launch_bounds__(kThreads, 2) void attn_bwd_dq_fast_kernel(BwdArgs a) {
+// kParts 2 (scored kernels, grids that leave at most one workgroup on a CU): eight
+// waves, of which waves 4 .. 7 take the odd key tiles of the same 128 queries through
+// stage buffers of their own, as in the forward; the two sums meet in LDS.
+template <int D, int kScore, int kParts>
+__global__ __launch_bounds__(kThreads * kParts, 2) void attn_bwd_dq_fast_kernel(BwdArgs a) {
   using C = DqFastCfg<D>;
   using M = Mma<bf16>;
   constexpr int BN = C::kBN, KC = C::kKC, DB = C::kDB, NKB = BN / 32;
-  __shared__ __attribute__((aligned(1024))) char bufA[C::kStageBytes];
-  __shared__ __attribute__((aligned(1024))) char bufB[C::kStageBytes];
+  constexpr int kSumBytes = kThreads * 16 * DB * 4;  // the second part's dQ (kParts 2)
+  __shared__ __attribute__((aligned(1024))) char
+      bufA[kParts == 2 && kSumBytes > 2 * C::kStageBytes ? kSumBytes : kParts * C::kStageBytes];
+  __shared__ __attribute__((aligned(1024))) char bufB[kParts * C::kStageBytes];
   __shared__ int s_bounds[2][kWaves];
 
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int tid = threadIdx.x, lane = tid & 63;
+  int wave = tid >> 6, part = 0;
+  if (kParts == 2) {  // waves 4 .. 7 are the second part
+    wave = __builtin_amdgcn_readfirstlane(wave);
+    part = wave / kWaves;
+    wave %= kWaves;
+  }
   const int g = lane >> 5, l32 = lane & 31;
   const int T = a.T;
   const int n_qt = (T + C::kBM - 1) / C::kBM;
@@ -99,6 +110,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_bwd_dq_fast_kernel(BwdArgs a
   }
   FragOffsets<C::kW> fo;
   fo.init(lane);
+  if (kParts > 1) fo.shift(part * C::kStageBytes);
   DmaPlan<D, BN> plan;
   plan.init(wave, lane, kpitch);
 
@@ -130,7 +142,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_bwd_dq_fast_kernel(BwdArgs a
     }
   };
   auto issue = [&](int it, char* buf) {
-    nx_at = lds_addr(buf);
+    nx_at = lds_addr(buf) + part * C::kStageBytes;
     if (it < ntiles) {
       const int64_t row0 = (int64_t)(kt0 + it * BN) * kpitch;
       nx_k = tile_words(Kb, krec, row0);
@@ -142,7 +154,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_bwd_dq_fast_kernel(BwdArgs a
   };
   // The first tile's loads go out before anything waits for the loads above.
   if (ntiles > 0) {
-    issue(0, bufA);
+    issue(part, bufA);
 #pragma unroll
     for (int k = 0; k < NPH; ++k) dma_part(k);
   }
@@ -184,7 +196,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_bwd_dq_fast_kernel(BwdArgs a
       e = __builtin_fmaf(-slope2, __builtin_fabsf((float)(q - k0 - 4 * g) - (float)acc_row(r, 0)), e);
     return __builtin_amdgcn_exp2f(e);
   };
-  if constexpr (kScore != 0) {
+  if constexpr (kScore != 0 && kParts == 1) {
     // Delta from a bf16 O carries O's rounding into every dS of its row, as large an
     // error as the rounding of dS itself.  Over many rows it stays under 4e-3 of dQ
     // and dK; over few it does not (up to 9e-3 at 32 rows, 5e-3 at 129, against 3e-3
@@ -311,14 +323,41 @@ __global__ __launch_bounds__(kThreads, 2) void attn_bwd_dq_fast_kernel(BwdArgs a
   };
 
   dma_wait_barrier();
-  for (int it = 0; it < ntiles; it += 2) {
-    issue(it + 1, bufB);
-    compute(it, bufA);
+  // (A part without a tile in a step sees nothing of the tile past the last.)
+  for (int it = 0; it < ntiles; it += 2 * kParts) {
+    issue(it + part + kParts, bufB);
+    compute(it + part, bufA);
     dma_wait_barrier();
-    if (it + 1 >= ntiles) break;
-    issue(it + 2, bufA);
-    compute(it + 1, bufB);
+    if (it + kParts >= ntiles) break;
+    issue(it + part + 2 * kParts, bufA);
+    compute(it + part + kParts, bufB);
     dma_wait_barrier();
+  }
+
+  if constexpr (kParts == 2) {
+    f32x4* const so = reinterpret_cast<f32x4*>(bufA) + (64 * wave + lane);
+    if (part == 1) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          so[(4 * db + j) * kThreads] = f32x4{dq[db][4 * j], dq[db][4 * j + 1], dq[db][4 * j + 2], dq[db][4 * j + 3]};
+      }
+    }
+    __syncthreads();
+    if (part == 0) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f32x4 v = so[(4 * db + j) * kThreads];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) dq[db][4 * j + t] += v[t];
+        }
+      }
+    }
+    __syncthreads();  // dQ leaves through the same memory
+    if (part == 1) return;
   }
 
   // Delta and lse2 for the dK/dV kernel, stored after the tile loop so that
@@ -409,7 +448,15 @@ static hipError_t launch_dq_fast_t(const Problem& p, const BwdArgs& a, hipStream
   const int n_qt = (p.T + DqFastCfg<D>::kBM - 1) / DqFastCfg<D>::kBM;
   const dim3 grid(n_qt * p.H * p.B), block(kThreads);
   const ProfileMark mk = profile_begin(s);
-  hipLaunchKernelGGL((attn_bwd_dq_fast_kernel<D, kScore>), grid, block, 0, s, a);
+  if constexpr (kScore != 0) {
+    if (score_parts(p, a.cus, grid.x)) {
+      hipLaunchKernelGGL((attn_bwd_dq_fast_kernel<D, kScore, 2>), grid, dim3(2 * kThreads), 0, s, a);
+      const hipError_t e = hipGetLastError();
+      profile_end(mk, "attn_bwd_dq_score_bf16", s);
+      return e;
+    }
+  }
+  hipLaunchKernelGGL((attn_bwd_dq_fast_kernel<D, kScore, 1>), grid, block, 0, s, a);
   const hipError_t e = hipGetLastError();
   profile_end(mk, kScore ? "attn_bwd_dq_score_bf16" : "attn_bwd_dq_bf16", s);
   return e;

@@ -202,10 +202,12 @@ __global__ __launch_bounds__(kThreads * kParts, 2 / kParts) void attn_fwd_fast_k
     m_true[qb] = -INFINITY;  // row maximum of c2 * S (same on both half-waves)
     l_half[qb] = 0.0f;       // sum of P over this half-wave's keys, against m_ref
   }
-  // Scores reach the softmax in base 2 times c2: raw products, or with a cap or a
-  // bias the finished scores (c2 = 1).
-  constexpr bool kFinished = (kScore & (kCap | kBias)) != 0;
-  const float c2 = kFinished ? 1.0f : a.scale_log2;
+  // A base-2 score is c2 s + c0: of raw products, of a capped score's -r, or with a
+  // bias of the finished score (1 and 0).
+  constexpr bool kFinished = (kScore & (kCap | kBias)) != 0, kCapAlone = (kScore & (kCap | kBias)) == kCap;
+  const float c2 = kCapAlone ? 2.0f * a.score.cap_out : kFinished ? 1.0f : a.scale_log2;
+  const float c0 = kCapAlone ? a.score.cap_out : 0.0f;
+  auto base2 = [&](float s) __attribute__((always_inline)) { return kCapAlone ? __builtin_fmaf(s, c2, c0) : s * c2; };
   const float slope2 = (kScore & kBias) ? a.score.slopes[h] * kLog2e : 0.0f;
   auto finish = [&](f32x16& sv, int qb, int k0) __attribute__((always_inline)) {
     if constexpr (kFinished)
@@ -256,13 +258,13 @@ __global__ __launch_bounds__(kThreads * kParts, 2 / kParts) void attn_fwd_fast_k
   // Softmax pieces for one 32-key block of one query block: the row maximum
   // (combined over the half-waves) and P with its unrounded sum.
   auto block_max = [&](f32x16& sv, int qb) -> float {
-    const float mx = max16(sv) * c2;
+    const float mx = base2(max16(sv));
     const float mq = nan_max(mx, other_half(mx));
     m_true[qb] = nan_max(m_true[qb], mq);
     return mq;
   };
   auto exp_block = [&](f32x16& sv, int qb, bf16x8* pfo) {
-    const float neg_m = m_ref[qb] == -INFINITY ? 0.0f : -m_ref[qb];
+    const float neg_m = m_ref[qb] == -INFINITY ? 0.0f : kCapAlone ? c0 - m_ref[qb] : -m_ref[qb];
     float psum = 0.0f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -454,7 +456,7 @@ __global__ __launch_bounds__(kThreads * kParts, 2 / kParts) void attn_fwd_fast_k
         return sv;
       };
       float mx = -INFINITY;
-      for (int k0 = klo; k0 <= khi; k0 += 32) mx = nan_max(mx, max16(scores(k0)) * c2);
+      for (int k0 = klo; k0 <= khi; k0 += 32) mx = nan_max(mx, base2(max16(scores(k0))));
       const float mq = nan_max(mx, other_half(mx));
       m_true[qb] = mq;
       m_ref[qb] = mq;
@@ -569,7 +571,7 @@ static hipError_t launch_fwd_fast_t(const Problem& p, const FwdArgs& a, hipStrea
   // 50 to 800 on average take 0.83 to 1.02 times as long, order kernels included.
   constexpr int kPartTiles = 10;
   const int64_t span = std::min((int64_t)p.T, (int64_t)a.left + a.right + FwdFastCfg<D>::kBM);
-  const bool parts = (int64_t)grid.x <= a.cus && span > kPartTiles * FwdFastCfg<D>::kBN;
+  const bool parts = kScore ? score_parts(p, a.cus, grid.x) : (int64_t)grid.x <= a.cus && span > kPartTiles * FwdFastCfg<D>::kBN;
   if (parts) hipLaunchKernelGGL((attn_fwd_fast_kernel<D, 2, kScore>), grid, dim3(2 * kThreads), 0, s, a);
   else hipLaunchKernelGGL((attn_fwd_fast_kernel<D, 1, kScore>), grid, dim3(kThreads), 0, s, a);
   const hipError_t e = hipGetLastError();

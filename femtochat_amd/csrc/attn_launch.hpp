@@ -103,7 +103,21 @@ struct BwdArgs {
   float scale_log2;  // log2(e)/sqrt(D)
   ScoreArgs score;
   const int32_t* chunk_ub;  // with a prefix: per 32 queries the (min, max) last visible key, or null
+  int split_heads, split_tiles;  // DkdvSplit; split items write float32 parts to dK and dV, part after part
 };
+
+// The sums of a split dK/dV's parts, into (or added to) the gradients.
+struct JoinArgs {
+  const float* part_k;
+  const float* part_v;
+  void* dK;
+  void* dV;
+  int64_t n;  // values of each gradient, a multiple of 16
+  int parts;
+  int grad_bf16, accumulate;
+};
+hipError_t launch_join(const JoinArgs& a, hipStream_t s);
+
 
 // Attention prologue (rope_norm.hip): rotary embedding then RMS norm x 1.2
 // of one tensor (Q or K) with NH heads; vectors = B*T*NH head vectors.

@@ -47,8 +47,16 @@ constexpr int kOrderMaxItems = 4096;    // largest B * ceil(T / 128) the order k
 inline bool order_fits(int T, int B) { return (int64_t)B * ((T + kOrderRows - 1) / kOrderRows) <= kOrderMaxItems; }
 
 // Fast mode with positions takes the tiles in the work order when the order
-// kernel's tables fit.
-inline bool ordered(const Problem& p) { return p.bf16 && p.positions && order_fits(p.T, p.B); }
+// kernel's tables fit.  Scored kernels do so only for query grids of more than
+// kOrderGrid workgroups: below, most tiles run at once, and the order costs more than
+// it gives (us of a step with and without it, order and bounds kernels included:
+// 2 x 1900 tokens, H8 D128, 240 workgroups 170 and 151; 5 x 866, H16 D128, 560 158 and
+// 146; 4 x 4096, H8/4 D128, 1024 354 and 400; 13 x 959, H16/4 D64, 1664 314 and 345).
+constexpr int kOrderGrid = 640;
+inline bool ordered(const Problem& p) {
+  if (!p.bf16 || !p.positions || !order_fits(p.T, p.B)) return false;
+  return p.score == 0 || (int64_t)((p.T + kOrderRows - 1) / kOrderRows) * p.H * p.B > kOrderGrid;
+}
 
 // A sliding window at most half the sequence (no positions): the tiles of a
 // row do about the same work and consecutive tiles share most of their keys,
@@ -152,6 +160,60 @@ inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 inline size_t chunk_bounds_bytes(const Problem& p) { return (size_t)p.B * ((p.T + 31) / 32) * 2 * sizeof(int32_t); }
 inline size_t order_bytes(const Problem& p) { return (size_t)p.B * ((p.T + kOrderRows - 1) / kOrderRows) * sizeof(int32_t); }
 
+// The dK/dV kernel with scores beyond the plain ones: a (128-key tile, batch, KV
+// head) item is one workgroup's, which takes the group's heads and their query
+// tiles one after another, so few items leave CUs idle behind long chains of steps.
+// Then an item is split: over the heads of the group (`heads` divides it), and over
+// the query tiles, every `tiles`-th for each part; the parts' sums meet in float32 in
+// the workspace, added in order.  The split is the one with the least estimated time:
+// the longer of the longest chain and a CU's share of all steps (with a third of a
+// chain more, which the last ones stand alone for), an item's own cost, and joining
+// the parts.  us of dK/dV and the join, whole -> split as chosen: 1 x 6792 tokens,
+// H8/2 D96 775 -> 242 (4 heads x 2 tiles); 1 x 2048, H8/1 D128 518 -> 62 (8 x 2);
+// 1 x 4096, H16/8 D128 287 -> 219 (2 x 2); 1 x 415, H16/4 D80 73 -> 31 (4 x 2);
+// 1 x 8192, H2/2 D64 210 -> 110 (1 x 4); 2 x 512, H8/8 D128 stays whole (28, split 34).
+struct DkdvSplit {
+  int heads, tiles;
+  int parts() const { return heads * tiles; }
+};
+inline DkdvSplit dkdv_split(const Problem& p) {
+  DkdvSplit best{1, 1};
+  if (p.score == 0) return best;
+  constexpr double kCus = 256, kItem = 2, kJoin = 7, kJoinBytesPerUs = 8e6;
+  const double step = 4 * (0.55 + 0.45 * p.D / 128);
+  const int n = (p.T + kOrderRows - 1) / kOrderRows;  // key tiles, and query tiles
+  // Query tiles that see a key tile, at most; a window's split has no more parts than
+  // the whole row's, whose workspace then serves every window.
+  const int reach = (int)std::min<int64_t>(n, std::max<int64_t>(0, (int64_t)p.left + p.right) / kOrderRows + 2);
+  int most = INT32_MAX;
+  if (p.left != p.T || p.right != 0) {
+    Problem whole = p;
+    whole.left = p.T;
+    whole.right = 0;
+    most = dkdv_split(whole).parts();
+  }
+  // (Documents hide most tiles from each other, by how many only the device knows:
+  // they are taken as a window of a thousand tokens.)
+  const int tiles_seen = p.positions ? std::min(reach, 8) : reach;
+  const double items = (double)n * p.Hkv * p.B, mean = std::min(0.5 * (n + 1), p.positions ? 0.5 * tiles_seen : reach);
+  const double part_bytes = 2.0 * p.B * p.T * p.Hkv * p.D * sizeof(float) * 2;  // written and read
+  double least = 0;
+  for (int h = 1; h <= p.group; ++h) {
+    if (p.group % h != 0) continue;
+    for (int t = 1; t <= 16 && (t == 1 || 2 * t <= tiles_seen); t *= 2) {
+      if (h * t > most) continue;
+      const double chain = (double)(p.group / h) * ((tiles_seen + t - 1) / t), share = items * p.group * mean / kCus;
+      double us = step * std::max(chain, share + 0.35 * chain) + kItem * std::max(1.0, items * h * t / kCus);
+      if (h * t > 1) us += kJoin + h * t * part_bytes / kJoinBytesPerUs;
+      if ((h == 1 && t == 1) || us < least || (us == least && t < best.tiles)) {
+        least = us;
+        best = DkdvSplit{h, t};
+      }
+    }
+  }
+  return best;
+}
+
 // Workspace layout of the forward pass (byte offsets, 256-aligned): PadWorkspace
 // (required where it is not empty), and when the work order applies the
 // per-32-query key bounds and the query tiles' order (optional: without a
@@ -214,10 +276,10 @@ inline FwdWorkspace fwd_workspace(const Problem& p) {
 // PadWorkspace, then Delta and the base-2
 // log-sum-exp per query, per-32-query key bounds with
 // positions (or a prefix, which also has upper ones), a bf16 copy of an fp32 dO in fast mode, in fast mode the
-// dK/dV kernel's work counters, and the dQ and dK/dV orders when the work
-// order applies.
+// dK/dV kernel's work counters, the dQ and dK/dV orders when the work
+// order applies, a prefix's upper bounds, and the parts of a split dK/dV.
 struct BwdWorkspace {
-  size_t delta, lse2, chunk_lb, dO16, queue, qorder, korder, chunk_ub, total;
+  size_t delta, lse2, chunk_lb, dO16, queue, qorder, korder, chunk_ub, part_k, part_v, total;
 };
 
 inline BwdWorkspace bwd_workspace(const Problem& p) {
@@ -240,6 +302,12 @@ inline BwdWorkspace bwd_workspace(const Problem& p) {
   if (ordered(p)) off = align256(off + order_bytes(p));
   w.chunk_ub = off;
   if (p.prefix) off = align256(off + chunk_bounds_bytes(p));
+  const int parts = dkdv_split(p).parts();
+  const size_t part = (size_t)p.B * p.T * p.Hkv * p.D * sizeof(float);
+  w.part_k = off;
+  if (parts > 1) off = align256(off + parts * part);
+  w.part_v = off;
+  if (parts > 1) off = align256(off + parts * part);
   w.total = off;
   return w;
 }

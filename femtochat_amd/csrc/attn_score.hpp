@@ -25,6 +25,19 @@ __device__ inline float cap_part(float x, float cap_in) {
   return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * cap_in) + 1.0f);
 }
 
+// Whether the forward and dQ take a query tile's key tiles in two parts (eight
+// waves): grids that leave at most one workgroup on a CU and have tiles that see more
+// than ten key tiles, and those of up to 1.75 a CU where that is more than twenty
+// (the longest tiles then no longer run alone at the end).  us of the forward and dQ,
+// one part -> two: 1 x 4096 tokens, H8 D128 (256 workgroups) 101, 113 -> 83, 98;
+// 1 x 6792, H8 D96 (432) 191, 226 -> 146, 177; 3 x 1500, H8 D80 (288) 48, 52 -> 39, 46;
+// 4 x 1024, H12 D64 (384, sixteen key tiles) 26, 30 -> 29, 36; 4 x 2048, H8 D128 (512)
+// 61, 76 -> 71, 91.
+inline bool score_parts(const Problem& p, int cus, unsigned workgroups) {
+  const int64_t span = p.prefix ? p.T : std::min((int64_t)p.T, (int64_t)p.left + p.right + kOrderRows);
+  return (workgroups <= (unsigned)cus && span > 10 * kOrderTile) || (4 * (int64_t)workgroups <= 7 * (int64_t)cus && span > 20 * kOrderTile);
+}
+
 // The last visible key of query q: the window's, or the end of the prefix of the
 // query's document (of the row without positions), -1 past the sequence.
 __device__ inline int prefix_ub(int q, int T, int right, int pos_q, bool documents, int prefix_q) {
@@ -39,14 +52,20 @@ __device__ inline int score_ub(int q, int T, int right, const int32_t* pos, cons
   return prefix_ub(q, T, right, pos != nullptr ? pos[q] : 0, pos != nullptr, prefix[per_token ? q : 0]);
 }
 
-// Base-2 scores of a 32-key block of S^T (lane = query): key k0 + acc_row(r, g),
-// d0 = q - k0 - 4 g.
+// Scores of a 32-key block of S^T (lane = query): key k0 + acc_row(r, g), d0 = q -
+// k0 - 4 g.  Finished base-2 scores, except with a cap alone: then -r, which the
+// softmax scales by 2 cap_out and moves by cap_out in the operation that subtracts
+// its reference (one multiply-add per score less).
 template <int kScore>
 __device__ inline void score_block(f32x16& s, int d0, float c2, float cap_in, float cap_out, float slope2) {
   const float d = (float)d0;
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
     float v = s[r];
+    if ((kScore & (kCap | kBias)) == kCap) {
+      s[r] = -cap_part(v, cap_in);
+      continue;
+    }
     if (kScore & kCap) v = __builtin_fmaf(-2.0f * cap_out, cap_part(v, cap_in), cap_out);
     else v *= c2;
     if (kScore & kBias) v = __builtin_fmaf(-slope2, __builtin_fabsf(d - (float)(8 * (r >> 2) + (r & 3))), v);

@@ -270,11 +270,12 @@ def _desc(A, Q, K, window, out_dtype, dout_dtype, grad_dtype, overwrite=False) -
 
 
 @lru_cache(maxsize=256)
-def _workspace_bytes(fields: bytes, which: int, with_positions: bool, with_prefix: bool = False) -> int:
+def _workspace_bytes(fields: bytes, which: int, with_positions: bool, scores: int = 0) -> int:
     """fc_attn_workspace_bytes of a descriptor (its bytes: sizes and options only)."""
     n = ctypes.c_size_t(0)
     d = _lib.AttnDesc.from_buffer_copy(fields)
-    score = _lib.AttnScore(0.0, 0, None, 4 if with_prefix else None)  # only whether there is a prefix counts
+    # only which of a cap (1), slopes (2) and a prefix (4) there are counts
+    score = _lib.AttnScore(float(scores & 1), 0, 4 if scores & 2 else None, 4 if scores & 4 else None)
     _lib.check(_lib.lib().fc_attn_score_workspace_bytes(ctypes.byref(d), ctypes.byref(score), which,
                                                         int(with_positions), ctypes.byref(n)))
     return n.value
@@ -282,12 +283,12 @@ def _workspace_bytes(fields: bytes, which: int, with_positions: bool, with_prefi
 
 @lru_cache(maxsize=256)
 def _plan(D: int, H: int, Hkv: int, T: int, B: int, left: int, right: int, mode: int, in_dtype, out_dtype, dout_dtype,
-          grad_dtype, overwrite: bool, which: int, with_positions: bool, with_prefix: bool):
+          grad_dtype, overwrite: bool, which: int, with_positions: bool, scores: int):
     """(descriptor, its workspace bytes) of a call: sizes and options only, so the
     same call again finds them here."""
     d = _lib.AttnDesc(D, H, Hkv, T, B, left, right, mode, _dtype_code(in_dtype), _dtype_code(out_dtype),
                       _dtype_code(dout_dtype), _dtype_code(grad_dtype), _lib.FC_FLAG_OVERWRITE if overwrite else 0)
-    return d, _workspace_bytes(bytes(d), which, with_positions, with_prefix)
+    return d, _workspace_bytes(bytes(d), which, with_positions, scores)
 
 
 def _score(softcap, slopes, prefix, device, B: int, T: int, H: int) -> Optional[_lib.AttnScore]:
@@ -300,6 +301,10 @@ def _score(softcap, slopes, prefix, device, B: int, T: int, H: int) -> Optional[
     if prefix is not None:
         _check_tensor("prefix", prefix, (B, T) if per_token else (B,), (torch.int32,), device)
     return _lib.AttnScore(float(softcap), int(per_token), _ptr(slopes), _ptr(prefix))
+
+
+def _kinds(softcap, slopes, prefix) -> int:
+    return (1 if softcap else 0) + (2 if slopes is not None else 0) + (4 if prefix is not None else 0)
 
 
 def _call(device: torch.device, entry, *args) -> None:
@@ -358,7 +363,7 @@ def _forward(A, O, l, m, Q, K, V, window, positions, workspace=None, score=None)
     device, dt = Q.device, O.dtype
     B, T, H, D = Q.shape
     d, nbytes = _plan(D, H, K.shape[2], T, B, int(window[0]), int(window[1]), A.mode, Q.dtype, dt, dt, dt, False,
-                      _lib.FC_PASS_FORWARD, positions is not None, score is not None and score.prefix is not None)
+                      _lib.FC_PASS_FORWARD, positions is not None, 0 if score is None else _kinds(score.softcap, score.slopes, score.prefix))
     aligned = None
     if nbytes > 0:
         if workspace is None:
@@ -401,7 +406,7 @@ def _backward(A, dQ, dK, dV, dO, Q, K, V, O, l, m, window, positions, accumulate
     B, T, H, D = Q.shape
     d, nbytes = _plan(D, H, K.shape[2], T, B, int(window[0]), int(window[1]), A.mode, Q.dtype, O.dtype, dO.dtype, dQ.dtype,
                       not accumulate, _lib.FC_PASS_BACKWARD, positions is not None,
-                      score is not None and score.prefix is not None)
+                      0 if score is None else _kinds(score.softcap, score.slopes, score.prefix))
     if workspace is None:  # freed to this stream's pool on return, so later work on the stream comes after the kernels
         workspace = torch.empty(max(nbytes, 256) + 256, dtype=torch.uint8, device=device)
     elif workspace.device != device or workspace.numel() * workspace.element_size() < nbytes + 256:
@@ -411,21 +416,22 @@ def _backward(A, dQ, dK, dV, dO, Q, K, V, O, l, m, window, positions, accumulate
           dV.data_ptr(), (workspace.data_ptr() + 255) & ~255, nbytes)
 
 
-def forward_workspace_bytes(A, Q, K, *, positions=None, prefix=None) -> int:
+def forward_workspace_bytes(A, Q, K, *, positions=None, softcap: float = 0.0, slopes=None, prefix=None) -> int:
     """Bytes of the caller-owned workspace ``attention_(…, workspace=)``
     accepts (the library's requirement plus 256 bytes of alignment slack; 0
     when the problem needs none)."""
     d = _desc(A, Q, K, (-1, 0), _dtype_code(Q.dtype), _dtype_code(Q.dtype), _dtype_code(Q.dtype))
-    n = _workspace_bytes(bytes(d), _lib.FC_PASS_FORWARD, positions is not None, prefix is not None)
+    n = _workspace_bytes(bytes(d), _lib.FC_PASS_FORWARD, positions is not None, _kinds(softcap, slopes, prefix))
     return n + 256 if n > 0 else 0
 
 
-def backward_workspace_bytes(A, Q, K, *, positions=None, dout_dtype=None, prefix=None) -> int:
+def backward_workspace_bytes(A, Q, K, *, positions=None, dout_dtype=None, softcap: float = 0.0, slopes=None,
+                             prefix=None) -> int:
     """Bytes of the caller-owned workspace ``delta_attention_(…, workspace=)``
     accepts (the library's requirement plus 256 bytes of alignment slack)."""
     dd = _dtype_code(dout_dtype or Q.dtype)
     d = _desc(A, Q, K, (-1, 0), dd, dd, dd)
-    return _workspace_bytes(bytes(d), _lib.FC_PASS_BACKWARD, positions is not None, prefix is not None) + 256
+    return _workspace_bytes(bytes(d), _lib.FC_PASS_BACKWARD, positions is not None, _kinds(softcap, slopes, prefix)) + 256
 
 
 def _reject_unknown(options: dict) -> None:

@@ -95,18 +95,23 @@ def test_the_calls_checks_still_hold():
     assert lib.fc_attn_score_bwd(ctypes.byref(d), score, *[AT] * 7, None, *[AT] * 3, None, 0, None) == L.FC_ERR_WORKSPACE
 
 
-@pytest.mark.parametrize("T,B,positions", [(1, 1, 0), (333, 3, 0), (333, 3, 1), (40000, 2, 1)])
-def test_a_prefix_adds_its_tables_to_the_workspace(T, B, positions):
-    """Per 32 queries two upper bounds, and the lower ones where positions do not bring them."""
+@pytest.mark.parametrize("T,B,positions,parts", [(1, 1, 0, 1), (333, 3, 0, 2), (333, 3, 1, 2), (2048, 1, 0, 8), (40000, 2, 1, 1)])
+def test_scores_need_their_tables_and_parts_in_the_workspace(T, B, positions, parts):
+    """A prefix: per 32 queries two upper bounds, and the lower ones where positions do not
+    bring them.  Any score: the float32 parts of a split dK/dV where there are few key tiles."""
     lib = L.lib()
     d = L.AttnDesc(64, 4, 2, T, B, -1, 0, L.FC_MODE_FAST, *[L.FC_BF16] * 4, 0)
     got = []
-    for score in (L.AttnScore(0.0, 0, None, None), L.AttnScore(0.0, 0, None, AT)):
+    for score in (None, L.AttnScore(1.0, 0, None, None), L.AttnScore(0.0, 0, None, AT)):
         n = ctypes.c_size_t(0)
         assert lib.fc_attn_score_workspace_bytes(ctypes.byref(d), score, L.FC_PASS_BACKWARD, positions, ctypes.byref(n)) == 0
         got.append(n.value)
-    table = (B * -(-T // 32) * 8 + 255) // 256 * 256
-    assert got[1] - got[0] == table * (1 if positions else 2)
+    room = lambda n: (n + 255) // 256 * 256  # noqa: E731
+    split = 2 * room(parts * B * T * 2 * 64 * 4) if parts > 1 else 0
+    n128 = B * -(-T // 128)
+    order = 2 * room(n128 * 4) if positions and n128 * 4 <= 640 else 0  # small query grids take no work order
+    assert got[1] - got[0] == split - order
+    assert got[2] - got[1] == room(B * -(-T // 32) * 8) * (1 if positions else 2)
 
 
 def test_python_refusals():

@@ -125,6 +125,30 @@ def test_many_workgroups(gpu, kind, D):
     _check(_run(gpu, host, (-1, 0), None, how), host, (-1, 0), None, how)
 
 
+@pytest.mark.parametrize("B,T,H,Hkv,D", [(1, 1300, 8, 1, 128), (1, 1300, 8, 2, 48), (2, 700, 4, 1, 64), (1, 2100, 2, 2, 32), (3, 140, 10, 2, 96)])
+@pytest.mark.parametrize("kind", ["cap", "all", "prefix"])
+@pytest.mark.parametrize("documents", [False, True])
+def test_few_key_tiles(gpu, B, T, H, Hkv, D, kind, documents):
+    """Problems whose dK/dV items are split over heads and query tiles and joined, with
+    gradients overwritten and added to, in both types."""
+    host = _inputs(24, B, T, H, Hkv, D)
+    pos = W.document_positions(T, B, 25, mean=400) if documents else None
+    how = _options(kind, 26, B, T, H, per_token=documents)
+    if documents and how["prefix"] is not None:
+        how["prefix"] = (how["prefix"] % 300).astype(np.int32)
+    for window in ((-1, 0), (200, 0)):
+        got = _run(gpu, host, window, pos, how)
+        _check(got, host, window, pos, how)
+    for x, y in zip(got, _run(gpu, host, window, pos, how)):
+        assert torch.equal(x, y)
+    for grad in (torch.bfloat16, torch.float32):
+        added = _run(gpu, host, window, pos, how, grad=grad, init=-0.5)
+        for x, y in zip(got[3:], added[3:]):
+            # got is rounded to bf16 once, added once in its own type
+            room = 2.0 ** -8 * x.float().abs() + (2.0 ** -8 * y.float().abs() if grad == torch.bfloat16 else 1e-6)
+            assert ((y.float() - x.float() + 0.5).abs() <= room + 1e-6).all()
+
+
 def test_prefixes_of_any_value(gpu):
     """Below 0, past T, and of each token its own: nothing monotone."""
     B, T, H, Hkv, D = 3, 290, 2, 2, 64
@@ -251,7 +275,7 @@ def test_the_same_bits_again_and_captured(gpu):
     d = _dev(gpu, how)
     O, l, m = torch.empty_like(Q), torch.empty(B, H, T, device=gpu), torch.empty(B, H, T, device=gpu)
     grads = [torch.empty_like(x) for x in (Q, K, V)]
-    n = F.backward_workspace_bytes(A, Q, K, prefix=d["prefix"])
+    n = F.backward_workspace_bytes(A, Q, K, **d)
     ws = torch.full((n,), 255, dtype=torch.uint8, device=gpu)
 
     def step():
