@@ -198,12 +198,12 @@ __global__ __launch_bounds__(kThreads * kParts, 2) void attn_bwd_dq_fast_kernel(
   };
   if constexpr (kScore != 0 && kParts == 1) {
     // Delta from a bf16 O carries O's rounding into every dS of its row, as large an
-    // error as the rounding of dS itself.  Over many rows it stays under 4e-3 of dQ
-    // and dK; over few it does not (up to 9e-3 at 32 rows, 5e-3 at 129, against 3e-3
-    // without it), so short sequences, whose kernels are bound by latency, sum
-    // Delta = P dP over their keys first.
-    constexpr int kShort = 256;
-    if (a.stats && T <= kShort) {
+    // error as the rounding of dS itself.  Where rows see many keys and there are many
+    // of them, it stays under 4e-3 of dQ and dK (2-norm); over few rows it does not (up
+    // to 9e-3 at 32 rows, 5e-3 at 129), nor with few keys each (6e-3 with two, 3.5e-3
+    // with 64), against 3e-3 without it.  So short sequences, whose kernels are bound
+    // by latency, and narrow windows sum Delta = P dP over their keys first.
+    if (a.stats && exact_delta(T, a.left, a.right)) {
       float sum = 0.0f;
       dma_wait_barrier();
       for (int it = 0; it < ntiles; ++it) {

@@ -25,6 +25,9 @@ __device__ inline float cap_part(float x, float cap_in) {
   return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * cap_in) + 1.0f);
 }
 
+// Whether the dQ kernel sums Delta over the keys (attn_bwd_dq_fast.hpp).
+__host__ __device__ inline bool exact_delta(int T, int left, int right) { return T <= 256 || left + imax(right, 0) <= 64; }
+
 // Whether the forward and dQ take a query tile's key tiles in two parts (eight
 // waves): grids that leave at most one workgroup on a CU and have tiles that see more
 // than ten key tiles, and those of up to 1.75 a CU where that is more than twenty
@@ -34,6 +37,7 @@ __device__ inline float cap_part(float x, float cap_in) {
 // 4 x 1024, H12 D64 (384, sixteen key tiles) 26, 30 -> 29, 36; 4 x 2048, H8 D128 (512)
 // 61, 76 -> 71, 91.
 inline bool score_parts(const Problem& p, int cus, unsigned workgroups) {
+  if (exact_delta(p.T, p.left, p.right)) return false;
   const int64_t span = p.prefix ? p.T : std::min((int64_t)p.T, (int64_t)p.left + p.right + kOrderRows);
   return (workgroups <= (unsigned)cus && span > 10 * kOrderTile) || (4 * (int64_t)workgroups <= 7 * (int64_t)cus && span > 20 * kOrderTile);
 }
