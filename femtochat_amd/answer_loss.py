@@ -200,7 +200,8 @@ class PolicyLossFunction(torch.autograd.Function):
         room = torch.empty(4 * n + 1, dtype=torch.float32, device=dev)
         out = torch.empty(tokens.shape if reduction == "none" else (), dtype=torch.float32, device=dev)
         at = room.data_ptr()
-        stats, weights, losses, count = at, at + 8 * n, at + 12 * n, at + 16 * n
+        stats, weights, losses = at, at + 8 * n, at + 12 * n
+        count = at + 16 * n if reduction == "mean" else None
         reduced = out.data_ptr()
         if reduction == "none":
             losses, reduced = reduced, None
@@ -215,7 +216,7 @@ class PolicyLossFunction(torch.autograd.Function):
         else:
             _call(dev, _lib.lib().fc_policy_loss_fwd, ctypes.byref(d), ctypes.byref(o), *inputs, reduced, count)
         ctx.save_for_backward(logits, tokens, room)
-        ctx.desc, ctx.count = d, n
+        ctx.desc, ctx.n, ctx.count = d, n, count
         return out
 
     @staticmethod
@@ -228,9 +229,9 @@ class PolicyLossFunction(torch.autograd.Function):
                   dout.data_ptr())
         else:
             delta = _gradient_like(logits)
-            at, n = room.data_ptr(), ctx.count
+            at, n = room.data_ptr(), ctx.n
             _call(delta.device, _lib.lib().fc_policy_loss_bwd, ctypes.byref(ctx.desc), delta.data_ptr(),
-                  logits.data_ptr(), tokens.data_ptr(), at, at + 8 * n, dout.data_ptr(), at + 16 * n)
+                  logits.data_ptr(), tokens.data_ptr(), at, at + 8 * n, dout.data_ptr(), ctx.count)
         return (delta,) + (None,) * 8
 
 
@@ -337,7 +338,7 @@ class PreferenceLossFunction(torch.autograd.Function):
               tokens.data_ptr(), ref_logprobs.data_ptr(), losses, rewards.data_ptr(), None, stats, weights, reduced, at,
               8 * n)
         ctx.save_for_backward(logits, tokens, room)
-        ctx.desc, ctx.count = d, n
+        ctx.desc, ctx.n = d, n
         ctx.mark_non_differentiable(rewards)
         return out, rewards
 
@@ -346,7 +347,7 @@ class PreferenceLossFunction(torch.autograd.Function):
         logits, tokens, room = ctx.saved_tensors
         dout = _as_floats(dout)
         delta = _gradient_like(logits)
-        at, n = room.data_ptr(), ctx.count
+        at, n = room.data_ptr(), ctx.n
         _call(delta.device, _lib.lib().fc_preference_loss_bwd, ctypes.byref(ctx.desc), delta.data_ptr(), logits.data_ptr(),
               tokens.data_ptr(), at + 8 * n, at + 16 * n, dout.data_ptr())
         return (delta,) + (None,) * 6

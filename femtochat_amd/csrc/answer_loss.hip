@@ -280,43 +280,51 @@ __global__ __launch_bounds__(256) void answer_fwd_wave_kernel(AnswerArgs a) {
   if (lane == 0) finish_token(a, token, col, r);
 }
 
-// A pair of answers: the sums of their log-probabilities, in a fixed order, then
-// the loss, the two rewards and the two weights.
+// Pairs of answers: the sums of their log-probabilities, in a fixed order, then the
+// loss, the two rewards and the two weights.  A workgroup per pair, or one for all of
+// a few, which then reduces the losses too (a launch less).
 __global__ __launch_bounds__(1024) void preference_pair_kernel(AnswerArgs a) {
   __shared__ double slots[16];
-  const int pair = blockIdx.x, T = a.per_answer;
-  double sums[2];
-  for (int side = 0; side < 2; ++side) {
-    const double* lp = a.lp + ((int64_t)pair + (int64_t)side * a.pairs) * T;
-    double s = 0.0;
-    for (int t = threadIdx.x; t < T; t += 1024) s += lp[t];
-    s = wave_sum(s);
-    if ((threadIdx.x & 63) == 0) slots[threadIdx.x / 64] = s;
-    __syncthreads();
-    s = 0.0;
-    for (int w = 0; w < 16; ++w) s += slots[w];
-    sums[side] = s;
-    __syncthreads();
+  const int T = a.per_answer;
+  double total = 0.0;
+  for (int pair = blockIdx.x; pair < a.pairs; pair += gridDim.x) {
+    double sums[2];
+    for (int side = 0; side < 2; ++side) {
+      const double* lp = a.lp + ((int64_t)pair + (int64_t)side * a.pairs) * T;
+      double s = 0.0;
+      for (int t = threadIdx.x; t < T; t += 1024) s += lp[t];
+      s = wave_sum(s);
+      if ((threadIdx.x & 63) == 0) slots[threadIdx.x / 64] = s;
+      __syncthreads();
+      s = 0.0;
+      for (int w = 0; w < 16; ++w) s += slots[w];
+      sums[side] = s;
+      __syncthreads();
+    }
+    if (threadIdx.x != 0) continue;
+    const double rw = a.beta * (sums[0] - (double)a.ref[pair]), rl = a.beta * (sums[1] - (double)a.ref[pair + a.pairs]);
+    const double h = rw - rl, e = a.smoothing;
+    // softplus(z) = log(1 + exp(z)) and the logistic function without overflow
+    const double q = log1p(exp(-fabs(h)));
+    const double up = fmax(h, 0.0) + q, down = fmax(-h, 0.0) + q;  // softplus(h), softplus(-h)
+    const double sig = 1.0 / (1.0 + exp(-h));                      // exp(inf) gives 0
+    const double sig_neg = 1.0 / (1.0 + exp(h));
+    const double dh = a.beta * (e * sig - (1.0 - e) * sig_neg);
+    // fmax ignores a NaN: h says it
+    const float loss = h != h ? __builtin_nanf("") : (float)((1.0 - e) * down + (e == 0.0 ? 0.0 : e * up));
+    a.losses[pair] = loss;
+    total += (double)loss;
+    if (a.rewards != nullptr) {
+      a.rewards[pair] = (float)rw;
+      a.rewards[pair + a.pairs] = (float)rl;
+    }
+    if (a.weights != nullptr) {
+      a.weights[pair] = (float)dh;
+      a.weights[pair + a.pairs] = (float)-dh;
+    }
   }
-  if (threadIdx.x != 0) return;
-  const double rw = a.beta * (sums[0] - (double)a.ref[pair]), rl = a.beta * (sums[1] - (double)a.ref[pair + a.pairs]);
-  const double h = rw - rl, e = a.smoothing;
-  // softplus(z) = log(1 + exp(z)) and the logistic function without overflow
-  const double q = log1p(exp(-fabs(h)));
-  const double up = fmax(h, 0.0) + q, down = fmax(-h, 0.0) + q;  // softplus(h), softplus(-h)
-  const double sig = 1.0 / (1.0 + exp(-h));                      // exp(inf) gives 0
-  const double sig_neg = 1.0 / (1.0 + exp(h));
-  const double dh = a.beta * (e * sig - (1.0 - e) * sig_neg);
-  // fmax ignores a NaN: h says it
-  a.losses[pair] = h != h ? __builtin_nanf("") : (float)((1.0 - e) * down + (e == 0.0 ? 0.0 : e * up));
-  if (a.rewards != nullptr) {
-    a.rewards[pair] = (float)rw;
-    a.rewards[pair + a.pairs] = (float)rl;
-  }
-  if (a.weights != nullptr) {
-    a.weights[pair] = (float)dh;
-    a.weights[pair + a.pairs] = (float)-dh;
-  }
+  if (gridDim.x == 1 && threadIdx.x == 0 && a.reduced != nullptr)
+    a.reduced[0] = (float)(a.reduction == 2 ? total / a.pairs : total);
 }
 
 // reduced = the sum of the losses or their mean (over the tokens of answers, or
@@ -638,7 +646,7 @@ hipError_t launch_reduce(const AnswerArgs& a, hipStream_t s) {
   return e;
 }
 
-// N V < 2^40 values (answer_args): fewer than 2^30 workgroups.
+// N V <= 2^33 values (answer_args): at most 2^23 + 1 workgroups.
 template <typename E>
 hipError_t launch_grad(const AnswerArgs& a, bool overwrite, hipStream_t s) {
   const int64_t n = a.N * a.V;
@@ -705,9 +713,9 @@ fc_status answer_args(const char* who, const fc_answer_desc* d, const void* logi
   if (d == nullptr) return bad(who, "descriptor is null");
   if (d->V <= 0 || d->answers <= 0 || d->T <= 0) return bad(who, "V, answers and T must be positive");
   const int64_t N = (int64_t)d->answers * d->T;
-  if (N > INT32_MAX) return bad(who, "at most 2^31-1 tokens per call", FC_ERR_UNSUPPORTED);
-  // A block of the gradient covers 1024 values or more.
-  if (N >= (((int64_t)1 << 40) / d->V)) return bad(who, "2^40 logits or more", FC_ERR_UNSUPPORTED);
+  // A launch holds fewer than 2^32 threads: 256 per token, or per 1024 values of the gradient.
+  if (N >= (int64_t)1 << 22) return bad(who, "at most 2^22 - 1 tokens per call", FC_ERR_UNSUPPORTED);
+  if (N * d->V > (int64_t)1 << 33) return bad(who, "more than 2^33 logits", FC_ERR_UNSUPPORTED);
   if (d->index_base != 0 && d->index_base != 1) return bad(who, "index_base must be 0 or 1");
   if (d->index_type != FC_INDEX_I32 && d->index_type != FC_INDEX_I64) return bad(who, "index_type must be FC_INDEX_I32 or FC_INDEX_I64");
   if (d->reduction < FC_REDUCE_NONE || d->reduction > FC_REDUCE_MEAN) return bad(who, "unknown reduction");
@@ -895,14 +903,14 @@ fc_status fc_preference_loss_fwd(const fc_answer_desc* desc, const fc_preference
   a.losses = losses;
   a.rewards = rewards;
   a.weights = weights;
+  a.reduced = reduced;
+  // One workgroup up to eight pairs, each at most four values per thread and side.
+  const bool few = a.pairs <= 8 && desc->T <= 4096;
   const fc::ProfileMark mk = fc::profile_begin(s);
-  hipLaunchKernelGGL(fc::preference_pair_kernel, dim3((unsigned)a.pairs), dim3(1024), 0, s, a);
+  hipLaunchKernelGGL(fc::preference_pair_kernel, dim3(few ? 1u : (unsigned)a.pairs), dim3(1024), 0, s, a);
   e = hipGetLastError();
   fc::profile_end(mk, "preference_pair", s);
-  if (e == hipSuccess && reduced != nullptr) {
-    a.reduced = reduced;
-    e = fc::launch_reduce(a, s);
-  }
+  if (e == hipSuccess && reduced != nullptr && !few && a.pairs > 1) e = fc::launch_reduce(a, s);
   return done(who, e);
 }
 

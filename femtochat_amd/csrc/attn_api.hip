@@ -168,8 +168,10 @@ namespace {
 // The scores' part of the problem; a score without a cap, slopes and a prefix is a plain one.
 fc_status score_problem(const fc_attn_score* score, fc::Problem* p) {
   if (score == nullptr) return FC_OK;
-  if (!(score->softcap >= 0.0f && score->softcap < INFINITY))
-    return fail(FC_ERR_INVALID_ARGUMENT, "softcap must be finite and at least 0 (0: none)");
+  // Beyond 4096 a capped score would be off by more than 2^-9, beside its rounding as
+  // the bf16 operand of the next product; below 2^-10 every score is at its cap.
+  if (!(score->softcap == 0.0f || (score->softcap >= 0x1p-10f && score->softcap <= 4096.0f)))
+    return fail(FC_ERR_INVALID_ARGUMENT, "softcap must be 0 (none) or from 2^-10 to 4096");
   if (((reinterpret_cast<uintptr_t>(score->slopes) | reinterpret_cast<uintptr_t>(score->prefix)) & 3) != 0)
     return fail(FC_ERR_INVALID_ARGUMENT, "slopes and prefix must be 4-byte aligned");
   p->prefix = score->prefix != nullptr;

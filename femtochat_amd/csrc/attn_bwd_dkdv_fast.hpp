@@ -48,6 +48,10 @@ struct DkdvStep {
   static constexpr int NPH = NQB + 2;            // phases of the body
   static constexpr int NTR = 2 * DB;             // transposed fragments per operand and block
   static constexpr int NPRE = NTR < 2 ? NTR : 2;  // of them requested one phase early
+  // Where MFMA results land in ordinary registers (D <= 64), the scored kernels' dP
+  // starts at -Delta, which the published array then holds, instead of zero: one
+  // subtraction per score less.
+  static constexpr bool kDeltaFirst = kScore != 0 && D <= 64;
   static constexpr int kNoUpper = -2;            // in place of chunk upper bounds: the window's own
   static constexpr int kMoreValu = ((kScore & kCap) ? 4 : 0) + ((kScore & kBias) ? 2 : 0);  // per score
   static constexpr int kSchedVALU = 0x2, kSchedMFMA = 0x8, kSchedDSRead = 0x100;
@@ -154,7 +158,7 @@ struct DkdvStep {
         float p = __builtin_amdgcn_exp2f(e);
         if (kSides & kUpper) p = (kScore ? key <= UB[j][t] : x >= -(8 * j + t)) ? p : 0.0f;
         if (kSides & kLower) p = key >= LB[j][t] ? p : 0.0f;
-        float ds = p * (dp[r] - Dl[j][t]);
+        float ds = p * (kDeltaFirst ? dp[r] : dp[r] - Dl[j][t]);
         if constexpr ((kScore & kCap) != 0) ds *= __builtin_fmaf(-u, u, u);
         if (kSides) ds *= Z[j][t];
         s[r] = p;
@@ -204,6 +208,10 @@ struct DkdvStep {
         if (kSides) bounds(lbs, b1, g, LB[b1], Z[b1], UB[b1]);
         s[b1] = zero16();
         dp[b1] = zero16();
+        if constexpr (kDeltaFirst) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[b1][r] = Dl[b1][r >> 2][r & 3];
+        }
 #pragma unroll
         for (int c = 0; c < KC; ++c) {
           s[b1] = M::mma(qa[c], kf[c], s[b1]);
@@ -497,7 +505,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
     if (tid < BQ) {
       const bool in = st_q < T;
       s_lse[slot][tid] = in ? ((kScore & kCap) ? st_lse - a.score.cap_out : st_lse) : INFINITY;
-      s_delta[slot][tid] = in ? st_delta : 0.0f;
+      s_delta[slot][tid] = !in ? 0.0f : DkdvStep<D, kScore>::kDeltaFirst ? -st_delta : st_delta;
       int lb = T;
       if (in) lb = max(0, max(st_q - a.left, pos != nullptr ? st_q - st_pos : 0));
       s_lb[slot][tid] = lb;

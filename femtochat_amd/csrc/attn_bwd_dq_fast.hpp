@@ -239,6 +239,15 @@ __global__ __launch_bounds__(kThreads * kParts, 2) void attn_bwd_dq_fast_kernel(
     }
   }
 
+  // Scored kernels with registers to spare start dP at -Delta instead of zero: one
+  // subtraction per score less (as in dK/dV).
+  constexpr bool kDeltaFirst = kScore != 0 && D <= 64;
+  f32x16 minus_delta;
+  if constexpr (kDeltaFirst) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) minus_delta[r] = -dlt;
+  }
+
   // Tile body: a pipeline over the tile's two 32-key blocks, phase i holding
   // S^T, dP^T of block i, the softmax of block i-1 and dQ^T += K^T dS^T of
   // block i-2, with MFMAs, LDS reads and VALU interleaved.
@@ -257,7 +266,7 @@ __global__ __launch_bounds__(kThreads * kParts, 2) void attn_bwd_dq_fast_kernel(
       __builtin_amdgcn_sched_barrier(0);
       if (b1 < NKB) {
         s[b1] = zero16();
-        dp[b1] = zero16();
+        dp[b1] = kDeltaFirst ? minus_delta : zero16();
 #pragma unroll
         for (int c = 0; c < KC; ++c) {
           const bf16x8 ka = as_bf16x8(lds_load16(Ks + 32 * b1 * 2 * C::kW, fo.nat(c)));
@@ -286,7 +295,7 @@ __global__ __launch_bounds__(kThreads * kParts, 2) void attn_bwd_dq_fast_kernel(
         for (int r = 0; r < 16; ++r) {
           float u = 0.0f;
           const float p = prob(s[bs][r], kt + 32 * bs, r, u);
-          float ds = p * (dp[bs][r] - dlt);
+          float ds = p * (kDeltaFirst ? dp[bs][r] : dp[bs][r] - dlt);
           if constexpr ((kScore & kCap) != 0) ds *= __builtin_fmaf(-u, u, u);
           if (need_mask) {
             const int kk = kt + 32 * bs + acc_row(r, g);

@@ -179,7 +179,7 @@ struct DkdvSplit {
 inline DkdvSplit dkdv_split(const Problem& p) {
   DkdvSplit best{1, 1};
   if (p.score == 0) return best;
-  constexpr double kCus = 256, kItem = 2, kJoin = 7, kJoinBytesPerUs = 8e6;
+  constexpr double kCus = 256, kItem = 2, kJoin = 7, kJoinBytesPerUs = 4e6;
   const double step = 4 * (0.55 + 0.45 * p.D / 128);
   const int n = (p.T + kOrderRows - 1) / kOrderRows;  // key tiles, and query tiles
   // Query tiles that see a key tile, at most; a window's split has no more parts than

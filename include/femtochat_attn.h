@@ -134,7 +134,8 @@ fc_status fc_attn_bwd_noalloc(const fc_attn_desc* desc, const void* dO,
  * The forward and the backward with scores beyond q.k/sqrt(D).  No reference
  * counterpart.
  *   softcap c > 0 : S <- c tanh(S / c)                       (S = q.k/sqrt(D))
- *   slopes  (H)   : S <- S - slopes[h] |q - k|, after the cap; any finite values
+ *   slopes  (H)   : S <- S - slopes[h] |q - k|, after the cap; any finite values,
+ *                   fastest where scores fall with the distance (at least 0)
  *   prefix        : a query also sees the keys up to the end of its prefix,
  *                   k <= max(q + right, start + n - 1), where start is the
  *                   query's document's first token (q - positions[q], 0 without
@@ -143,13 +144,14 @@ fc_status fc_attn_bwd_noalloc(const fc_attn_desc* desc, const void* dO,
  *                   prefix[b] (one value per row), taken as 0 below 0 and T
  *                   above T.
  * Everything else is as above: rows with no visible key, the statistics (of the
- * finished scores), the document mask, GQA, the workspace, the gradients (dS = 0
- * for a query with a single visible key).  slopes and prefix have no gradient.
+ * finished scores), the document mask, GQA, the gradients (dS = 0 for a query
+ * with a single visible key).  The workspace is that of
+ * fc_attn_score_workspace_bytes; the one for a causal window serves any window.  slopes and prefix have no gradient.
  * Fast mode only (FC_ERR_UNSUPPORTED otherwise); a score with softcap 0 and null
  * slopes and prefix is the plain one in either mode.  A capped score is off by at
  * most c 2^-21. */
 typedef struct {
-  float softcap;             /* 0: none */
+  float softcap;             /* 0: none, else 2^-10 to 4096 */
   int32_t prefix_per_token;  /* prefix is (T,B), one value per token; else (B) */
   const float* slopes;       /* device, H values, or NULL */
   const int32_t* prefix;     /* device, or NULL */

@@ -143,7 +143,7 @@ fc_status fc_embedding_bwd_sorted(const fc_embed_desc* desc, float* dweights, co
  * A token's log-probability is lp = x[y] - max - log(sum(exp(x - max))) over its
  * column; a token outside the vocabulary that is not ignore_index makes its loss,
  * and its column of the gradient, NaN.  logits and dlogits must lie alike against
- * 16 bytes. */
+ * 16 bytes.  At most 2^22 - 1 tokens and 2^33 logits per call. */
 typedef struct {
   int32_t V;            /* vocabulary size */
   int32_t answers, T;   /* answers and tokens of each */

@@ -100,6 +100,8 @@ def test_bad_descriptors(kw, entry):
 def test_too_many():
     assert _policy(_desc(answers=1 << 16, T=1 << 15)) == L.FC_ERR_UNSUPPORTED
     assert _policy(_desc(V=1 << 30, answers=1 << 10, T=1)) == L.FC_ERR_UNSUPPORTED
+    assert _policy(_desc(V=2, answers=1 << 11, T=1 << 11)) == L.FC_ERR_UNSUPPORTED
+    assert _policy(_desc(V=1 << 13, answers=(1 << 20) + 1, T=1)) == L.FC_ERR_UNSUPPORTED
     assert _policy(_desc(V=1 << 17), entry="fused", dlogits=AT + (1 << 30)) == L.FC_ERR_UNSUPPORTED  # 512 KB columns
 
 

@@ -70,6 +70,8 @@ def _desc(mode=L.FC_MODE_FAST):
     (L.AttnScore(-1.0, 0, None, None), L.FC_ERR_INVALID_ARGUMENT),
     (L.AttnScore(float("nan"), 0, None, None), L.FC_ERR_INVALID_ARGUMENT),
     (L.AttnScore(float("inf"), 0, None, None), L.FC_ERR_INVALID_ARGUMENT),
+    (L.AttnScore(4097.0, 0, None, None), L.FC_ERR_INVALID_ARGUMENT),
+    (L.AttnScore(0.0009, 0, None, None), L.FC_ERR_INVALID_ARGUMENT),
     (L.AttnScore(0.0, 0, AT + 2, None), L.FC_ERR_INVALID_ARGUMENT),
     (L.AttnScore(0.0, 0, None, AT + 1), L.FC_ERR_INVALID_ARGUMENT),
 ])
@@ -112,6 +114,21 @@ def test_scores_need_their_tables_and_parts_in_the_workspace(T, B, positions, pa
     order = 2 * room(n128 * 4) if positions and n128 * 4 <= 640 else 0  # small query grids take no work order
     assert got[1] - got[0] == split - order
     assert got[2] - got[1] == room(B * -(-T // 32) * 8) * (1 if positions else 2)
+
+
+def test_the_causal_workspace_serves_every_window():
+    lib = L.lib()
+    n = ctypes.c_size_t(0)
+    for T in (1, 130, 500, 1500, 4000, 9000):
+        for H, Hkv in ((1, 1), (8, 1), (16, 4), (6, 3)):
+            for positions in (0, 1):
+                sizes = []
+                for window in ((-1, 0), (0, 0), (100, 0), (700, 50), (T, T), (5, -9)):
+                    d = L.AttnDesc(64, H, Hkv, T, 2, *window, L.FC_MODE_FAST, *[L.FC_BF16] * 4, 0)
+                    assert lib.fc_attn_score_workspace_bytes(ctypes.byref(d), L.AttnScore(1.0, 0, None, None), L.FC_PASS_BACKWARD,
+                                                             positions, ctypes.byref(n)) == 0
+                    sizes.append(n.value)
+                assert max(sizes) == sizes[0], (T, H, Hkv, positions, sizes)
 
 
 def test_python_refusals():

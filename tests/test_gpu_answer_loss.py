@@ -200,7 +200,7 @@ def test_columns_longer_than_the_fused_kernel_holds(gpu, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("P,T,V", [(1, 1, 2), (2, 33, 1000), (3, 17, 4099), (1, 1500, 64), (5, 4, 50257)])
+@pytest.mark.parametrize("P,T,V", [(1, 1, 2), (2, 33, 1000), (3, 17, 4099), (1, 1500, 64), (5, 4, 50257), (9, 6, 200), (40, 3, 33), (1, 5000, 16)])
 @pytest.mark.parametrize("smoothing", [0.0, 0.1])
 def test_preference(gpu, P, T, V, dtype, smoothing):
     x, xd = _logits(gpu, 20 + V, 2 * P, T, V, dtype)
@@ -291,6 +291,39 @@ def test_scale_gradient(gpu, n, off, dtype):
         y = x.clone()
         _scale(y[off:], torch.tensor(f, device=gpu))
         assert torch.equal(y[off:], (x[off:].float() * torch.tensor(f, device=gpu)).to(x.dtype)) and torch.equal(y[:off], x[:off])
+
+
+@pytest.mark.parametrize("V", [32768, 50257])
+def test_beyond_32_bit_offsets(gpu, V):
+    """More than 2^31 bf16 logits (and 2^32 bytes): the last answers give the bits that
+    they give by themselves, in both losses."""
+    T, B = 1024, 2 * (-(-(1 << 31) // (2 * 1024 * V)) + 1)
+    g = torch.Generator(device=gpu).manual_seed(50)
+    x = torch.empty(B, T, V, dtype=torch.bfloat16, device=gpu)
+    for i in range(B):
+        x[i].normal_(0.0, 2.0, generator=g)
+    tok = torch.randint(0, V, (B, T), device=gpu, generator=g)
+    tok[:, ::3] = -1
+    old, adv = torch.full((B, T), -9.0, device=gpu), torch.randn(B, device=gpu, generator=g)
+
+    def policy(x, tok, old, adv):
+        losses, delta = torch.empty(tok.shape, device=gpu), torch.empty_like(x)
+        F.policy_loss_fused_(losses, delta, x, tok, old, adv, reduction="sum")
+        return losses, delta
+
+    losses, delta = policy(x, tok, old, adv)
+    l2, d2 = policy(x[-2:].contiguous(), tok[-2:].contiguous(), old[-2:].contiguous(), adv[-2:].contiguous())
+    assert torch.equal(losses[-2:], l2) and torch.equal(delta[-2:], d2)
+    del delta, d2
+    ref = torch.full((B,), -6000.0, device=gpu)
+    pair = torch.tensor([B // 2 - 1, B - 1], device=gpu)
+    xs = x[pair].requires_grad_()
+    small, _ = F.PreferenceLossFunction.apply(xs, tok[pair], ref[:2], 0.1, 0.0, -1, "sum")
+    want = torch.autograd.grad(small, xs)[0]
+    x.requires_grad_()
+    loss, rewards = F.PreferenceLossFunction.apply(x, tok, ref, 0.1, 0.0, -1, "sum")
+    got = torch.autograd.grad(loss, x)[0]
+    assert torch.equal(got[pair], want)
 
 
 def test_gpu_refusals(gpu):

@@ -181,7 +181,7 @@ def test_steep_and_rising_biases(gpu, slopes, prefix, D):
     _check(_run(gpu, host, (-1, 0), None, how), host, (-1, 0), None, how)
 
 
-@pytest.mark.parametrize("softcap,scale", [(0.5, 3.0), (30.0, 300.0), (50.0, 8.0), (1000.0, 2.0)])
+@pytest.mark.parametrize("softcap,scale", [(2.0 ** -10, 3.0), (0.5, 3.0), (30.0, 300.0), (50.0, 8.0), (4096.0, 2.0)])
 @pytest.mark.parametrize("D", [32, 128])
 def test_saturated_and_loose_caps(gpu, softcap, scale, D):
     B, T, H, Hkv = 1, 333, 2, 1
