@@ -280,51 +280,80 @@ __global__ __launch_bounds__(256) void answer_fwd_wave_kernel(AnswerArgs a) {
   if (lane == 0) finish_token(a, token, col, r);
 }
 
-// Pairs of answers: the sums of their log-probabilities, in a fixed order, then the
-// loss, the two rewards and the two weights.  A workgroup per pair, or one for all of
-// a few, which then reduces the losses too (a launch less).
+// A pair from the sums of its answers' log-probabilities: the loss (returned too),
+// the two rewards and the two weights.
+__device__ inline float finish_pair(const AnswerArgs& a, int pair, double chosen, double rejected) {
+  const double rw = a.beta * (chosen - (double)a.ref[pair]), rl = a.beta * (rejected - (double)a.ref[pair + a.pairs]);
+  const double h = rw - rl, e = a.smoothing;
+  // softplus(z) = log(1 + exp(z)) and the logistic function without overflow
+  const double q = log1p(exp(-fabs(h)));
+  const double up = fmax(h, 0.0) + q, down = fmax(-h, 0.0) + q;  // softplus(h), softplus(-h)
+  const double sig = 1.0 / (1.0 + exp(-h));                      // exp(inf) gives 0
+  const double sig_neg = 1.0 / (1.0 + exp(h));
+  const double dh = a.beta * (e * sig - (1.0 - e) * sig_neg);
+  // fmax ignores a NaN: h says it
+  const float loss = h != h ? __builtin_nanf("") : (float)((1.0 - e) * down + (e == 0.0 ? 0.0 : e * up));
+  a.losses[pair] = loss;
+  if (a.rewards != nullptr) {
+    a.rewards[pair] = (float)rw;
+    a.rewards[pair + a.pairs] = (float)rl;
+  }
+  if (a.weights != nullptr) {
+    a.weights[pair] = (float)dh;
+    a.weights[pair + a.pairs] = (float)-dh;
+  }
+  return loss;
+}
+
+// A workgroup per pair; the sums in a fixed order.
 __global__ __launch_bounds__(1024) void preference_pair_kernel(AnswerArgs a) {
   __shared__ double slots[16];
-  const int T = a.per_answer;
-  double total = 0.0;
-  for (int pair = blockIdx.x; pair < a.pairs; pair += gridDim.x) {
-    double sums[2];
-    for (int side = 0; side < 2; ++side) {
-      const double* lp = a.lp + ((int64_t)pair + (int64_t)side * a.pairs) * T;
-      double s = 0.0;
-      for (int t = threadIdx.x; t < T; t += 1024) s += lp[t];
-      s = wave_sum(s);
-      if ((threadIdx.x & 63) == 0) slots[threadIdx.x / 64] = s;
-      __syncthreads();
-      s = 0.0;
-      for (int w = 0; w < 16; ++w) s += slots[w];
-      sums[side] = s;
-      __syncthreads();
-    }
-    if (threadIdx.x != 0) continue;
-    const double rw = a.beta * (sums[0] - (double)a.ref[pair]), rl = a.beta * (sums[1] - (double)a.ref[pair + a.pairs]);
-    const double h = rw - rl, e = a.smoothing;
-    // softplus(z) = log(1 + exp(z)) and the logistic function without overflow
-    const double q = log1p(exp(-fabs(h)));
-    const double up = fmax(h, 0.0) + q, down = fmax(-h, 0.0) + q;  // softplus(h), softplus(-h)
-    const double sig = 1.0 / (1.0 + exp(-h));                      // exp(inf) gives 0
-    const double sig_neg = 1.0 / (1.0 + exp(h));
-    const double dh = a.beta * (e * sig - (1.0 - e) * sig_neg);
-    // fmax ignores a NaN: h says it
-    const float loss = h != h ? __builtin_nanf("") : (float)((1.0 - e) * down + (e == 0.0 ? 0.0 : e * up));
-    a.losses[pair] = loss;
-    total += (double)loss;
-    if (a.rewards != nullptr) {
-      a.rewards[pair] = (float)rw;
-      a.rewards[pair + a.pairs] = (float)rl;
-    }
-    if (a.weights != nullptr) {
-      a.weights[pair] = (float)dh;
-      a.weights[pair + a.pairs] = (float)-dh;
-    }
+  const int pair = blockIdx.x, T = a.per_answer;
+  double sums[2];
+  for (int side = 0; side < 2; ++side) {
+    const double* lp = a.lp + ((int64_t)pair + (int64_t)side * a.pairs) * T;
+    double s = 0.0;
+    for (int t = threadIdx.x; t < T; t += 1024) s += lp[t];
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) slots[threadIdx.x / 64] = s;
+    __syncthreads();
+    s = 0.0;
+    for (int w = 0; w < 16; ++w) s += slots[w];
+    sums[side] = s;
+    __syncthreads();
   }
-  if (gridDim.x == 1 && threadIdx.x == 0 && a.reduced != nullptr)
+  if (threadIdx.x == 0) finish_pair(a, pair, sums[0], sums[1]);
+}
+
+// Up to kFewPairs pairs of up to kFewTokens tokens in one workgroup, a wave per
+// answer, the losses reduced too: a launch less, which is what small steps take.
+constexpr int kFewPairs = 8, kFewTokens = 2048;
+__global__ __launch_bounds__(128 * kFewPairs) void preference_few_kernel(AnswerArgs a) {
+  __shared__ double sums[2 * kFewPairs];
+  __shared__ float loss[kFewPairs];
+  const int wave = threadIdx.x / 64, lane = threadIdx.x & 63, T = a.per_answer;
+  if (wave < 2 * a.pairs) {
+    const double* lp = a.lp + (int64_t)wave * T;
+    constexpr int kRun = 8;  // loads in flight per lane
+    double s = 0.0;
+    for (int base = lane; base < T; base += 64 * kRun) {
+      double v[kRun];
+#pragma unroll
+      for (int k = 0; k < kRun; ++k) v[k] = lp[min(base + 64 * k, T - 1)];
+#pragma unroll
+      for (int k = 0; k < kRun; ++k) s += base + 64 * k < T ? v[k] : 0.0;
+    }
+    s = wave_sum(s);
+    if (lane == 0) sums[wave] = s;
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < a.pairs) loss[threadIdx.x] = finish_pair(a, threadIdx.x, sums[threadIdx.x], sums[threadIdx.x + a.pairs]);
+  __syncthreads();
+  if (threadIdx.x == 0 && a.reduced != nullptr) {
+    double total = 0.0;
+    for (int i = 0; i < a.pairs; ++i) total += (double)loss[i];
     a.reduced[0] = (float)(a.reduction == 2 ? total / a.pairs : total);
+  }
 }
 
 // reduced = the sum of the losses or their mean (over the tokens of answers, or
@@ -904,13 +933,13 @@ fc_status fc_preference_loss_fwd(const fc_answer_desc* desc, const fc_preference
   a.rewards = rewards;
   a.weights = weights;
   a.reduced = reduced;
-  // One workgroup up to eight pairs, each at most four values per thread and side.
-  const bool few = a.pairs <= 8 && desc->T <= 4096;
+  const bool few = a.pairs <= fc::kFewPairs && desc->T <= fc::kFewTokens;
   const fc::ProfileMark mk = fc::profile_begin(s);
-  hipLaunchKernelGGL(fc::preference_pair_kernel, dim3(few ? 1u : (unsigned)a.pairs), dim3(1024), 0, s, a);
+  if (few) hipLaunchKernelGGL(fc::preference_few_kernel, dim3(1), dim3(128 * fc::kFewPairs), 0, s, a);
+  else hipLaunchKernelGGL(fc::preference_pair_kernel, dim3((unsigned)a.pairs), dim3(1024), 0, s, a);
   e = hipGetLastError();
   fc::profile_end(mk, "preference_pair", s);
-  if (e == hipSuccess && reduced != nullptr && !few && a.pairs > 1) e = fc::launch_reduce(a, s);
+  if (e == hipSuccess && reduced != nullptr && !few) e = fc::launch_reduce(a, s);
   return done(who, e);
 }
 
