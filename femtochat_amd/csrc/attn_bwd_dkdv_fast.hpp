@@ -40,7 +40,14 @@ struct DkdvFastCfg {
 struct StepScore {
   float cap_in, cap_out, slope2;
 };
-template <int D, int kScore>
+// kTwo (capped scores, D <= 64, grids of two items a CU and more): two workgroups on
+// a CU, so that one's products run under the other's exponentials, which bound these
+// kernels; half the registers each, for which the row statistics and bounds are read
+// where the softmax needs them instead of a phase before.  us, one workgroup -> two:
+// 16 x 2048 tokens, H8 D64 272 -> 252; 4 x 2048, H8 D64 96 -> 93, H16 D32 113 -> 97,
+// H16 D16 110 -> 92; fewer items run alone on their CU: 2 x 1000, H8 D64 36 -> 44.
+// (Not capped, 4 x 2048, H8/4 D64 with a bias: 81 -> 94.)
+template <int D, int kScore, bool kTwo>
 struct DkdvStep {
   using C = DkdvFastCfg<D>;
   using M = Mma<bf16>;
@@ -204,8 +211,8 @@ struct DkdvStep {
           qa[c] = as_bf16x8(lds_load16(qt, fo.nat(c)));
           oa[c] = as_bf16x8(lds_load16(ot, fo.nat(c)));
         }
-        stats(lse, delta, b1, g, L[b1], Dl[b1]);
-        if (kSides) bounds(lbs, b1, g, LB[b1], Z[b1], UB[b1]);
+        stats(lse, delta, b1, g, L[b1], Dl[b1]);  // (kTwo: only Delta is used from here)
+        if (kSides && !kTwo) bounds(lbs, b1, g, LB[b1], Z[b1], UB[b1]);
         s[b1] = zero16();
         dp[b1] = zero16();
         if constexpr (kDeltaFirst) {
@@ -232,6 +239,11 @@ struct DkdvStep {
         }
       }
       if (bs >= 0 && bs < NQB) {
+        if constexpr (kTwo) {
+          f32x4 unused[4];
+          stats(lse, delta, bs, g, L[bs], unused);
+          if (kSides) bounds(lbs, bs, g, LB[bs], Z[bs], UB[bs]);
+        }
         softmax<kSides>(s[bs], dp[bs], L[bs], Dl[bs], LB[bs], Z[bs], UB[bs], bs, q0, key, g, T, right, c2, sc, pf[bs],
                            sf[bs]);
         // First transposed fragments of the block, for the next phase.
@@ -260,8 +272,8 @@ struct DkdvStep {
   }
 };
 
-template <int D, int kScore>
-__global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs a) {
+template <int D, int kScore, bool kTwo>
+__global__ __launch_bounds__(kThreads, kTwo ? 2 : 1) void attn_bwd_dkdv_fast_kernel(BwdArgs a) {
   using C = DkdvFastCfg<D>;
   constexpr int BQ = C::kBQ, KC = C::kKC, DB = C::kDB;
   // Two stage buffers as distinct objects, so the compiler can tell the LDS
@@ -456,7 +468,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
   uint32_t nx_at = 0;
   // Phases 0..3 of a step issue the loads, so they have the rest of the step
   // to land; later phases issue none.
-  constexpr int NPH = DkdvStep<D, kScore>::NPH, NDMA = NPH < 4 ? NPH : 4;
+  constexpr int NPH = DkdvStep<D, kScore, kTwo>::NPH, NDMA = NPH < 4 ? NPH : 4;
   constexpr int kPer = (DmaPlan<D, BQ>::kPerWave + NDMA - 1) / NDMA;
   auto dma_part = [&](int k) {
 #pragma unroll
@@ -505,7 +517,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
     if (tid < BQ) {
       const bool in = st_q < T;
       s_lse[slot][tid] = in ? ((kScore & kCap) ? st_lse - a.score.cap_out : st_lse) : INFINITY;
-      s_delta[slot][tid] = !in ? 0.0f : DkdvStep<D, kScore>::kDeltaFirst ? -st_delta : st_delta;
+      s_delta[slot][tid] = !in ? 0.0f : DkdvStep<D, kScore, kTwo>::kDeltaFirst ? -st_delta : st_delta;
       int lb = T;
       if (in) lb = max(0, max(st_q - a.left, pos != nullptr ? st_q - st_pos : 0));
       s_lb[slot][tid] = lb;
@@ -530,7 +542,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
       s_lbc[slot][1][tid] = hi;
       if constexpr (kScore != 0) {
         // (a chunk the sequence's end cuts has queries without keys)
-        s_lbc[slot][2][tid] = cub == nullptr ? DkdvStep<D, kScore>::kNoUpper : qc0 + 31 < T ? st_umin : -1;
+        s_lbc[slot][2][tid] = cub == nullptr ? DkdvStep<D, kScore, kTwo>::kNoUpper : qc0 + 31 < T ? st_umin : -1;
         s_lbc[slot][3][tid] = qc0 < T ? st_umax : -1;
       }
     }
@@ -545,7 +557,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_dkdv_fast_kernel(BwdArgs
       sc.cap_out = a.score.cap_out;
     }
     if constexpr ((kScore & kBias) != 0) sc.slope2 = a.score.slopes[kvh * a.group + h_first + st.h] * kLog2e;
-    DkdvStep<D, kScore>::run(dma_part, buf, buf + C::kTileBytes, s_lse[slot], s_delta[slot], s_lb[slot], s_lbc[slot][0], kf, vf, dk, dv,
+    DkdvStep<D, kScore, kTwo>::run(dma_part, buf, buf + C::kTileBytes, s_lse[slot], s_delta[slot], s_lb[slot], s_lbc[slot][0], kf, vf, dk, dv,
                              fo, q0, key, kw0, kw1, g, T, a.right, c2, sc);
   };
 
@@ -792,7 +804,15 @@ static hipError_t launch_dkdv_fast_t(const Problem& p, const BwdArgs& a, hipStre
   const int slots = cus >= kXcds && cus < n_items ? cus : n_items;
   const dim3 grid(slots), block(kThreads);
   const ProfileMark mk = profile_begin(s);
-  hipLaunchKernelGGL((attn_bwd_dkdv_fast_kernel<D, kScore>), grid, block, 0, s, a);
+  if constexpr ((kScore & kCap) != 0 && D <= 64) {
+    if (cus >= kXcds && n_items >= 2 * cus) {
+      hipLaunchKernelGGL((attn_bwd_dkdv_fast_kernel<D, kScore, true>), dim3(2 * cus), block, 0, s, a);
+      const hipError_t e = hipGetLastError();
+      profile_end(mk, "attn_bwd_dkdv_score_bf16", s);
+      return e;
+    }
+  }
+  hipLaunchKernelGGL((attn_bwd_dkdv_fast_kernel<D, kScore, false>), grid, block, 0, s, a);
   const hipError_t e = hipGetLastError();
   profile_end(mk, kScore ? "attn_bwd_dkdv_score_bf16" : "attn_bwd_dkdv_bf16", s);
   return e;
