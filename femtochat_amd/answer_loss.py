@@ -216,7 +216,7 @@ class PolicyLossFunction(torch.autograd.Function):
         else:
             _call(dev, _lib.lib().fc_policy_loss_fwd, ctypes.byref(d), ctypes.byref(o), *inputs, reduced, count)
         ctx.save_for_backward(logits, tokens, room)
-        ctx.desc, ctx.n, ctx.count = d, n, count
+        ctx.desc, ctx.n = d, n
         return out
 
     @staticmethod
@@ -229,9 +229,11 @@ class PolicyLossFunction(torch.autograd.Function):
                   dout.data_ptr())
         else:
             delta = _gradient_like(logits)
+            # (room may lie elsewhere now: saved-tensor hooks move what is saved)
             at, n = room.data_ptr(), ctx.n
+            count = at + 16 * n if ctx.desc.reduction == _REDUCTIONS["mean"] else None
             _call(delta.device, _lib.lib().fc_policy_loss_bwd, ctypes.byref(ctx.desc), delta.data_ptr(),
-                  logits.data_ptr(), tokens.data_ptr(), at, at + 8 * n, dout.data_ptr(), ctx.count)
+                  logits.data_ptr(), tokens.data_ptr(), at, at + 8 * n, dout.data_ptr(), count)
         return (delta,) + (None,) * 8
 
 

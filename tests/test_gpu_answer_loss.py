@@ -342,3 +342,27 @@ def test_gpu_refusals(gpu):
         F.policy_loss(x, t, o, o, kl=0.1)
     with pytest.raises(F._lib.AttentionError):
         F.preference_loss(x, t, o[:, 0].contiguous(), beta=-1.0)
+
+
+@pytest.mark.parametrize("V", [1003, 4 * 1024 * 16 + 9])
+def test_saved_tensors_that_move(gpu, V):
+    """Saved-tensor hooks may hand the backward copies: what lay where the forward
+    left it is overwritten here."""
+    B, T = 2, 5
+    x, xd = _logits(gpu, 41, B, T, V, "f32")
+    tok = _tokens(42, B, T, V, "some")
+    old, ref, adv = _policy_inputs(43, x, tok, per_answer=True)
+    td, od, rd, ad = _dev(gpu, tok, old, ref, adv)
+    xd.requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(), lambda t: t.clone()):
+        out = F.PolicyLossFunction.apply(xd, td, od, ad, rd, CLIP, 0.1, -1, "mean")
+        pref, _ = F.PreferenceLossFunction.apply(xd, td, ad, 0.1, 0.0, -1, "mean")
+    dirt = [torch.full((4 * B * T + k,), float("nan"), device=gpu) for k in (1, 1, B + 1, B + 1)]
+    _, g, w = O.policy(x, tok, old, adv, ref, CLIP, 0.1, dy=1.0 / (tok != -1).sum())
+    wd = np.abs(w) / (tok != -1).sum()
+    one = torch.ones((), device=gpu)
+    _check_gradient(torch.autograd.grad(out, xd, one, retain_graph=True)[0], g, wd, "f32")
+    _check_gradient(torch.autograd.grad(out, xd, one)[0], g, wd, "f32")
+    again, _ = F.PreferenceLossFunction.apply(xd, td, ad, 0.1, 0.0, -1, "mean")
+    assert torch.equal(torch.autograd.grad(pref, xd)[0], torch.autograd.grad(again, xd)[0])
+    assert all(d.isnan().all() for d in dirt)
