@@ -276,8 +276,8 @@ def preference_loss_(losses: torch.Tensor, logits: torch.Tensor, tokens: torch.T
     o = _lib.PreferenceOptions(float(beta), float(label_smoothing))
     if workspace is None:
         workspace = torch.empty(shape, dtype=torch.float64, device=dev)
-    elif workspace.device != dev:
-        raise ValueError(f"workspace is on {workspace.device}, expected {dev}")
+    elif workspace.device != dev or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous tensor on {dev}")
     _call(dev, _lib.lib().fc_preference_loss_fwd, ctypes.byref(d), ctypes.byref(o), _ptr(logits), _ptr(tokens),
           _ptr(ref_logprobs), _ptr(losses), _ptr(rewards), _ptr(logprobs), _ptr(stats), _ptr(weights), _ptr(reduced),
           _ptr(workspace), workspace.numel() * workspace.element_size())

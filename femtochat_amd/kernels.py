@@ -368,8 +368,8 @@ def _forward(A, O, l, m, Q, K, V, window, positions, workspace=None, score=None)
     if nbytes > 0:
         if workspace is None:
             workspace = torch.empty(nbytes + 256, dtype=torch.uint8, device=device)
-        elif workspace.device != device or workspace.numel() * workspace.element_size() < nbytes + 256:
-            raise ValueError(f"workspace must be a {nbytes + 256}-byte tensor on {device}")
+        elif workspace.device != device or not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < nbytes + 256:
+            raise ValueError(f"workspace must be a {nbytes + 256}-byte contiguous tensor on {device}")
         aligned = (workspace.data_ptr() + 255) & ~255
     _call(device, _lib.lib().fc_attn_score_fwd, ctypes.byref(d), score, Q.data_ptr(), K.data_ptr(), V.data_ptr(),
           _ptr(positions), O.data_ptr(), l.data_ptr(), m.data_ptr(), aligned, nbytes)
@@ -409,8 +409,8 @@ def _backward(A, dQ, dK, dV, dO, Q, K, V, O, l, m, window, positions, accumulate
                       0 if score is None else _kinds(score.softcap, score.slopes, score.prefix))
     if workspace is None:  # freed to this stream's pool on return, so later work on the stream comes after the kernels
         workspace = torch.empty(max(nbytes, 256) + 256, dtype=torch.uint8, device=device)
-    elif workspace.device != device or workspace.numel() * workspace.element_size() < nbytes + 256:
-        raise ValueError(f"workspace must be a {nbytes + 256}-byte tensor on {device}")
+    elif workspace.device != device or not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < nbytes + 256:
+        raise ValueError(f"workspace must be a {nbytes + 256}-byte contiguous tensor on {device}")
     _call(device, _lib.lib().fc_attn_score_bwd, ctypes.byref(d), score, dO.data_ptr(), Q.data_ptr(), K.data_ptr(),
           V.data_ptr(), O.data_ptr(), l.data_ptr(), m.data_ptr(), _ptr(positions), dQ.data_ptr(), dK.data_ptr(),
           dV.data_ptr(), (workspace.data_ptr() + 255) & ~255, nbytes)
@@ -490,10 +490,12 @@ class AttentionFunction(torch.autograd.Function):
     """``AttentionFunction.apply(Q, K, V, window, A, positions, softcap, slopes,
     prefix)``: differentiable attention, the role of the reference's Enzyme rule
     (ext/FemtoChatEnzymeExt.jl:221-278): forward = ``attention_state``; reverse =
-    ``Δattention!`` overwriting fresh gradient buffers."""
+    ``Δattention!`` overwriting fresh gradient buffers.  Slopes are constants."""
 
     @staticmethod
     def forward(ctx, Q, K, V, window, A=None, positions=None, softcap=0.0, slopes=None, prefix=None):
+        if ctx.needs_input_grad[7]:
+            raise ValueError("slopes have no gradient; pass them detached")
         A = A if A is not None else instruction(Q.dtype, Q.device, Q.shape[-1])
         st = attention_state(A, Q, K, V, window, positions=positions, softcap=softcap, slopes=slopes, prefix=prefix)
         ctx.save_for_backward(st.Q, st.K, st.V, st.O, st.l, st.m, positions, slopes, prefix)

@@ -375,3 +375,56 @@ def test_gpu_refusals(gpu):
     with pytest.raises(F._lib.AttentionError, match="fast mode"):
         F.attention(F.MFMAExact(), *f, (-1, 0), softcap=3.0)
     assert torch.equal(F.attention(F.MFMAExact(), *f, (-1, 0), softcap=0.0), F.attention(F.MFMAExact(), *f, (-1, 0)))
+
+
+def test_slopes_that_ask_for_a_gradient_are_refused(gpu):
+    Q, K, V, _ = (x.to(gpu) for x in _inputs(25, 1, 40, 4, 2, 32))
+    slopes = torch.full((4,), 0.1, device=gpu, requires_grad=True)
+    with pytest.raises(ValueError, match="slopes"):
+        F.AttentionFunction.apply(Q, K, V, (-1, 0), None, None, 0.0, slopes)
+    F.AttentionFunction.apply(Q, K, V, (-1, 0), None, None, 0.0, slopes.detach())
+
+
+def test_workspaces_that_repeat_their_memory_are_refused(gpu):
+    """A broadcast tensor has the values but not the bytes."""
+    Q, K, V, dO = (x.to(gpu) for x in _inputs(26, 1, 300, 4, 2, 32))
+    n = F.backward_workspace_bytes(A, Q, K, softcap=5.0)
+    O, l, m = torch.empty_like(Q), torch.empty(1, 4, 300, device=gpu), torch.empty(1, 4, 300, device=gpu)
+    F.attention_(A, O, l, m, Q, K, V, (-1, 0), softcap=5.0)
+    grads = [torch.empty_like(x) for x in (Q, K, V)]
+    ws = torch.empty(1, dtype=torch.uint8, device=gpu).expand(n)
+    with pytest.raises(ValueError, match="contiguous"):
+        F.delta_attention_(A, *grads, dO, Q, K, V, O, l, m, (-1, 0), softcap=5.0, workspace=ws)
+    x, t, r = torch.zeros(2, 3, 5, device=gpu), torch.zeros(2, 3, dtype=torch.int64, device=gpu), torch.zeros(2, device=gpu)
+    with pytest.raises(ValueError, match="contiguous"):
+        F.preference_loss(x, t, r, workspace=torch.empty(1, 1, dtype=torch.float64, device=gpu).expand(2, 3))
+
+
+def test_two_streams_at_once(gpu):
+    """Scored steps and losses on two streams at a time, the same bits as alone."""
+    def step(seed):
+        Q, K, V, dO = (x.to(gpu).requires_grad_(i < 3) for i, x in enumerate(_inputs(seed, 2, 700, 4, 2, 64)))
+        prefix = torch.tensor([40, 650], dtype=torch.int32, device=gpu)
+        x = torch.randn(4, 33, 1000, device=gpu, generator=torch.Generator(device=gpu).manual_seed(seed)).requires_grad_()
+        t = torch.randint(0, 1000, (4, 33), device=gpu, generator=torch.Generator(device=gpu).manual_seed(seed))
+        r = torch.zeros(4, device=gpu)
+        torch.cuda.current_stream(gpu).synchronize()
+
+        def run():
+            out = F.AttentionFunction.apply(Q, K, V, (-1, 0), None, None, 5.0, None, prefix)
+            loss = F.PreferenceLossFunction.apply(x, t, r, 0.1, 0.0, -1, "mean")[0]
+            return torch.autograd.grad([out, loss], [Q, K, V, x], [dO, torch.ones_like(loss)])
+        return run
+
+    runs = [step(27), step(28)]
+    want = [[g.clone() for g in run()] for run in runs]
+    streams = [torch.cuda.Stream(gpu), torch.cuda.Stream(gpu)]
+    torch.cuda.synchronize(gpu)
+    got = [None, None]
+    for _ in range(3):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i] = runs[i]()
+    torch.cuda.synchronize(gpu)
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
