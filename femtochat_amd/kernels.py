@@ -494,7 +494,7 @@ class AttentionFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, Q, K, V, window, A=None, positions=None, softcap=0.0, slopes=None, prefix=None):
-        if ctx.needs_input_grad[7]:
+        if slopes is not None and ctx.needs_input_grad[7]:
             raise ValueError("slopes have no gradient; pass them detached")
         A = A if A is not None else instruction(Q.dtype, Q.device, Q.shape[-1])
         st = attention_state(A, Q, K, V, window, positions=positions, softcap=softcap, slopes=slopes, prefix=prefix)
