@@ -194,7 +194,19 @@ __global__ __launch_bounds__(kOrderThreads) void attn_order_kernel(OrderArgs a) 
       const int qlo = a.chunk_ub != nullptr ? 0 : max(0, k0 - a.right), qhi = min(T - 1, k1 + a.left);
       int n = 0;
       if (a.chunk_ub != nullptr) {
-        for (int u = 0; u <= qhi / kOrderKStep; ++u) n += (s_lb[b * n128 + u] <= k1 && s_ub[b * n128 + u] >= k0) ? 1 : 0;
+        const int* lbs = s_lb + b * n128;
+        const int* ubs = s_ub + b * n128;
+        const int ulast = qhi / kOrderKStep;
+        for (int u0 = 0; u0 <= ulast; u0 += kOrderRun) {
+          int lb[kOrderRun], ub[kOrderRun];
+#pragma unroll
+          for (int e = 0; e < kOrderRun; ++e) {  // within the padded tables
+            lb[e] = lbs[u0 + e];
+            ub[e] = ubs[u0 + e];
+          }
+#pragma unroll
+          for (int e = 0; e < kOrderRun; ++e) n += (u0 + e <= ulast && lb[e] <= k1 && ub[e] >= k0) ? 1 : 0;
+        }
       } else if (qhi >= qlo) {
         const int* row = s_lb + b * n128;
         const int ulast = qhi / kOrderKStep;

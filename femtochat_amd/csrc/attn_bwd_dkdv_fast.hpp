@@ -287,6 +287,7 @@ __global__ __launch_bounds__(kThreads, kTwo ? 2 : 1) void attn_bwd_dkdv_fast_ker
   __shared__ __attribute__((aligned(16))) int s_lbc[2][kScore ? 4 : 2][BQ / 32];  // per slot: chunk min, max of lb, then of ub
   constexpr int kVisTiles = 256;  // query tiles whose visibility is tabulated in LDS
   __shared__ unsigned char s_vis[kVisTiles];
+  __shared__ int s_ends[2][kWaves];  // of the tabulated tiles, the first and last visible one per wave (scored kernels)
 
   __shared__ int s_next;
 
@@ -440,11 +441,40 @@ __global__ __launch_bounds__(kThreads, kTwo ? 2 : 1) void attn_bwd_dkdv_fast_ker
     qt_begin = qlo / BQ;
     n_qt_tiles = qhi >= qlo ? qhi / BQ - qt_begin + 1 : 0;
     vis_table = clb != nullptr && n_qt_tiles <= kVisTiles;
-    if (vis_table) {
-      for (int t = tid; t < n_qt_tiles; t += kThreads) s_vis[t] = tile_visible_global(qt_begin + t) ? 1 : 0;
+    t_first = 0;
+    if constexpr (kScore != 0) {
+      // One tile per thread, and from the first visible one to the last: a search
+      // through a row of documents, a dependent LDS read per tile at the start and at
+      // the end of every head, took up to 12% of the kernel (2 x 8192 tokens of documents, H16/8:
+      // D128 capped 257 -> 229 us, D64 biased 154 -> 137; 1 x 8192 D128 prefixes 149 -> 142).
+      static_assert(kVisTiles == kThreads, "one tile per thread");
+      if (vis_table) {
+        const bool seen = tid < n_qt_tiles && tile_visible_global(qt_begin + tid);
+        s_vis[tid] = seen ? 1 : 0;
+        const uint64_t mask = __ballot(seen);
+        if (lane == 0) {
+          s_ends[0][wave] = mask != 0 ? 64 * wave + __builtin_ctzll(mask) : kVisTiles;
+          s_ends[1][wave] = mask != 0 ? 64 * wave + 64 - __builtin_clzll(mask) : 0;
+        }
+        __syncthreads();
+        int first = kVisTiles, end = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          first = min(first, s_ends[0][w]);
+          end = max(end, s_ends[1][w]);
+        }
+        n_qt_tiles = __builtin_amdgcn_readfirstlane(end);
+        t_first = __builtin_amdgcn_readfirstlane(first);
+      } else {
+        __syncthreads();
+      }
+    } else {
+      if (vis_table) {
+        for (int t = tid; t < n_qt_tiles; t += kThreads) s_vis[t] = tile_visible_global(qt_begin + t) ? 1 : 0;
+      }
+      __syncthreads();
     }
-    __syncthreads();
-    t_first = first_tile(0);
+    t_first = first_tile(t_first);
     G = t_first < n_qt_tiles ? (kScore ? a.group / a.split_heads : a.group) : 0;  // no visible tile: no step
   };
   FragOffsets<DkdvFastCfg<D>::kW> fo;
