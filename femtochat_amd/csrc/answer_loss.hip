@@ -57,6 +57,7 @@ struct AnswerArgs {
   const float* dy;      // null (1), 1 value, or one per loss (reduction 0)
   int64_t N;
   int64_t ignore_index;
+  int64_t keep_from;    // the forward's columns from here on are to stay in the Infinity Cache
   int V;
   int index_base, index_type;
   int reduction;        // 0 none, 1 sum, 2 mean
@@ -158,7 +159,7 @@ __device__ inline Column combine4(const Column* c) {
 // 16-byte boundary and behind the last one go to the first threads, the chunks
 // between them to thread tid, tid + kThreads, ..., kBatch loads in flight; the sum
 // moves to a new maximum once per round.
-template <typename E, int kThreads, int kBatch>
+template <typename E, int kThreads, int kBatch, bool kKeep>
 __device__ inline Lse column_pass(const E* col, int V, int tid) {
   constexpr int kPer = Chunk<E>::kPer;
   const int head = min((int)((16 - (reinterpret_cast<uintptr_t>(col) & 15)) & 15) / (int)sizeof(E), V);
@@ -174,7 +175,8 @@ __device__ inline Lse column_pass(const E* col, int V, int tid) {
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       const int c = min(base + kThreads * k, chunks - 1);  // a chunk past the end is the last one again, not counted below
-      u[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(body + (int64_t)kPer * c));
+      const u32x4* p = reinterpret_cast<const u32x4*>(body + (int64_t)kPer * c);
+      u[k] = kKeep ? *p : __builtin_nontemporal_load(p);
     }
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
@@ -259,7 +261,8 @@ __global__ __launch_bounds__(256) void answer_fwd_kernel(AnswerArgs a) {
     return;
   }
   const E* col = static_cast<const E*>(a.logits) + token * (int64_t)a.V;
-  const Column v = wave_combine(column_pass<E, 256, 8>(col, a.V, threadIdx.x));
+  const Column v = wave_combine(token >= a.keep_from ? column_pass<E, 256, 8, true>(col, a.V, threadIdx.x)
+                                                     : column_pass<E, 256, 8, false>(col, a.V, threadIdx.x));
   if ((threadIdx.x & 63) == 0) slots[threadIdx.x / 64] = v;
   __syncthreads();
   if (threadIdx.x == 0) finish_token(a, token, col, combine4(slots));
@@ -276,7 +279,8 @@ __global__ __launch_bounds__(256) void answer_fwd_wave_kernel(AnswerArgs a) {
     return;
   }
   const E* col = static_cast<const E*>(a.logits) + token * (int64_t)a.V;
-  const Column r = wave_combine(column_pass<E, 64, 8>(col, a.V, lane));
+  const Column r = wave_combine(token >= a.keep_from ? column_pass<E, 64, 8, true>(col, a.V, lane)
+                                                     : column_pass<E, 64, 8, false>(col, a.V, lane));
   if (lane == 0) finish_token(a, token, col, r);
 }
 
@@ -458,7 +462,7 @@ __global__ __launch_bounds__(256) void answer_grad_kernel(AnswerArgs a, int head
     out[e] = from_f32<E>(kOverwrite ? v : v + to_f32(out[e]));
   };
   // From the array's end: the forward's last reads are still in the Infinity Cache
-  // (8192 x 32768 bf16, forward and gradient: 278 -> 271 us; 2262 x 50257 fp32: 240 -> 232).
+  // (kKeepBytes).
   const int64_t b0 = head + (int64_t)(gridDim.x - 1 - blockIdx.x) * (256 * kPer);  // the block's first value
   const int64_t e = b0 + (int64_t)threadIdx.x * kPer;
   if (blockIdx.x == 0 && (int)threadIdx.x < head) value(threadIdx.x);
@@ -655,8 +659,18 @@ int column_chunks(const AnswerArgs& a, int per) {
 template <typename E>
 int column_chunks(const AnswerArgs& a) { return column_chunks(a, Chunk<E>::kPer); }
 
+// What the forward reads last the gradient, which sweeps from the array's end, reads
+// first: the last kKeepBytes are read without the streaming hint, which would keep
+// them out of the Infinity Cache (256 MB), everything before them with it, and so is
+// everything where no gradient follows (no statistics wanted).  us of the forward and
+// the gradient of a preference step, for kKeepBytes of 0, 128, 192, 256, 320 MB and
+// everything: 8192 x 32768 bf16 64 + 185, 67 + 177, 68 + 174, 68 + 170, 69 + 168,
+// 73 + 166; 2262 x 50257 fp32 62 + 150, 63 + 141, 63 + 135, 64 + 130, 64 + 130, 65 + 136.
+constexpr int64_t kKeepBytes = (int64_t)256 << 20;
+
 template <typename E>
-hipError_t launch_fwd(const AnswerArgs& a, hipStream_t s) {
+hipError_t launch_fwd(AnswerArgs a, hipStream_t s) {
+  a.keep_from = a.stats == nullptr ? a.N : a.N - std::min(a.N, kKeepBytes / ((int64_t)a.V * (int64_t)sizeof(E)));
   const ProfileMark mk = profile_begin(s);
   if (column_chunks<E>(a) <= kWaveChunks)
     hipLaunchKernelGGL((answer_fwd_wave_kernel<E>), dim3((unsigned)((a.N + 3) / 4)), dim3(256), 0, s, a);
