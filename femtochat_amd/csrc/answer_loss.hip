@@ -663,10 +663,16 @@ int column_chunks(const AnswerArgs& a) { return column_chunks(a, Chunk<E>::kPer)
 // first: the last kKeepBytes are read without the streaming hint, which would keep
 // them out of the Infinity Cache (256 MB), everything before them with it, and so is
 // everything where no gradient follows (no statistics wanted).  us of the forward and
-// the gradient of a preference step, for kKeepBytes of 0, 128, 192, 256, 320 MB and
-// everything: 8192 x 32768 bf16 64 + 185, 67 + 177, 68 + 174, 68 + 170, 69 + 168,
-// 73 + 166; 2262 x 50257 fp32 62 + 150, 63 + 141, 63 + 135, 64 + 130, 64 + 130, 65 + 136.
-constexpr int64_t kKeepBytes = (int64_t)256 << 20;
+// the gradient of a preference step together, for 0, 128, 192, 256 MB and everything,
+// a quarter of the tokens outside the answers:
+//                        the logits just written         the same step again
+//   8192 x 32768 bf16    248 236 235 240 263             255 246 249 243 248
+//   2262 x 50257 fp32    224 205 202 205 229             209 201 196 192 200
+//   4096 x 32768 bf16    127 121 120 126 126             123 122 118 114 115
+//   2048 x 32768 bf16     71  60  60  60  59              69  62  62  62  61
+// Behind 1 GB of foreign writes the kept columns take the forward 10-45 us more: it
+// is the one that waits for those to leave the cache (8192 x 32768: 242 256 263 270 292).
+constexpr int64_t kKeepBytes = (int64_t)192 << 20;
 
 template <typename E>
 hipError_t launch_fwd(AnswerArgs a, hipStream_t s) {
