@@ -366,3 +366,31 @@ def test_saved_tensors_that_move(gpu, V):
     again, _ = F.PreferenceLossFunction.apply(xd, td, ad, 0.1, 0.0, -1, "mean")
     assert torch.equal(torch.autograd.grad(pref, xd)[0], torch.autograd.grad(again, xd)[0])
     assert all(d.isnan().all() for d in dirt)
+
+
+@pytest.mark.parametrize("B,T", [(1, 1), (3, 21), (1, 64), (1, 513), (4, 256), (5, 205), (3, 700)])
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+def test_the_mean_of_any_number_of_tokens(gpu, B, T, index):
+    """The divisor, also where only the gradient asks for it, and the count."""
+    V = 50
+    x, xd = _logits(gpu, 51, B, T, V, "f32")
+    tok = _tokens(52, B, T, V, "some")
+    tok[0, 0] = 3
+    old, ref, adv = _policy_inputs(53, x, tok, per_answer=True)
+    td, od, rd, ad = _dev(gpu, tok, old, ref, adv)
+    n = int((tok != -1).sum())
+    loss, g, w = O.policy(x, tok, old, adv, ref, CLIP, 0.1, dy=1.0 / n)
+    # A token whose two terms cancel has a small w and moves with lp all the same:
+    # w = -A r + kl (1 - exp(d)), so |dw / dlp| <= |A| r + kl exp(d).
+    lp, _ = O.log_probs(x, tok)
+    slope = np.where(tok != -1, np.abs(adv)[:, None] * np.exp(lp - old) + 0.1 * np.exp(ref - lp), 0.0)
+    for wants in (True, False):
+        losses, delta = torch.full((B, T), float("nan"), device=gpu), torch.full_like(xd, float("nan"))
+        reduced, count = (torch.full((1,), float("nan"), device=gpu) for _ in range(2))
+        F.policy_loss_fused_(losses, delta, xd, td.to(index), od, ad, ref_logprobs=rd, clip=CLIP, kl=0.1,
+                             reduced=reduced if wants else None, count=count)
+        assert float(count) == n
+        _check_gradient(delta, g, (np.abs(w) + slope) / n, "f32")
+        if wants:
+            total = losses.double().sum().item() / n
+            assert abs(float(reduced) - total) <= 2.0 ** -24 * abs(total) + 1e-30
