@@ -22,7 +22,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .kernels import _call, _check_tensor, _dtype_code, _ptr
+from .kernels import _as_saved, _call, _check_tensor, _dtype_code, _ptr
 from .loss import _INDEX, _REDUCTIONS, valid_target_count
 
 __all__ = [
@@ -180,6 +180,15 @@ def policy_loss_fused_(losses: torch.Tensor, delta: torch.Tensor, logits: torch.
           _ptr(weights), _ptr(reduced), _ptr(count), _ptr(delta), _ptr(dy))
 
 
+def _save(ctx, desc, logits, tokens, room) -> None:
+    ctx.save_for_backward(logits, tokens, room)
+    ctx.desc, ctx.n, ctx.device = desc, tokens.numel(), logits.device
+    ctx.saved_as = ((logits.shape, logits.dtype), (tokens.shape, tokens.dtype), (room.shape, room.dtype))
+
+
+_SAVED = ("logits", "tokens", "statistics")
+
+
 class PolicyLossFunction(torch.autograd.Function):
     """``PolicyLossFunction.apply(logits, tokens, old_logprobs, advantages,
     ref_logprobs, clip, kl, ignore_index, reduction)``: gradients for the logits
@@ -215,21 +224,19 @@ class PolicyLossFunction(torch.autograd.Function):
                   ctx.delta.data_ptr(), None)
         else:
             _call(dev, _lib.lib().fc_policy_loss_fwd, ctypes.byref(d), ctypes.byref(o), *inputs, reduced, count)
-        ctx.save_for_backward(logits, tokens, room)
-        ctx.desc, ctx.n = d, n
+        _save(ctx, d, logits, tokens, room)
         return out
 
     @staticmethod
     def backward(ctx, dout):
         delta, ctx.delta = ctx.delta, None
-        logits, tokens, room = ctx.saved_tensors
+        logits, tokens, room = _as_saved(ctx.saved_tensors, _SAVED, ctx.saved_as, ctx.device)
         dout = _as_floats(dout)
         if delta is not None:
             _call(delta.device, _lib.lib().fc_scale_gradient, delta.data_ptr(), ctx.desc.dtype, delta.numel(),
                   dout.data_ptr())
         else:
             delta = _gradient_like(logits)
-            # (room may lie elsewhere now: saved-tensor hooks move what is saved)
             at, n = room.data_ptr(), ctx.n
             count = at + 16 * n if ctx.desc.reduction == _REDUCTIONS["mean"] else None
             _call(delta.device, _lib.lib().fc_policy_loss_bwd, ctypes.byref(ctx.desc), delta.data_ptr(),
@@ -339,14 +346,13 @@ class PreferenceLossFunction(torch.autograd.Function):
         _call(dev, _lib.lib().fc_preference_loss_fwd, ctypes.byref(d), ctypes.byref(o), logits.data_ptr(),
               tokens.data_ptr(), ref_logprobs.data_ptr(), losses, rewards.data_ptr(), None, stats, weights, reduced, at,
               8 * n)
-        ctx.save_for_backward(logits, tokens, room)
-        ctx.desc, ctx.n = d, n
+        _save(ctx, d, logits, tokens, room)
         ctx.mark_non_differentiable(rewards)
         return out, rewards
 
     @staticmethod
     def backward(ctx, dout, _):
-        logits, tokens, room = ctx.saved_tensors
+        logits, tokens, room = _as_saved(ctx.saved_tensors, _SAVED, ctx.saved_as, ctx.device)
         dout = _as_floats(dout)
         delta = _gradient_like(logits)
         at, n = room.data_ptr(), ctx.n

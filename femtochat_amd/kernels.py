@@ -316,6 +316,21 @@ def _call(device: torch.device, entry, *args) -> None:
         _lib.check(entry(*args, _stream_ptr(device)))
 
 
+def _as_saved(tensors, names, like, device):
+    """What save_for_backward hands back, as the kernels read it.  Saved-tensor hooks
+    return the values, in whatever strides; anything but the (shape, dtype) of ``like``
+    on ``device`` is refused as an argument would be."""
+    for t, (shape, dtype) in zip(tensors, like):
+        if not (t.is_contiguous() and t.shape == shape and t.dtype is dtype and t.device == device):
+            break
+    else:
+        return tensors
+    tensors = tuple(t if t.is_contiguous() else t.contiguous() for t in tensors)
+    for name, t, (shape, dtype) in zip(names, tensors, like):
+        _check_tensor(f"the saved {name}", t, shape, (dtype,), device)
+    return tensors
+
+
 def _check_common(A, Q, K, V, positions):
     device = Q.device
     if not isinstance(A, Instruction):
@@ -486,6 +501,9 @@ def attention(*args, positions=None, forward=None, backward=None, **options) -> 
     return attention_state(A, Q, K, V, window, positions=positions, **opts).O
 
 
+_SAVED = ("Q", "K", "V", "O", "l", "m") + ("positions, slopes or prefix",) * 3
+
+
 class AttentionFunction(torch.autograd.Function):
     """``AttentionFunction.apply(Q, K, V, window, A, positions, softcap, slopes,
     prefix)``: differentiable attention, the role of the reference's Enzyme rule
@@ -498,14 +516,26 @@ class AttentionFunction(torch.autograd.Function):
             raise ValueError("slopes have no gradient; pass them detached")
         A = A if A is not None else instruction(Q.dtype, Q.device, Q.shape[-1])
         st = attention_state(A, Q, K, V, window, positions=positions, softcap=softcap, slopes=slopes, prefix=prefix)
-        ctx.save_for_backward(st.Q, st.K, st.V, st.O, st.l, st.m, positions, slopes, prefix)
+        saved = st[1:]
+        given = tuple(t for t in (positions, slopes, prefix) if t is not None)
+        if given:
+            saved += given
+        ctx.save_for_backward(*saved)
+        ctx.given = (positions is not None, slopes is not None, prefix is not None)
+        ctx.saved_as = [(t.shape, t.dtype) for t in saved]
         ctx.A, ctx.window, ctx.softcap = A, window, softcap
+        ctx.device = Q.device
         ctx.dtypes = (Q.dtype, K.dtype, V.dtype)
         return st.O
 
     @staticmethod
     def backward(ctx, dO):
-        Q, K, V, O, l, m, positions, slopes, prefix = ctx.saved_tensors
+        # (hooks may have moved what the forward checked; one look at each: delta_attention_'s
+        # checks take 14 us of a toy layer's step, which is all host time)
+        device = ctx.device
+        Q, K, V, O, l, m, *given = _as_saved(ctx.saved_tensors, _SAVED, ctx.saved_as, device)
+        positions, slopes, prefix = (given.pop(0) if there else None for there in ctx.given)
+        B, T, H, _ = Q.shape
         if not dO.is_contiguous():
             dO = dO.contiguous()
         if dO.dtype != O.dtype:
@@ -517,11 +547,7 @@ class AttentionFunction(torch.autograd.Function):
         gdtype = torch.float32
         if isinstance(ctx.A, MFMAFast) and all(dt == torch.bfloat16 for dt in ctx.dtypes):
             gdtype = torch.bfloat16
-        device = Q.device
         dQ, dK, dV = (torch.empty(x.shape, dtype=gdtype, device=device) for x in (Q, K, V))
-        # The forward checked what it saved (a toy layer's step is all host time: 149
-        # us with delta_attention_'s checks again, 135 without).
-        B, T, H, _ = Q.shape
         _backward(ctx.A, dQ, dK, dV, dO, Q, K, V, O, l, m, ctx.window, positions, False, None,
                   _score(ctx.softcap, slopes, prefix, device, B, T, H))
         out = [g.to(dt) if g.dtype != dt else g for g, dt in zip((dQ, dK, dV), ctx.dtypes)]
