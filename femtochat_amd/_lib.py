@@ -25,6 +25,7 @@ FC_BF16 = 1
 FC_MODE_EXACT = 0
 FC_MODE_FAST = 1
 FC_FLAG_OVERWRITE = 1
+FC_FLAG_FORMED = 2
 FC_PASS_FORWARD = 0
 FC_PASS_BACKWARD = 1
 FC_REDUCE_NONE = 0

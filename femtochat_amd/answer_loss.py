@@ -193,9 +193,9 @@ class PolicyLossFunction(torch.autograd.Function):
     """``PolicyLossFunction.apply(logits, tokens, old_logprobs, advantages,
     ref_logprobs, clip, kl, ignore_index, reduction)``: gradients for the logits
     only.  With a reduction, the forward forms the gradient of the value itself
-    beside it, in one pass over the logits, and the backward multiplies it by the
-    incoming gradient (and touches nothing where that is 1); a second backward
-    through the same node forms it again."""
+    beside it, in one pass over the logits; the backward touches nothing where the
+    incoming gradient is 1, and forms it again (rounded once, as any further backward
+    through the same node does) where it is not."""
 
     @staticmethod
     def forward(ctx, logits, tokens, old_logprobs, advantages, ref_logprobs=None, clip=(0.2, 0.2), kl=0.0,
@@ -232,15 +232,15 @@ class PolicyLossFunction(torch.autograd.Function):
         delta, ctx.delta = ctx.delta, None
         logits, tokens, room = _as_saved(ctx.saved_tensors, _SAVED, ctx.saved_as, ctx.device)
         dout = _as_floats(dout)
-        if delta is not None:
-            _call(delta.device, _lib.lib().fc_scale_gradient, delta.data_ptr(), ctx.desc.dtype, delta.numel(),
-                  dout.data_ptr())
-        else:
+        # (copies that hooks hand back may lie otherwise against 16 bytes)
+        formed = delta is not None and (delta.data_ptr() ^ logits.data_ptr()) & 15 == 0
+        if not formed:
             delta = _gradient_like(logits)
-            at, n = room.data_ptr(), ctx.n
-            count = at + 16 * n if ctx.desc.reduction == _REDUCTIONS["mean"] else None
-            _call(delta.device, _lib.lib().fc_policy_loss_bwd, ctypes.byref(ctx.desc), delta.data_ptr(),
-                  logits.data_ptr(), tokens.data_ptr(), at, at + 8 * n, dout.data_ptr(), count)
+        ctx.desc.flags = _lib.FC_FLAG_OVERWRITE | (_lib.FC_FLAG_FORMED if formed else 0)
+        at, n = room.data_ptr(), ctx.n
+        count = at + 16 * n if ctx.desc.reduction == _REDUCTIONS["mean"] else None
+        _call(delta.device, _lib.lib().fc_policy_loss_bwd, ctypes.byref(ctx.desc), delta.data_ptr(), logits.data_ptr(),
+              tokens.data_ptr(), at, at + 8 * n, dout.data_ptr(), count)
         return (delta,) + (None,) * 8
 
 

@@ -456,13 +456,18 @@ __device__ inline int target_from(int64_t y, int V, int64_t j) {
   return y >= 0 && y < V ? (int)max((int64_t)-1, min(y - j, (int64_t)INT_MAX)) : -1;
 }
 
+// What the gradient's sweep does with what dlogits holds: adds to it, writes over it,
+// or writes over a gradient that has its zeros already (answer_reform_kernel).
+constexpr int kAdd = 0, kWrite = 1, kReform = 2;
+
 // The whole (token, vocabulary) array in one sweep, a 16-byte chunk per thread,
 // whatever V is; a chunk across two columns goes value by value, and so do the
 // values in front of the array's first 16-byte boundary and behind its last one
 // (chunk 0 starts at `head` values).  Columns outside the answers are written as
-// zeros (overwriting) or left alone, and not read.
-template <typename E, bool kOverwrite>
-__global__ __launch_bounds__(256) void answer_grad_kernel(AnswerArgs a, int head) {
+// zeros (kWrite) or left alone, and not read.  `block` is one of `blocks` parts of
+// 256 chunks.
+template <typename E, int kInto>
+__device__ __attribute__((always_inline)) inline void grad_block(const AnswerArgs& a, int head, int64_t block, int64_t blocks) {
   constexpr int kPer = Chunk<E>::kPer;
   const E* x = static_cast<const E*>(a.logits);
   E* out = static_cast<E*>(a.dlogits);
@@ -471,20 +476,20 @@ __global__ __launch_bounds__(256) void answer_grad_kernel(AnswerArgs a, int head
     const int64_t token = e / V, j = e - token * V;
     const int64_t raw = index_at(a.tokens, token, a.index_type);
     if (raw == a.ignore_index) {
-      if (kOverwrite) out[e] = from_f32<E>(0.0f);
+      if (kInto == kWrite) out[e] = from_f32<E>(0.0f);
       return;
     }
     const float2 st = a.stats[token];
     const float f = grad_factor(a, token, a.weights[a.pairs > 0 ? answer_of(a, token) : token], a.reduction == 2 ? mean_divisor(a) : 1.0f);
     float v = to_f32(x[e]);
     grad_values<1>(&v, st.x, f / st.y, f, j == raw - a.index_base ? 0 : -1);
-    out[e] = from_f32<E>(kOverwrite ? v : v + to_f32(out[e]));
+    out[e] = from_f32<E>(kInto == kAdd ? v + to_f32(out[e]) : v);
   };
   // From the array's end: the forward's last reads are still in the Infinity Cache
   // (kKeepBytes).
-  const int64_t b0 = head + (int64_t)(gridDim.x - 1 - blockIdx.x) * (256 * kPer);  // the block's first value
+  const int64_t b0 = head + (blocks - 1 - block) * (256 * kPer);  // the block's first value
   const int64_t e = b0 + (int64_t)threadIdx.x * kPer;
-  if (blockIdx.x == 0 && (int)threadIdx.x < head) value(threadIdx.x);
+  if (block == 0 && (int)threadIdx.x < head) value(threadIdx.x);
   // A block inside one column has its token and what belongs to it in scalar registers.
   const int64_t t0 = b0 / V, j0 = b0 - t0 * V;
   int64_t token = t0, j = j0 + (int64_t)threadIdx.x * kPer;
@@ -501,24 +506,39 @@ __global__ __launch_bounds__(256) void answer_grad_kernel(AnswerArgs a, int head
   const int64_t raw = index_at(a.tokens, token, a.index_type);
   u32x4* o = reinterpret_cast<u32x4*>(out + e);
   if (raw == a.ignore_index) {
-    if (kOverwrite) __builtin_nontemporal_store(u32x4{0u, 0u, 0u, 0u}, o);
+    if (kInto == kWrite) __builtin_nontemporal_store(u32x4{0u, 0u, 0u, 0u}, o);
     return;
   }
   const u32x4 u = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(x + e));
   u32x4 prior;
-  if (!kOverwrite) prior = __builtin_nontemporal_load(o);
+  if (kInto == kAdd) prior = __builtin_nontemporal_load(o);
   const float2 st = a.stats[token];
   const float f = grad_factor(a, token, a.weights[a.pairs > 0 ? answer_of(a, token) : token], a.reduction == 2 ? mean_divisor(a) : 1.0f);
   float v[kPer];
   Chunk<E>::unpack(u, v);
   grad_values<kPer>(v, st.x, f / st.y, f, target_from(raw - a.index_base, a.V, j));
-  if (!kOverwrite) {
+  if (kInto == kAdd) {
     float w[kPer];
     Chunk<E>::unpack(prior, w);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) v[i] += w[i];
   }
   __builtin_nontemporal_store(Chunk<E>::pack(v), o);
+}
+
+template <typename E, int kInto>
+__global__ __launch_bounds__(256) void answer_grad_kernel(AnswerArgs a, int head) {
+  grad_block<E, kInto>(a, head, blockIdx.x, gridDim.x);
+}
+
+// The gradient of a loss that policy_fused_kernel has formed for dy = 1: kept where
+// dy[0] is 1 (the loss as the step's last node; the grid reads one value and ends),
+// formed again from the logits elsewhere.  That reads and writes what scaling the
+// formed one would, less the columns outside the answers, and rounds once.
+template <typename E>
+__global__ __launch_bounds__(256) void answer_reform_kernel(AnswerArgs a, int head, int64_t blocks) {
+  if (a.dy[0] == 1.0f) return;
+  for (int64_t i = blockIdx.x; i < blocks; i += gridDim.x) grad_block<E, kReform>(a, head, i, blocks);
 }
 
 // ---- the policy loss and its gradient in one pass -------------------------------
@@ -723,15 +743,17 @@ hipError_t launch_reduce(const AnswerArgs& a, hipStream_t s) {
 
 // N V <= 2^33 values (answer_args): at most 2^23 + 1 workgroups.
 template <typename E>
-hipError_t launch_grad(const AnswerArgs& a, bool overwrite, hipStream_t s) {
+hipError_t launch_grad(const AnswerArgs& a, int into, hipStream_t s) {
   const int64_t n = a.N * a.V;
   const int head = (int)std::min<int64_t>(n, ((16 - (reinterpret_cast<uintptr_t>(a.logits) & 15)) & 15) / sizeof(E));
   const int64_t blocks = std::max<int64_t>(1, (n - head + 256 * Chunk<E>::kPer - 1) / (256 * Chunk<E>::kPer));
   const ProfileMark mk = profile_begin(s);
-  if (overwrite) hipLaunchKernelGGL((answer_grad_kernel<E, true>), dim3((unsigned)blocks), dim3(256), 0, s, a, head);
-  else hipLaunchKernelGGL((answer_grad_kernel<E, false>), dim3((unsigned)blocks), dim3(256), 0, s, a, head);
+  if (into == kReform)  // eight workgroups a CU sweep the array
+    hipLaunchKernelGGL((answer_reform_kernel<E>), dim3((unsigned)std::min<int64_t>(2048, blocks)), dim3(256), 0, s, a, head, blocks);
+  else if (into == kWrite) hipLaunchKernelGGL((answer_grad_kernel<E, kWrite>), dim3((unsigned)blocks), dim3(256), 0, s, a, head);
+  else hipLaunchKernelGGL((answer_grad_kernel<E, kAdd>), dim3((unsigned)blocks), dim3(256), 0, s, a, head);
   const hipError_t e = hipGetLastError();
-  profile_end(mk, "answer_grad", s);
+  profile_end(mk, into == kReform ? "answer_reform" : "answer_grad", s);
   return e;
 }
 
@@ -788,7 +810,7 @@ bool off4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) != 0; }
 
 // Checks of what every entry point takes; fills the arguments they share.
 fc_status answer_args(const char* who, const fc_answer_desc* d, const void* logits, const void* dlogits, bool grad,
-                      const void* tokens, AnswerArgs* a) {
+                      const void* tokens, AnswerArgs* a, uint32_t flags = FC_FLAG_OVERWRITE) {
   if (d == nullptr) return bad(who, "descriptor is null");
   if (d->V <= 0 || d->answers <= 0 || d->T <= 0) return bad(who, "V, answers and T must be positive");
   const int64_t N = (int64_t)d->answers * d->T;
@@ -799,7 +821,7 @@ fc_status answer_args(const char* who, const fc_answer_desc* d, const void* logi
   if (d->index_type != FC_INDEX_I32 && d->index_type != FC_INDEX_I64) return bad(who, "index_type must be FC_INDEX_I32 or FC_INDEX_I64");
   if (d->reduction < FC_REDUCE_NONE || d->reduction > FC_REDUCE_MEAN) return bad(who, "unknown reduction");
   if (d->dtype != FC_F32 && d->dtype != FC_BF16) return bad(who, "dtype must be FC_F32 or FC_BF16");
-  if ((d->flags & ~FC_FLAG_OVERWRITE) != 0) return bad(who, "unknown flag bits");
+  if ((d->flags & ~flags) != 0) return bad(who, "unknown flag bits");
   if (logits == nullptr || tokens == nullptr || (grad && dlogits == nullptr)) return bad(who, "a required pointer is null");
   if ((reinterpret_cast<uintptr_t>(tokens) & (d->index_type == FC_INDEX_I64 ? 7 : 3)) != 0)
     return bad(who, "tokens are not aligned to their element size");
@@ -848,8 +870,9 @@ fc_status policy_args(const char* who, const fc_answer_desc* d, const fc_policy_
 }
 
 hipError_t run_fwd(const AnswerArgs& a, bool b16, hipStream_t s) { return b16 ? launch_fwd<bf16>(a, s) : launch_fwd<float>(a, s); }
-hipError_t run_grad(const AnswerArgs& a, bool b16, bool overwrite, hipStream_t s) {
-  return b16 ? launch_grad<bf16>(a, overwrite, s) : launch_grad<float>(a, overwrite, s);
+hipError_t run_grad(const AnswerArgs& a, const fc_answer_desc* d, hipStream_t s) {
+  const int into = (d->flags & FC_FLAG_FORMED) != 0 ? kReform : (d->flags & FC_FLAG_OVERWRITE) != 0 ? kWrite : kAdd;
+  return d->dtype == FC_BF16 ? launch_grad<bf16>(a, into, s) : launch_grad<float>(a, into, s);
 }
 
 }  // namespace
@@ -891,8 +914,11 @@ fc_status fc_policy_loss_bwd(const fc_answer_desc* desc, void* dlogits, const vo
                              const float* stats, const float* weights, const float* dy, const float* count, void* stream) {
   const char* who = "fc_policy_loss_bwd";
   AnswerArgs a;
-  const fc_status st = fc::answer_args(who, desc, logits, dlogits, true, tokens, &a);
+  const fc_status st = fc::answer_args(who, desc, logits, dlogits, true, tokens, &a, FC_FLAG_OVERWRITE | FC_FLAG_FORMED);
   if (st != FC_OK) return st;
+  if ((desc->flags & FC_FLAG_FORMED) != 0 &&
+      ((desc->flags & FC_FLAG_OVERWRITE) == 0 || desc->reduction == FC_REDUCE_NONE || dy == nullptr || logits == dlogits))
+    return bad(who, "a formed gradient is overwritten, of a sum or a mean, and has a dy and an array of its own");
   if (stats == nullptr || weights == nullptr || (desc->reduction == FC_REDUCE_MEAN && count == nullptr))
     return bad(who, "stats, weights and (for the mean) count are required");
   if (off4(weights) || off4(dy) || off4(count)) return bad(who, "float buffers must be 4-byte aligned");
@@ -901,7 +927,7 @@ fc_status fc_policy_loss_bwd(const fc_answer_desc* desc, void* dlogits, const vo
   a.weights = const_cast<float*>(weights);
   a.dy = dy;
   a.count = const_cast<float*>(count);
-  return done(who, fc::run_grad(a, desc->dtype == FC_BF16, (desc->flags & FC_FLAG_OVERWRITE) != 0, static_cast<hipStream_t>(stream)));
+  return done(who, fc::run_grad(a, desc, static_cast<hipStream_t>(stream)));
 }
 
 fc_status fc_policy_loss_fused(const fc_answer_desc* desc, const fc_policy_options* options, const void* logits,
@@ -1008,7 +1034,7 @@ fc_status fc_preference_loss_bwd(const fc_answer_desc* desc, void* dlogits, cons
   a.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
   a.weights = const_cast<float*>(weights);
   a.dy = dy;
-  return done(who, fc::run_grad(a, desc->dtype == FC_BF16, (desc->flags & FC_FLAG_OVERWRITE) != 0, static_cast<hipStream_t>(stream)));
+  return done(who, fc::run_grad(a, desc, static_cast<hipStream_t>(stream)));
 }
 
 fc_status fc_scale_gradient(void* x, int32_t dtype, int64_t n, const float* dy, void* stream) {

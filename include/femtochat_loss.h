@@ -155,6 +155,11 @@ typedef struct {
   uint32_t flags;       /* FC_FLAG_OVERWRITE: the backward writes dlogits instead of adding */
 } fc_answer_desc;
 
+/* Beside FC_FLAG_OVERWRITE in fc_policy_loss_bwd, for a sum or a mean: dlogits holds
+   what fc_policy_loss_fused wrote for dy = 1 on the same logits; where dy[0] is 1 it is
+   not touched (nor are the logits read), elsewhere it is formed again. */
+#define FC_FLAG_FORMED 2u
+
 typedef struct {
   double clip_low, clip_high;    /* the ratio is clipped to [1 - clip_low, 1 + clip_high] */
   double kl;                     /* factor of the KL term, 0: none */
@@ -213,7 +218,8 @@ fc_status fc_preference_loss_bwd(const fc_answer_desc* desc, void* dlogits, cons
 
 /* x[i] *= dy[0] for 0 <= i < n (float32 or bfloat16, the product rounded once);
    where dy[0] is 1, x is not touched.  For a gradient that was formed beside its
-   loss and is scaled once the loss's own gradient is known. */
+   loss and is scaled once the loss's own gradient is known, where a second rounding
+   does no harm (fc_policy_loss_bwd with FC_FLAG_FORMED rounds once). */
 fc_status fc_scale_gradient(void* x, int32_t dtype, int64_t n, const float* dy, void* stream);
 
 #ifdef __cplusplus

@@ -152,3 +152,20 @@ def test_scale_refusals():
     for args in ((None, L.FC_F32, 4, AT), (AT, L.FC_F32, 4, None), (AT, L.FC_F32, 0, AT), (AT, 9, 4, AT), (AT + 2, L.FC_F32, 4, AT),
                  (AT, L.FC_F32, 4, AT + 1)):
         assert lib.fc_scale_gradient(*args, None) == L.FC_ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("kw,swap", [
+    (dict(flags=L.FC_FLAG_FORMED), {}), (dict(reduction=L.FC_REDUCE_NONE), {}), ({}, dict(dy=None)), ({}, dict(dlogits=AT)),
+])
+def test_a_formed_gradient_refusals(kw, swap):
+    """It is overwritten, of a sum or a mean, under a dy, in an array of its own."""
+    d = dict(flags=L.FC_FLAG_OVERWRITE | L.FC_FLAG_FORMED)
+    d.update(kw)
+    s = dict(stats=AT, weights=AT, dy=AT)
+    s.update(swap)
+    assert _policy(_desc(**d), entry="bwd", **s) == L.FC_ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("entry", ["fwd", "fused"])
+def test_only_the_gradient_takes_a_formed_one(entry):
+    assert _policy(_desc(flags=L.FC_FLAG_FORMED | L.FC_FLAG_OVERWRITE), entry=entry) == L.FC_ERR_INVALID_ARGUMENT
