@@ -39,7 +39,7 @@ __all__ = [
 
 _LOGITS = (torch.float32, torch.bfloat16)
 _F32 = (torch.float32,)
-_FUSED_BYTES = (1 << 18) - 16  # the longest column that fc_policy_loss_fused holds
+_FUSED_BYTES = 1 << 18  # what fc_policy_loss_fused holds of a column, in whole 16-byte pieces
 
 
 def _desc(logits, tokens, ignore_index, reduction, index_base, overwrite=False) -> _lib.AnswerDesc:
@@ -84,6 +84,14 @@ def _dy(dy, dev, n: int) -> Optional[torch.Tensor]:
     if dy.numel() != n:
         raise ValueError(f"dy must hold {n} value(s), got {dy.numel()}")
     return dy
+
+
+def _held_at_once(logits: torch.Tensor) -> bool:
+    """Whether fc_policy_loss_fused takes these columns: one that may begin inside a
+    16-byte piece has up to a piece less one value fewer."""
+    size = logits.element_size()
+    n = logits.shape[-1] * size
+    return n <= _FUSED_BYTES - (16 - size) or (n == _FUSED_BYTES and logits.data_ptr() % 16 == 0)
 
 
 def _gradient_like(logits: torch.Tensor) -> torch.Tensor:
@@ -163,8 +171,9 @@ def policy_loss_fused_(losses: torch.Tensor, delta: torch.Tensor, logits: torch.
                        count: Optional[torch.Tensor] = None) -> None:
     """``policy_loss_`` and its gradient (written to ``delta``, zeros outside the
     answers) with the logits read once: the loss as the step's last node.
-    ``dy``: None (1), a number or a device tensor.  Columns of up to 262128 bytes (the
-    library raises FC_ERR_UNSUPPORTED above)."""
+    ``dy``: None (1), a number or a device tensor.  Columns of up to 256 KB (less
+    14 bytes in bfloat16, 12 in float32, where a column may begin inside a 16-byte
+    piece of memory); the library raises FC_ERR_UNSUPPORTED above."""
     d = _desc(logits, tokens, ignore_index, reduction, index_base, overwrite=True)
     o = _options(logits, tokens, old_logprobs, advantages, ref_logprobs, clip, kl)
     dev, shape = logits.device, tuple(tokens.shape)
@@ -217,8 +226,7 @@ class PolicyLossFunction(torch.autograd.Function):
         inputs = (logits.data_ptr(), tokens.data_ptr(), old_logprobs.data_ptr(), advantages.data_ptr(), _ptr(ref_logprobs),
                   losses, None, stats, weights)
         ctx.delta = None
-        if (ctx.needs_input_grad[0] and reduction != "none"
-                and logits.shape[-1] * logits.element_size() <= _FUSED_BYTES):
+        if ctx.needs_input_grad[0] and reduction != "none" and _held_at_once(logits):
             ctx.delta = _gradient_like(logits)
             _call(dev, _lib.lib().fc_policy_loss_fused, ctypes.byref(d), ctypes.byref(o), *inputs, reduced, count,
                   ctx.delta.data_ptr(), None)

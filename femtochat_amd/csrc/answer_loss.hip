@@ -946,7 +946,7 @@ fc_status fc_policy_loss_fused(const fc_answer_desc* desc, const fc_policy_optio
   if (logits == dlogits) return bad(who, "the gradient overlaps the logits");
   const bool b16 = desc->dtype == FC_BF16;
   if (fc::column_chunks(a, b16 ? 8 : 4) > fc::kFusedMost)
-    return bad(who, "a column of more than 256 KB is not held at once (use fc_policy_loss_fwd and fc_policy_loss_bwd)", FC_ERR_UNSUPPORTED);
+    return bad(who, "a column of more than 256 KB, with what it may begin inside, is not held at once (use fc_policy_loss_fwd and fc_policy_loss_bwd)", FC_ERR_UNSUPPORTED);
   a.count = count;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   hipError_t e = hipSuccess;

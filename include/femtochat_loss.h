@@ -191,7 +191,8 @@ fc_status fc_policy_loss_bwd(const fc_answer_desc* desc, void* dlogits, const vo
 
 /* Both in one pass: the logits are read once and dlogits is written once
    (whatever desc->flags says).  count is written too, and required for the mean.
-   Columns of up to 256 KB less 16 bytes (FC_ERR_UNSUPPORTED above). */
+   Columns of up to 256 KB where all begin and end on a 16-byte boundary, else of
+   up to 256 KB less 14 bytes (bfloat16) or 12 (float32); FC_ERR_UNSUPPORTED above. */
 fc_status fc_policy_loss_fused(const fc_answer_desc* desc, const fc_policy_options* options, const void* logits,
                                const void* tokens, const float* old_logprobs, const float* advantages,
                                const float* ref_logprobs, float* losses, float* logprobs, float* stats,
