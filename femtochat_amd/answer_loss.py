@@ -209,6 +209,8 @@ class PolicyLossFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, old_logprobs, advantages, ref_logprobs=None, clip=(0.2, 0.2), kl=0.0,
                 ignore_index=-1, reduction="mean"):
+        if any(ctx.needs_input_grad[2:5]):
+            raise ValueError("old_logprobs, advantages and ref_logprobs have no gradient; pass them detached")
         logits = logits.contiguous()
         d = _desc(logits, tokens, ignore_index, reduction, 0, overwrite=True)
         o = _options(logits, tokens, old_logprobs, advantages, ref_logprobs, clip, kl)
@@ -335,6 +337,8 @@ class PreferenceLossFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, tokens, ref_logprobs, beta=0.1, label_smoothing=0.0, ignore_index=-1, reduction="mean"):
+        if ctx.needs_input_grad[2]:
+            raise ValueError("ref_logprobs have no gradient; pass them detached")
         logits = logits.contiguous()
         d = _desc(logits, tokens, ignore_index, reduction, 0, overwrite=True)
         dev, n, B = logits.device, tokens.numel(), tokens.shape[0]

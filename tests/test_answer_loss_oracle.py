@@ -169,3 +169,16 @@ def test_a_formed_gradient_refusals(kw, swap):
 @pytest.mark.parametrize("entry", ["fwd", "fused"])
 def test_only_the_gradient_takes_a_formed_one(entry):
     assert _policy(_desc(flags=L.FC_FLAG_FORMED | L.FC_FLAG_OVERWRITE), entry=entry) == L.FC_ERR_INVALID_ARGUMENT
+
+
+def test_inputs_without_a_gradient_are_refused_one():
+    """What the losses take as constants is not silently left without a gradient."""
+    x, t, o = torch.zeros(2, 3, 5), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3)
+    asks = o.clone().requires_grad_()
+    for old, adv, ref in ((asks, o, None), (o, asks, None), (o, o, asks), (o, o[:, 0].clone().requires_grad_(), o)):
+        with pytest.raises(ValueError, match="no gradient"):
+            F.PolicyLossFunction.apply(x, t, old, adv, ref, (0.2, 0.2), 0.1, -1, "mean")
+    with pytest.raises(ValueError, match="no gradient"):
+        F.PreferenceLossFunction.apply(x, t, asks[:, 0], 0.1, 0.0, -1, "mean")
+    with pytest.raises(ValueError, match="HIP device"):  # detached: the next check speaks
+        F.PolicyLossFunction.apply(x, t, asks.detach(), o, None, (0.2, 0.2), 0.0, -1, "mean")

@@ -15,7 +15,8 @@ B, T, H, HKV, D, V = 2, 5, 4, 2, 16, 7
 class Ctx:
     """The context of a node: what its forward set, and the tensors it saved as
     `swap` returns them."""
-    needs_input_grad = (True,) * 3 + (False,) * 6
+    def __init__(self, wanted=1):
+        self.needs_input_grad = (True,) * wanted + (False,) * (9 - wanted)
 
     def save_for_backward(self, *tensors):
         self.saved = tensors
@@ -40,7 +41,7 @@ def calls(monkeypatch):
 
 
 def _attention(swap):
-    ctx = Ctx()
+    ctx = Ctx(3)
     Q, K, W = (torch.randn(B, T, h, D).bfloat16() for h in (H, HKV, HKV))
     pos = torch.arange(T, dtype=torch.int32).repeat(B, 1)
     F.AttentionFunction.forward(ctx, Q, K, W, (-1, 0), None, pos, 5.0, torch.ones(H), torch.full((B, T), 2, dtype=torch.int32))
