@@ -22,7 +22,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .kernels import _as_saved, _call, _check_tensor, _dtype_code, _ptr
+from .kernels import _OnceOnly, _as_saved, _call, _check_tensor, _dtype_code, _ptr
 from .loss import _INDEX, _REDUCTIONS, valid_target_count
 
 __all__ = [
@@ -251,6 +251,8 @@ class PolicyLossFunction(torch.autograd.Function):
         count = at + 16 * n if ctx.desc.reduction == _REDUCTIONS["mean"] else None
         _call(delta.device, _lib.lib().fc_policy_loss_bwd, ctypes.byref(ctx.desc), delta.data_ptr(), logits.data_ptr(),
               tokens.data_ptr(), at, at + 8 * n, dout.data_ptr(), count)
+        if torch.is_grad_enabled():
+            delta = _OnceOnly.apply("the policy loss", delta, logits, dout)
         return (delta,) + (None,) * 8
 
 
@@ -370,4 +372,6 @@ class PreferenceLossFunction(torch.autograd.Function):
         at, n = room.data_ptr(), ctx.n
         _call(delta.device, _lib.lib().fc_preference_loss_bwd, ctypes.byref(ctx.desc), delta.data_ptr(), logits.data_ptr(),
               tokens.data_ptr(), at + 8 * n, at + 16 * n, dout.data_ptr())
+        if torch.is_grad_enabled():
+            delta = _OnceOnly.apply("the preference loss", delta, logits, dout)
         return (delta,) + (None,) * 6

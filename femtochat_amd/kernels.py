@@ -501,6 +501,20 @@ def attention(*args, positions=None, forward=None, backward=None, **options) -> 
     return attention_state(A, Q, K, V, window, positions=positions, **opts).O
 
 
+class _OnceOnly(torch.autograd.Function):
+    """``_OnceOnly.apply(what, gradient, *inputs)``: the gradient itself, which raises
+    where it is differentiated by what it was formed from (create_graph)."""
+
+    @staticmethod
+    def forward(ctx, what, gradient, *inputs):
+        ctx.what = what
+        return gradient.view_as(gradient)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError(f"the gradient of {ctx.what} has no gradient of its own")
+
+
 _SAVED = ("Q", "K", "V", "O", "l", "m") + ("positions, slopes or prefix",) * 3
 
 
@@ -548,9 +562,11 @@ class AttentionFunction(torch.autograd.Function):
         if isinstance(ctx.A, MFMAFast) and all(dt == torch.bfloat16 for dt in ctx.dtypes):
             gdtype = torch.bfloat16
         dQ, dK, dV = (torch.empty(x.shape, dtype=gdtype, device=device) for x in (Q, K, V))
-        _backward(ctx.A, dQ, dK, dV, dO, Q, K, V, O, l, m, ctx.window, positions, False, None,
-                  _score(ctx.softcap, slopes, prefix, device, B, T, H))
+        score = _score(ctx.softcap, slopes, prefix, device, B, T, H)
+        _backward(ctx.A, dQ, dK, dV, dO, Q, K, V, O, l, m, ctx.window, positions, False, None, score)
         out = [g.to(dt) if g.dtype != dt else g for g, dt in zip((dQ, dK, dV), ctx.dtypes)]
+        if score is not None and torch.is_grad_enabled():
+            out = [_OnceOnly.apply("attention with capped, biased or prefix-masked scores", g, Q, K, V, dO) for g in out]
         return (out[0], out[1], out[2]) + (None,) * 6
 
 
