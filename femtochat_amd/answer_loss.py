@@ -22,7 +22,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .kernels import _OnceOnly, _as_saved, _call, _check_tensor, _dtype_code, _ptr
+from .kernels import _OnceOnly, _as_saved, _call, _check_tensor, _check_workspace, _dtype_code, _ptr
 from .loss import _INDEX, _REDUCTIONS, valid_target_count
 
 __all__ = [
@@ -295,8 +295,8 @@ def preference_loss_(losses: torch.Tensor, logits: torch.Tensor, tokens: torch.T
     o = _lib.PreferenceOptions(float(beta), float(label_smoothing))
     if workspace is None:
         workspace = torch.empty(shape, dtype=torch.float64, device=dev)
-    elif workspace.device != dev or not workspace.is_contiguous():
-        raise ValueError(f"workspace must be a contiguous tensor on {dev}")
+    else:
+        _check_workspace(workspace, 0, dev)  # (its size is the library's to refuse)
     _call(dev, _lib.lib().fc_preference_loss_fwd, ctypes.byref(d), ctypes.byref(o), _ptr(logits), _ptr(tokens),
           _ptr(ref_logprobs), _ptr(losses), _ptr(rewards), _ptr(logprobs), _ptr(stats), _ptr(weights), _ptr(reduced),
           _ptr(workspace), workspace.numel() * workspace.element_size())

@@ -331,6 +331,14 @@ def _as_saved(tensors, names, like, device):
     return tensors
 
 
+def _check_workspace(t: torch.Tensor, nbytes: int, device) -> None:
+    """A workspace lends its bytes: dense memory in any order of its dimensions, but no
+    tensor that repeats or leaves out memory."""
+    dense = t.is_contiguous() or t.permute(sorted(range(t.dim()), key=t.stride, reverse=True)).is_contiguous()
+    if t.device != device or not dense or t.numel() * t.element_size() < nbytes:
+        raise ValueError(f"workspace must be a {f'{nbytes}-byte ' if nbytes else ''}contiguous tensor on {device} (in some order of its dimensions)")
+
+
 def _check_common(A, Q, K, V, positions):
     device = Q.device
     if not isinstance(A, Instruction):
@@ -383,8 +391,8 @@ def _forward(A, O, l, m, Q, K, V, window, positions, workspace=None, score=None)
     if nbytes > 0:
         if workspace is None:
             workspace = torch.empty(nbytes + 256, dtype=torch.uint8, device=device)
-        elif workspace.device != device or not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < nbytes + 256:
-            raise ValueError(f"workspace must be a {nbytes + 256}-byte contiguous tensor on {device}")
+        else:
+            _check_workspace(workspace, nbytes + 256, device)
         aligned = (workspace.data_ptr() + 255) & ~255
     _call(device, _lib.lib().fc_attn_score_fwd, ctypes.byref(d), score, Q.data_ptr(), K.data_ptr(), V.data_ptr(),
           _ptr(positions), O.data_ptr(), l.data_ptr(), m.data_ptr(), aligned, nbytes)
@@ -424,8 +432,8 @@ def _backward(A, dQ, dK, dV, dO, Q, K, V, O, l, m, window, positions, accumulate
                       0 if score is None else _kinds(score.softcap, score.slopes, score.prefix))
     if workspace is None:  # freed to this stream's pool on return, so later work on the stream comes after the kernels
         workspace = torch.empty(max(nbytes, 256) + 256, dtype=torch.uint8, device=device)
-    elif workspace.device != device or not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < nbytes + 256:
-        raise ValueError(f"workspace must be a {nbytes + 256}-byte contiguous tensor on {device}")
+    else:
+        _check_workspace(workspace, nbytes + 256, device)
     _call(device, _lib.lib().fc_attn_score_bwd, ctypes.byref(d), score, dO.data_ptr(), Q.data_ptr(), K.data_ptr(),
           V.data_ptr(), O.data_ptr(), l.data_ptr(), m.data_ptr(), _ptr(positions), dQ.data_ptr(), dK.data_ptr(),
           dV.data_ptr(), (workspace.data_ptr() + 255) & ~255, nbytes)
