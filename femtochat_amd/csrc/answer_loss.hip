@@ -296,8 +296,9 @@ __device__ inline float finish_pair(const AnswerArgs& a, int pair, double chosen
   const double sig = 1.0 / (1.0 + exp(-h));                      // exp(inf) gives 0
   const double sig_neg = 1.0 / (1.0 + exp(h));
   const double dh = a.beta * (e * sig - (1.0 - e) * sig_neg);
-  // fmax ignores a NaN: h says it
-  const float loss = h != h ? __builtin_nanf("") : (float)((1.0 - e) * down + (e == 0.0 ? 0.0 : e * up));
+  // fmax ignores a NaN: h says it.  A side without a share adds nothing, also where h is
+  // infinite (an answer whose token has a logit of -inf).
+  const float loss = h != h ? __builtin_nanf("") : (float)((e == 1.0 ? 0.0 : (1.0 - e) * down) + (e == 0.0 ? 0.0 : e * up));
   a.losses[pair] = loss;
   if (a.rewards != nullptr) {
     a.rewards[pair] = (float)rw;
