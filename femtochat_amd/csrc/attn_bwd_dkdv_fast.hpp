@@ -586,7 +586,7 @@ __global__ __launch_bounds__(kThreads, kTwo ? 2 : 1) void attn_bwd_dkdv_fast_ker
       sc.cap_in = a.score.cap_in;
       sc.cap_out = a.score.cap_out;
     }
-    if constexpr ((kScore & kBias) != 0) sc.slope2 = a.score.slopes[kvh * a.group + h_first + st.h] * kLog2e;
+    if constexpr ((kScore & kBias) != 0) sc.slope2 = base2_slope(a.score.slopes[kvh * a.group + h_first + st.h]);
     DkdvStep<D, kScore, kTwo>::run(dma_part, buf, buf + C::kTileBytes, s_lse[slot], s_delta[slot], s_lb[slot], s_lbc[slot][0], kf, vf, dk, dv,
                              fo, q0, key, kw0, kw1, g, T, a.right, c2, sc);
   };

@@ -181,7 +181,7 @@ __global__ __launch_bounds__(kThreads * kParts, 2) void attn_bwd_dq_fast_kernel(
 #pragma unroll
   for (int i = 0; i < DB; ++i) dq[i] = zero16();
   const float c2 = a.scale_log2;
-  const float slope2 = (kScore & kBias) ? a.score.slopes[h] * kLog2e : 0.0f;
+  const float slope2 = (kScore & kBias) ? base2_slope(a.score.slopes[h]) : 0.0f;
   const float base = (kScore & kCap) ? neg_lse + a.score.cap_out : neg_lse;
   // P of key k0 + acc_row(r, g), and the cap's r (attn_score.hpp) in u.
   auto prob = [&](float x, int k0, int r, float& u) __attribute__((always_inline)) -> float {

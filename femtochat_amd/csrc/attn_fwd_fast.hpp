@@ -208,7 +208,7 @@ __global__ __launch_bounds__(kThreads * kParts, 2 / kParts) void attn_fwd_fast_k
   const float c2 = kCapAlone ? 2.0f * a.score.cap_out : kFinished ? 1.0f : a.scale_log2;
   const float c0 = kCapAlone ? a.score.cap_out : 0.0f;
   auto base2 = [&](float s) __attribute__((always_inline)) { return kCapAlone ? __builtin_fmaf(s, c2, c0) : s * c2; };
-  const float slope2 = (kScore & kBias) ? a.score.slopes[h] * kLog2e : 0.0f;
+  const float slope2 = (kScore & kBias) ? base2_slope(a.score.slopes[h]) : 0.0f;
   auto finish = [&](f32x16& sv, int qb, int k0) __attribute__((always_inline)) {
     if constexpr (kFinished)
       score_block<kScore>(sv, qv[qb] - k0 - 4 * g, a.scale_log2, a.score.cap_in, a.score.cap_out, slope2);

@@ -25,6 +25,13 @@ __device__ inline float cap_part(float x, float cap_in) {
   return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * cap_in) + 1.0f);
 }
 
+// A head's slope in base 2, finite whatever the slope is, so that a query's own key (a
+// distance of 0) keeps its score.
+__device__ inline float base2_slope(float slope) {
+  const float s = slope * kLog2e;
+  return __builtin_fabsf(s) == INFINITY ? __builtin_copysignf(kFltMax, s) : s;
+}
+
 // Whether the dQ kernel sums Delta over the keys (attn_bwd_dq_fast.hpp).
 __host__ __device__ inline bool exact_delta(int T, int left, int right) { return T <= 256 || left + imax(right, 0) <= 64; }
 
