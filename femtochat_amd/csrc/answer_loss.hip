@@ -557,7 +557,8 @@ __device__ inline void forget(u32x4& u) {
 template <typename E, int kThreads, int kChunks, int kWavesPerSimd>
 __global__ __launch_bounds__(kThreads == 64 ? 256 : kThreads, kWavesPerSimd) void policy_fused_kernel(AnswerArgs a) {
   constexpr int kPer = Chunk<E>::kPer, kRows = kThreads == 64 ? 4 : 1, kWaves = kThreads / 64;
-  __shared__ float smax[kWaves], ssum[kWaves], sw;
+  __shared__ float smax[kWaves], sw;
+  __shared__ double ssum[kWaves];
   const int64_t token = (int64_t)blockIdx.x * kRows + (kRows > 1 ? threadIdx.x / kThreads : 0);
   const int tid = kRows > 1 ? threadIdx.x % kThreads : threadIdx.x;
   if (token >= a.N) return;  // kRows > 1 only: no barrier follows
@@ -614,23 +615,24 @@ __global__ __launch_bounds__(kThreads == 64 ? 256 : kThreads, kWavesPerSimd) voi
       for (int i = 0; i < kPer; ++i) part += exp_sum(v[i], ref);
       s += part;
     }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
+    // The threads' sums meet in float64, as in the forward: 64 to 1024 of them against
+    // one that holds the maximum.
+    double sum = wave_sum((double)s);
     if (kWaves > 1) {
-      if ((tid & 63) == 0) ssum[tid / 64] = s;
+      if ((tid & 63) == 0) ssum[tid / 64] = sum;
       __syncthreads();
-      s = ssum[0];
+      sum = ssum[0];
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) s += ssum[w];
+      for (int w = 1; w < kWaves; ++w) sum += ssum[w];
     }
     float w = 0.0f;
-    if (tid < 64) w = finish_token(a, token, col, Column{mx, (double)s});  // every lane of the first wave the same
+    if (tid < 64) w = finish_token(a, token, col, Column{mx, sum});  // every lane of the first wave the same
     if (kWaves > 1) {
       if (tid == 0) sw = w;
       __syncthreads();
       w = sw;
     }
-    const float f = grad_factor(a, token, w, divisor), scaled = f / s;
+    const float f = grad_factor(a, token, w, divisor), scaled = f / (float)sum;
     const int64_t y = index_at(a.tokens, token, a.index_type) - a.index_base;
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
