@@ -168,14 +168,19 @@ inline size_t order_bytes(const Problem& p) { return (size_t)p.B * ((p.T + kOrde
 // the workspace, added in order.  The split is the one with the least estimated time:
 // the longer of the longest chain and a CU's share of all steps (with a third of a
 // chain more, which the last ones stand alone for), an item's own cost, and joining
-// the parts.  us of dK/dV and the join, whole -> split as chosen: 1 x 6792 tokens,
+// the parts, which a problem has at most kPartBytes of.  us of dK/dV and the join,
+// whole -> split as chosen: 1 x 6792 tokens,
 // H8/2 D96 775 -> 242 (4 heads x 2 tiles); 1 x 2048, H8/1 D128 518 -> 62 (8 x 2);
 // 1 x 4096, H16/8 D128 287 -> 219 (2 x 2); 1 x 415, H16/4 D80 73 -> 31 (4 x 2);
 // 1 x 8192, H2/2 D64 210 -> 110 (1 x 4); 2 x 512, H8/8 D128 stays whole (28, split 34).
+// Whole backwards with several items a CU: 4 x 4096, H16/4 D128 (2 a CU) 1237 -> 1096
+// (2 x 1); 4 x 5000, H12/4 D64 (2.5) 984 -> 850 (1 x 2); 1 x 16384, H32/8 D128 (4) 8290
+// -> 7945 (4 x 1, 512 MB), with 8 a CU 16970 -> 17145 (8 x 8192, H32/4 D128, 2 x 1, 512 MB).
 struct DkdvSplit {
   int heads, tiles;
   int parts() const { return heads * tiles; }
 };
+constexpr int64_t kPartBytes = (int64_t)256 << 20;
 inline DkdvSplit dkdv_split(const Problem& p) {
   DkdvSplit best{1, 1};
   if (p.score == 0) return best;
@@ -201,7 +206,7 @@ inline DkdvSplit dkdv_split(const Problem& p) {
   for (int h = 1; h <= p.group; ++h) {
     if (p.group % h != 0) continue;
     for (int t = 1; t <= 16 && (t == 1 || 2 * t <= tiles_seen); t *= 2) {
-      if (h * t > most) continue;
+      if (h * t > most || h * t * part_bytes / 2 > kPartBytes) continue;
       const double chain = (double)(p.group / h) * ((tiles_seen + t - 1) / t), share = items * p.group * mean / kCus;
       double us = step * std::max(chain, share + 0.35 * chain) + kItem * std::max(1.0, items * h * t / kCus);
       if (h * t > 1) us += kJoin + h * t * part_bytes / kJoinBytesPerUs;

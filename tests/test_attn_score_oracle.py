@@ -137,3 +137,24 @@ def test_python_refusals():
         F.attention(x, x, x, (-1, 0), softcap=30.0)
     with pytest.raises(TypeError, match="unexpected"):
         F.attention(x, x, x, (-1, 0), softcaps=30.0)
+
+
+def _parts_bytes(T, B, H, Hkv, D, window, positions=0):
+    """What a capped score adds to the backward's workspace beside the plain one's (the work
+    order aside, which a score may do without)."""
+    lib, got = L.lib(), []
+    d = L.AttnDesc(D, H, Hkv, T, B, *window, L.FC_MODE_FAST, *[L.FC_BF16] * 4, 0)
+    for score in (None, L.AttnScore(1.0, 0, None, None)):
+        n = ctypes.c_size_t(0)
+        assert lib.fc_attn_score_workspace_bytes(ctypes.byref(d), score, L.FC_PASS_BACKWARD, positions, ctypes.byref(n)) == 0
+        got.append(n.value)
+    return got[1] - got[0]
+
+
+@pytest.mark.parametrize("T,B,H,Hkv,D", [(8192, 1, 64, 4, 128), (14000, 1, 64, 4, 128), (16384, 1, 128, 1, 128), (50000, 1, 32, 1, 128),
+                                         (128, 440, 16, 1, 128), (6000, 9, 64, 1, 128), (4096, 1, 16, 8, 128), (1, 1, 64, 1, 16),
+                                         (16384, 1, 32, 8, 128), (32768, 1, 32, 8, 128), (32768, 8, 64, 4, 128), (8192, 8, 32, 4, 128)])
+def test_the_parts_of_a_split_are_bounded(T, B, H, Hkv, D):
+    """At most 256 MB of float32 parts, whatever the problem's size."""
+    for window in ((-1, 0), (1024, 0), (600, 300)):
+        assert _parts_bytes(T, B, H, Hkv, D, window) <= (256 << 20) + 512
