@@ -121,6 +121,10 @@ __global__ __launch_bounds__(kThreads * kParts, 2) void attn_bwd_dq_fast_kernel(
     kmin = min(kmin, s_bounds[0][w]);
     kmax = max(kmax, s_bounds[1][w]);
   }
+  if constexpr (kScore != 0) {  // the same on every lane: scalar branches
+    kmin = __builtin_amdgcn_readfirstlane(kmin);
+    kmax = __builtin_amdgcn_readfirstlane(kmax);
+  }
   const int kt0 = (kmin / BN) * BN;
   const int ntiles = kmax >= kmin ? (kmax - kt0) / BN + 1 : 0;
 
@@ -196,20 +200,21 @@ __global__ __launch_bounds__(kThreads * kParts, 2) void attn_bwd_dq_fast_kernel(
       e = __builtin_fmaf(-slope2, __builtin_fabsf((float)(q - k0 - 4 * g) - (float)acc_row(r, 0)), e);
     return __builtin_amdgcn_exp2f(e);
   };
-  if constexpr (kScore != 0 && kParts == 1) {
+  if constexpr (kScore != 0) {
     // Delta from a bf16 O carries O's rounding into every dS of its row, as large an
     // error as the rounding of dS itself.  Where rows see many keys and there are many
     // of them, it stays under 4e-3 of dQ and dK (2-norm); over few rows it does not (up
     // to 9e-3 at 32 rows, 5e-3 at 129), nor with few keys each (6e-3 with two, 3.5e-3
-    // with 64), against 3e-3 without it.  So short sequences, whose kernels are bound
-    // by latency, and narrow windows sum Delta = P dP over their keys first.
-    if (a.stats && exact_delta(T, a.left, a.right)) {
+    // with 64), against 3e-3 without it.  So query tiles whose keys span little, which
+    // are the short ones, and narrow windows sum Delta = P dP over their keys first.
+    if (a.stats && (kmax - kmin < kExactSpan || narrow_window(a.left, a.right))) {
       float sum = 0.0f;
       dma_wait_barrier();
-      for (int it = 0; it < ntiles; ++it) {
-        const int kt = kt0 + it * BN;
-        const char* Ks = it & 1 ? bufB : bufA;
-        issue(it + 1, it & 1 ? bufA : bufB);
+      bool odd = false;
+      for (int it = 0; it < ntiles; it += kParts, odd = !odd) {
+        const int kt = kt0 + (it + part) * BN;
+        const char* Ks = odd ? bufB : bufA;
+        issue(it + part + kParts, odd ? bufA : bufB);
 #pragma unroll
         for (int k = 0; k < NPH; ++k) dma_part(k);
 #pragma unroll
@@ -230,9 +235,15 @@ __global__ __launch_bounds__(kThreads * kParts, 2) void attn_bwd_dq_fast_kernel(
         }
         dma_wait_barrier();
       }
+      if constexpr (kParts == 2) {  // both parts go on with the row's whole sum
+        __shared__ float s_sum[2][kThreads];
+        s_sum[part][64 * wave + lane] = sum;
+        __syncthreads();
+        sum = s_sum[0][64 * wave + lane] + s_sum[1][64 * wave + lane];
+      }
       dlt = q < T ? sum + __shfl_xor(sum, 32) : 0.0f;
       if (ntiles > 0) {  // the first tile again
-        issue(0, bufA);
+        issue(part, bufA);
 #pragma unroll
         for (int k = 0; k < NPH; ++k) dma_part(k);
       }

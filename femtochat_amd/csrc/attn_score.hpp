@@ -32,8 +32,11 @@ __device__ inline float base2_slope(float slope) {
   return __builtin_fabsf(s) == INFINITY ? __builtin_copysignf(kFltMax, s) : s;
 }
 
-// Whether the dQ kernel sums Delta over the keys (attn_bwd_dq_fast.hpp).
-__host__ __device__ inline bool exact_delta(int T, int left, int right) { return T <= 256 || left + imax(right, 0) <= 64; }
+// Whether the dQ kernel sums Delta over the keys (attn_bwd_dq_fast.hpp): windows of up
+// to 64 tokens, and query tiles whose keys span at most 256, as those of short sequences
+// and of short documents packed into a long row do.
+__host__ __device__ inline bool narrow_window(int left, int right) { return left + imax(right, 0) <= 64; }
+constexpr int kExactSpan = 256;
 
 // Whether the forward and dQ take a query tile's key tiles in two parts (eight
 // waves): grids that leave at most one workgroup on a CU and have tiles that see more
@@ -44,7 +47,7 @@ __host__ __device__ inline bool exact_delta(int T, int left, int right) { return
 // 4 x 1024, H12 D64 (384, sixteen key tiles) 26, 30 -> 29, 36; 4 x 2048, H8 D128 (512)
 // 61, 76 -> 71, 91.
 inline bool score_parts(const Problem& p, int cus, unsigned workgroups) {
-  if (exact_delta(p.T, p.left, p.right)) return false;
+  if (narrow_window(p.left, p.right)) return false;
   const int64_t span = p.prefix ? p.T : std::min((int64_t)p.T, (int64_t)p.left + p.right + kOrderRows);
   return (workgroups <= (unsigned)cus && span > 10 * kOrderTile) || (4 * (int64_t)workgroups <= 7 * (int64_t)cus && span > 20 * kOrderTile);
 }
