@@ -91,8 +91,8 @@ __device__ inline float max16(const f32x16& s) {
   return m;
 }
 
-// kParts 2 (grids that leave at most one workgroup on a CU): eight waves, of
-// which waves 4 .. 7 take the odd key tiles of the same 128 queries through
+// kParts 2 (small grids: the launcher's rule, score_parts for scored kernels): eight
+// waves, of which waves 4 .. 7 take the odd key tiles of the same 128 queries through
 // stage buffers of their own, so that a wave's chain of tiles is half as long
 // and each SIMD has two waves, as with two workgroups per CU.
 template <int D, int kParts, int kScore>
