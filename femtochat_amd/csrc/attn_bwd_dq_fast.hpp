@@ -23,8 +23,9 @@ struct DqFastCfg {
   static constexpr int kStageBytes = 2 * kTileBytes;  // K, V
 };
 
-// kParts 2 (scored kernels on small grids, score_parts): eight waves, of which waves 4 .. 7 take the odd key tiles of the same 128 queries through
-// stage buffers of their own, as in the forward; the two sums meet in LDS.
+// kParts 2 (scored kernels on small grids, score_parts): eight waves, of which waves
+// 4 .. 7 take the odd key tiles of the same 128 queries through stage buffers of their
+// own, as in the forward; the two sums meet in LDS.
 template <int D, int kScore, int kParts>
 __global__ __launch_bounds__(kThreads * kParts, 2) void attn_bwd_dq_fast_kernel(BwdArgs a) {
   using C = DqFastCfg<D>;
