@@ -20,9 +20,10 @@
 //    both, so the logits are read once and the gradient written once.
 // The preference loss has no such form: w needs a whole answer's log-probability
 // before the first gradient.
-// exp and the sums over the vocabulary are float32; a token's log-probability, its
-// ratio and the sums over an answer are float64 (a ratio next to its clip decides a
-// whole column, and an answer's sum is in the thousands while h is near 1).
+// exp is float32, and so are the sums over 16 bytes of logits; the sums over the
+// vocabulary, a token's log-probability, its ratio and the sums over an answer are
+// float64 (a ratio next to its clip decides a whole column, and an answer's sum is in
+// the thousands while h is near 1).
 #include "attn_device.hpp"
 #include "attn_launch.hpp"
 
@@ -122,19 +123,12 @@ __device__ inline float exp_sum(float x, float m) {
   return __builtin_amdgcn_exp2f(__builtin_fmaf(t, kLog2e, t * kLog2eLow));
 }
 
-// (maximum, sum of exp(x - maximum)) of what a thread or a group has seen; s = 0:
-// nothing yet, or only -inf.
-struct Lse {
-  float m, s;
-};
-__device__ inline Lse combine(Lse a, Lse b) {
-  const float m = fmaxf(a.m, b.m);
-  return Lse{m, (a.s == 0.0f ? 0.0f : a.s * exp_sum(a.m, m)) + (b.s == 0.0f ? 0.0f : b.s * exp_sum(b.m, m))};
-}
-
-// (maximum, sum) of a column: the sum in float64, each part moved to the maximum
-// of its group once (a tree of pairs would move it by the exponential's rounding,
-// which leans to one side, at every level).
+// (maximum, sum of exp(x - maximum)) of what a thread, a group or a column has seen;
+// s = 0: nothing yet, or only -inf.
+// The sums are float64, of float32 sums of a chunk's values: a thread that holds a value
+// near the maximum would lose most of its others to a float32 one, up to 1e-7 of the
+// column where few values carry it (logits with a standard deviation of 6), always to
+// the same side.
 struct Column {
   float m;
   double s;
@@ -145,11 +139,14 @@ __device__ inline double wave_sum(double s) {
   return s;
 }
 __device__ inline double moved(double s, float from, float to) { return s == 0.0 ? 0.0 : s * (double)exp_sum(from, to); }
-__device__ inline Column wave_combine(Lse v) {
+// A column's threads, waves: each part is moved to the maximum of its group once (a
+// tree of pairs would move it by the exponential's rounding, which leans to one side,
+// at every level).
+__device__ inline Column wave_combine(Column v) {
   float m = v.m;
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  return Column{m, wave_sum(moved((double)v.s, v.m, m))};
+  return Column{m, wave_sum(moved(v.s, v.m, m))};
 }
 __device__ inline Column combine4(const Column* c) {
   const float m = fmaxf(fmaxf(c[0].m, c[1].m), fmaxf(c[2].m, c[3].m));
@@ -161,15 +158,18 @@ __device__ inline Column combine4(const Column* c) {
 // between them to thread tid, tid + kThreads, ..., kBatch loads in flight; the sum
 // moves to a new maximum once per round.
 template <typename E, int kThreads, int kBatch, bool kKeep>
-__device__ inline Lse column_pass(const E* col, int V, int tid) {
+__device__ inline Column column_pass(const E* col, int V, int tid) {
   constexpr int kPer = Chunk<E>::kPer;
   const int head = min((int)((16 - (reinterpret_cast<uintptr_t>(col) & 15)) & 15) / (int)sizeof(E), V);
   const int chunks = (V - head) / kPer, tail = V - head - kPer * chunks;
   const E* body = col + head;
-  Lse acc{-INFINITY, 0.0f};
-  auto one = [](float x) { return Lse{x, x == -INFINITY ? 0.0f : 1.0f}; };
-  if (tid < head) acc = combine(acc, one(to_f32(col[tid])));
-  if (tid < tail) acc = combine(acc, one(to_f32(body[kPer * chunks + tid])));
+  Column acc{-INFINITY, 0.0};
+  auto one = [&](float x) {
+    const float m = fmaxf(acc.m, x);
+    acc = Column{m, moved(acc.s, acc.m, m) + (x == -INFINITY ? 0.0 : (double)exp_sum(x, m))};
+  };
+  if (tid < head) one(to_f32(col[tid]));
+  if (tid < tail) one(to_f32(body[kPer * chunks + tid]));
   for (int base = tid; base < chunks; base += kThreads * kBatch) {
     u32x4 u[kBatch];
     float bm = -INFINITY;
@@ -188,16 +188,16 @@ __device__ inline Lse column_pass(const E* col, int V, int tid) {
     }
     const float m = fmaxf(acc.m, bm);
     const float ref = m == -INFINITY ? 0.0f : m;  // only -inf so far: every exponential is 0
-    float s = acc.s == 0.0f ? 0.0f : acc.s * exp_sum(acc.m, ref);
+    double s = moved(acc.s, acc.m, ref);
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       float v[kPer], part = 0.0f;
       Chunk<E>::unpack(u[k], v);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) part += exp_sum(v[i], ref);
-      s += base + kThreads * k < chunks ? part : 0.0f;
+      s += base + kThreads * k < chunks ? (double)part : 0.0;
     }
-    acc = Lse{m, s};
+    acc = Column{m, s};
   }
   return acc;
 }
@@ -605,7 +605,7 @@ __global__ __launch_bounds__(kThreads == 64 ? 256 : kThreads, kWavesPerSimd) voi
       for (int w = 1; w < kWaves; ++w) mx = fmaxf(mx, smax[w]);
     }
     const float ref = mx == -INFINITY ? 0.0f : mx;
-    float s = 0.0f;
+    double sum = 0.0;  // (as in the forward)
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
       float v[kPer], part = 0.0f;
@@ -613,11 +613,9 @@ __global__ __launch_bounds__(kThreads == 64 ? 256 : kThreads, kWavesPerSimd) voi
       Chunk<E>::unpack(u[k], v);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) part += exp_sum(v[i], ref);
-      s += part;
+      sum += (double)part;
     }
-    // The threads' sums meet in float64, as in the forward: 64 to 1024 of them against
-    // one that holds the maximum.
-    double sum = wave_sum((double)s);
+    sum = wave_sum(sum);
     if (kWaves > 1) {
       if ((tid & 63) == 0) ssum[tid / 64] = sum;
       __syncthreads();
