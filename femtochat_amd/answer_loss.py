@@ -206,12 +206,18 @@ class PolicyLossFunction(torch.autograd.Function):
     incoming gradient is 1, and forms it again (rounded once, as any further backward
     through the same node does) where it is not."""
 
+    @classmethod
+    def apply(cls, logits, *args):
+        # (a copy that autograd knows, so that what the node saves leads to the caller's logits)
+        if isinstance(logits, torch.Tensor) and not logits.is_contiguous():
+            logits = logits.contiguous()
+        return super().apply(logits, *args)
+
     @staticmethod
     def forward(ctx, logits, tokens, old_logprobs, advantages, ref_logprobs=None, clip=(0.2, 0.2), kl=0.0,
                 ignore_index=-1, reduction="mean"):
         if any(ctx.needs_input_grad[2:5]):
             raise ValueError("old_logprobs, advantages and ref_logprobs have no gradient; pass them detached")
-        logits = logits.contiguous()
         d = _desc(logits, tokens, ignore_index, reduction, 0, overwrite=True)
         o = _options(logits, tokens, old_logprobs, advantages, ref_logprobs, clip, kl)
         dev, n = logits.device, tokens.numel()
@@ -337,11 +343,17 @@ class PreferenceLossFunction(torch.autograd.Function):
     label_smoothing, ignore_index, reduction)`` -> (loss, rewards): gradients for
     the logits, through the loss only."""
 
+    @classmethod
+    def apply(cls, logits, *args):
+        # (a copy that autograd knows, so that what the node saves leads to the caller's logits)
+        if isinstance(logits, torch.Tensor) and not logits.is_contiguous():
+            logits = logits.contiguous()
+        return super().apply(logits, *args)
+
     @staticmethod
     def forward(ctx, logits, tokens, ref_logprobs, beta=0.1, label_smoothing=0.0, ignore_index=-1, reduction="mean"):
         if ctx.needs_input_grad[2]:
             raise ValueError("ref_logprobs have no gradient; pass them detached")
-        logits = logits.contiguous()
         d = _desc(logits, tokens, ignore_index, reduction, 0, overwrite=True)
         dev, n, B = logits.device, tokens.numel(), tokens.shape[0]
         if B % 2 != 0:

@@ -574,7 +574,8 @@ class AttentionFunction(torch.autograd.Function):
         _backward(ctx.A, dQ, dK, dV, dO, Q, K, V, O, l, m, ctx.window, positions, False, None, score)
         out = [g.to(dt) if g.dtype != dt else g for g, dt in zip((dQ, dK, dV), ctx.dtypes)]
         if score is not None and torch.is_grad_enabled():
-            out = [_OnceOnly.apply("attention with capped, biased or prefix-masked scores", g, Q, K, V, dO) for g in out]
+            # (O leads to the leaves, also where Q, K and V are conversions of them)
+            out = [_OnceOnly.apply("attention with capped, biased or prefix-masked scores", g, O, dO) for g in out]
         return (out[0], out[1], out[2]) + (None,) * 6
 
 
