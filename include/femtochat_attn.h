@@ -134,8 +134,9 @@ fc_status fc_attn_bwd_noalloc(const fc_attn_desc* desc, const void* dO,
  * The forward and the backward with scores beyond q.k/sqrt(D).  No reference
  * counterpart.
  *   softcap c > 0 : S <- c tanh(S / c)                       (S = q.k/sqrt(D))
- *   slopes  (H)   : S <- S - slopes[h] |q - k|, after the cap; any finite values,
- *                   fastest where scores fall with the distance (at least 0)
+ *   slopes  (H)   : S <- S - slopes[h] |q - k|, after the cap; any finite values of
+ *                   which -slopes[h] T stays in float32's range, fastest where
+ *                   scores fall with the distance (at least 0)
  *   prefix        : a query also sees the keys up to the end of its prefix,
  *                   k <= max(q + right, start + n - 1), where start is the
  *                   query's document's first token (q - positions[q], 0 without
