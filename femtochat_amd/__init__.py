@@ -7,8 +7,10 @@ host-side mirror of the reference's ``Kernels`` attention API, and
 ``CausalSelfAttention`` applies to Q and K before it, and
 ``femtochat_amd.loss`` the cross-entropy and token-embedding kernels either
 side of the model (include/femtochat_loss.h), ``femtochat_amd.answer_loss`` the
-policy and preference losses over its answers, ``femtochat_amd.optim`` the
-optimizer kernels (include/femtochat_optim.h).
+policy and preference losses over its answers, ``femtochat_amd.cache`` and
+``femtochat_amd.drafts`` the cache, its attention and the verification of drafted tokens
+that generate text (include/femtochat_cache.h), ``femtochat_amd.optim`` the optimizer
+kernels (include/femtochat_optim.h).
 """
 from .kernels import (  # noqa: F401
     AttentionFunction,
@@ -59,6 +61,18 @@ from .answer_loss import (  # noqa: F401
     preference_loss_,
     preference_loss_gradient_,
 )
+from .cache import (  # noqa: F401
+    KVCache,
+    cache_keep_,
+    cache_read,
+    cache_read_,
+    cache_write_,
+    cached_attention,
+    cached_attention_,
+    cached_attention_workspace_bytes,
+    kv_cache,
+)
+from .drafts import verify_drafts, verify_drafts_, verify_drafts_workspace_bytes  # noqa: F401
 from .optim import (  # noqa: F401
     AdamW,
     adam_update_,

@@ -1,5 +1,6 @@
 """ctypes binding of libfemtochat_attn.so (the C ABI in include/femtochat_attn.h
-include/femtochat_loss.h, include/femtochat_optim.h and include/femtochat_xla.h).
+include/femtochat_loss.h, include/femtochat_cache.h, include/femtochat_optim.h and
+include/femtochat_xla.h).
 
 The shared library is built in-tree by ``femtochat_amd.build`` (hipcc,
 gfx950).  Loading fails loudly when it is missing: there is no CPU fallback
@@ -33,6 +34,9 @@ FC_REDUCE_SUM = 1
 FC_REDUCE_MEAN = 2
 FC_INDEX_I32 = 0
 FC_INDEX_I64 = 1
+FC_CACHE_BF16 = 1
+FC_CACHE_I8 = 2
+FC_CACHE_F8 = 3
 
 STATUS_NAMES = {
     FC_OK: "FC_OK",
@@ -133,6 +137,53 @@ class EmbedDesc(ctypes.Structure):
         ("index_type", ctypes.c_int32),
         ("y_dtype", ctypes.c_int32),
         ("flags", ctypes.c_uint32),
+    ]
+
+
+class CacheDesc(ctypes.Structure):
+    _fields_ = [
+        ("D", ctypes.c_int32),
+        ("Hkv", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("layers", ctypes.c_int32),
+        ("pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("type", ctypes.c_int32),
+    ]
+
+
+class Cache(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("table", ctypes.c_void_p),
+    ]
+
+
+class CachedAttnOptions(ctypes.Structure):
+    _fields_ = [
+        ("H", ctypes.c_int32),
+        ("N", ctypes.c_int32),
+        ("left", ctypes.c_int32),
+        ("tree", ctypes.c_int32),
+        ("softcap", ctypes.c_float),
+        ("slopes", ctypes.c_void_p),
+    ]
+
+
+class VerifyDesc(ctypes.Structure):
+    _fields_ = [
+        ("B", ctypes.c_int32),
+        ("N", ctypes.c_int32),
+        ("V", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("index_type", ctypes.c_int32),
+        ("tree", ctypes.c_int32),
+        ("has_draft", ctypes.c_int32),
+        ("temperature", ctypes.c_double),
     ]
 
 
@@ -244,6 +295,17 @@ _SIGNATURES = {
                                + [ctypes.c_size_t, _P]),
     "fc_preference_loss_bwd": (ctypes.c_int, [ctypes.POINTER(AnswerDesc)] + [_P] * 7),
     "fc_scale_gradient": (ctypes.c_int, [_P, ctypes.c_int32, ctypes.c_int64, _P, _P]),
+    "fc_cache_write": (ctypes.c_int, [ctypes.POINTER(CacheDesc), ctypes.POINTER(Cache), _P, _P, ctypes.c_int32, ctypes.c_int32,
+                                      _P, _P, _P]),
+    "fc_cache_read": (ctypes.c_int, [ctypes.POINTER(CacheDesc), ctypes.POINTER(Cache), _P, _P, ctypes.c_int32, ctypes.c_int32,
+                                     _P, _P, _P]),
+    "fc_cache_keep": (ctypes.c_int, [ctypes.POINTER(CacheDesc), ctypes.POINTER(Cache), ctypes.c_int32, _P, _P, _P, _P]),
+    "fc_cached_attn_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(CacheDesc), ctypes.POINTER(CachedAttnOptions),
+                                                      ctypes.POINTER(ctypes.c_size_t)]),
+    "fc_cached_attn": (ctypes.c_int, [ctypes.POINTER(CacheDesc), ctypes.POINTER(Cache), ctypes.POINTER(CachedAttnOptions)]
+                       + [_P] * 6 + [ctypes.c_size_t, _P]),
+    "fc_verify_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(VerifyDesc), ctypes.POINTER(ctypes.c_size_t)]),
+    "fc_verify_drafts": (ctypes.c_int, [ctypes.POINTER(VerifyDesc)] + [_P] * 10 + [ctypes.c_size_t, _P]),
     "fc_embedding_fwd": (ctypes.c_int, [ctypes.POINTER(EmbedDesc), _P, _P, _P, _P]),
     "fc_embedding_bwd": (ctypes.c_int, [ctypes.POINTER(EmbedDesc), _P, _P, _P, _P]),
     "fc_embedding_bwd_full": (ctypes.c_int, [ctypes.POINTER(EmbedDesc), _P, _P, _P, _P]),

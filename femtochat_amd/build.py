@@ -15,7 +15,7 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
-SOURCES = ["attn_api.hip", "attn_fwd.hip", "attn_bwd.hip", "attn_fwd_fast.hip", "attn_bwd_fast.hip", "attn_bwd_dkdv_vgpr.hip", "attn_score_join.hip", "rope_norm.hip", "loss.hip", "answer_loss.hip", "xla_bridge.hip", "optim.hip", "embed_sort.hip", "embed_grad.hip", "convert.hip"]
+SOURCES = ["attn_api.hip", "attn_fwd.hip", "attn_bwd.hip", "attn_fwd_fast.hip", "attn_bwd_fast.hip", "attn_bwd_dkdv_vgpr.hip", "attn_score_join.hip", "rope_norm.hip", "loss.hip", "answer_loss.hip", "xla_bridge.hip", "optim.hip", "embed_sort.hip", "embed_grad.hip", "convert.hip", "cache.hip", "cached_attn_api.hip", "drafts.hip"]
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [
@@ -43,6 +43,10 @@ EXTRA_FLAGS = {"attn_bwd_dkdv_vgpr.hip": _VGPR_FORM, "attn_bwd.hip": _VGPR_FORM,
 SCORE_SOURCES = ["attn_score_dkdv.hip", "attn_score_dkdv_vgpr.hip", "attn_score_dq.hip", "attn_score_fwd.hip"]
 SCORES = (1, 3, 5, 7)
 
+# Sources compiled once for each type of cache (include/femtochat_cache.h).
+CACHE_SOURCES = ["cached_attn.hip"]
+CACHE_TYPES = (1, 2, 3)
+
 
 def hipcc() -> str:
     for cand in (os.environ.get("HIPCC"), "/opt/rocm/bin/hipcc", shutil.which("hipcc")):
@@ -64,6 +68,7 @@ def build(verbose: bool = False) -> Path:
     cc = hipcc()
     BUILD.mkdir(exist_ok=True)
     units = [(s, f"{Path(s).stem}{n}.o", [f"-DFC_SCORE={n}"]) for s in SCORE_SOURCES for n in SCORES]
+    units += [(s, f"{Path(s).stem}{n}.o", [f"-DFC_CACHE={n}"]) for s in CACHE_SOURCES for n in CACHE_TYPES]
     units += [(s, Path(s).stem + ".o", []) for s in SOURCES]
     objs = [BUILD / o for _, o, _ in units]
     cmds = [[cc, *HIPCC_FLAGS, *EXTRA_FLAGS.get(s, []), *define, "-c", str(CSRC / s), "-o", str(BUILD / o)]

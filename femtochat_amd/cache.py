@@ -1,0 +1,331 @@
+"""Text generation on the MI355X: a cache of keys and values, and attention of the
+newest tokens over it.
+
+They stand beside ``attention`` for what follows training: a prompt's keys and
+values (after the attention prologue) are written once, and each new token, or tree
+of drafted ones, attends to them with the scores that ``attention`` gives (causal or
+windowed, capped, biased).  The reference has no counterpart.
+
+A ``KVCache`` holds tokens in pages::
+
+    k, v              (pages, Hkv, page, D), bfloat16, int8 or float8_e4m3fn
+    k_scale, v_scale  (pages, Hkv, page) float32, one per token and head (8-bit types)
+    pages             (B, M) int32: the pages of each sequence's tokens in order, or
+                      None, where page b is sequence b's own
+
+or, with a leading dimension, those of all layers (``cache.layer(i)`` is one).  An
+8-bit value is code * scale, with scale = max |x| / 127 (int8) or / 448 (float8) over a
+token's head.  ``lengths`` (B,) int32 are the tokens that the cache holds before a
+call; the call's own tokens lie behind them, ``counts`` (B,) int32 of them where a
+batch is ragged.  A step of generation with drafted tokens is::
+
+    for i in range(layers):                       # nodes: the last token and the drafts
+        cache_write_(cache.layer(i), K, V, lengths, counts)
+        O = cached_attention(Q, cache.layer(i), lengths, window, parents=parents, counts=counts)
+    path, kept, token = verify_drafts(logits, nodes, uniforms, parents=parents, counts=counts)
+    cache_keep_(cache, lengths, path, kept)
+    lengths += kept                               # token is the next step's first node
+"""
+from __future__ import annotations
+
+import ctypes
+from functools import lru_cache
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from . import _lib
+from .kernels import _call, _check_tensor, _check_workspace, _dtype_code, _ptr
+
+__all__ = [
+    "KVCache",
+    "kv_cache",
+    "cache_write_",
+    "cache_read",
+    "cache_read_",
+    "cache_keep_",
+    "cached_attention",
+    "cached_attention_",
+    "cached_attention_workspace_bytes",
+]
+
+_TYPES = {torch.bfloat16: _lib.FC_CACHE_BF16, torch.int8: _lib.FC_CACHE_I8, torch.float8_e4m3fn: _lib.FC_CACHE_F8}
+_VALUES = (torch.float32, torch.bfloat16)
+_I32 = (torch.int32,)
+
+
+class KVCache(NamedTuple):
+    """A cache's buffers (module documentation)."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: Optional[torch.Tensor] = None
+    v_scale: Optional[torch.Tensor] = None
+    pages: Optional[torch.Tensor] = None
+
+    def layer(self, i: int) -> "KVCache":
+        """Layer i of a cache of several."""
+        if self.k.dim() != 5:
+            raise ValueError("the cache holds one layer")
+        pick = lambda t: None if t is None else t[i]  # noqa: E731
+        return KVCache(self.k[i], self.v[i], pick(self.k_scale), pick(self.v_scale), self.pages)
+
+    @property
+    def capacity(self) -> int:
+        """The tokens a sequence has room for."""
+        return self.k.shape[-2] * (1 if self.pages is None else self.pages.shape[1])
+
+
+def kv_cache(sequences: int, capacity: int, n_kv_head: int, head_dim: int, dtype: torch.dtype = torch.bfloat16, *,
+             layers: Optional[int] = None, page: Optional[int] = None, pool: Optional[int] = None, device="cuda") -> KVCache:
+    """An empty cache for ``sequences`` of up to ``capacity`` tokens (rounded up to whole
+    pages, of 16 tokens at least).  With ``page`` (a power of two from 16) it is a pool of ``pool``
+    pages (default: enough for every sequence) and a table, filled in order as far as the
+    pool goes and with -1 behind it; the caller may hand out pages otherwise."""
+    if dtype not in _TYPES:
+        raise TypeError(f"unsupported dtype {dtype}; a cache holds bfloat16, int8 or float8_e4m3fn")
+    if min(sequences, capacity, n_kv_head, head_dim) <= 0 or (layers is not None and layers <= 0) or (pool is not None and pool <= 0):
+        raise ValueError("sequences, capacity, n_kv_head, head_dim, layers and pool must be positive")
+    table = None
+    if page is None:
+        if pool is not None:
+            raise ValueError("a pool has pages")
+        size, count = -(-capacity // 16) * 16, sequences
+    else:
+        if page < 16 or page & (page - 1):
+            raise ValueError("a page holds a power of two of tokens, 16 at least")
+        each = -(-capacity // page)
+        size, count = page, sequences * each if pool is None else pool
+        table = torch.arange(sequences * each, dtype=torch.int32)
+        table = torch.where(table < count, table, -1).view(sequences, each).to(device)
+    shape = ((layers,) if layers is not None else ()) + (count, n_kv_head, size)
+    k, v = (torch.zeros(shape + (head_dim,), dtype=dtype, device=device) for _ in range(2))
+    if dtype == torch.bfloat16:
+        return KVCache(k, v, None, None, table)
+    return KVCache(k, v, torch.zeros(shape, device=device), torch.zeros(shape, device=device), table)
+
+
+class _Buffers:
+    """A checked cache: its descriptor, pointers, device and sizes."""
+
+    __slots__ = ("desc", "pointers", "device", "lead", "B", "Hkv", "D")
+
+    def __init__(self, cache: KVCache, B: int):
+        k, v, ks, vs, pages = cache
+        if not isinstance(k, torch.Tensor) or k.dim() not in (4, 5) or k.dtype not in _TYPES:
+            raise ValueError("a cache's k must be a ([layers,] pages, Hkv, page, D) tensor of bfloat16, int8 or float8_e4m3fn")
+        device = k.device
+        if device.type != "cuda":
+            raise ValueError("the MI355X cache kernels need tensors on a HIP device (torch 'cuda'); there is no CPU path")
+        shape = k.shape
+        _check_tensor("k", k, shape, (k.dtype,), device)
+        _check_tensor("v", v, shape, (k.dtype,), device)
+        if k.dtype is torch.bfloat16:
+            if ks is not None or vs is not None:
+                raise ValueError("a bfloat16 cache has no scales")
+        else:
+            _check_tensor("k_scale", ks, shape[:-1], (torch.float32,), device)
+            _check_tensor("v_scale", vs, shape[:-1], (torch.float32,), device)
+        M = 0
+        if pages is not None:
+            if not isinstance(pages, torch.Tensor) or pages.dim() != 2 or pages.shape[1] == 0:
+                raise ValueError("a cache's pages must be a (B, M) int32 tensor")
+            M = pages.shape[1]
+            _check_tensor("pages", pages, (B, M), _I32, device)
+        lead = tuple(shape[:-4])
+        P, Hkv, S, D = shape[-4:]
+        self.desc = _lib.CacheDesc(D, Hkv, B, lead[0] if lead else 1, P, S, M, _TYPES[k.dtype])
+        self.pointers = _lib.Cache(k.data_ptr(), v.data_ptr(), _ptr(ks), _ptr(vs), _ptr(pages))
+        self.device, self.lead, self.B, self.Hkv, self.D = device, lead, B, Hkv, D
+
+
+def _batch(cache: KVCache, like) -> int:
+    """The sequences of a call: those of ``like`` (B, ...), or of the cache's table."""
+    if isinstance(like, torch.Tensor) and like.dim() >= 1:
+        return like.shape[0]
+    return cache.k.shape[-4] if cache.pages is None else cache.pages.shape[0]
+
+
+def _check_counts(c: _Buffers, lengths, counts, name: str = "lengths") -> None:
+    if lengths is not None:
+        _check_tensor(name, lengths, (c.B,), _I32, c.device)
+    if counts is not None:
+        _check_tensor("counts", counts, (c.B,), _I32, c.device)
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """An input as the kernels read it, 16 bytes at a time."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def cache_write_(cache: KVCache, K: torch.Tensor, V: torch.Tensor, lengths: torch.Tensor,
+                 counts: Optional[torch.Tensor] = None) -> None:
+    """Writes K and V ([layers,] B, T, Hkv, D), float32 or bfloat16, as each sequence's
+    tokens ``lengths[b]`` to ``lengths[b] + counts[b] - 1`` (T of them without ``counts``),
+    quantised to the cache's type.  Tokens beyond the capacity are not written."""
+    c = _Buffers(cache, _batch(cache, lengths))
+    T = _check_values(c, K, V, None)
+    _check_tensor("lengths", lengths, (c.B,), _I32, c.device)
+    _check_counts(c, None, counts)
+    if T == 0:
+        return
+    K, V = _aligned(K), _aligned(V)
+    _call(c.device, _lib.lib().fc_cache_write, ctypes.byref(c.desc), ctypes.byref(c.pointers), K.data_ptr(), V.data_ptr(),
+          _dtype_code(K.dtype), T, lengths.data_ptr(), _ptr(counts))
+
+
+def _check_values(c: _Buffers, K, V, T: Optional[int]) -> int:
+    if not isinstance(K, torch.Tensor) or K.dim() != len(c.lead) + 4:
+        raise ValueError("K and V must be ([layers,] B, T, Hkv, D) tensors, with layers where the cache has them")
+    T = K.shape[-3] if T is None else T
+    shape = c.lead + (c.B, T, c.Hkv, c.D)
+    _check_tensor("K", K, shape, _VALUES, c.device)
+    _check_tensor("V", V, shape, (K.dtype,), c.device)
+    return T
+
+
+def cache_read_(K: torch.Tensor, V: torch.Tensor, cache: KVCache, starts: Optional[torch.Tensor] = None,
+                counts: Optional[torch.Tensor] = None) -> None:
+    """``cache_read`` into the caller's K and V."""
+    c = _Buffers(cache, _batch(cache, starts if starts is not None else counts))
+    T = _check_values(c, K, V, None)
+    _check_counts(c, starts, counts, "starts")
+    if T == 0:
+        return
+    if (K.data_ptr() | V.data_ptr()) % 16:
+        raise ValueError("K and V must start on a 16-byte boundary")
+    _call(c.device, _lib.lib().fc_cache_read, ctypes.byref(c.desc), ctypes.byref(c.pointers), K.data_ptr(), V.data_ptr(),
+          _dtype_code(K.dtype), T, _ptr(starts), _ptr(counts))
+
+
+def cache_read(cache: KVCache, starts: Optional[torch.Tensor], T: int, counts: Optional[torch.Tensor] = None, *,
+               dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values ([layers,] B, T, Hkv, D) of each sequence's tokens ``starts[b]`` (None:
+    0) to ``starts[b] + counts[b] - 1``, with zeros behind them, in float32 or bfloat16:
+    ``cache_read(cache, None, T, lengths)`` is all that the cache holds, for ``attention``.
+    Tokens beyond the capacity read as NaN."""
+    if dtype not in _VALUES:
+        raise TypeError(f"unsupported dtype {dtype}; a cache reads back as float32 or bfloat16")
+    if T < 0:
+        raise ValueError("T must not be negative")
+    k = cache.k
+    if not isinstance(k, torch.Tensor) or k.dim() not in (4, 5):
+        raise ValueError("a cache's k must be a ([layers,] pages, Hkv, page, D) tensor of bfloat16, int8 or float8_e4m3fn")
+    B = _batch(cache, starts if starts is not None else counts)
+    shape = tuple(k.shape[:-4]) + (B, T, k.shape[-3], k.shape[-1])
+    K, V = torch.empty(shape, dtype=dtype, device=k.device), torch.empty(shape, dtype=dtype, device=k.device)
+    cache_read_(K, V, cache, starts, counts)
+    return K, V
+
+
+def cache_keep_(cache: KVCache, lengths: torch.Tensor, path: torch.Tensor, counts: torch.Tensor) -> None:
+    """Keeps a path of the tokens behind ``lengths``: token ``lengths[b] + path[b, j]`` moves to
+    ``lengths[b] + j`` for j < counts[b], in every layer that the cache holds.  ``path`` (B, N)
+    int32 increases along a row, as ``verify_drafts`` gives it."""
+    c = _Buffers(cache, _batch(cache, lengths))
+    if not isinstance(path, torch.Tensor) or path.dim() != 2:
+        raise ValueError("path must be a (B, N) int32 tensor")
+    N = path.shape[1]
+    _check_tensor("path", path, (c.B, N), _I32, c.device)
+    _check_tensor("lengths", lengths, (c.B,), _I32, c.device)
+    _check_tensor("counts", counts, (c.B,), _I32, c.device)
+    if N == 0:
+        return
+    _call(c.device, _lib.lib().fc_cache_keep, ctypes.byref(c.desc), ctypes.byref(c.pointers), N, lengths.data_ptr(),
+          path.data_ptr(), counts.data_ptr())
+
+
+@lru_cache(maxsize=256)
+def _workspace_bytes(D, Hkv, B, P, S, M, kind, H, N, left) -> int:
+    n = ctypes.c_size_t(0)
+    _lib.check(_lib.lib().fc_cached_attn_workspace_bytes(
+        ctypes.byref(_lib.CacheDesc(D, Hkv, B, 1, P, S, M, kind)),
+        ctypes.byref(_lib.CachedAttnOptions(H, N, left, 0, 0.0, None)), ctypes.byref(n)))
+    return n.value
+
+
+def _left(window) -> int:
+    left, right = window
+    if int(right) != 0 or int(left) < -1:
+        raise ValueError(f"a window over a cache is (left, 0), or (-1, 0) for all tokens, got {tuple(window)}")
+    return int(left)
+
+
+def _options(c: _Buffers, N: int, H: int, window, parents, softcap, slopes) -> _lib.CachedAttnOptions:
+    tree = 0
+    if parents is not None:
+        tree = 2 if isinstance(parents, torch.Tensor) and parents.dim() == 2 else 1
+        _check_tensor("parents", parents, (c.B, N) if tree == 2 else (N,), _I32, c.device)
+    if slopes is not None:
+        _check_tensor("slopes", slopes, (H,), (torch.float32,), c.device)
+    return _lib.CachedAttnOptions(H, N, _left(window), tree, float(softcap), _ptr(slopes))
+
+
+def _bytes(c: _Buffers, o: _lib.CachedAttnOptions) -> int:
+    d = c.desc
+    return _workspace_bytes(d.D, d.Hkv, d.B, d.pages, d.page_size, d.max_pages, d.type, o.H, o.N, o.left)
+
+
+def cached_attention_workspace_bytes(Q: torch.Tensor, cache: KVCache, window=(-1, 0)) -> int:
+    """Bytes of the caller-owned workspace ``cached_attention_(…, workspace=)`` accepts (the
+    library's requirement plus 256 bytes of alignment slack; 0 when the problem needs none)."""
+    if not isinstance(Q, torch.Tensor) or Q.dim() != 4:
+        raise ValueError("Q must have shape (B, N, H, D)")
+    c = _Buffers(cache, Q.shape[0])
+    n = _bytes(c, _lib.CachedAttnOptions(Q.shape[2], Q.shape[1], _left(window), 0, 0.0, None))
+    return n + 256 if n > 0 else 0
+
+
+def cached_attention_(O: torch.Tensor, Q: torch.Tensor, cache: KVCache, lengths: torch.Tensor,
+                      window: Tuple[int, int] = (-1, 0), *, counts: Optional[torch.Tensor] = None,
+                      parents: Optional[torch.Tensor] = None, softcap: float = 0.0,
+                      slopes: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> None:
+    """``cached_attention`` into the caller's O (bfloat16, as Q)."""
+    if not isinstance(Q, torch.Tensor) or Q.dim() != 4:
+        raise ValueError("Q must have shape (B, N, H, D)")
+    B, N, H, D = Q.shape
+    c = _Buffers(cache, B)
+    shape = (B, N, H, c.D)
+    _check_tensor("Q", Q, shape, (torch.bfloat16,), c.device)
+    _check_tensor("O", O, shape, (torch.bfloat16,), c.device)
+    _check_tensor("lengths", lengths, (B,), _I32, c.device)
+    _check_counts(c, None, counts)
+    if O.data_ptr() % 16:
+        raise ValueError("O must start on a 16-byte boundary")
+    o = _options(c, N, H, window, parents, softcap, slopes)
+    nbytes = _bytes(c, o)
+    at = None
+    if nbytes > 0:
+        if workspace is None:  # freed to this stream's pool on return, so later work on the stream comes after the kernels
+            workspace = torch.empty(nbytes + 256, dtype=torch.uint8, device=c.device)
+        else:
+            _check_workspace(workspace, nbytes + 256, c.device)
+        at = (workspace.data_ptr() + 255) & ~255
+    Q = _aligned(Q)
+    _call(c.device, _lib.lib().fc_cached_attn, ctypes.byref(c.desc), ctypes.byref(c.pointers), ctypes.byref(o), Q.data_ptr(),
+          O.data_ptr(), lengths.data_ptr(), _ptr(counts), _ptr(parents), at, nbytes)
+
+
+def cached_attention(Q: torch.Tensor, cache: KVCache, lengths: torch.Tensor, window: Tuple[int, int] = (-1, 0), *,
+                     counts: Optional[torch.Tensor] = None, parents: Optional[torch.Tensor] = None, softcap: float = 0.0,
+                     slopes: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the newest tokens over one layer's cache: Q (B, N, H, D), N from 1 to 64, for
+    the tokens that ``cache_write_`` has put behind ``lengths``; bfloat16, or float32 or float16
+    that is rounded to it, and the result in the same type.
+
+    Each token sees the cache's and the new ones before it, or with ``parents`` (int32, (N,) or
+    (B, N)) the cache's and its ancestors: a drafted node's parent is a node before it, -1 where
+    it follows the sequence itself.  ``window`` (left, 0), ``softcap`` and ``slopes`` are those of
+    ``attention``, over positions in the text (a node's is ``lengths[b]`` plus its ancestors).
+    Nodes from ``counts[b]`` on get zeros; one beyond the cache's capacity, or whose
+    parents are no tree's, gets NaN."""
+    if isinstance(Q, torch.Tensor) and Q.dtype in (torch.float32, torch.float16):
+        x = Q.to(torch.bfloat16)
+        O = torch.empty_like(x)
+        cached_attention_(O, x, cache, lengths, window, counts=counts, parents=parents, softcap=softcap, slopes=slopes,
+                          workspace=workspace)
+        return O.to(Q.dtype)
+    O = torch.empty_like(Q)
+    cached_attention_(O, Q, cache, lengths, window, counts=counts, parents=parents, softcap=softcap, slopes=slopes,
+                      workspace=workspace)
+    return O

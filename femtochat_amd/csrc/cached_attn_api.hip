@@ -1,0 +1,146 @@
+// Attention over a cache: the entry points, the rules that size a call, and the
+// join of a sequence's parts.
+#include "cached_attn.hpp"
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <cstdio>
+
+namespace fc {
+
+hipError_t launch_cached_attn_join(const CachedAttnArgs& a, int rows_per_group, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)a.g.B * a.N * a.H));
+  const ProfileMark mk = profile_begin(s);
+  switch (a.g.D) {
+    case 16: hipLaunchKernelGGL(cached_attn_join_kernel<16>, grid, dim3(256), 0, s, a, rows_per_group); break;
+    case 32: hipLaunchKernelGGL(cached_attn_join_kernel<32>, grid, dim3(256), 0, s, a, rows_per_group); break;
+    case 48: hipLaunchKernelGGL(cached_attn_join_kernel<48>, grid, dim3(256), 0, s, a, rows_per_group); break;
+    case 64: hipLaunchKernelGGL(cached_attn_join_kernel<64>, grid, dim3(256), 0, s, a, rows_per_group); break;
+    case 80: hipLaunchKernelGGL(cached_attn_join_kernel<80>, grid, dim3(256), 0, s, a, rows_per_group); break;
+    case 96: hipLaunchKernelGGL(cached_attn_join_kernel<96>, grid, dim3(256), 0, s, a, rows_per_group); break;
+    case 112: hipLaunchKernelGGL(cached_attn_join_kernel<112>, grid, dim3(256), 0, s, a, rows_per_group); break;
+    default: hipLaunchKernelGGL(cached_attn_join_kernel<128>, grid, dim3(256), 0, s, a, rows_per_group); break;
+  }
+  const hipError_t e = hipGetLastError();
+  profile_end(mk, "cached_attn_join", s);
+  return e;
+}
+
+namespace {
+
+fc_status bad(const char* who, const char* what, fc_status code = FC_ERR_INVALID_ARGUMENT) {
+  char msg[256];
+  snprintf(msg, sizeof(msg), "%s: %s", who, what);
+  return set_error(code, msg);
+}
+bool off(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; }
+
+constexpr int kLeastTiles = 8;      // of a slot: two per wave
+constexpr int kSlotsPerLaunch = 1024;  // four workgroups per CU
+
+// The sizes of a call that follow from its descriptor alone (not from the lengths,
+// which lie on the device).
+struct Plan {
+  int row_blocks, groups, share, items;
+  bool parts;          // a sequence may have several slots
+  size_t o_bytes, s_bytes;
+};
+
+Plan plan_of(const CacheGeom& g, int H, int N, int left) {
+  Plan p;
+  const int rows = H / g.Hkv * N;
+  const int most = g.type == FC_CACHE_BF16 && g.D > 64 ? 2 : 4;
+  p.row_blocks = rows <= 16 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
+  p.groups = (rows + 16 * p.row_blocks - 1) / (16 * p.row_blocks);
+  p.share = std::max(1, std::min(1024, kSlotsPerLaunch / (g.Hkv * p.groups)));
+  // A sequence's tiles, at most: one slot holds them all where these are few.
+  const int64_t span = std::min<int64_t>(g.capacity, (int64_t)left + N + kTileKeys);
+  p.parts = (span + kTileKeys - 1) / kTileKeys + 1 > kLeastTiles;
+  p.items = p.parts ? p.share + g.B : g.B;
+  if (!p.parts) p.share = 1;
+  const int64_t slots = p.parts ? (int64_t)g.Hkv * p.groups * p.items * 16 * p.row_blocks : 0;
+  p.o_bytes = (size_t)slots * g.D * 4;
+  p.s_bytes = (size_t)slots * sizeof(float2);
+  return p;
+}
+
+fc_status options_of(const char* who, const CacheGeom& g, const fc_cached_attn_options* o) {
+  if (o == nullptr) return bad(who, "options are null");
+  if (g.layers != 1) return bad(who, "attention takes one layer's cache");
+  if (o->H <= 0 || o->H % g.Hkv != 0) return bad(who, "H must be a multiple of Hkv");
+  if (o->H / g.Hkv > 1024) return bad(who, "at most 1024 query heads per KV head", FC_ERR_UNSUPPORTED);
+  if (o->N < 1 || o->N > kMaxNodes) return bad(who, "a call takes 1 to 64 new tokens", o->N < 1 ? FC_ERR_INVALID_ARGUMENT : FC_ERR_UNSUPPORTED);
+  if (o->left < -1) return bad(who, "left must be -1 (all) or at least 0");
+  if (o->tree < 0 || o->tree > 2) return bad(who, "unknown kind of tree");
+  if (!(o->softcap == 0.0f || (o->softcap >= 0x1p-10f && o->softcap <= 4096.0f)))
+    return bad(who, "softcap must be 0 (none) or from 2^-10 to 4096");
+  if (off(o->slopes, 4)) return bad(who, "slopes must be 4-byte aligned");
+  if ((int64_t)g.B * o->N * o->H > (int64_t)1 << 24) return bad(who, "at most 2^24 rows (sequences times new tokens times heads)", FC_ERR_UNSUPPORTED);
+  return FC_OK;
+}
+int left_of(const fc_cached_attn_options* o) { return o->left < 0 ? INT_MAX / 2 : std::min(o->left, INT_MAX / 2); }
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+}  // namespace fc
+
+extern "C" {
+
+fc_status fc_cached_attn_workspace_bytes(const fc_cache_desc* desc, const fc_cached_attn_options* options, size_t* bytes) {
+  const char* who = "fc_cached_attn_workspace_bytes";
+  fc::CacheGeom g;
+  char msg[200];
+  fc_status st = fc::make_cache(desc, &g, msg, sizeof(msg));
+  if (st != FC_OK) return fc::bad(who, msg, st);
+  if ((st = fc::options_of(who, g, options)) != FC_OK) return st;
+  if (bytes == nullptr) return fc::bad(who, "bytes is null");
+  const fc::Plan p = fc::plan_of(g, options->H, options->N, fc::left_of(options));
+  *bytes = fc::round256(p.o_bytes) + fc::round256(p.s_bytes);
+  fc::clear_error();
+  return FC_OK;
+}
+
+fc_status fc_cached_attn(const fc_cache_desc* desc, const fc_cache* cache, const fc_cached_attn_options* options,
+                         const void* Q, void* O, const int32_t* lengths, const int32_t* counts, const int32_t* parents,
+                         void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "fc_cached_attn";
+  fc::CachedAttnArgs a{};
+  fc_status st = fc::check_cache(who, desc, cache, &a.g);
+  if (st != FC_OK) return st;
+  if ((st = fc::options_of(who, a.g, options)) != FC_OK) return st;
+  if (Q == nullptr || O == nullptr || lengths == nullptr) return fc::bad(who, "a required pointer is null");
+  if ((options->tree != 0) != (parents != nullptr)) return fc::bad(who, "parents and the kind of tree do not agree");
+  if (fc::off(Q, 16) || fc::off(O, 16)) return fc::bad(who, "Q and O must be 16-byte aligned");
+  if (fc::off(lengths, 4) || fc::off(counts, 4) || fc::off(parents, 4)) return fc::bad(who, "integer buffers must be 4-byte aligned");
+  const int left = fc::left_of(options);
+  const fc::Plan p = fc::plan_of(a.g, options->H, options->N, left);
+  const size_t need = fc::round256(p.o_bytes) + fc::round256(p.s_bytes);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return fc::bad(who, "the workspace is missing or too small", FC_ERR_WORKSPACE);
+  if (need > 0 && fc::off(workspace, 256)) return fc::bad(who, "the workspace must be 256-byte aligned", FC_ERR_WORKSPACE);
+  a.k = cache->k, a.v = cache->v, a.k_scale = cache->k_scale, a.v_scale = cache->v_scale;
+  a.table = desc->max_pages > 0 ? cache->table : nullptr;
+  a.Q = Q, a.O = O, a.lengths = lengths, a.counts = counts, a.parents = parents, a.slopes = options->slopes;
+  a.part_o = reinterpret_cast<float*>(workspace);
+  a.part_s = reinterpret_cast<float2*>(static_cast<char*>(workspace) + fc::round256(p.o_bytes));
+  a.H = options->H, a.N = options->N, a.G = options->H / desc->Hkv, a.rows = a.G * a.N;
+  a.left = left, a.tree = options->tree;
+  a.groups = p.groups, a.items = p.items, a.share = p.share, a.least = p.parts ? fc::kLeastTiles : 1 << 30;
+  const double scale = 1.0 / std::sqrt((double)desc->D);
+  a.scale_log2 = (float)(1.4426950408889634 * scale);
+  if (options->softcap > 0.0f) {
+    a.cap_in = (float)(2.0 * 1.4426950408889634 * scale / (double)options->softcap);
+    a.cap_out = (float)(1.4426950408889634 * options->softcap);
+  }
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  hipError_t e = desc->type == FC_CACHE_BF16 ? fc::launch_cached_attn<FC_CACHE_BF16>(a, p.row_blocks, s)
+                 : desc->type == FC_CACHE_I8 ? fc::launch_cached_attn<FC_CACHE_I8>(a, p.row_blocks, s)
+                                             : fc::launch_cached_attn<FC_CACHE_F8>(a, p.row_blocks, s);
+  if (e == hipSuccess && p.parts) e = fc::launch_cached_attn_join(a, 16 * p.row_blocks, s);
+  if (e != hipSuccess) return fc::bad(who, hipGetErrorString(e), FC_ERR_HIP);
+  fc::clear_error();
+  return FC_OK;
+}
+
+}  // extern "C"
