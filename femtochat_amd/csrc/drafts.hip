@@ -1,20 +1,24 @@
 // Verification of drafted tokens against the target's logits, from given random
 // numbers (gfx950).
 //
-// What is drawn is a comparison of u with ratios of exponentials of the logits, and
-// the place of u's share among the vocabulary's cumulative weights, of which one in
-// V lies next to any u: so exponentials, sums and weights are float64 (a float32
-// sum would draw another token about once in a hundred rows of 2^15), and the
-// exponential is a polynomial of 2^f, f in [-1/2, 1/2], within 2^-47 (v_exp_f32 has
-// 2^-22).
+// The next token is the place of u's share among the vocabulary's cumulative weights,
+// of which one in V lies next to any u: those are exponentials and sums in float64 (in
+// float32 another token would be drawn about once in a hundred rows of 2^15).  An
+// acceptance is one comparison of u with a ratio of two probabilities, for which
+// float32 exponentials summed in float64 (1e-7) are enough.  float64 operations are what
+// costs here, not the bytes (22 us of them for 704 rows of 2^15 bf16 logits that
+// are read in 10), so they are kept for the row where a sequence's walk ends.
 //
 //  * draft_stats_kernel reads every row of logits (target and draft) once: each
 //    workgroup leaves a chunk's maximum and the sum of its exponentials.
-//  * draft_walk_kernel, a workgroup per sequence and chunk: one wave takes a node per
-//    lane, tests all of them at once and follows the accepted ones from the root;
-//    then the workgroup sums the weights of its chunk of the row where the walk ended.
-//  * draft_pick_kernel finds the chunk that u's share falls into and the token in it.
-// The first is bound by HBM, the others are a few microseconds of latency.
+//  * draft_pick_kernel, a workgroup per sequence and chunk: one wave takes a node per
+//    lane, tests all of them at once and follows the accepted ones from the root; the
+//    workgroup sums the weights of its chunk of the row where the walk ended; and the last
+//    one of a sequence to get there (the first kernel zeroed their counter) finds the part
+//    that u's share falls into and the token in it.
+//  * With the drafts' distributions a weight is p - q, whose two sums have to be there
+//    first: draft_walk_kernel, before the pick, walks and forms them.
+//  * Vocabularies of up to 2048 run whole in draft_small_kernel, a workgroup per sequence.
 #include "attn_device.hpp"
 #include "attn_launch.hpp"
 
@@ -35,7 +39,7 @@ constexpr int kPerThread = kChunkValues / kDraftThreads;
 
 // A chunk's part of a row's softmax, or of its largest value.
 struct ChunkStat {
-  float most;  // largest logit
+  float most;  // largest logit, NaN where there is one
   int index;   // temperature 0: its first index, -1 where the chunk holds a NaN or +infinity
   double sum;  // of exp((x - most) / temperature)
 };
@@ -48,6 +52,7 @@ struct RowStat {
 struct Walk {
   int last;         // node, -1: nothing is kept
   int residual;     // draws: weights max(p - q, 0)
+  int next;         // temperature 0
   uint64_t struck;  // candidates: the nodes whose tokens were tried there
   RowStat p, q;
 };
@@ -60,34 +65,53 @@ struct DraftArgs {
   const int32_t *parents, *counts;
   int32_t *path, *kept, *next;
   ChunkStat* stats;  // [B N target rows, B (N - 1) draft rows][chunks]
-  Walk* walks;       // [B]
-  double* sums;      // [B][chunks], of the weights
+  Walk* walks;       // [B] (draws)
+  double2* both;     // [B][chunks][kParts]: sums of the two exponentials (draws)
+  double* sums;      // [B][chunks][kParts], of the weights
+  int32_t* arrived;  // [B]: workgroups of the pick that left their sums
   int B, N, V, chunks;
   int index64, tree;
   double to_log2;    // log2(e) / temperature
 };
 
 template <typename E> constexpr int kPiece = 16 / (int)sizeof(E);
+constexpr int kParts = 4;                            // of a chunk: a wave's values
+constexpr int kPartValues = kChunkValues / kParts;   // 2048
 
-// exp of (x - most) / temperature, x <= most: 0 for -infinity, NaN where either is no number.
-__device__ inline double weight_of(float x, float most, double to_log2) {
-  if (x == -INFINITY) return 0.0;
-  double t = ((double)x - (double)most) * to_log2;
-  t = t < -1080.0 ? -1080.0 : t;
-  const double n = __builtin_rint(t), z = (t - n) * 0.69314718055994530942;
-  double e = 1.0 / 39916800.0;  // Taylor's sum up to z^11: |z| <= ln(2) / 2 leaves 2^-47 of the value
-  e = __builtin_fma(e, z, 1.0 / 3628800.0);
-  e = __builtin_fma(e, z, 1.0 / 362880.0);
-  e = __builtin_fma(e, z, 1.0 / 40320.0);
-  e = __builtin_fma(e, z, 1.0 / 5040.0);
-  e = __builtin_fma(e, z, 1.0 / 720.0);
-  e = __builtin_fma(e, z, 1.0 / 120.0);
-  e = __builtin_fma(e, z, 1.0 / 24.0);
-  e = __builtin_fma(e, z, 1.0 / 6.0);
-  e = __builtin_fma(e, z, 0.5);
-  e = __builtin_fma(e, z, 1.0);
-  e = __builtin_fma(e, z, 1.0);
-  return __builtin_ldexp(e, (int)n);
+// exp((x - most) / temperature) for x <= most.  2^t = 2^n 2^f, n the nearest whole number
+// (its bits come from adding 1.5 2^52) and f in [-1/2, 1/2]: a polynomial of degree 10 through
+// the Chebyshev points, within 2^-51 (v_exp_f32 has 2^-22); 17 instructions.
+struct Exponent {
+  double to_log2, most2;  // log2(e) / temperature, most times that
+  float low;              // logits below it have no weight: 2^-1000
+};
+__device__ inline Exponent exponent_of(float most, double to_log2) {
+  return Exponent{to_log2, (double)most * to_log2, (float)((double)most - 1000.0 / to_log2)};
+}
+__device__ inline float nan_max(float x, float y) { return __builtin_elementwise_maximum(x, y); }
+// A logit without weight has 2^-1000, which a sum does not notice (weight_of: 0).
+__device__ inline double term_of(float x, const Exponent& e) {
+  const double t = __builtin_fma((double)nan_max(x, e.low), e.to_log2, -e.most2);
+  const double s = t + 0x1.8p52, f = t - (s - 0x1.8p52);
+  double v = 0x1.e6064532b85cep-28;
+  v = __builtin_fma(v, f, 0x1.b675bd731322bp-24);
+  v = __builtin_fma(v, f, 0x1.62bfd472702f4p-20);
+  v = __builtin_fma(v, f, 0x1.ffcb5405401d9p-17);
+  v = __builtin_fma(v, f, 0x1.4309130972597p-13);
+  v = __builtin_fma(v, f, 0x1.5d87fe9d7ab38p-10);
+  v = __builtin_fma(v, f, 0x1.3b2ab6fba1dcfp-7);
+  v = __builtin_fma(v, f, 0x1.c6b08d703ce45p-5);
+  v = __builtin_fma(v, f, 0x1.ebfbdff82c598p-3);
+  v = __builtin_fma(v, f, 0x1.62e42fefa3a19p-1);
+  v = __builtin_fma(v, f, 1.0);
+  const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+  const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, s);
+  // (a NaN's n is a multiple of 2^29: it stays one)
+  return __builtin_bit_cast(double, (uint64_t)((uint32_t)(bits >> 32) + (n << 20)) << 32 | (uint32_t)bits);
+}
+__device__ inline double weight_of(float x, const Exponent& e) {
+  const double v = term_of(x, e);
+  return x <= e.low ? 0.0 : v;
 }
 
 // The values of the row from element e on, as many as 16 bytes hold; -infinity outside
@@ -120,6 +144,16 @@ __device__ inline double wave_sum(double v) {
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
   return v;
 }
+// Sums of the lanes up to each.
+__device__ inline double wave_scan(double v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double s = __shfl_up(v, o);
+    if (lane >= o) v += s;
+  }
+  return v;
+}
 
 // One chunk of one row.
 template <typename E, bool kGreedy>
@@ -129,6 +163,7 @@ __global__ __launch_bounds__(kDraftThreads) void draft_stats_kernel(DraftArgs a)
   __shared__ int index4[4];
   __shared__ double sum4[4];
   const int tid = threadIdx.x, wave = tid >> 6;
+  if (tid == 0 && blockIdx.x < (unsigned)a.B) a.arrived[blockIdx.x] = 0;
   const int r = blockIdx.x / a.chunks, chunk = blockIdx.x - r * a.chunks;
   const int targets = a.B * a.N;
   const E* row = r < targets ? static_cast<const E*>(a.logits) + (int64_t)r * a.V
@@ -137,43 +172,42 @@ __global__ __launch_bounds__(kDraftThreads) void draft_stats_kernel(DraftArgs a)
   float x[kRounds][P];
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) load_piece(row, a.V, first + k * kDraftThreads * P, x[k]);
-  float m = -INFINITY;
+  float all = -INFINITY;
 #pragma unroll
   for (int k = 0; k < kRounds; ++k)
 #pragma unroll
-    for (int i = 0; i < P; ++i) m = fmaxf(m, x[k][i]);
-  float all = m;
+    for (int i = 0; i < P; ++i) all = nan_max(all, x[k][i]);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor(all, o));
+  for (int o = 32; o > 0; o >>= 1) all = nan_max(all, __shfl_xor(all, o));
   if ((tid & 63) == 0) most4[wave] = all;
   __syncthreads();
-  all = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3]));
+  all = nan_max(nan_max(most4[0], most4[1]), nan_max(most4[2], most4[3]));
   ChunkStat out;
   out.most = all;
   out.index = INT_MAX;
   out.sum = 0.0;
   if (kGreedy) {
     int at = INT_MAX;
-    bool bad = all == INFINITY;
 #pragma unroll
     for (int k = kRounds - 1; k >= 0; --k)
 #pragma unroll
-      for (int i = P - 1; i >= 0; --i) {
+      for (int i = P - 1; i >= 0; --i)
         if (x[k][i] == all && all != -INFINITY) at = first + k * kDraftThreads * P + i;
-        bad |= x[k][i] != x[k][i];
-      }
-    at = bad ? -1 : at;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o));
     if ((tid & 63) == 0) index4[wave] = at;
     __syncthreads();
-    out.index = min(min(index4[0], index4[1]), min(index4[2], index4[3]));
-  } else {
+    out.index = all != all || all == INFINITY ? -1 : min(min(index4[0], index4[1]), min(index4[2], index4[3]));
+  } else if (all != -INFINITY) {
+    const float c = (float)a.to_log2;
     double s = 0.0;
 #pragma unroll
-    for (int k = 0; k < kRounds; ++k)
+    for (int k = 0; k < kRounds; ++k) {
+      float t = 0.0f;
 #pragma unroll
-      for (int i = 0; i < P; ++i) s += weight_of(x[k][i], all, a.to_log2);
+      for (int i = 0; i < P; ++i) t += __builtin_amdgcn_exp2f((x[k][i] - all) * c);
+      s += (double)t;
+    }
     s = wave_sum(s);
     if ((tid & 63) == 0) sum4[wave] = s;
     __syncthreads();
@@ -184,14 +218,19 @@ __global__ __launch_bounds__(kDraftThreads) void draft_stats_kernel(DraftArgs a)
 
 __device__ inline RowStat row_stat(const DraftArgs& a, int64_t row) {
   const ChunkStat* st = a.stats + row * a.chunks;
-  RowStat r;
-  r.most = -INFINITY;
-  for (int c = 0; c < a.chunks; ++c) r.most = fmaxf(r.most, st[c].most);
-  r.sum = 0.0;
-  for (int c = 0; c < a.chunks; ++c) {
-    const ChunkStat s = st[c];
-    // (a chunk of -infinities has the sum 0, or NaN where it holds one)
-    r.sum += s.most == -INFINITY ? s.sum : s.sum * weight_of(s.most, r.most, a.to_log2);
+  const float to_log2 = (float)a.to_log2;
+  RowStat r{-INFINITY, 0.0};
+  for (int c0 = 0; c0 < a.chunks; c0 += 8) {
+    ChunkStat s[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) s[c] = c0 + c < a.chunks ? st[c0 + c] : ChunkStat{-INFINITY, 0, 0.0};
+    const float before = r.most;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) r.most = nan_max(r.most, s[c].most);
+    if (before != -INFINITY) r.sum *= (double)__builtin_amdgcn_exp2f((before - r.most) * to_log2);
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (s[c].most != -INFINITY) r.sum += s[c].sum * (double)__builtin_amdgcn_exp2f((s[c].most - r.most) * to_log2);
   }
   return r;
 }
@@ -212,70 +251,87 @@ __device__ inline int row_best(const DraftArgs& a, int64_t row) {
 __device__ inline int64_t token_at(const DraftArgs& a, int64_t i) {
   return a.index64 ? static_cast<const int64_t*>(a.tokens)[i] : static_cast<const int32_t*>(a.tokens)[i];
 }
-__device__ inline double shfl64(double v, int from) { return __shfl(v, from); }
+__device__ inline double read_lane(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)u, lane), hi = __builtin_amdgcn_readlane((uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+__device__ inline RowStat stat_at(const RowStat& s, int lane) {  // lane: any, of 64
+  return RowStat{__shfl(s.most, lane), __shfl(s.sum, lane)};
+}
 
 // Sequence b's walk, by one whole wave, a node per lane; the same in every lane.
+// kGreedy: best is the index of the largest logit of the lane's row; else p (and with
+// draft_logits q) that row's softmax.
 template <typename E, bool kGreedy>
-__device__ inline Walk walk_nodes(const DraftArgs& a, int b, bool write) {
+__device__ inline Walk walk_nodes(const DraftArgs& a, int b, bool write, int best, const RowStat& row_p, const RowStat& row_q) {
   const int i = threadIdx.x & 63;
+  const bool node = i >= 1 && i < a.N;
   const int count = a.counts == nullptr ? a.N : min(max(a.counts[b], 0), a.N);
-  const bool there = i >= 1 && i < count;
+  const int64_t token = node ? token_at(a, (int64_t)b * a.N + i) : -1;
   int up = i - 1;
-  if (a.parents != nullptr && there) up = a.parents[(a.tree == 2 ? (int64_t)b * a.N : 0) + i];
-  const bool linked = there && up >= 0 && up < i;
-  const int64_t token = there ? token_at(a, (int64_t)b * a.N + i) : -1;
-  const bool known = linked && token >= 0 && token < a.V;
+  if (a.parents != nullptr && node) up = a.parents[(a.tree == 2 ? (int64_t)b * a.N : 0) + i];
+  const double u = !kGreedy && node ? (double)a.u[(int64_t)b * a.N + i] : 1.0;
+  const bool known = node && i < count && up >= 0 && up < i && token >= 0 && token < a.V;
   const int64_t row = (int64_t)b * a.N + up;
-  bool chosen = false;
+  bool chosen = false;  // tested by itself: all but candidates, whose test depends on those before them
+  double p = 0.0;
   if (kGreedy) {
-    chosen = known && row_best(a, row) == (int)token;
+    chosen = __shfl(best, known ? up : 0) == (int)token && known;
   } else {
-    double p = 0.0, q = 0.0;
+    const RowStat st = stat_at(row_p, known ? up : 0), dt = a.draft != nullptr ? stat_at(row_q, known ? up : 0) : st;
     if (known) {
-      const RowStat st = row_stat(a, row);
-      p = weight_of(static_cast<float>(static_cast<const E*>(a.logits)[row * a.V + token]), st.most, a.to_log2) / st.sum;
-      if (a.draft != nullptr) {
-        const int64_t drow = (int64_t)b * (a.N - 1) + up;
-        const RowStat dt = row_stat(a, (int64_t)a.B * a.N + drow);
-        q = weight_of(static_cast<float>(static_cast<const E*>(a.draft)[drow * a.V + token]), dt.most, a.to_log2) / dt.sum;
-      }
-    }
-    const double u = there ? (double)a.u[(int64_t)b * a.N + i] : 1.0;
-    if (a.draft != nullptr) {
-      chosen = known && u * q < p;
-    } else {
-      // Siblings before this node: whether one has its token, and what they have of p.
-      bool again = false;
-      const int token32 = (int)token;
-      for (int j = 1; j < count; ++j) {
-        const int uj = __shfl(up, j), tj = __shfl(token32, j), kj = __shfl((int)known, j);
-        again |= j < i && kj != 0 && uj == up && tj == token32;
-      }
-      double left = 1.0;
-      for (int j = 1; j < count; ++j) {
-        const int uj = __shfl(up, j), fresh = __shfl((int)(known && !again), j);
-        const double pj = shfl64(p, j);
-        left -= j < i && fresh != 0 && uj == up ? pj : 0.0;
-      }
-      chosen = known && !again && u * left < p;
+      const float x = static_cast<float>(static_cast<const E*>(a.logits)[row * a.V + token]);
+      float d = 0.0f;
+      if (a.draft != nullptr) d = static_cast<float>(static_cast<const E*>(a.draft)[((int64_t)b * (a.N - 1) + up) * a.V + token]);
+      p = weight_of(x, exponent_of(st.most, a.to_log2)) / st.sum;
+      if (a.draft != nullptr) chosen = u * (weight_of(d, exponent_of(dt.most, a.to_log2)) / dt.sum) < p;
     }
   }
   // From the root to the first accepted child, and on.
+  const int token32 = (int)token;
   Walk w;
   w.last = count > 0 ? 0 : -1;
-  w.residual = 0, w.struck = 0;
-  w.p = w.q = RowStat{-INFINITY, 0.0};
+  w.struck = 0;
   int kept = count > 0 ? 1 : 0, mine = -1;  // path[lane]
   if (i == 0 && count > 0) mine = 0;
   while (w.last >= 0) {
-    const uint64_t hit = __ballot(chosen && up == w.last);
+    const uint64_t children = __ballot(known && up == w.last);
+    uint64_t hit = kGreedy || a.draft != nullptr ? __ballot(chosen) & children : 0;
+    if (!kGreedy && a.draft == nullptr) {
+      // In order, each against what those before it have left of p; a token that was tried is not taken.
+      double left = 1.0;
+      uint64_t tried = 0;
+      for (uint64_t todo = children; todo != 0; todo &= todo - 1) {
+        const int j = __ffsll((long long)todo) - 1;
+        if (__ballot((tried >> i & 1) != 0 && token32 == __builtin_amdgcn_readlane(token32, j)) != 0) continue;
+        const double pj = read_lane(p, j);
+        if (read_lane(u, j) * left < pj) {
+          hit = 1ull << j;
+          break;
+        }
+        left -= pj;
+        tried |= 1ull << j;
+      }
+      w.struck = hit == 0 ? children : 0;
+    }
     if (hit == 0) break;
     w.last = __ffsll((long long)hit) - 1;
     if (i == kept) mine = w.last;
     ++kept;
   }
-  w.struck = a.draft == nullptr ? __ballot(known && up == w.last) : 0;
   w.residual = a.draft != nullptr && kept < count;
+  w.next = -1;
+  w.p = w.q = RowStat{-INFINITY, 0.0};
+  if (w.last >= 0) {
+    if (kGreedy) {
+      w.next = __shfl(best, w.last);
+    } else {
+      w.p = stat_at(row_p, w.last);
+      if (w.residual) w.q = stat_at(row_q, w.last);
+    }
+  }
   if (write) {
     if (i < a.N) a.path[(int64_t)b * a.N + i] = mine;
     if (i == 0) a.kept[b] = kept;
@@ -283,7 +339,61 @@ __device__ inline Walk walk_nodes(const DraftArgs& a, int b, bool write) {
   return w;
 }
 
-// Which of a chunk's values are struck out: a bit each, from element `first` of the row on.
+// What the weights of a row come from.
+template <typename E>
+struct Weights {
+  const E *row, *draft;  // draft: residual, else null
+  Exponent p, q;
+  double ip, iq;         // residual: 1 / sum
+  int V;
+  bool alike;            // the two rows lie alike against 16 bytes
+};
+template <typename E>
+__device__ inline Weights<E> weights_of(const DraftArgs& a, const Walk& w, int b) {
+  Weights<E> r;
+  r.row = static_cast<const E*>(a.logits) + ((int64_t)b * a.N + w.last) * a.V;
+  r.draft = w.residual ? static_cast<const E*>(a.draft) + ((int64_t)b * (a.N - 1) + w.last) * a.V : nullptr;
+  r.p = exponent_of(w.p.most, a.to_log2);
+  r.q = exponent_of(w.q.most, a.to_log2);
+  r.ip = r.iq = 1.0;
+  r.V = a.V;
+  r.alike = row_head(r.row) == row_head(r.draft);
+  return r;
+}
+
+// The weights of the piece at element e: p (times its sum), less q where the row is a residual's, and 0
+// where bits (null: none) strike a value out; bits begin at element `first`.
+template <typename E>
+__device__ inline void weights(const Weights<E>& w, const uint32_t* bits, int first, int e, double (&out)[kPiece<E>]) {
+  constexpr int P = kPiece<E>;
+  float x[P], d[P];
+  load_piece(w.row, w.V, e, x);
+  if (w.draft != nullptr) {
+    if (w.alike) {
+      load_piece(w.draft, w.V, e, d);
+    } else {
+#pragma unroll
+      for (int i = 0; i < P; ++i) d[i] = e + i >= 0 && e + i < w.V ? static_cast<float>(w.draft[e + i]) : -INFINITY;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < P; ++i) out[i] = weight_of(x[i], w.p);
+  if (w.draft != nullptr) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const double rest = __builtin_fma(out[i], w.ip, -(weight_of(d[i], w.q) * w.iq));
+      out[i] = rest <= 0.0 ? 0.0 : rest;  // (NaN stays)
+    }
+  } else if (bits != nullptr) {
+    const int at = e - first;
+    const uint32_t struck = bits[at >> 5] >> (at & 31);
+#pragma unroll
+    for (int i = 0; i < P; ++i) out[i] = (struck >> i & 1) != 0 ? 0.0 : out[i];
+  }
+}
+
+// Which of a chunk's values are struck out: a bit each, from element `first` of the row on
+// (pieces begin at multiples of their length, so one word holds a piece's).
 __device__ inline void strike(uint32_t* bits, const DraftArgs& a, int b, uint64_t struck, int first) {
   for (int i = threadIdx.x; i < kChunkValues / 32; i += kDraftThreads) bits[i] = 0;
   __syncthreads();
@@ -295,73 +405,49 @@ __device__ inline void strike(uint32_t* bits, const DraftArgs& a, int b, uint64_
   __syncthreads();
 }
 
-// The weights of the piece at element e: p, less q where the row is a residual's, and 0
-// where bits (null: none) strike a value out.
+// A wave's part of a chunk: the sum of its weights, in every lane.
 template <typename E>
-__device__ inline void weights(const DraftArgs& a, const Walk& w, const E* row, const E* drow, const uint32_t* bits, int first,
-                               int e, double (&out)[kPiece<E>]) {
+__device__ inline double part_sum(const Weights<E>& w, const uint32_t* bits, int first, int part) {
   constexpr int P = kPiece<E>;
-  float x[P];
-  load_piece(row, a.V, e, x);
-  const double ip = 1.0 / w.p.sum;
-#pragma unroll
-  for (int i = 0; i < P; ++i) out[i] = weight_of(x[i], w.p.most, a.to_log2) * ip;
-  if (drow != nullptr) {
-    const double iq = 1.0 / w.q.sum;
-    float d[P];
-    if (row_head(drow) == row_head(row)) {
-      load_piece(drow, a.V, e, d);
-    } else {  // the draft's row lies otherwise against 16 bytes: its values one by one
-#pragma unroll
-      for (int i = 0; i < P; ++i) d[i] = e + i >= 0 && e + i < a.V ? static_cast<float>(drow[e + i]) : -INFINITY;
-    }
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const double rest = out[i] - weight_of(d[i], w.q.most, a.to_log2) * iq;
-      out[i] = rest > 0.0 ? rest : rest != rest ? rest : 0.0;
-    }
-  } else if (bits != nullptr) {
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const int at = e + i - first;
-      if ((bits[at >> 5] >> (at & 31) & 1) != 0) out[i] = 0.0;
-    }
-  }
-}
-
-// Their sum over a chunk, in every thread.
-template <typename E>
-__device__ inline double chunk_sum(const DraftArgs& a, const Walk& w, const E* row, const E* drow, const uint32_t* bits, int first,
-                                   double* sum4) {
-  constexpr int P = kPiece<E>, kRounds = kPerThread / P;
-  const int tid = threadIdx.x;
+  const int lane = threadIdx.x & 63;
   double s = 0.0;
 #pragma unroll 2
-  for (int k = 0; k < kRounds; ++k) {
+  for (int k = 0; k < kPartValues / (64 * P); ++k) {
     double v[P];
-    weights<E>(a, w, row, drow, bits, first, first + (k * kDraftThreads + tid) * P, v);
+    weights<E>(w, bits, first, first + part * kPartValues + (k * 64 + lane) * P, v);
 #pragma unroll
     for (int i = 0; i < P; ++i) s += v[i];
   }
-  s = wave_sum(s);
-  __syncthreads();
-  if ((tid & 63) == 0) sum4[tid >> 6] = s;
-  __syncthreads();
-  return sum4[0] + sum4[1] + sum4[2] + sum4[3];
+  return wave_sum(s);
 }
 
+// The stats of the lane's rows, by one whole wave.
+template <bool kGreedy>
+__device__ inline void node_stats(const DraftArgs& a, int b, int* best, RowStat* p, RowStat* q) {
+  const int i = threadIdx.x & 63;
+  *best = -1;
+  *p = *q = RowStat{-INFINITY, 0.0};
+  if (i >= a.N) return;
+  if (kGreedy) {
+    *best = row_best(a, (int64_t)b * a.N + i);
+    return;
+  }
+  *p = row_stat(a, (int64_t)b * a.N + i);
+  if (a.draft != nullptr && i < a.N - 1) *q = row_stat(a, (int64_t)a.B * a.N + (int64_t)b * (a.N - 1) + i);
+}
+
+// Draws: the walk, and the sums of the two exponentials where it ended in a refusal.
 template <typename E>
 __global__ __launch_bounds__(kDraftThreads) void draft_walk_kernel(DraftArgs a) {
+  constexpr int P = kPiece<E>;
   __shared__ Walk walk;
-  __shared__ uint32_t bits[kChunkValues / 32];
-  __shared__ double sum4[4];
-  const int tid = threadIdx.x, b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
   if (tid < 64) {
-    Walk w = walk_nodes<E, false>(a, b, chunk == 0);
-    if (w.last >= 0) {
-      w.p = row_stat(a, (int64_t)b * a.N + w.last);
-      if (w.residual) w.q = row_stat(a, (int64_t)a.B * a.N + (int64_t)b * (a.N - 1) + w.last);
-    }
+    int best;
+    RowStat p, q;
+    node_stats<false>(a, b, &best, &p, &q);
+    const Walk w = walk_nodes<E, false>(a, b, chunk == 0, best, p, q);
     if (tid == 0) {
       walk = w;
       if (chunk == 0) a.walks[b] = w;
@@ -369,84 +455,151 @@ __global__ __launch_bounds__(kDraftThreads) void draft_walk_kernel(DraftArgs a) 
   }
   __syncthreads();
   const Walk w = walk;
-  if (w.last < 0) return;
-  const E* row = static_cast<const E*>(a.logits) + ((int64_t)b * a.N + w.last) * a.V;
-  const E* drow = w.residual ? static_cast<const E*>(a.draft) + ((int64_t)b * (a.N - 1) + w.last) * a.V : nullptr;
-  const int first = chunk * kChunkValues - row_head(row);
-  if (w.struck != 0) strike(bits, a, b, w.struck, first);
-  const double s = chunk_sum(a, w, row, drow, w.struck != 0 ? bits : nullptr, first, sum4);
-  if (tid == 0) a.sums[(int64_t)b * a.chunks + chunk] = s;
+  if (w.last < 0 || w.residual == 0) return;
+  const Weights<E> ws = weights_of<E>(a, w, b);
+  double sp = 0.0, sq = 0.0;
+  const auto add = [&](const E* row, const Exponent& e, double& s) {
+    const int first = chunk * kChunkValues + wave * kPartValues - row_head(row);
+#pragma unroll 2
+    for (int k = 0; k < kPartValues / (64 * P); ++k) {
+      float x[P];
+      load_piece(row, a.V, first + (k * 64 + lane) * P, x);
+#pragma unroll
+      for (int i = 0; i < P; ++i) s += term_of(x[i], e);
+    }
+  };
+  add(ws.row, ws.p, sp);
+  add(ws.draft, ws.q, sq);
+  sp = wave_sum(sp);
+  sq = wave_sum(sq);
+  if (lane == 0) a.both[((int64_t)b * a.chunks + chunk) * kParts + wave] = make_double2(sp, sq);
 }
 
-template <typename E>
+// kDraws: the walk is done.
+template <typename E, bool kDraws>
 __global__ __launch_bounds__(kDraftThreads) void draft_pick_kernel(DraftArgs a) {
-  constexpr int P = kPiece<E>, kPieces = kPerThread / P;
+  constexpr int P = kPiece<E>;
+  constexpr int kMine = kPartValues / kDraftThreads, kPieces = kMine / P;  // the pick: 8 values of a thread
+  static_assert(kMine % P == 0, "a thread's values are whole pieces");
+  __shared__ Walk walk;
   __shared__ uint32_t bits[kChunkValues / 32];
   __shared__ double sum4[4];
   __shared__ int found4[4], last4[4];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, b = blockIdx.x;
-  const Walk w = a.walks[b];
-  if (w.last < 0) {
-    if (tid == 0) a.next[b] = -1;
-    return;
-  }
-  const double* sums = a.sums + (int64_t)b * a.chunks;
-  double total = 0.0;
-  for (int c = 0; c < a.chunks; ++c) total += sums[c];
-  if (!(total >= 0.0 && total < 1e300)) {
-    if (tid == 0) a.next[b] = -1;
-    return;
-  }
-  const double u = (double)fminf(fmaxf(a.u[(int64_t)b * a.N], 0.0f), 0x1.fffffep-1f);
-  const E* row = static_cast<const E*>(a.logits) + ((int64_t)b * a.N + w.last) * a.V;
-  const E* drow = w.residual ? static_cast<const E*>(a.draft) + ((int64_t)b * (a.N - 1) + w.last) * a.V : nullptr;
-  const uint32_t* strikes = w.struck != 0 ? bits : nullptr;
-  const int head = row_head(row);
-  int chunk = 0;
-  double before = 0.0, target = u * total;
-  if (total > 0.0) {
-    for (; chunk < a.chunks - 1; ++chunk) {
-      const double upto = before + sums[chunk];
-      if (upto > target) break;
-      before = upto;
-    }
-  } else {  // nothing is left of p (it was rounded away): p itself, which sums up to 1
-    drow = nullptr, strikes = nullptr, target = u;
-    for (; chunk < a.chunks - 1; ++chunk) {
-      const double upto = before + chunk_sum(a, w, row, drow, strikes, chunk * kChunkValues - head, sum4);
-      if (upto > target) break;
-      before = upto;
+  __shared__ int is_last;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
+  const int parts = a.chunks * kParts;
+  if (!kDraws) {
+    if (tid < 64) {
+      int best;
+      RowStat p, q;
+      node_stats<false>(a, b, &best, &p, &q);
+      const Walk w = walk_nodes<E, false>(a, b, chunk == 0, best, p, q);
+      if (tid == 0) walk = w;
     }
     __syncthreads();
   }
+  // (draws: the sums come with the walk, whether it needs them or not)
+  double sp = 0.0, sq = 0.0;
+  if (kDraws) {
+    for (int i0 = 0; i0 < parts; i0 += 64) {
+      const double2 s = i0 + lane < parts ? a.both[(int64_t)b * parts + i0 + lane] : make_double2(0.0, 0.0);
+      sp += s.x;
+      sq += s.y;
+    }
+  }
+  const Walk w = kDraws ? a.walks[b] : walk;
+  // (a row with a NaN or +infinity, or of -infinities, has no sum)
+  if (w.last < 0 || !(w.p.sum > 0.0 && w.p.sum < 1e300) || (w.residual != 0 && !(w.q.sum > 0.0 && w.q.sum < 1e300))) {
+    if (chunk == 0 && tid == 0) a.next[b] = -1;
+    return;
+  }
+  Weights<E> ws = weights_of<E>(a, w, b);
+  const int head = row_head(ws.row);
+  if (kDraws && w.residual != 0) {
+    ws.ip = 1.0 / wave_sum(sp);
+    ws.iq = 1.0 / wave_sum(sq);
+  }
+  const uint32_t* strikes = w.struck != 0 ? bits : nullptr;
+  double* sums = a.sums + (int64_t)b * parts;
+  {
+    const int first = chunk * kChunkValues - head;
+    if (strikes != nullptr) strike(bits, a, b, w.struck, first);
+    const double s = part_sum(ws, strikes, first, wave);
+    if (a.chunks == 1) {
+      if (lane == 0) sum4[wave] = s;
+    } else {
+      // What the last workgroup reads is written and read at the agent's scope, past the
+      // XCDs' own caches; the wave waits for its store before the barrier, and the counter
+      // moves behind that.  (A release at that scope would write the whole L2 back.)
+      if (lane == 0) __hip_atomic_store(&sums[chunk * kParts + wave], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+  }
+  __syncthreads();
+  if (a.chunks > 1) {
+    if (tid == 0)
+      is_last = __hip_atomic_fetch_add(&a.arrived[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.chunks - 1;
+    __syncthreads();
+    if (is_last == 0) return;
+  }
+  // The last one: the part that u's share falls into.  Every wave looks by itself.
+  const auto part_at = [&](int i) {
+    return a.chunks == 1 ? sum4[i] : __hip_atomic_load(&sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
+  double total = 0.0;
+  for (int i0 = 0; i0 < parts; i0 += 64) total += wave_sum(i0 + lane < parts ? part_at(i0 + lane) : 0.0);
+  const double u = (double)fminf(fmaxf(a.u[(int64_t)b * a.N], 0.0f), 0x1.fffffep-1f);
+  double before = 0.0, target = u * total;
+  int part = parts - 1;
+  if (total > 0.0) {
+    for (int i0 = 0; i0 < parts; i0 += 64) {
+      const double upto = before + wave_scan(i0 + lane < parts ? part_at(i0 + lane) : 0.0);
+      const uint64_t hit = __ballot(upto > target);
+      if (hit != 0) {
+        const int at = __ffsll((long long)hit) - 1;
+        part = i0 + at;
+        before = at > 0 ? __shfl(upto, at - 1) : before;
+        break;
+      }
+      before = __shfl(upto, 63);
+    }
+  } else {  // nothing is left of p (it was rounded away): p itself
+    ws.draft = nullptr, strikes = nullptr;
+    for (int i = 0; i < parts; ++i) total += part_sum(ws, strikes, i / kParts * kChunkValues - head, i % kParts);
+    target = u * total;
+    for (part = 0; part < parts - 1; ++part) {
+      const double upto = before + part_sum(ws, strikes, part / kParts * kChunkValues - head, part % kParts);
+      if (upto > target) break;
+      before = upto;
+    }
+  }
   target -= before;
-  const int first = chunk * kChunkValues - head;
-  if (strikes != nullptr) strike(bits, a, b, w.struck, first);
-  // A thread's values are neighbours here, so that the order of the sum is theirs.
+  // The token in it.  A thread's values are neighbours here: the order of the sum is theirs.
+  const int first = part / kParts * kChunkValues - head;
+  if (strikes != nullptr) {
+    __syncthreads();
+    strike(bits, a, b, w.struck, first);
+  }
   double v[kPieces][P];
   double mine = 0.0;
   int last_positive = -1;
-  const int e0 = first + tid * kPerThread;
+  const int e0 = first + part % kParts * kPartValues + tid * kMine;
 #pragma unroll
   for (int k = 0; k < kPieces; ++k) {
-    weights<E>(a, w, row, drow, strikes, first, e0 + k * P, v[k]);
+    weights<E>(ws, strikes, first, e0 + k * P, v[k]);
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       mine += v[k][i];
       if (v[k][i] > 0.0) last_positive = e0 + k * P + i;
     }
   }
-  double upto = mine;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double s = __shfl_up(upto, o);
-    if (lane >= o) upto += s;
-  }
+  double upto = wave_scan(mine);
+  __syncthreads();
   if (lane == 63) sum4[wave] = upto;
   __syncthreads();
   for (int i = 0; i < wave; ++i) upto += sum4[i];
-  const uint64_t hit = __ballot(upto > target);
-  const uint64_t some = __ballot(last_positive >= 0);
+  const uint64_t hit = __ballot(upto > target), some = __ballot(last_positive >= 0);
   const int top = __shfl(last_positive, some == 0 ? 0 : 63 - __clzll((long long)some));
   if (lane == 0) {
     found4[wave] = hit == 0 ? INT_MAX : wave * 64 + __ffsll((long long)hit) - 1;
@@ -475,8 +628,132 @@ __global__ __launch_bounds__(kDraftThreads) void draft_pick_kernel(DraftArgs a) 
 template <typename E>
 __global__ __launch_bounds__(64) void draft_greedy_kernel(DraftArgs a) {
   const int b = blockIdx.x;
-  const Walk w = walk_nodes<E, true>(a, b, true);
-  if (threadIdx.x == 0) a.next[b] = w.last < 0 ? -1 : row_best(a, (int64_t)b * a.N + w.last);
+  int best;
+  RowStat p, q;
+  node_stats<true>(a, b, &best, &p, &q);
+  const Walk w = walk_nodes<E, true>(a, b, true, best, p, q);
+  if (threadIdx.x == 0) a.next[b] = w.next;
+}
+
+// A vocabulary of up to kSmallValues, a workgroup per sequence: its rows one to a wave,
+// the walk, and the row where it ended, two values to a thread.
+constexpr int kSmallThreads = 1024, kSmallValues = 2048, kSmallWaves = kSmallThreads / 64;
+
+template <typename E, bool kGreedy>
+__global__ __launch_bounds__(kSmallThreads) void draft_small_kernel(DraftArgs a) {
+  __shared__ RowStat rows[2][64];
+  __shared__ int bests[64];
+  __shared__ Walk walk;
+  __shared__ uint32_t bits[kSmallValues / 32];
+  __shared__ double sums[2][kSmallWaves];
+  __shared__ int found[kSmallWaves], tops[kSmallWaves];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, b = blockIdx.x;
+  const int drafts = a.draft != nullptr ? a.N - 1 : 0;
+  for (int r = wave; r < a.N + drafts; r += kSmallWaves) {
+    const bool target = r < a.N;
+    const E* row = target ? static_cast<const E*>(a.logits) + ((int64_t)b * a.N + r) * a.V
+                          : static_cast<const E*>(a.draft) + ((int64_t)b * (a.N - 1) + r - a.N) * a.V;
+    float most = -INFINITY;
+    int at = INT_MAX;
+    for (int i0 = 0; i0 < a.V; i0 += 512) {  // eight loads at a time
+      float x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = i0 + k * 64 + lane < a.V ? static_cast<float>(row[i0 + k * 64 + lane]) : -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (kGreedy && x[k] > most) at = i0 + k * 64 + lane;
+        most = nan_max(most, x[k]);
+      }
+    }
+    float all = most;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) all = nan_max(all, __shfl_xor(all, o));
+    if (kGreedy) {
+      at = most == all ? at : INT_MAX;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o));
+      if (lane == 0) bests[r] = all != all || all == INFINITY || at == INT_MAX ? -1 : at;
+    } else {
+      const Exponent e = exponent_of(all, a.to_log2);
+      double s = 0.0;
+      for (int i0 = 0; i0 < a.V; i0 += 512) {
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = i0 + k * 64 + lane < a.V ? static_cast<float>(row[i0 + k * 64 + lane]) : -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += weight_of(x[k], e);
+      }
+      s = wave_sum(s);
+      // (a row of -infinities: no sum)
+      if (lane == 0) rows[target ? 0 : 1][target ? r : r - a.N] = RowStat{all, all == -INFINITY ? 0.0 : s};
+    }
+  }
+  if (tid < kSmallValues / 32) bits[tid] = 0;
+  __syncthreads();
+  if (tid < 64) {
+    const RowStat none{-INFINITY, 0.0};
+    const Walk w = walk_nodes<E, kGreedy>(a, b, true, kGreedy && lane < a.N ? bests[lane] : -1, !kGreedy && lane < a.N ? rows[0][lane] : none,
+                                          !kGreedy && lane < drafts ? rows[1][lane] : none);
+    if (kGreedy) {
+      if (tid == 0) a.next[b] = w.next;
+      return;
+    }
+    if (tid == 0) walk = w;
+    if ((w.struck >> lane & 1) != 0) {
+      const int at = (int)token_at(a, (int64_t)b * a.N + lane);
+      atomicOr(&bits[at >> 5], 1u << (at & 31));
+    }
+  }
+  if (kGreedy) return;
+  __syncthreads();
+  const Walk w = walk;
+  if (w.last < 0 || !(w.p.sum > 0.0 && w.p.sum < 1e300) || (w.residual != 0 && !(w.q.sum > 0.0 && w.q.sum < 1e300))) {
+    if (tid == 0) a.next[b] = -1;
+    return;
+  }
+  const Weights<E> ws = weights_of<E>(a, w, b);
+  const double ip = 1.0 / w.p.sum, iq = w.residual != 0 ? 1.0 / w.q.sum : 0.0;
+  double p[2], v[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int i = 2 * tid + k;
+    p[k] = v[k] = 0.0;
+    if (i < a.V) {
+      p[k] = weight_of(static_cast<float>(ws.row[i]), ws.p) * ip;
+      v[k] = p[k];
+      if (w.residual != 0) v[k] = fmax(p[k] - weight_of(static_cast<float>(ws.draft[i]), ws.q) * iq, 0.0);
+      else if ((bits[i >> 5] >> (i & 31) & 1) != 0) v[k] = 0.0;
+    }
+  }
+  double total = 0.0, upto = 0.0;
+  for (int round = 0; round < 2; ++round) {  // a second one where nothing is left of p (it was rounded away): p itself
+    upto = wave_scan(v[0] + v[1]);
+    if (lane == 63) sums[round][wave] = upto;
+    __syncthreads();
+    total = 0.0;
+    for (int i = 0; i < kSmallWaves; ++i) {
+      if (i == wave) upto += total;
+      total += sums[round][i];
+    }
+    if (total > 0.0) break;
+    v[0] = p[0], v[1] = p[1];
+  }
+  const double u = (double)fminf(fmaxf(a.u[(int64_t)b * a.N], 0.0f), 0x1.fffffep-1f), target = u * total;
+  const int top = v[1] > 0.0 ? 2 * tid + 1 : v[0] > 0.0 ? 2 * tid : -1;
+  const uint64_t hit = __ballot(upto > target && top >= 0), some = __ballot(top >= 0);
+  const int wave_top = __shfl(top, some == 0 ? 0 : 63 - __clzll((long long)some));
+  if (lane == 0) {
+    found[wave] = hit == 0 ? INT_MAX : tid + __ffsll((long long)hit) - 1;
+    tops[wave] = wave_top;
+  }
+  __syncthreads();
+  int owner = INT_MAX, last = -1;
+  for (int i = 0; i < kSmallWaves; ++i) owner = min(owner, found[i]), last = max(last, tops[i]);
+  if (owner == INT_MAX) {  // the two sums' roundings differ: the last one with any weight
+    if (tid == 0) a.next[b] = last;
+  } else if (tid == owner) {
+    a.next[b] = v[0] > 0.0 && (upto - v[1] > target || !(v[1] > 0.0)) ? 2 * tid : 2 * tid + 1;
+  }
 }
 
 fc_status bad(const char* who, const char* what, fc_status code = FC_ERR_INVALID_ARGUMENT) {
@@ -512,35 +789,48 @@ fc_status check(const char* who, const fc_verify_desc* d) {
 }
 
 struct Layout {
-  size_t stats, walks, sums, total;
+  size_t stats, walks, both, sums, arrived, total;
 };
 Layout layout_of(const fc_verify_desc* d) {
   Layout l;
-  const int chunks = chunks_of(d);
+  const size_t chunks = (size_t)chunks_of(d), B = (size_t)d->B;
+  const bool draws = rows_of(d) > (int64_t)d->B * d->N;
   l.stats = 0;
   l.walks = round256((size_t)rows_of(d) * chunks * sizeof(ChunkStat));
-  l.sums = l.walks + round256((size_t)d->B * sizeof(Walk));
-  l.total = l.sums + round256((size_t)d->B * chunks * sizeof(double));
+  l.both = l.walks + (draws ? round256(B * sizeof(Walk)) : 0);
+  l.sums = l.both + (draws ? round256(B * chunks * kParts * sizeof(double2)) : 0);
+  l.arrived = l.sums + round256(B * chunks * kParts * sizeof(double));
+  l.total = l.arrived + round256(B * sizeof(int32_t));
   return l;
 }
 
 template <typename E>
 hipError_t launch_verify(const DraftArgs& a, int64_t rows, bool greedy, hipStream_t s) {
   ProfileMark mk = profile_begin(s);
-  const dim3 all((unsigned)(rows * a.chunks));
+  if (a.V <= kSmallValues) {
+    if (greedy) hipLaunchKernelGGL((draft_small_kernel<E, true>), dim3((unsigned)a.B), dim3(kSmallThreads), 0, s, a);
+    else hipLaunchKernelGGL((draft_small_kernel<E, false>), dim3((unsigned)a.B), dim3(kSmallThreads), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    profile_end(mk, "draft_small", s);
+    return e;
+  }
+  const dim3 all((unsigned)(rows * a.chunks)), ends((unsigned)(a.B * a.chunks));
   if (greedy) hipLaunchKernelGGL((draft_stats_kernel<E, true>), all, dim3(kDraftThreads), 0, s, a);
   else hipLaunchKernelGGL((draft_stats_kernel<E, false>), all, dim3(kDraftThreads), 0, s, a);
   hipError_t e = hipGetLastError();
   profile_end(mk, "draft_stats", s);
   if (e != hipSuccess) return e;
+  if (a.draft != nullptr) {
+    mk = profile_begin(s);
+    hipLaunchKernelGGL((draft_walk_kernel<E>), ends, dim3(kDraftThreads), 0, s, a);
+    e = hipGetLastError();
+    profile_end(mk, "draft_walk", s);
+    if (e != hipSuccess) return e;
+  }
   mk = profile_begin(s);
   if (greedy) hipLaunchKernelGGL((draft_greedy_kernel<E>), dim3((unsigned)a.B), dim3(64), 0, s, a);
-  else hipLaunchKernelGGL((draft_walk_kernel<E>), dim3((unsigned)(a.B * a.chunks)), dim3(kDraftThreads), 0, s, a);
-  e = hipGetLastError();
-  profile_end(mk, "draft_walk", s);
-  if (e != hipSuccess || greedy) return e;
-  mk = profile_begin(s);
-  hipLaunchKernelGGL((draft_pick_kernel<E>), dim3((unsigned)a.B), dim3(kDraftThreads), 0, s, a);
+  else if (a.draft != nullptr) hipLaunchKernelGGL((draft_pick_kernel<E, true>), ends, dim3(kDraftThreads), 0, s, a);
+  else hipLaunchKernelGGL((draft_pick_kernel<E, false>), ends, dim3(kDraftThreads), 0, s, a);
   e = hipGetLastError();
   profile_end(mk, "draft_pick", s);
   return e;
@@ -587,7 +877,9 @@ fc_status fc_verify_drafts(const fc_verify_desc* desc, const void* logits, const
   char* ws = static_cast<char*>(workspace);
   a.stats = reinterpret_cast<fc::ChunkStat*>(ws + l.stats);
   a.walks = reinterpret_cast<fc::Walk*>(ws + l.walks);
+  a.both = reinterpret_cast<double2*>(ws + l.both);
   a.sums = reinterpret_cast<double*>(ws + l.sums);
+  a.arrived = reinterpret_cast<int32_t*>(ws + l.arrived);
   a.B = desc->B, a.N = desc->N, a.V = desc->V, a.chunks = fc::chunks_of(desc);
   a.index64 = desc->index_type == FC_INDEX_I64, a.tree = desc->tree;
   a.to_log2 = greedy ? 0.0 : 1.4426950408889634074 / desc->temperature;
