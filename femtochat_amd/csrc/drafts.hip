@@ -66,17 +66,17 @@ struct DraftArgs {
   int32_t *path, *kept, *next;
   ChunkStat* stats;  // [B N target rows, B (N - 1) draft rows][chunks]
   Walk* walks;       // [B] (draws)
-  double2* both;     // [B][chunks][kParts]: sums of the two exponentials (draws)
-  double* sums;      // [B][chunks][kParts], of the weights
+  double2* both;     // [B][groups][kWaves4]: sums of the two exponentials (draws)
+  double* sums;      // [B][groups][kWaves4], of the weights
   int32_t* arrived;  // [B]: workgroups of the pick that left their sums
   int B, N, V, chunks;
+  int groups;        // workgroups of a sequence in the walk and the pick, a part to each of their waves
   int index64, tree;
   double to_log2;    // log2(e) / temperature
 };
 
 template <typename E> constexpr int kPiece = 16 / (int)sizeof(E);
-constexpr int kParts = 4;                            // of a chunk: a wave's values
-constexpr int kPartValues = kChunkValues / kParts;   // 2048
+constexpr int kWaves4 = kDraftThreads / 64;
 
 // exp((x - most) / temperature) for x <= most.  2^t = 2^n 2^f, n the nearest whole number
 // (its bits come from adding 1.5 2^52) and f in [-1/2, 1/2]: a polynomial of degree 10 through
@@ -392,29 +392,35 @@ __device__ inline void weights(const Weights<E>& w, const uint32_t* bits, int fi
   }
 }
 
-// Which of a chunk's values are struck out: a bit each, from element `first` of the row on
-// (pieces begin at multiples of their length, so one word holds a piece's).
+// Which of kCount values are struck out: a bit each, from element `first` of the row on
+// (pieces begin at multiples of their length, so one word holds a piece's).  All of a
+// workgroup's threads call it, or (kThreads 64) one wave for itself.
+template <int kCount, int kThreads>
 __device__ inline void strike(uint32_t* bits, const DraftArgs& a, int b, uint64_t struck, int first) {
-  for (int i = threadIdx.x; i < kChunkValues / 32; i += kDraftThreads) bits[i] = 0;
-  __syncthreads();
-  const int i = threadIdx.x;
+  const int i = threadIdx.x % kThreads;
+  const auto sync = [] {
+    if (kThreads > 64) __syncthreads();
+    else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  };
+  for (int k = i; k < kCount / 32; k += kThreads) bits[k] = 0;
+  sync();
   if (i < 64 && (struck >> i & 1) != 0) {
     const int at = (int)token_at(a, (int64_t)b * a.N + i) - first;
-    if (at >= 0 && at < kChunkValues) atomicOr(&bits[at >> 5], 1u << (at & 31));
+    if (at >= 0 && at < kCount) atomicOr(&bits[at >> 5], 1u << (at & 31));
   }
-  __syncthreads();
+  sync();
 }
 
-// A wave's part of a chunk: the sum of its weights, in every lane.
-template <typename E>
-__device__ inline double part_sum(const Weights<E>& w, const uint32_t* bits, int first, int part) {
+// The sum of kPart weights from element `first` on, by a wave, in every lane; bits begin there too.
+template <typename E, int kPart>
+__device__ inline double part_sum(const Weights<E>& w, const uint32_t* bits, int first) {
   constexpr int P = kPiece<E>;
   const int lane = threadIdx.x & 63;
   double s = 0.0;
 #pragma unroll 2
-  for (int k = 0; k < kPartValues / (64 * P); ++k) {
+  for (int k = 0; k < kPart / (64 * P); ++k) {
     double v[P];
-    weights<E>(w, bits, first, first + part * kPartValues + (k * 64 + lane) * P, v);
+    weights<E>(w, bits, first, first + (k * 64 + lane) * P, v);
 #pragma unroll
     for (int i = 0; i < P; ++i) s += v[i];
   }
@@ -437,20 +443,20 @@ __device__ inline void node_stats(const DraftArgs& a, int b, int* best, RowStat*
 }
 
 // Draws: the walk, and the sums of the two exponentials where it ended in a refusal.
-template <typename E>
+template <typename E, int kPart>
 __global__ __launch_bounds__(kDraftThreads) void draft_walk_kernel(DraftArgs a) {
   constexpr int P = kPiece<E>;
   __shared__ Walk walk;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
+  const int b = blockIdx.x / a.groups, group = blockIdx.x - b * a.groups;
   if (tid < 64) {
     int best;
     RowStat p, q;
     node_stats<false>(a, b, &best, &p, &q);
-    const Walk w = walk_nodes<E, false>(a, b, chunk == 0, best, p, q);
+    const Walk w = walk_nodes<E, false>(a, b, group == 0, best, p, q);
     if (tid == 0) {
       walk = w;
-      if (chunk == 0) a.walks[b] = w;
+      if (group == 0) a.walks[b] = w;
     }
   }
   __syncthreads();
@@ -459,9 +465,9 @@ __global__ __launch_bounds__(kDraftThreads) void draft_walk_kernel(DraftArgs a) 
   const Weights<E> ws = weights_of<E>(a, w, b);
   double sp = 0.0, sq = 0.0;
   const auto add = [&](const E* row, const Exponent& e, double& s) {
-    const int first = chunk * kChunkValues + wave * kPartValues - row_head(row);
+    const int first = (group * kWaves4 + wave) * kPart - row_head(row);
 #pragma unroll 2
-    for (int k = 0; k < kPartValues / (64 * P); ++k) {
+    for (int k = 0; k < kPart / (64 * P); ++k) {
       float x[P];
       load_piece(row, a.V, first + (k * 64 + lane) * P, x);
 #pragma unroll
@@ -472,29 +478,27 @@ __global__ __launch_bounds__(kDraftThreads) void draft_walk_kernel(DraftArgs a) 
   add(ws.draft, ws.q, sq);
   sp = wave_sum(sp);
   sq = wave_sum(sq);
-  if (lane == 0) a.both[((int64_t)b * a.chunks + chunk) * kParts + wave] = make_double2(sp, sq);
+  if (lane == 0) a.both[((int64_t)b * a.groups + group) * kWaves4 + wave] = make_double2(sp, sq);
 }
 
 // kDraws: the walk is done.
-template <typename E, bool kDraws>
+template <typename E, bool kDraws, int kPart>
 __global__ __launch_bounds__(kDraftThreads) void draft_pick_kernel(DraftArgs a) {
   constexpr int P = kPiece<E>;
-  constexpr int kMine = kPartValues / kDraftThreads, kPieces = kMine / P;  // the pick: 8 values of a thread
-  static_assert(kMine % P == 0, "a thread's values are whole pieces");
+  constexpr int kMine = kPart / 64, kPieces = kMine / P;  // the pick: values of a lane
+  static_assert(kMine % P == 0, "a lane's values are whole pieces");
   __shared__ Walk walk;
-  __shared__ uint32_t bits[kChunkValues / 32];
-  __shared__ double sum4[4];
-  __shared__ int found4[4], last4[4];
+  __shared__ uint32_t bits[kWaves4 * kPart / 32];
   __shared__ int is_last;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
-  const int parts = a.chunks * kParts;
+  const int b = blockIdx.x / a.groups, group = blockIdx.x - b * a.groups;
+  const int parts = a.groups * kWaves4;
   if (!kDraws) {
     if (tid < 64) {
       int best;
       RowStat p, q;
       node_stats<false>(a, b, &best, &p, &q);
-      const Walk w = walk_nodes<E, false>(a, b, chunk == 0, best, p, q);
+      const Walk w = walk_nodes<E, false>(a, b, group == 0, best, p, q);
       if (tid == 0) walk = w;
     }
     __syncthreads();
@@ -511,7 +515,7 @@ __global__ __launch_bounds__(kDraftThreads) void draft_pick_kernel(DraftArgs a) 
   const Walk w = kDraws ? a.walks[b] : walk;
   // (a row with a NaN or +infinity, or of -infinities, has no sum)
   if (w.last < 0 || !(w.p.sum > 0.0 && w.p.sum < 1e300) || (w.residual != 0 && !(w.q.sum > 0.0 && w.q.sum < 1e300))) {
-    if (chunk == 0 && tid == 0) a.next[b] = -1;
+    if (group == 0 && tid == 0) a.next[b] = -1;
     return;
   }
   Weights<E> ws = weights_of<E>(a, w, b);
@@ -520,41 +524,39 @@ __global__ __launch_bounds__(kDraftThreads) void draft_pick_kernel(DraftArgs a) 
     ws.ip = 1.0 / wave_sum(sp);
     ws.iq = 1.0 / wave_sum(sq);
   }
-  const uint32_t* strikes = w.struck != 0 ? bits : nullptr;
   double* sums = a.sums + (int64_t)b * parts;
+  const uint32_t* strikes = nullptr;
   {
-    const int first = chunk * kChunkValues - head;
-    if (strikes != nullptr) strike(bits, a, b, w.struck, first);
-    const double s = part_sum(ws, strikes, first, wave);
-    if (a.chunks == 1) {
-      if (lane == 0) sum4[wave] = s;
-    } else {
-      // What the last workgroup reads is written and read at the agent's scope, past the
-      // XCDs' own caches; the wave waits for its store before the barrier, and the counter
-      // moves behind that.  (A release at that scope would write the whole L2 back.)
-      if (lane == 0) __hip_atomic_store(&sums[chunk * kParts + wave], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const int first = group * kWaves4 * kPart - head;
+    if (w.struck != 0) {
+      strike<kWaves4 * kPart, kDraftThreads>(bits, a, b, w.struck, first);
+      strikes = bits + wave * (kPart / 32);
     }
+    const double s = part_sum<E, kPart>(ws, strikes, first + wave * kPart);
+    // What the last workgroup reads is written and read at the agent's scope, past the
+    // XCDs' own caches; the wave waits for its store before the barrier, and the counter
+    // moves behind that.  (A release at that scope would write the whole L2 back: 20 us.)
+    if (lane == 0) __hip_atomic_store(&sums[group * kWaves4 + wave], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
   __syncthreads();
-  if (a.chunks > 1) {
-    if (tid == 0)
-      is_last = __hip_atomic_fetch_add(&a.arrived[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.chunks - 1;
-    __syncthreads();
-    if (is_last == 0) return;
-  }
-  // The last one: the part that u's share falls into.  Every wave looks by itself.
+  if (tid == 0)
+    is_last = __hip_atomic_fetch_add(&a.arrived[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.groups - 1;
+  __syncthreads();
+  if (is_last == 0 || wave != 0) return;
+  // The last one's first wave: the part that u's share falls into.
   const auto part_at = [&](int i) {
-    return a.chunks == 1 ? sum4[i] : __hip_atomic_load(&sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return i < parts ? __hip_atomic_load(&sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
   };
   double total = 0.0;
-  for (int i0 = 0; i0 < parts; i0 += 64) total += wave_sum(i0 + lane < parts ? part_at(i0 + lane) : 0.0);
+  for (int i0 = 0; i0 < parts; i0 += 64) total += part_at(i0 + lane);
+  total = wave_sum(total);
   const double u = (double)fminf(fmaxf(a.u[(int64_t)b * a.N], 0.0f), 0x1.fffffep-1f);
   double before = 0.0, target = u * total;
   int part = parts - 1;
   if (total > 0.0) {
     for (int i0 = 0; i0 < parts; i0 += 64) {
-      const double upto = before + wave_scan(i0 + lane < parts ? part_at(i0 + lane) : 0.0);
+      const double upto = before + wave_scan(part_at(i0 + lane));
       const uint64_t hit = __ballot(upto > target);
       if (hit != 0) {
         const int at = __ffsll((long long)hit) - 1;
@@ -566,25 +568,25 @@ __global__ __launch_bounds__(kDraftThreads) void draft_pick_kernel(DraftArgs a) 
     }
   } else {  // nothing is left of p (it was rounded away): p itself
     ws.draft = nullptr, strikes = nullptr;
-    for (int i = 0; i < parts; ++i) total += part_sum(ws, strikes, i / kParts * kChunkValues - head, i % kParts);
+    for (int i = 0; i < parts; ++i) total += part_sum<E, kPart>(ws, nullptr, i * kPart - head);
     target = u * total;
     for (part = 0; part < parts - 1; ++part) {
-      const double upto = before + part_sum(ws, strikes, part / kParts * kChunkValues - head, part % kParts);
+      const double upto = before + part_sum<E, kPart>(ws, nullptr, part * kPart - head);
       if (upto > target) break;
       before = upto;
     }
   }
   target -= before;
-  // The token in it.  A thread's values are neighbours here: the order of the sum is theirs.
-  const int first = part / kParts * kChunkValues - head;
+  // The token in it.  A lane's values are neighbours here: the order of the sum is theirs.
+  const int first = part * kPart - head;
   if (strikes != nullptr) {
-    __syncthreads();
-    strike(bits, a, b, w.struck, first);
+    strike<kPart, 64>(bits, a, b, w.struck, first);
+    strikes = bits;
   }
   double v[kPieces][P];
   double mine = 0.0;
   int last_positive = -1;
-  const int e0 = first + part % kParts * kPartValues + tid * kMine;
+  const int e0 = first + lane * kMine;
 #pragma unroll
   for (int k = 0; k < kPieces; ++k) {
     weights<E>(ws, strikes, first, e0 + k * P, v[k]);
@@ -594,27 +596,14 @@ __global__ __launch_bounds__(kDraftThreads) void draft_pick_kernel(DraftArgs a) 
       if (v[k][i] > 0.0) last_positive = e0 + k * P + i;
     }
   }
-  double upto = wave_scan(mine);
-  __syncthreads();
-  if (lane == 63) sum4[wave] = upto;
-  __syncthreads();
-  for (int i = 0; i < wave; ++i) upto += sum4[i];
-  const uint64_t hit = __ballot(upto > target), some = __ballot(last_positive >= 0);
-  const int top = __shfl(last_positive, some == 0 ? 0 : 63 - __clzll((long long)some));
-  if (lane == 0) {
-    found4[wave] = hit == 0 ? INT_MAX : wave * 64 + __ffsll((long long)hit) - 1;
-    last4[wave] = top;
-  }
-  __syncthreads();
-  const int owner = min(min(found4[0], found4[1]), min(found4[2], found4[3]));
-  if (owner == INT_MAX) {  // the two sums' roundings differ: the last one with any weight
-    if (tid == 0) a.next[b] = max(max(last4[0], last4[1]), max(last4[2], last4[3]));
-    return;
-  }
-  if (tid != owner) return;
+  const double upto = wave_scan(mine);
+  const uint64_t hit = __ballot(upto > target && last_positive >= 0), some = __ballot(last_positive >= 0);
+  // (where the two sums' roundings differ, and no value is beyond the target: the last one with any weight)
+  const int owner = hit != 0 ? __ffsll((long long)hit) - 1 : some != 0 ? 63 - __clzll((long long)some) : 0;
+  if (lane != owner) return;
   double c = upto - mine;
   int at = last_positive;
-  bool open = true;
+  bool open = hit != 0;
 #pragma unroll
   for (int k = 0; k < kPieces; ++k)
 #pragma unroll
@@ -788,24 +777,52 @@ fc_status check(const char* who, const fc_verify_desc* d) {
   return FC_OK;
 }
 
+// The values of a wave in the walk and the pick: 512 (a workgroup's 2048 take it 4 us of
+// float64, at 2048 a wave they take 12) unless that makes more workgroups than the GPU holds
+// at once, each of which walks its sequence's nodes again.
+constexpr int kShort = 512, kLong = 2048;
+int groups_of(const fc_verify_desc* d, int part) {
+  const int per = d->dtype == FC_BF16 ? 8 : 4;
+  return (int)(((int64_t)d->V + per - 1 + kWaves4 * part - 1) / (kWaves4 * part));
+}
+int part_of(const fc_verify_desc* d) { return (int64_t)d->B * groups_of(d, kShort) <= 1280 ? kShort : kLong; }
+
 struct Layout {
   size_t stats, walks, both, sums, arrived, total;
 };
 Layout layout_of(const fc_verify_desc* d) {
   Layout l;
-  const size_t chunks = (size_t)chunks_of(d), B = (size_t)d->B;
+  const size_t chunks = (size_t)chunks_of(d), B = (size_t)d->B, parts = (size_t)groups_of(d, part_of(d)) * kWaves4;
   const bool draws = rows_of(d) > (int64_t)d->B * d->N;
   l.stats = 0;
   l.walks = round256((size_t)rows_of(d) * chunks * sizeof(ChunkStat));
   l.both = l.walks + (draws ? round256(B * sizeof(Walk)) : 0);
-  l.sums = l.both + (draws ? round256(B * chunks * kParts * sizeof(double2)) : 0);
-  l.arrived = l.sums + round256(B * chunks * kParts * sizeof(double));
+  l.sums = l.both + (draws ? round256(B * parts * sizeof(double2)) : 0);
+  l.arrived = l.sums + round256(B * parts * sizeof(double));
   l.total = l.arrived + round256(B * sizeof(int32_t));
   return l;
 }
 
+template <typename E, int kPart>
+hipError_t launch_ends(const DraftArgs& a, hipStream_t s) {
+  const dim3 ends((unsigned)(a.B * a.groups));
+  if (a.draft != nullptr) {
+    const ProfileMark mk = profile_begin(s);
+    hipLaunchKernelGGL((draft_walk_kernel<E, kPart>), ends, dim3(kDraftThreads), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    profile_end(mk, "draft_walk", s);
+    if (e != hipSuccess) return e;
+  }
+  const ProfileMark mk = profile_begin(s);
+  if (a.draft != nullptr) hipLaunchKernelGGL((draft_pick_kernel<E, true, kPart>), ends, dim3(kDraftThreads), 0, s, a);
+  else hipLaunchKernelGGL((draft_pick_kernel<E, false, kPart>), ends, dim3(kDraftThreads), 0, s, a);
+  const hipError_t e = hipGetLastError();
+  profile_end(mk, "draft_pick", s);
+  return e;
+}
+
 template <typename E>
-hipError_t launch_verify(const DraftArgs& a, int64_t rows, bool greedy, hipStream_t s) {
+hipError_t launch_verify(const DraftArgs& a, int64_t rows, bool greedy, int part, hipStream_t s) {
   ProfileMark mk = profile_begin(s);
   if (a.V <= kSmallValues) {
     if (greedy) hipLaunchKernelGGL((draft_small_kernel<E, true>), dim3((unsigned)a.B), dim3(kSmallThreads), 0, s, a);
@@ -814,25 +831,17 @@ hipError_t launch_verify(const DraftArgs& a, int64_t rows, bool greedy, hipStrea
     profile_end(mk, "draft_small", s);
     return e;
   }
-  const dim3 all((unsigned)(rows * a.chunks)), ends((unsigned)(a.B * a.chunks));
+  const dim3 all((unsigned)(rows * a.chunks));
   if (greedy) hipLaunchKernelGGL((draft_stats_kernel<E, true>), all, dim3(kDraftThreads), 0, s, a);
   else hipLaunchKernelGGL((draft_stats_kernel<E, false>), all, dim3(kDraftThreads), 0, s, a);
   hipError_t e = hipGetLastError();
   profile_end(mk, "draft_stats", s);
   if (e != hipSuccess) return e;
-  if (a.draft != nullptr) {
-    mk = profile_begin(s);
-    hipLaunchKernelGGL((draft_walk_kernel<E>), ends, dim3(kDraftThreads), 0, s, a);
-    e = hipGetLastError();
-    profile_end(mk, "draft_walk", s);
-    if (e != hipSuccess) return e;
-  }
+  if (!greedy) return part == kShort ? launch_ends<E, kShort>(a, s) : launch_ends<E, kLong>(a, s);
   mk = profile_begin(s);
-  if (greedy) hipLaunchKernelGGL((draft_greedy_kernel<E>), dim3((unsigned)a.B), dim3(64), 0, s, a);
-  else if (a.draft != nullptr) hipLaunchKernelGGL((draft_pick_kernel<E, true>), ends, dim3(kDraftThreads), 0, s, a);
-  else hipLaunchKernelGGL((draft_pick_kernel<E, false>), ends, dim3(kDraftThreads), 0, s, a);
+  hipLaunchKernelGGL((draft_greedy_kernel<E>), dim3((unsigned)a.B), dim3(64), 0, s, a);
   e = hipGetLastError();
-  profile_end(mk, "draft_pick", s);
+  profile_end(mk, "draft_greedy", s);
   return e;
 }
 
@@ -880,12 +889,14 @@ fc_status fc_verify_drafts(const fc_verify_desc* desc, const void* logits, const
   a.both = reinterpret_cast<double2*>(ws + l.both);
   a.sums = reinterpret_cast<double*>(ws + l.sums);
   a.arrived = reinterpret_cast<int32_t*>(ws + l.arrived);
-  a.B = desc->B, a.N = desc->N, a.V = desc->V, a.chunks = fc::chunks_of(desc);
+  const int part = fc::part_of(desc);
+  a.B = desc->B, a.N = desc->N, a.V = desc->V, a.chunks = fc::chunks_of(desc), a.groups = fc::groups_of(desc, part);
   a.index64 = desc->index_type == FC_INDEX_I64, a.tree = desc->tree;
   a.to_log2 = greedy ? 0.0 : 1.4426950408889634074 / desc->temperature;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t rows = (int64_t)a.B * a.N + (draft ? (int64_t)a.B * (a.N - 1) : 0);
-  const hipError_t e = desc->dtype == FC_BF16 ? fc::launch_verify<fc::bf16>(a, rows, greedy, s) : fc::launch_verify<float>(a, rows, greedy, s);
+  const hipError_t e = desc->dtype == FC_BF16 ? fc::launch_verify<fc::bf16>(a, rows, greedy, part, s)
+                                               : fc::launch_verify<float>(a, rows, greedy, part, s);
   if (e != hipSuccess) return fc::bad(who, hipGetErrorString(e), FC_ERR_HIP);
   fc::clear_error();
   return FC_OK;
