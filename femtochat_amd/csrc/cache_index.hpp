@@ -62,13 +62,30 @@ FC_HD inline Span span_of(int length, int count, int N, int left, int capacity) 
   s.tiles = s.count == 0 ? 1 : imax(1, (end + kTileKeys - 1) / kTileKeys - s.first);
   return s;
 }
-// Tiles per slot: the sequences' tiles in `share` equal parts, so that a batch's long
-// sequences are spread as widely as its lengths ask for, and no part below `least`.  A
-// sequence's tiles in parts of this size make at most share + B slots in all.
-FC_HD inline int slot_tiles(int64_t total, int share, int least) {
-  const int64_t part = (total + share - 1) / share;
-  return (int)((imax(least, (int)(part < (1 << 30) ? part : 1 << 30)) + 3) / 4 * 4);
+// A batch's work is shared out as one line, each sequence's tiles behind the ones before,
+// with room in front for what beginning a sequence costs (in tiles): workgroup x takes the
+// x-th stretch of the line.  One share, and with it one workgroup, may end a sequence,
+// hold others whole and begin another.
+constexpr int kBegin = 8;
+
+FC_HD inline int64_t share_of(int64_t total, int shares, int least) {
+  const int64_t s = (total + shares - 1) / shares;
+  return s > least ? s : least;
 }
+// The tiles (first, last: counted from the sequence's first) of a sequence at `start` of the
+// line that share x holds: none where it has only the room in front, or nothing, of it.
+struct Stretch {
+  int first, last;
+};
+FC_HD inline Stretch stretch_of(int64_t start, int tiles, int64_t x, int64_t share) {
+  const int64_t from = x * share - start, upto = from + share;
+  Stretch s;
+  s.first = from <= kBegin ? 0 : (int)(from - kBegin < tiles ? from - kBegin : tiles);
+  s.last = upto <= kBegin ? 0 : (int)(upto - kBegin < tiles ? upto - kBegin : tiles);
+  return s;
+}
+// Where share x leaves its part of a sequence: it has at most two parts that are not whole.
+FC_HD inline int64_t part_slot(int64_t start, int64_t x, int64_t share) { return 2 * x + (start >= x * share ? 1 : 0); }
 
 // Which of the 32 keys from key0 on are seen: those of the sequence (below length)
 // from `low` on, and the nodes' behind it.

@@ -10,10 +10,7 @@
 // rounding does (2.3e-3 of O for 1.7e-3, in the 2-norm).
 //
 // The work is the reading of the cache, once per KV head, so what a wave needs is
-// loads in flight and few instructions per byte; there is no LDS and no barrier
-// in the loop:
-//  * A wave takes 32 keys at a time, the next ones' bytes on their way into
-//    registers.  Waves, and workgroups, split a sequence's keys among them.
+// loads in flight and few instructions per byte:
 //  * K's rows are the first product's A operand as they lie: lane (n, g) = (l % 16,
 //    l / 16) reads units g ceil(U / 4) + s of row n (8 values each, U = D / 8), and Q's
 //    operand holds the same units, as the order of a sum is free.
@@ -26,6 +23,22 @@
 //    own registers), whose row n is then column C n + c of O.
 //  * Row maxima are not kept from tile to tile: a row's reference moves only
 //    where a score exceeds it by 2^8, which a wave asks of its lanes with one vote.
+// Each wave reads keys of its own for sixteen or 32 rows, with neither LDS (but for the queries)
+// nor barriers in the loop: its operands are used twice at most, and eight waves that shared
+// them through LDS in steps of 128 keys waited for each other longer than for the bytes
+// (16 sequences of 4096 int8 keys, 64 rows, 8 KV heads: 75 us for 61).
+//
+// The lengths lie on the device, so the launch is the same whatever they are: as many
+// workgroups as the GPU holds at once, each of which finds its equal share of all
+// sequences' tiles (cache_index.hpp).  A sequence in several shares is joined by a
+// second, small kernel.
+//
+// Measured, codes of 8 bits, heads of 128, the kernel alone: 64 sequences of up to 4096 keys,
+// 5 KV heads, one token each, 40 us (192 MB, 4.8 TB/s; a copy reaches 5.1); one of 131072 keys,
+// 8 KV heads, 50 us (277 MB; part of it stays in the 256 MB cache between calls); 16 of up to
+// 8192 keys, 8 KV heads, 32 nodes of two heads each, 61 us (168 MB, 2.8 TB/s), where the vector
+// units are busy for four fifths: a third of it turns codes into numbers and a fourth makes
+// two numbers of each probability.
 //
 // Rows that do not see a key have P = 0 there, but 0 * infinity is not 0: in tiles
 // that some row sees only in part, values that no row sees are taken as zeros,
@@ -47,69 +60,94 @@ struct CachedAttnArgs {
   void* O;
   const int32_t *lengths, *counts, *parents;
   const float* slopes;
-  float* part_o;   // [slot][16 R][D]
-  float2* part_s;  // [slot][16 R] (reference, sum)
+  float* part_o;   // [KV head, row group][2 shares][16 R][D]
+  float2* part_s;  // [KV head, row group][2 shares][16 R] (reference, sum)
   int H, N, G, rows;      // rows = G N
   int left;               // INT_MAX / 2: all
   int tree;               // 0 a run, 1 one tree, 2 a tree per sequence
   int groups;             // row groups of 16 R
-  int items, share;       // slots per row group, and how many of them share the tiles
-  int least;              // tiles of a slot, at least
+  int shares;             // workgroups per KV head and row group, each with a share of all tiles; 0: one per sequence
+  int least;              // tiles of a share, at least
   float scale_log2, cap_in, cap_out;
 };
 
 // ---- which keys a workgroup takes ---------------------------------------------
 
-__device__ inline int wave_sum(int v) {
+__device__ inline int64_t wave_sum(int64_t v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
   return v;
 }
-__device__ inline Span span_at(const CachedAttnArgs& a, int b) {
-  return span_of(a.lengths[b], a.counts != nullptr ? a.counts[b] : a.N, a.N, a.left, a.g.capacity);
+
+__device__ inline int64_t of_lane(int64_t v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, lane), hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)v >> 32), lane);
+  return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-struct Slot {
-  int b, part, parts, first;  // sequence (-1: none), which of its parts, its first slot
-  int tiles;                  // of a part
+// The lengths and counts of 64 sequences, one to each lane.
+struct Chunk {
+  int b0, length, count;
+  __device__ inline void load(const CachedAttnArgs& a, int from) {
+    b0 = from;
+    const int b = from + (int)(threadIdx.x & 63);
+    length = b < a.g.B ? a.lengths[b] : 0;
+    count = b < a.g.B ? (a.counts != nullptr ? a.counts[b] : a.N) : 0;
+  }
+  __device__ inline Span mine(const CachedAttnArgs& a) const { return span_of(length, count, a.N, a.left, a.g.capacity); }
+  // Of sequence b, which may lie behind the chunk.
+  __device__ inline Span of(const CachedAttnArgs& a, int b) {
+    if (b - b0 >= 64) load(a, b);
+    return span_of(__builtin_amdgcn_readlane(length, b - b0), __builtin_amdgcn_readlane(count, b - b0), a.N, a.left, a.g.capacity);
+  }
 };
-// The sequence of slot x, or (x < 0) the slots of sequence of_b.  Every lane of a
-// wave calls it and gets the same.
-__device__ inline Slot find_slot(const CachedAttnArgs& a, int x, int of_b) {
+
+// A place on the line of all sequences' work (cache_index.hpp).
+struct Line {
+  int64_t share;  // its stretches' length
+  int64_t start;  // where a sequence begins
+  int b;          // which, B past the end
+  Chunk chunk;    // from or around it
+};
+// The first sequence of share x, or (x < 0) sequence of_b.  Every lane of a wave calls it
+// and gets the same.
+__device__ inline Line find_on_line(const CachedAttnArgs& a, int x, int of_b) {
   const int lane = threadIdx.x & 63;
-  int64_t total = 0;
-  for (int b0 = 0; b0 < a.g.B; b0 += 64) total += wave_sum(b0 + lane < a.g.B ? span_at(a, b0 + lane).tiles : 0);
-  Slot s;
-  s.tiles = slot_tiles(total, a.share, a.least);
-  s.b = -1, s.part = 0, s.parts = 0, s.first = 0;
-  int before = 0;
+  const auto cost = [&](const Chunk& c) { return c.b0 + lane < a.g.B ? c.mine(a).tiles + kBegin : 0; };
+  Line l;
+  l.chunk.load(a, 0);
+  int64_t total = wave_sum(cost(l.chunk));
+  for (int b0 = 64; b0 < a.g.B; b0 += 64) {
+    Chunk c;
+    c.load(a, b0);
+    total += wave_sum(cost(c));
+  }
+  l.share = share_of(total, a.shares, a.least);
+  l.b = a.g.B;
+  l.start = total;
+  const int64_t at = x * l.share;
+  int64_t before = 0;
   for (int b0 = 0; b0 < a.g.B; b0 += 64) {
-    const int b = b0 + lane;
-    const int n = b < a.g.B ? (span_at(a, b).tiles + s.tiles - 1) / s.tiles : 0;
-    int upto = n;  // slots of the sequences up to this lane's
+    if (b0 > 0) l.chunk.load(a, b0);
+    const int n = cost(l.chunk);
+    int64_t upto = n;  // with the sequences up to this lane's
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-      const int v = __shfl_up(upto, o);
+      const int64_t v = __shfl_up(upto, o);
       if (lane >= o) upto += v;
     }
-    const int mine = before + upto - n;
-    const uint64_t hit = __ballot(x >= 0 ? (x >= mine && x < mine + n) : b == of_b);
+    const uint64_t hit = __ballot(n > 0 && (x >= 0 ? at < before + upto : b0 + lane == of_b));
     if (hit != 0) {
-      const int at = __ffsll((long long)hit) - 1;
-      s.b = b0 + at;
-      s.parts = __shfl(n, at);
-      s.first = __shfl(mine, at);
-      s.part = x - s.first;
+      const int i = __ffsll((long long)hit) - 1;
+      l.b = b0 + i;
+      l.start = before + of_lane(upto - n, i);
       break;
     }
-    before += __shfl(upto, 63);
+    before += of_lane(upto, 63);
   }
-  s.b = __builtin_amdgcn_readfirstlane(s.b);
-  s.part = __builtin_amdgcn_readfirstlane(s.part);
-  s.parts = __builtin_amdgcn_readfirstlane(s.parts);
-  s.first = __builtin_amdgcn_readfirstlane(s.first);
-  s.tiles = __builtin_amdgcn_readfirstlane(s.tiles);
-  return s;
+  l.share = of_lane(l.share, 0);
+  l.start = of_lane(l.start, 0);
+  l.b = __builtin_amdgcn_readfirstlane(l.b);
+  return l;
 }
 
 // ---- the nodes --------------------------------------------------------------------
@@ -119,17 +157,16 @@ struct Nodes {
   uint64_t sees[kMaxNodes];  // itself and its ancestors within the window
   int depth[kMaxNodes];      // ancestors; -1 where its parents are not a tree's
 };
-// Called by one whole wave; lane i walks from node i to the root.
-__device__ inline void trace_nodes(Nodes* to, const int32_t* parents, int N, int left) {
+// Called by one whole wave; lane i, which holds node i's parent, walks from it to the root.
+__device__ inline void trace_nodes(Nodes* to, bool tree, int up, int N, int left) {
   const int i = threadIdx.x & 63;
   uint64_t sees = i < N ? 1ull << i : 0;
   int depth = 0, at = i;
   bool good = true;
-  if (parents == nullptr) {
+  if (!tree) {
     depth = i;
     sees = left >= i ? (2ull << i) - 1 : ((2ull << left) - 1) << (i - left);  // (left < i < 64)
   } else {
-    const int up = i < N ? parents[i] : -1;
     while (true) {
       const int next = __shfl(up, at);  // every lane's `at` is below 64
       const bool ok = next >= -1 && next < at;
@@ -172,31 +209,24 @@ __device__ inline uint32_t code_pair(uint32_t w) {
 __device__ inline uint32_t low_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ inline uint32_t high_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-template <int kBytes> struct Raw;  // kBytes of a row, in words
-template <> struct Raw<1> {
-  uint32_t w[1];
-  __device__ inline void load(const uint8_t* p) { w[0] = *p; }
-};
-template <> struct Raw<2> {
-  uint32_t w[1];
-  __device__ inline void load(const uint8_t* p) { w[0] = *reinterpret_cast<const uint16_t*>(p); }
-};
-template <> struct Raw<4> {
-  uint32_t w[1];
-  __device__ inline void load(const uint8_t* p) { w[0] = *reinterpret_cast<const uint32_t*>(p); }
-};
-template <> struct Raw<8> {
-  uint32_t w[2];
-  __device__ inline void load(const uint8_t* p) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x, w[1] = v.y;
-  }
-};
-template <> struct Raw<16> {
-  uint32_t w[4];
-  __device__ inline void load(const uint8_t* p) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+// kBytes of a row, in words.  They come through buffer descriptors: one without records
+// reads as zeros with no branch and no traffic, so a loop's last requests need no
+// condition (behind one the compiler would wait for them as if they had been made).
+template <int kBytes>
+struct Raw {
+  uint32_t w[kBytes < 4 ? 1 : kBytes / 4];
+  __device__ inline void load(__amdgpu_buffer_rsrc_t r, int offset) {
+    if constexpr (kBytes == 1) w[0] = __builtin_amdgcn_raw_buffer_load_b8(r, offset, 0, 0);
+    if constexpr (kBytes == 2) w[0] = __builtin_amdgcn_raw_buffer_load_b16(r, offset, 0, 0);
+    if constexpr (kBytes == 4) w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, offset, 0, 0);
+    if constexpr (kBytes == 8) {
+      const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(r, offset, 0, 0);
+      w[0] = v[0], w[1] = v[1];
+    }
+    if constexpr (kBytes == 16) {
+      const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0);
+      w[0] = v[0], w[1] = v[1], w[2] = v[2], w[3] = v[3];
+    }
   }
 };
 
@@ -210,195 +240,164 @@ struct CachedCfg {
   static constexpr int kRow = kD * kEsz;          // bytes
 };
 
-// A tile's bytes, as loaded.
-template <int kType, int kD>
-struct RawTile {
-  using C = CachedCfg<kType, kD>;
-  Raw<8 * C::kEsz> k[2][C::kSteps];
-  Raw<C::kC * C::kEsz> v[8];
-  f32x4 ks[2], vs[2];  // 8-bit types
+// What a call needs beside the sequence, the same for every row.
+struct CallScores {
+  float factor;  // of a product before its key's scale: log2(e) / sqrt(D), or what the cap takes
+  float cap_in, cap_out;
+  bool slopes;
 };
 
+// Reductions over the sixteen lanes of a row of the wave (n), left in all of them.
+template <typename Op>
+__device__ inline uint32_t reduce16(uint32_t v, Op op) {
+  const auto step = [&](auto ctrl) {
+    v = op(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, decltype(ctrl)::value, 0xf, 0xf, false));
+  };
+  step(std::integral_constant<int, 0xB1>{});   // quad_perm [1, 0, 3, 2]
+  step(std::integral_constant<int, 0x4E>{});   // quad_perm [2, 3, 0, 1]
+  step(std::integral_constant<int, 0x141>{});  // row_half_mirror
+  step(std::integral_constant<int, 0x140>{});  // row_mirror
+  return v;
+}
+
+// The rows' queries as operands, for all of a workgroup's waves.
 template <int kType, int kD, int kR>
-__global__ __launch_bounds__(256, kD > 64 && kR * (kType == FC_CACHE_BF16 ? 2 : 1) == 4 ? 1 : 2) void cached_attn_kernel(CachedAttnArgs a) {
+struct Queries {
   using C = CachedCfg<kType, kD>;
-  constexpr bool k8 = kType != FC_CACHE_BF16;
-  constexpr int kRows = 16 * kR;
-  constexpr int kPad = kD + 4;  // floats of a row of the exchange: its lanes' stores spread over the banks
-  __shared__ Nodes nodes;
-  __shared__ float exchange[4 * 16 * kPad];
-  __shared__ float2 wave_stats[4][kRows];
+  bf16x8 unit[kR][C::kSteps][64];
 
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
-  // Workgroups go to the XCDs in turn: the row groups of one slot, which read the
-  // same keys, are 8 workgroups apart, on one XCD and running together.
-  const int id = blockIdx.x, of8 = id / 8;
-  const int rg = of8 % a.groups, rest = of8 / a.groups * 8 + id % 8;
-  const int h = rest / a.items, x = rest - h * a.items;
-  if (h >= a.g.Hkv) return;
-  const Slot slot = find_slot(a, x, -1);
-  if (slot.b < 0) return;
-  const int b = slot.b;
-  const Span span = span_at(a, b);
-  const int length = __builtin_amdgcn_readfirstlane(span.length), count = __builtin_amdgcn_readfirstlane(span.count);
-  const int tile0 = __builtin_amdgcn_readfirstlane(span.first) + slot.part * slot.tiles;
-  const int tile1 = min(tile0 + slot.tiles, __builtin_amdgcn_readfirstlane(span.first + span.tiles));
-  const int end = min(length + count, a.g.capacity);
+  // All 256 threads, sixteen to a row: load, then store, which waits for the values.  Returns
+  // which there are; the others, of which any may be read, are stored as zeros.
+  __device__ static inline uint32_t load(bf16x8 (&to)[kR], const CachedAttnArgs& a, int b, int h, int first_row, int count) {
+    uint32_t there = 0;
+#pragma unroll
+    for (int rb = 0; rb < kR; ++rb) {
+      const int row = first_row + 16 * rb + (int)(threadIdx.x >> 4), node = row / a.G, u = threadIdx.x & 15;
+      const bool mine = node < count && u < C::kU;
+      const bf16* src = static_cast<const bf16*>(a.Q);
+      src += mine ? (((int64_t)b * a.N + node) * a.H + h * a.G + row - node * a.G) * kD + 8 * u : 0;
+      to[rb] = *reinterpret_cast<const bf16x8*>(src);
+      there |= mine ? 1u << rb : 0;
+    }
+    return there;
+  }
+  __device__ inline void store(const bf16x8 (&from)[kR], uint32_t there) {
+    const int n = threadIdx.x >> 4, u = threadIdx.x & 15;
+#pragma unroll
+    for (int rb = 0; rb < kR; ++rb)
+      if (u < 4 * C::kSteps) unit[rb][u % C::kSteps][n + 16 * (u / C::kSteps)] = (there >> rb & 1) != 0 ? from[rb] : Mma<bf16>::zero();
+  }
+};
 
-  if (wave == 0) trace_nodes(&nodes, a.parents == nullptr ? nullptr : a.parents + (a.tree == 2 ? (int64_t)b * a.N : 0), a.N, a.left);
-  __syncthreads();
-
-  // This lane's row of each block of 16: its node's view, and its slope.
-  uint64_t sees[kR];
-  int low[kR], at[kR];
+// kR blocks of sixteen rows of a KV head, one to each lane n: what they see, their queries
+// and their sums.
+template <int kType, int kD, int kR>
+struct Rows {
+  using C = CachedCfg<kType, kD>;
+  static constexpr bool k8 = kType != FC_CACHE_BF16;
+  uint64_t sees[kR], any_sees;  // nodes that the row, and that any of them all sees
+  int low[kR], any_low;         // first key of the sequence, likewise (INT_MAX: none)
+  int all_low;                  // behind which every row sees every key of the sequence
+  int at[kR];                   // the row's position in the text
   float slope2[kR];
-  bool broken[kR];  // NaN
-  bf16x8 q[kR][C::kSteps];
-  uint64_t any_sees = 0;
-  int any_low = INT_MAX, all_low = 0;  // the first key any row sees, and the first that all do
-#pragma unroll
-  for (int rb = 0; rb < kR; ++rb) {
-    const int row = rg * kRows + rb * 16 + n, node = row / a.G, head = h * a.G + row - node * a.G;
-    const bool there = row < a.rows && node < count;
-    const int depth = there ? nodes.depth[node] : 0;
-    broken[rb] = there && (depth < 0 || node >= a.g.capacity - length);
-    sees[rb] = there && !broken[rb] ? nodes.sees[node] : 0;
-    at[rb] = length + depth;
-    low[rb] = there && !broken[rb] ? max(at[rb] - a.left, 0) : INT_MAX;
-    slope2[rb] = a.slopes != nullptr && there ? base2_slope(a.slopes[head]) : 0.0f;
-    any_sees |= sees[rb];
-    any_low = min(any_low, low[rb]);
-    // (rows that are not there, or broken, may take whatever comes)
-    all_low = max(all_low, there && !broken[rb] ? low[rb] : 0);
-    const bf16* src = static_cast<const bf16*>(a.Q) + (((int64_t)b * a.N + node) * a.H + head) * kD;
-#pragma unroll
-    for (int s = 0; s < C::kSteps; ++s) {
-      const int u = g * C::kSteps + s;
-      q[rb][s] = there && u < C::kU ? *reinterpret_cast<const bf16x8*>(src + 8 * u) : Mma<bf16>::zero();
-    }
-  }
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) {
-    any_sees |= __shfl_xor(any_sees, o);
-    any_low = min(any_low, __shfl_xor(any_low, o));
-    all_low = max(all_low, __shfl_xor(all_low, o));
-  }
-  any_low = __builtin_amdgcn_readfirstlane(any_low);
-  all_low = __builtin_amdgcn_readfirstlane(all_low);
-
-  f32x4 acc[kR][C::kC];
+  bool broken[kR];              // NaN
+  f32x4 acc[kR][C::kC];         // column C (4 g + r) + c of lane n's row
   float ref[kR], sum[kR];
+
+  __device__ inline void begin(const CachedAttnArgs& a, const Nodes& nodes, int b, int h, int first_row, int length, int count) {
+    const int n = threadIdx.x & 15;
+    any_sees = 0;
+    any_low = INT_MAX;
+    all_low = 0;
 #pragma unroll
-  for (int rb = 0; rb < kR; ++rb) {
-    ref[rb] = -1e30f;
-    sum[rb] = 0.0f;
+    for (int rb = 0; rb < kR; ++rb) {
+      const int row = first_row + 16 * rb + n, node = row / a.G, head = h * a.G + row - node * a.G;
+      const bool there = row < a.rows && node < count;
+      const int depth = there ? nodes.depth[node] : 0;
+      broken[rb] = there && (depth < 0 || node >= a.g.capacity - length);
+      sees[rb] = there && !broken[rb] ? nodes.sees[node] : 0;
+      at[rb] = length + depth;
+      low[rb] = there && !broken[rb] ? max(at[rb] - a.left, 0) : INT_MAX;
+      slope2[rb] = a.slopes != nullptr && there ? base2_slope(a.slopes[head]) : 0.0f;
+      any_sees |= sees[rb];
+      any_low = min(any_low, low[rb]);
+      all_low = max(all_low, there && !broken[rb] ? low[rb] : 0);  // (rows that are not there, or broken, may take whatever comes)
+      ref[rb] = -1e30f;
+      sum[rb] = 0.0f;
 #pragma unroll
-    for (int c = 0; c < C::kC; ++c) acc[rb][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int c = 0; c < C::kC; ++c) acc[rb][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const auto either = [](uint32_t x, uint32_t y) { return x | y; };
+    any_sees = (uint64_t)reduce16((uint32_t)(any_sees >> 32), either) << 32 | reduce16((uint32_t)any_sees, either);
+    any_low = __builtin_amdgcn_readfirstlane((int)reduce16((uint32_t)any_low, [](uint32_t x, uint32_t y) { return min(x, y); }));
+    all_low = __builtin_amdgcn_readfirstlane((int)reduce16((uint32_t)all_low, [](uint32_t x, uint32_t y) { return max(x, y); }));
   }
 
-  // A block of 16 keys lies in one page: its first row, and whether that page is one.
-  struct Place {
-    int64_t row;
-    bool good;
-  };
-  const auto place = [&](int key) {
-    key = key < end ? key : end - 1 - (end - 1) % 16;  // (a tile's second block may begin past the end)
-    const int64_t page = cache_page(a.g, a.table, b, key);
-    Place p;
-    p.good = page >= 0;
-    const int64_t row = ((p.good ? page : 0) * a.g.Hkv + h) * a.g.page_size + cache_place(a.g, a.table, key);
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)row), hi = __builtin_amdgcn_readfirstlane((uint32_t)(row >> 32));
-    p.row = (int64_t)(((uint64_t)hi << 32) | lo);
-    return p;
-  };
-  RawTile<kType, kD> t;
-  Place here[2];  // of the tile whose bytes are in t or on their way
-  const float factor0 = a.cap_in > 0.0f ? a.cap_in : a.scale_log2;
-  const auto load_k = [&](const Place (&p)[2]) {
+  // Which of a lane's eight keys are set in a mask of 32 from key 4 g on, as halves of
+  // the operands' words: keys 2 i and 2 i + 1.
+  __device__ static inline u32x4 halves(uint32_t keys) {
+    u32x4 m;
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      const uint8_t* kr = static_cast<const uint8_t*>(a.k) + p[kb].row * C::kRow;
-#pragma unroll
-      for (int s = 0; s < C::kSteps; ++s) {
-        const int u = g * C::kSteps + s;  // (units past the row: its last one, left out below)
-        t.k[kb][s].load(kr + n * C::kRow + 8 * C::kEsz * (4 * C::kSteps == C::kU ? u : min(u, C::kU - 1)));
-      }
-      if (k8) t.ks[kb] = *reinterpret_cast<const f32x4*>(a.k_scale + p[kb].row + 4 * g);
+    for (int i = 0; i < 4; ++i) {
+      const int bit = 16 * (i >> 1) + 2 * (i & 1);
+      m[i] = ((keys >> bit & 1) != 0 ? 0xffffu : 0u) | ((keys >> bit & 2) != 0 ? 0xffff0000u : 0u);
     }
-  };
-  const auto load_v = [&](const Place (&p)[2]) {
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      const uint8_t* vr = static_cast<const uint8_t*>(a.v) + p[kb].row * C::kRow;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        t.v[4 * kb + r].load(vr + (4 * g + r) * C::kRow + C::kC * C::kEsz * (C::kLanes == 16 ? n : min(n, C::kLanes - 1)));
-      if (k8) t.vs[kb] = *reinterpret_cast<const f32x4*>(a.v_scale + p[kb].row + 4 * g);
-    }
-  };
+    return m;
+  }
 
-  // A tile; the next one's bytes are requested as soon as this one's leave their registers.
-  const auto process = [&](bool masked, int key0, bool more) {
-    // S^T of the two blocks: lane n's query, keys key0 + 16 kb + 4 g + r.
-    f32x4 s[kR][2], factor[2];
+  // Keys key0 .. key0 + 31.  Of `keys`: frag(kb, step), scale(kb) of keys 4 g + r, used() once
+  // both are; of `values`: frag(c), scale(kb), and for keys of which some row may be blind
+  // keep(mask: which of the 32 keys from 4 g on any row sees), finite() (non-finite values
+  // become zeros).
+  template <typename Keys, typename Values>
+  __device__ inline void tile(const CallScores& call, const Queries<kType, kD, kR>& queries, const Nodes& nodes, int N, int key0, int length, Keys& keys, Values& values) {
+    const int g = (threadIdx.x & 63) >> 4;
+    // Every row sees every key of a tile before the nodes and behind all rows' first keys.
+    const bool masked = key0 < all_low || key0 + kTileKeys > length;
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));  // (the queries would be kept in registers from tile to tile)
+    f32x4 s[kR][2];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
       for (int rb = 0; rb < kR; ++rb) s[rb][kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int st = 0; st < C::kSteps; ++st) {
-        uint32_t w[4];
-        if constexpr (k8) {
-          w[0] = code_pair<kType, false>(t.k[kb][st].w[0]);
-          w[1] = code_pair<kType, true>(t.k[kb][st].w[0]);
-          w[2] = code_pair<kType, false>(t.k[kb][st].w[1]);
-          w[3] = code_pair<kType, true>(t.k[kb][st].w[1]);
-        } else {
+        const bf16x8 f = keys.frag(kb, st);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = t.k[kb][st].w[i];
-        }
-        if (4 * C::kSteps != C::kU && g * C::kSteps + st >= C::kU) w[0] = w[1] = w[2] = w[3] = 0;
-        const bf16x8 kf = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
-#pragma unroll
-        for (int rb = 0; rb < kR; ++rb) s[rb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[rb][st], s[rb][kb], 0, 0, 0);
+        for (int rb = 0; rb < kR; ++rb) s[rb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, queries.unit[rb][st][lane], s[rb][kb], 0, 0, 0);
       }
-      const float c = here[kb].good ? factor0 : NAN;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) factor[kb][r] = k8 ? c * t.ks[kb][r] : c;
-    }
-    if (more) {
-      const int key = key0 + 4 * kTileKeys;
-      here[0] = place(key);
-      here[1] = place(key + 16);
-      load_k(here);
     }
     // Scores in base 2.
 #pragma unroll
-    for (int rb = 0; rb < kR; ++rb)
+    for (int kb = 0; kb < 2; ++kb) {
+      const f32x4 f = keys.scale(kb, call.factor);
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) s[rb][kb] *= factor[kb];
-    if (a.cap_in > 0.0f) {
+      for (int rb = 0; rb < kR; ++rb) s[rb][kb] *= f;
+    }
+    keys.used();
+    if (call.cap_in > 0.0f) {
 #pragma unroll
       for (int rb = 0; rb < kR; ++rb)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[rb][kb][r] = __builtin_fmaf(-2.0f * a.cap_out, cap_part(s[rb][kb][r], 1.0f), a.cap_out);
+          for (int r = 0; r < 4; ++r) s[rb][kb][r] = __builtin_fmaf(-2.0f * call.cap_out, cap_part(s[rb][kb][r], 1.0f), call.cap_out);
     }
-    if (a.slopes != nullptr) {
+    int g4 = 4 * g;
+    asm volatile("" : "+v"(g4));  // (what follows from it would be kept from tile to tile)
+    if (call.slopes) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int key = key0 + 16 * kb + 4 * g + r;
-          const int pos = masked && key >= length && key < length + a.N ? length + nodes.depth[key - length] : key;
+          const int key = key0 + 16 * kb + g4 + r;
+          const int pos = masked && key >= length && key < length + N ? length + nodes.depth[key - length] : key;
 #pragma unroll
           for (int rb = 0; rb < kR; ++rb) s[rb][kb][r] = __builtin_fmaf(-slope2[rb], (float)(at[rb] - pos), s[rb][kb][r]);
         }
     }
-    int g4 = 4 * g;
     if (masked) {
-      asm volatile("" : "+v"(g4));  // (what follows from it would be kept from tile to tile)
 #pragma unroll
       for (int rb = 0; rb < kR; ++rb) {
         const uint32_t seen = seen_keys(key0 + g4, low[rb], sees[rb], length);
@@ -430,234 +429,462 @@ __global__ __launch_bounds__(256, kD > 64 && kR * (kType == FC_CACHE_BF16 ? 2 : 
         for (int c = 0; c < C::kC; ++c) acc[rb][c] *= by;
       }
     }
-    bf16x8 pf[kR], pl[kR];
+    u32x4 ph[kR], pl[kR];
 #pragma unroll
     for (int rb = 0; rb < kR; ++rb) {
-      bf16x8 f, f2;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float e = __builtin_amdgcn_exp2f(s[rb][j >> 2][j & 3] - ref[rb]);
-        sum[rb] += e;
-        if (k8) e *= t.vs[j >> 2][j & 3];
-        f[j] = static_cast<bf16>(e);
-        f2[j] = static_cast<bf16>(e - static_cast<float>(f[j]));
+      for (int kb = 0; kb < 2; ++kb) {
+        f32x4 e;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          e[r] = __builtin_amdgcn_exp2f(s[rb][kb][r] - ref[rb]);
+          sum[rb] += e[r];
+        }
+        if (k8) e *= values.scale(kb);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t hi = pair(e[2 * i], e[2 * i + 1]);
+          ph[rb][2 * kb + i] = hi;
+          pl[rb][2 * kb + i] = pair(e[2 * i] - __builtin_bit_cast(float, hi << 16), e[2 * i + 1] - __builtin_bit_cast(float, hi & 0xffff0000u));
+        }
       }
-      pf[rb] = f;
-      pl[rb] = f2;
     }
-    // V's columns: word i of key j holds columns 2 i and 2 i + 1.
-    constexpr int kW = (C::kC + 1) / 2;
-    uint32_t col[8][kW];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int i = 0; i < kW; ++i)
-        col[j][i] = !k8 ? t.v[j].w[i] : (i & 1) != 0 ? code_pair<kType, true>(t.v[j].w[i / 2]) : code_pair<kType, false>(t.v[j].w[i / 2]);
-    // The c-th product's operand.
-    const auto column = [&](int c, auto word) {
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t x = word(2 * i, c / 2), y = word(2 * i + 1, c / 2);
-        w[i] = (c & 1) != 0 ? high_halves(x, y) : low_halves(x, y);
-      }
-      return as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
-    };
     if (masked) {
-      if (k8) {  // (a scale may be NaN)
+      values.keep(seen_keys(key0 + g4, any_low, any_sees, length));
+      if (k8) {  // (an unseen key's scale may be NaN; codes are finite)
 #pragma unroll
         for (int rb = 0; rb < kR; ++rb) {
-          const uint32_t seen = seen_keys(key0 + g4, low[rb], sees[rb], length);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const bool in = (seen >> (16 * (j >> 2) + (j & 3)) & 1) != 0;
-            pf[rb][j] = in ? pf[rb][j] : static_cast<bf16>(0.0f);
-            pl[rb][j] = in ? pl[rb][j] : static_cast<bf16>(0.0f);
-          }
+          const u32x4 mine = halves(seen_keys(key0 + g4, low[rb], sees[rb], length));
+          ph[rb] &= mine;
+          pl[rb] &= mine;
         }
-      }
-      const uint32_t any_seen = seen_keys(key0 + g4, any_low, any_sees, length);
-      bool odd = false;  // a value that is not finite where some row sees it
+      } else {
+        bool odd = false;  // a value that is not finite where some row sees it
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool in = (any_seen >> (16 * (j >> 2) + (j & 3)) & 1) != 0;
+        for (int c = 0; c < C::kC; ++c) {
+          const u32x4 v = __builtin_bit_cast(u32x4, values.frag(c));
 #pragma unroll
-        for (int i = 0; i < kW; ++i) {
-          col[j][i] = in ? col[j][i] : 0;
-          if (!k8) odd |= (col[j][i] & 0x7f80u) == 0x7f80u || (col[j][i] & 0x7f800000u) == 0x7f800000u;
+          for (int i = 0; i < 4; ++i) odd |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
         }
-      }
-      if (!k8 && __ballot(odd) != 0) {
-        // Rare (and codes of 8 bits are finite).  Which rows see +infinity, -infinity or NaN in which columns: products of
-        // ones; such a value is added to those rows alone and is 0 in the others' product.
+        if (__ballot(odd) != 0) {
+          // Rare.  Which rows see +infinity, -infinity or NaN in which columns: a product of
+          // ones; such a value is added to those rows alone and is 0 in the others' product.
 #pragma unroll 1
-        for (int kind = 0; kind < 3; ++kind) {
-          const auto is = [&](uint32_t half) {
-            return kind == 0 ? half == 0x7f80u : kind == 1 ? half == 0xff80u : (half & 0x7fffu) > 0x7f80u;
-          };
-          const auto flags = [&](int j, int i) {
-            return (is(col[j][i] & 0xffffu) ? 0x3f80u : 0) | (is(col[j][i] >> 16) ? 0x3f800000u : 0);
-          };
-          const float what = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN;
+          for (int kind = 0; kind < 3; ++kind) {
+            const auto is = [&](uint32_t half) {
+              return kind == 0 ? half == 0x7f80u : kind == 1 ? half == 0xff80u : (half & 0x7fffu) > 0x7f80u;
+            };
+            const float what = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN;
 #pragma unroll
-          for (int c = 0; c < C::kC; ++c) {
-            const bf16x8 vf = column(c, flags);
+            for (int c = 0; c < C::kC; ++c) {
+              const u32x4 v = __builtin_bit_cast(u32x4, values.frag(c));
+              u32x4 flags;
 #pragma unroll
-            for (int rb = 0; rb < kR; ++rb) {
-              const uint32_t seen = seen_keys(key0 + g4, low[rb], sees[rb], length);
-              bf16x8 ones;
+              for (int i = 0; i < 4; ++i) flags[i] = (is(v[i] & 0xffffu) ? 0x3f80u : 0) | (is(v[i] >> 16) ? 0x3f800000u : 0);
 #pragma unroll
-              for (int j = 0; j < 8; ++j) ones[j] = static_cast<bf16>((seen >> (16 * (j >> 2) + (j & 3)) & 1) != 0 ? 1.0f : 0.0f);
-              const f32x4 found = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, ones, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+              for (int rb = 0; rb < kR; ++rb) {
+                const bf16x8 ones = __builtin_bit_cast(bf16x8, halves(seen_keys(key0 + g4, low[rb], sees[rb], length)) & 0x3f803f80u);
+                const f32x4 found =
+                    __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, flags), ones, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
-              for (int r = 0; r < 4; ++r) acc[rb][c][r] += found[r] > 0.0f ? what : 0.0f;
+                for (int r = 0; r < 4; ++r) acc[rb][c][r] += found[r] > 0.0f ? what : 0.0f;
+              }
             }
           }
+          values.finite();
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int i = 0; i < kW; ++i) {
-            if ((col[j][i] & 0x7f80u) == 0x7f80u) col[j][i] &= 0xffff0000u;
-            if ((col[j][i] & 0x7f800000u) == 0x7f800000u) col[j][i] &= 0xffffu;
-          }
       }
     }
 #pragma unroll
     for (int c = 0; c < C::kC; ++c) {
-      const bf16x8 vf = column(c, [&](int j, int i) { return col[j][i]; });
+      const bf16x8 f = values.frag(c);
 #pragma unroll
-      for (int rb = 0; rb < kR; ++rb) acc[rb][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[rb], acc[rb][c], 0, 0, 0);
+      for (int rb = 0; rb < kR; ++rb) acc[rb][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, ph[rb]), acc[rb][c], 0, 0, 0);
 #pragma unroll
-      for (int rb = 0; rb < kR; ++rb) acc[rb][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl[rb], acc[rb][c], 0, 0, 0);
-    }
-    if (more) load_v(here);
-  };
-
-  int tile = tile0 + wave;
-  if (tile < tile1 && count > 0) {
-    here[0] = place(tile * kTileKeys);
-    here[1] = place(tile * kTileKeys + 16);
-    load_k(here);
-    load_v(here);
-    while (true) {
-      const int key0 = tile * kTileKeys;
-      const bool more = tile + 4 < tile1;
-      // Every row sees every key of a tile before the nodes and behind all rows' first keys.
-      process(key0 < all_low || key0 + kTileKeys > length, key0, more);
-      if (!more) break;
-      tile += 4;
+      for (int rb = 0; rb < kR; ++rb) acc[rb][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, pl[rb]), acc[rb][c], 0, 0, 0);
     }
   }
+};
+// A word's halves that are no finite bf16, as zeros.
+__device__ inline uint32_t finite_halves(uint32_t w) {
+  return w & ((w & 0x7f80u) == 0x7f80u ? 0xffff0000u : ~0u) & ((w & 0x7f800000u) == 0x7f800000u ? 0xffffu : ~0u);
+}
 
-  // Join the four waves: each row's largest reference, then the sums.
+// The K operand of 8 neighbouring values, and the V operands of eight keys' C columns.
+template <int kType>
+__device__ inline bf16x8 key_operand(const uint32_t* w) {
+  if constexpr (kType == FC_CACHE_BF16) return as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+  else return as_bf16x8(make_uint4(code_pair<kType, false>(w[0]), code_pair<kType, true>(w[0]), code_pair<kType, false>(w[1]), code_pair<kType, true>(w[1])));
+}
+// Column c of two keys' columns.
+template <int kType>
+__device__ inline uint32_t two_keys(const uint32_t* x, const uint32_t* y, int c) {
+  if constexpr (kType == FC_CACHE_I8) {  // (the rounding to bf16 pairs them)
+    return pair((float)(int8_t)(x[c / 4] >> 8 * (c % 4) & 0xff), (float)(int8_t)(y[c / 4] >> 8 * (c % 4) & 0xff));
+  } else {
+    uint32_t u, v;
+    if constexpr (kType == FC_CACHE_BF16) {
+      u = x[c / 2], v = y[c / 2];
+    } else if (c / 2 % 2 != 0) {
+      u = code_pair<kType, true>(x[c / 4]), v = code_pair<kType, true>(y[c / 4]);
+    } else {
+      u = code_pair<kType, false>(x[c / 4]), v = code_pair<kType, false>(y[c / 4]);
+    }
+    return c % 2 != 0 ? high_halves(u, v) : low_halves(u, v);
+  }
+}
+
+// Where a sequence's 16-key blocks lie.  Lane i holds the page of the wave's i-th block
+// from here, 64 at a time: a look at the table for each tile would wait for everything
+// the wave has on its way (64 x 4096 int8 keys in pages of 64: 64 us for 51).
+struct Blocks {
+  int page;
+  // Blocks at key, key + step, ...
+  __device__ inline void fetch(const CachedAttnArgs& a, int b, int key, int step, int end) {
+    const int mine = key + step * (int)(threadIdx.x & 63);
+    page = mine < end ? (int)cache_page(a.g, a.table, b, mine) : 0;
+  }
+  // The i-th block, which begins at key: its page's number (-1: none) and its first row.
+  __device__ inline int64_t row(const CachedAttnArgs& a, int h, int i, int key, int* number) const {
+    const int p = __builtin_amdgcn_readlane(page, i);
+    *number = p;
+    return ((int64_t)max(p, 0) * a.g.Hkv + h) * a.g.page_size + cache_place(a.g, a.table, key);
+  }
+};
+
+// The kSteps operands' bytes of a K row, from offset on.
+template <int kType, int kSteps>
+__device__ inline void load_steps(Raw<kType == FC_CACHE_BF16 ? 16 : 8> (&k)[kSteps], __amdgpu_buffer_rsrc_t r, int offset) {
+  if constexpr (kType != FC_CACHE_BF16 && kSteps % 2 == 0) {  // 16 bytes at a time
+#pragma unroll
+    for (int s = 0; s < kSteps; s += 2) {
+      Raw<16> two;
+      two.load(r, offset + 8 * s);
+      k[s].w[0] = two.w[0], k[s].w[1] = two.w[1], k[s + 1].w[0] = two.w[2], k[s + 1].w[1] = two.w[3];
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) k[s].load(r, offset + (kType == FC_CACHE_BF16 ? 16 : 8) * s);
+  }
+}
+
+// A block's sixteen rows, as descriptors without records where it is not there.
+template <int kType, int kD>
+struct BlockBytes {
+  using C = CachedCfg<kType, kD>;
+  __amdgpu_buffer_rsrc_t k, v, ks, vs;
+  __device__ inline void set(const CachedAttnArgs& a, int64_t row, bool there) {
+    const uint32_t rows = there ? 16 : 0;
+    k = make_rsrc(static_cast<const char*>(a.k) + row * C::kRow, rows * C::kRow);
+    v = make_rsrc(static_cast<const char*>(a.v) + row * C::kRow, rows * C::kRow);
+    if constexpr (kType != FC_CACHE_BF16) {
+      ks = make_rsrc(a.k_scale + row, 4 * rows);
+      vs = make_rsrc(a.v_scale + row, 4 * rows);
+    }
+  }
+};
+// Offsets in a block of lane (n, g)'s parts of K (step 0; a unit past the row reads the next
+// one's, or zeros, and is left out of the operand) and V (row 4 g).
+template <int kType, int kD>
+struct LaneOffsets {
+  using C = CachedCfg<kType, kD>;
+  int k, v;
+  __device__ inline LaneOffsets() {
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    k = n * C::kRow + 8 * C::kEsz * g * C::kSteps;
+    v = 4 * g * C::kRow + C::kC * C::kEsz * (C::kLanes == 16 ? n : min(n, C::kLanes - 1));
+  }
+};
+
+// The stretches of a workgroup, sequence by sequence: body(b, length, count, first tile, last tile, whole, slot).
+template <typename Body>
+__device__ inline void for_each_stretch(const CachedAttnArgs& a, int x, Body body) {
+  Line line{0, 0, x, {}};
+  if (a.shares > 0)
+    line = find_on_line(a, x, -1);
+  else
+    line.chunk.load(a, x);
+  bool again = false;
+  for (int b = line.b; b < a.g.B; ++b) {
+    const int64_t start = line.start;
+    if (a.shares > 0 && start >= (x + 1) * line.share) break;
+    const Span span = line.chunk.of(a, b);
+    Stretch st{0, span.tiles};
+    if (a.shares > 0) {
+      line.start += span.tiles + kBegin;
+      st = stretch_of(start, span.tiles, x, line.share);
+      if (st.first >= st.last) continue;
+    }
+    if (again) __syncthreads();  // the last sequence's LDS is read
+    again = true;
+    body(b, span.length, span.count, span.first + st.first, span.first + st.last, st.first == 0 && st.last == span.tiles,
+         part_slot(start, x, line.share));
+    if (a.shares == 0) break;
+  }
+}
+
+// Which KV head, row group and share a workgroup has.  Workgroups go to the XCDs in
+// turn: the row groups of one share, which read the same keys, are 8 workgroups apart, on
+// one XCD and running together.
+struct Place {
+  int h, group, x;
+};
+__device__ inline Place place_of(const CachedAttnArgs& a) {
+  const int id = blockIdx.x, of8 = id / 8, rest = of8 / a.groups * 8 + id % 8, per_head = a.shares > 0 ? a.shares : a.g.B;
+  Place p;
+  p.group = of8 % a.groups;
+  p.h = rest / per_head;
+  p.x = rest - p.h * per_head;
+  return p;
+}
+
+// A stretch's end: each of four waves holds sums of the workgroup's rows over some of its keys.
+template <int kD, int kR>
+struct Exchange {
+  static constexpr int kPad = kD + 4;  // floats of a row: the lanes' stores spread over the banks
+  float acc[kR][4][16 * kPad];
+  float2 stats[kR][4][16];
+};
+template <int kType, int kD, int kR>
+__device__ inline void finish(const CachedAttnArgs& a, const Rows<kType, kD, kR>& rows, Exchange<kD, kR>& x, int b, int h, int group,
+                              int count, bool whole, int64_t slot) {
+  using C = CachedCfg<kType, kD>;
+  constexpr int kPad = Exchange<kD, kR>::kPad, kRows = 16 * kR;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int rb = 0; rb < kR; ++rb) {
-    float l = sum[rb];
+    float l = rows.sum[rb];
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    if (g == 0) wave_stats[wave][rb * 16 + n] = make_float2(ref[rb], broken[rb] ? NAN : l);
+    if (g == 0) x.stats[rb][wave][n] = make_float2(rows.ref[rb], rows.broken[rb] ? NAN : l);
+    float* to = x.acc[rb][wave] + n * kPad;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int d = C::kC * (4 * g + r);
+      if (C::kLanes != 16 && d >= kD) continue;
+#pragma unroll
+      for (int c = 0; c < C::kC; ++c) to[d + c] = rows.acc[rb][c][r];
+    }
   }
   __syncthreads();
-  const bool whole = slot.parts == 1;
-  const int64_t out_slot = ((int64_t)h * a.groups + rg) * a.items + x;
-#pragma unroll
+  // Sixteen threads to a row, four columns each at a time.
+  const int of16 = tid >> 4;
+  const int64_t out = (((int64_t)h * a.groups + group) * 2 * a.shares + slot) * kRows;
+#pragma unroll 1
   for (int rb = 0; rb < kR; ++rb) {
-    const int rr = rb * 16 + n;
-    const float2 st0 = wave_stats[0][rr], st1 = wave_stats[1][rr], st2 = wave_stats[2][rr], st3 = wave_stats[3][rr];
-    const float m = fmaxf(fmaxf(st0.x, st1.x), fmaxf(st2.x, st3.x));
-    const float by = __builtin_amdgcn_exp2f(ref[rb] - m);
-    if (rb > 0) __syncthreads();
-    float* to = exchange + (wave * 16 + n) * kPad;
+    const int row = group * kRows + 16 * rb + of16, node = row / a.G, head = h * a.G + row - node * a.G;
+    if (row >= a.rows) break;
+    float by[4], m = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int w = 0; w < 4; ++w) m = fmaxf(m, x.stats[rb][w][of16].x);
 #pragma unroll
-      for (int c = 0; c < C::kC; ++c) {
-        const int d = C::kC * (4 * g + r) + c;
-        if (C::kLanes == 16 || d < kD) to[d] = acc[rb][c][r] * by;
-      }
-    if (wave == 0 && g == 0 && !whole) {
-      const float l = st0.y * __builtin_amdgcn_exp2f(st0.x - m) + st1.y * __builtin_amdgcn_exp2f(st1.x - m) +
-                      st2.y * __builtin_amdgcn_exp2f(st2.x - m) + st3.y * __builtin_amdgcn_exp2f(st3.x - m);
-      a.part_s[out_slot * kRows + rr] = make_float2(m, l);
+    for (int w = 0; w < 4; ++w) {
+      const float2 st = x.stats[rb][w][of16];
+      by[w] = __builtin_amdgcn_exp2f(st.x - m);
+      sum += st.y * by[w];
     }
-    __syncthreads();
-    // 256 threads: row tid / 16, columns of tid % 16.
-    const int orow = tid >> 4, ox = tid & 15;
-    const float2 w0 = wave_stats[0][rb * 16 + orow], w1 = wave_stats[1][rb * 16 + orow], w2 = wave_stats[2][rb * 16 + orow],
-                 w3 = wave_stats[3][rb * 16 + orow];
-    const float om = fmaxf(fmaxf(w0.x, w1.x), fmaxf(w2.x, w3.x));
-    const float l = w0.y * __builtin_amdgcn_exp2f(w0.x - om) + w1.y * __builtin_amdgcn_exp2f(w1.x - om) +
-                    w2.y * __builtin_amdgcn_exp2f(w2.x - om) + w3.y * __builtin_amdgcn_exp2f(w3.x - om);
-    const int row = rg * kRows + rb * 16 + orow, node = row / a.G, head = h * a.G + row - node * a.G;
-    const float inv = 1.0f / l;
-    if (row < a.rows) {
-      bf16* O = static_cast<bf16*>(a.O) + (((int64_t)b * a.N + node) * a.H + head) * kD;
-      float* P = a.part_o + (out_slot * kRows + rb * 16 + orow) * kD;
-      for (int d = 4 * ox; d < kD; d += 64) {
-        f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (!whole && (tid & 15) == 0) a.part_s[out + 16 * rb + of16] = make_float2(m, sum);
+    const float inv = 1.0f / sum;
+    bf16* O = static_cast<bf16*>(a.O) + (((int64_t)b * a.N + node) * a.H + head) * kD;
+    for (int d = 4 * (tid & 15); d < kD; d += 64) {
+      f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(exchange + (w * 16 + orow) * kPad + d);
-        if (whole) {
-          v = node < count ? v * inv : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-          *reinterpret_cast<uint2*>(O + d) = make_uint2(pair(v[0], v[1]), pair(v[2], v[3]));
-        } else {
-          *reinterpret_cast<f32x4*>(P + d) = v;
-        }
+      for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(x.acc[rb][w] + of16 * kPad + d) * by[w];
+      if (whole) {
+        v = node < count ? v * inv : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        *reinterpret_cast<uint2*>(O + d) = make_uint2(pair(v[0], v[1]), pair(v[2], v[3]));
+      } else {
+        *reinterpret_cast<f32x4*>(a.part_o + (out + 16 * rb + of16) * kD + d) = v;
       }
     }
   }
 }
 
-// The parts of a row's sequence, where there are several: a workgroup per row.
-template <int kD>
-__global__ __launch_bounds__(256) void cached_attn_join_kernel(CachedAttnArgs a, int rows_per_group) {
-  constexpr int kCols = kD / 4;           // threads of a part, four columns each
-  constexpr int kAtOnce = 256 / kCols;    // parts at a time
-  __shared__ float weight[1024];
-  __shared__ float wave_most[4], wave_sums[4];
-  __shared__ f32x4 part[kAtOnce * kCols];
-  const int tid = threadIdx.x, wave = tid >> 6;
-  const int row_id = blockIdx.x;  // (b, node, head)
-  const int head = row_id % a.H, bn = row_id / a.H, b = bn / a.N, node = bn - b * a.N;
-  const Slot slot = find_slot(a, -1, b);
-  if (slot.parts <= 1) return;
-  const int h = head / a.G, row = node * a.G + head - h * a.G, rg = row / rows_per_group, rr = row - rg * rows_per_group;
-  const int64_t first = ((int64_t)h * a.groups + rg) * a.items + slot.first;
-  const int parts = min(slot.parts, 1024);
-  float m = -1e30f;
-  for (int i = tid; i < parts; i += 256) m = fmaxf(m, a.part_s[(first + i) * rows_per_group + rr].x);
+__device__ inline CallScores scores_of(const CachedAttnArgs& a) {
+  return CallScores{a.cap_in > 0.0f ? a.cap_in : a.scale_log2, a.cap_in, a.cap_out, a.slopes != nullptr};
+}
+__device__ inline const int32_t* parents_of(const CachedAttnArgs& a, int b) {
+  return a.parents == nullptr ? nullptr : a.parents + (a.tree == 2 ? (int64_t)b * a.N : 0);
+}
+
+// Four waves take every fourth tile of 32 keys, each straight from memory through its
+// registers, for the 16 kR rows of their workgroup.
+template <int kType, int kD, int kR>
+__global__ __launch_bounds__(256, 2) void cached_attn_kernel(CachedAttnArgs a) {
+  using C = CachedCfg<kType, kD>;
+  constexpr bool k8 = kType != FC_CACHE_BF16;
+  __shared__ Nodes nodes;
+  __shared__ __attribute__((aligned(16))) Queries<kType, kD, kR> queries;
+  __shared__ __attribute__((aligned(16))) Exchange<kD, kR> exchange;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = (threadIdx.x & 63) >> 4;
+  const Place at = place_of(a);
+  if (at.h >= a.g.Hkv) return;
+  const CallScores call = scores_of(a);
+  for_each_stretch(a, at.x, [&](int b, int length, int count, int tile0, int tile1, bool whole, int64_t slot) {
+    const int end = min(length + count, a.g.capacity), first_row = at.group * 16 * kR;
+    if (count == 0) tile1 = tile0;  // (nothing to read)
+    Raw<8 * C::kEsz> k[2][C::kSteps];
+    Raw<C::kC * C::kEsz> v[8];
+    Raw<16> ks[2], vs[2];
+    Blocks blocks[2];
+    BlockBytes<kType, kD> bytes[2];  // of the tile whose bytes are in k and v or on their way
+    int page[2];
+    const LaneOffsets<kType, kD> off;
+    const auto locate = [&](int i, int key, bool there) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  if ((tid & 63) == 0) wave_most[wave] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(wave_most[0], wave_most[1]), fmaxf(wave_most[2], wave_most[3]));
-  float l = 0.0f;
-  for (int i = tid; i < parts; i += 256) {
-    const float2 st = a.part_s[(first + i) * rows_per_group + rr];
-    const float w = __builtin_amdgcn_exp2f(st.x - m);
-    weight[i] = w;
-    l += st.y * w;
+      for (int kb = 0; kb < 2; ++kb) {
+        const int64_t row = blocks[kb].row(a, at.h, i, key + 16 * kb, &page[kb]);
+        bytes[kb].set(a, row, there && key + 16 * kb < end);
+      }
+    };
+    const auto load_k = [&] {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        load_steps<kType>(k[kb], bytes[kb].k, off.k);
+        if (k8) ks[kb].load(bytes[kb].ks, 16 * g);
+      }
+    };
+    const auto load_v = [&] {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[4 * kb + r].load(bytes[kb].v, off.v + r * C::kRow);
+        if (k8) vs[kb].load(bytes[kb].vs, 16 * g);
+      }
+    };
+    const auto request_k = [&](int i, int key, bool there) {
+      locate(i, key, there);
+      load_k();
+    };
+    // What a stretch begins with is requested before any of it is waited for.
+    const auto fetch = [&](int key) {
+      blocks[0].fetch(a, b, key, 4 * kTileKeys, end);
+      blocks[1].fetch(a, b, key + 16, 4 * kTileKeys, end);
+    };
+    int tile = tile0 + wave, i = 0;
+    fetch(tile * kTileKeys);
+    bf16x8 q[kR];
+    const uint32_t asked = queries.load(q, a, b, at.h, first_row, count);
+    const int32_t* parents = parents_of(a, b);
+    const int up = parents != nullptr && (int)threadIdx.x < a.N ? parents[threadIdx.x] : -1;
+    locate(0, tile * kTileKeys, tile < tile1);
+    load_k();
+    load_v();
+    queries.store(q, asked);
+    if (wave == 0) trace_nodes(&nodes, parents != nullptr, up, a.N, a.left);
+    __syncthreads();
+    Rows<kType, kD, kR> rows;
+    rows.begin(a, nodes, b, at.h, first_row, length, count);
+    for (; tile < tile1; tile += 4) {
+      const int key0 = tile * kTileKeys, next = key0 + 4 * kTileKeys;
+      i = (i + 1) & 63;
+      if (i == 0) fetch(next);
+      // (each operand's next bytes are requested as soon as these have left their registers)
+      struct {
+        decltype(k)& bytes;
+        decltype(ks)& scales;
+        const int (&page)[2];
+        const int g;
+        decltype(request_k)& request;
+        const int i, next;
+        const bool more;
+        __device__ inline bf16x8 frag(int kb, int st) const {
+          const bf16x8 f = key_operand<kType>(bytes[kb][st].w);
+          return 4 * C::kSteps != C::kU && g * C::kSteps + st >= C::kU ? Mma<bf16>::zero() : f;
+        }
+        __device__ inline f32x4 scale(int kb, float by) const {
+          const float f = page[kb] >= 0 ? by : NAN;  // a page that is none
+          return k8 ? __builtin_bit_cast(f32x4, scales[kb]) * f : f32x4{f, f, f, f};
+        }
+        __device__ inline void used() const { request(i, next, more); }
+      } keys{k, ks, page, g, request_k, i, next, tile + 4 < tile1};
+      struct {
+        decltype(v)& bytes;
+        decltype(vs)& scales;
+        __device__ inline bf16x8 frag(int c) const {
+          return as_bf16x8(make_uint4(two_keys<kType>(bytes[0].w, bytes[1].w, c), two_keys<kType>(bytes[2].w, bytes[3].w, c),
+                                      two_keys<kType>(bytes[4].w, bytes[5].w, c), two_keys<kType>(bytes[6].w, bytes[7].w, c)));
+        }
+        __device__ inline f32x4 scale(int kb) const { return __builtin_bit_cast(f32x4, scales[kb]); }
+        __device__ inline void keep(uint32_t mask) const {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (uint32_t& w : bytes[j].w) w = (mask >> (16 * (j >> 2) + (j & 3)) & 1) != 0 ? w : 0;
+        }
+        __device__ inline void finite() const {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (uint32_t& w : bytes[j].w) w = finite_halves(w);
+        }
+      } values{v, vs};
+      rows.tile(call, queries, nodes, a.N, key0, length, keys, values);
+      load_v();
+    }
+    finish<kType, kD, kR>(a, rows, exchange, b, at.h, at.group, count, whole, slot);
+  });
+}
+
+// The parts of a row's sequence, where there are several: kWaves waves to a row, of a workgroup's
+// four.
+template <int kD, int kWaves>
+__global__ __launch_bounds__(256) void cached_attn_join_kernel(CachedAttnArgs a, int rows_per_group) {
+  constexpr int kCols = kD / 4;         // threads of a part, four columns each
+  constexpr int kAtOnce = 64 / kCols;   // parts of a wave at a time
+  __shared__ f32x4 sums[4][kCols];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row_id = blockIdx.x * (4 / kWaves) + wave / kWaves;  // (b, node, head)
+  if (kWaves == 1 && row_id >= a.g.B * a.N * a.H) return;
+  const int head = row_id % a.H, bn = row_id / a.H, b = bn / a.N, node = bn - b * a.N;
+  Line line = find_on_line(a, -1, b);
+  const Span span = line.chunk.of(a, b);
+  // The shares that hold some of its tiles; the first may hold only the room in front.
+  int64_t x0 = line.start / line.share;
+  const int64_t x1 = (line.start + span.tiles + kBegin - 1) / line.share;
+  if (stretch_of(line.start, span.tiles, x0, line.share).last == 0) ++x0;
+  if (x0 >= x1) return;
+  const int h = head / a.G, row = node * a.G + head - h * a.G, rg = row / rows_per_group, rr = row - rg * rows_per_group;
+  const int64_t slots = ((int64_t)h * a.groups + rg) * 2 * a.shares;
+  const auto place = [&](int i) { return (slots + part_slot(line.start, x0 + i, line.share)) * rows_per_group + rr; };
+  const int parts = (int)(x1 - x0) + 1;
+  float2 st = lane < parts ? a.part_s[place(lane)] : make_float2(-INFINITY, 0.0f);
+  float m = st.x, l = st.y;
+  for (int i = lane + 64; i < parts; i += 64) {
+    st = a.part_s[place(i)];
+    const float most = fmaxf(m, st.x);
+    l = l * __builtin_amdgcn_exp2f(m - most) + st.y * __builtin_amdgcn_exp2f(st.x - most);
+    m = most;
   }
+  float all = m;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor(all, o));
+  l *= __builtin_amdgcn_exp2f(m - all);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
-  if ((tid & 63) == 0) wave_sums[wave] = l;
-  __syncthreads();
-  l = wave_sums[0] + wave_sums[1] + wave_sums[2] + wave_sums[3];
-  const int q = tid / kCols, d = 4 * (tid % kCols);
+  const int q = lane / kCols, d = 4 * (lane - q * kCols);
   f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   if (q < kAtOnce) {
 #pragma unroll 4
-    for (int i = q; i < parts; i += kAtOnce)
-      v += *reinterpret_cast<const f32x4*>(a.part_o + ((first + i) * rows_per_group + rr) * kD + d) * weight[i];
-    part[tid] = v;
+    for (int i = wave % kWaves * kAtOnce + q; i < parts; i += kWaves * kAtOnce) {
+      const int64_t at = place(i);
+      v += *reinterpret_cast<const f32x4*>(a.part_o + at * kD + d) * __builtin_amdgcn_exp2f(a.part_s[at].x - all);
+    }
   }
-  __syncthreads();
-  if (tid < kCols) {
-#pragma unroll 4
-    for (int i = 1; i < kAtOnce; ++i) v += part[i * kCols + tid];
-    const Span span = span_at(a, b);
-    v = node < span.count ? v * (1.0f / l) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  f32x4 of_wave = v;
+#pragma unroll
+  for (int i = 1; i < kAtOnce; ++i)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) of_wave[c] += __shfl(v[c], lane + i * kCols);
+  if (kWaves > 1) {
+    if (lane < kCols) sums[wave][lane] = of_wave;
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) of_wave += sums[w][min(lane, kCols - 1)];
+  }
+  if (lane < kCols) {
+    v = node < span.count ? of_wave * (1.0f / l) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     bf16* O = static_cast<bf16*>(a.O) + (int64_t)row_id * kD;
     *reinterpret_cast<uint2*>(O + d) = make_uint2(pair(v[0], v[1]), pair(v[2], v[3]));
   }

@@ -9,18 +9,34 @@
 
 namespace fc {
 
+// A wave for each row, or where there are few rows a workgroup: 64 x 10 rows of 4 parts 3 us
+// either way, 16 x 32 x 16 rows of 3 parts 6.4 and 18.5 us, 16 rows of 51 parts 6.4 and 3.1 us.
+constexpr int kJoinRows = 2048;
+
+namespace {
+
+template <int kD>
+void launch_join(const CachedAttnArgs& a, int rows_per_group, hipStream_t s) {
+  const int rows = a.g.B * a.N * a.H;
+  if (rows <= kJoinRows)
+    hipLaunchKernelGGL((cached_attn_join_kernel<kD, 4>), dim3(rows), dim3(256), 0, s, a, rows_per_group);
+  else
+    hipLaunchKernelGGL((cached_attn_join_kernel<kD, 1>), dim3((rows + 3) / 4), dim3(256), 0, s, a, rows_per_group);
+}
+
+}  // namespace
+
 hipError_t launch_cached_attn_join(const CachedAttnArgs& a, int rows_per_group, hipStream_t s) {
-  const dim3 grid((unsigned)((int64_t)a.g.B * a.N * a.H));
   const ProfileMark mk = profile_begin(s);
   switch (a.g.D) {
-    case 16: hipLaunchKernelGGL(cached_attn_join_kernel<16>, grid, dim3(256), 0, s, a, rows_per_group); break;
-    case 32: hipLaunchKernelGGL(cached_attn_join_kernel<32>, grid, dim3(256), 0, s, a, rows_per_group); break;
-    case 48: hipLaunchKernelGGL(cached_attn_join_kernel<48>, grid, dim3(256), 0, s, a, rows_per_group); break;
-    case 64: hipLaunchKernelGGL(cached_attn_join_kernel<64>, grid, dim3(256), 0, s, a, rows_per_group); break;
-    case 80: hipLaunchKernelGGL(cached_attn_join_kernel<80>, grid, dim3(256), 0, s, a, rows_per_group); break;
-    case 96: hipLaunchKernelGGL(cached_attn_join_kernel<96>, grid, dim3(256), 0, s, a, rows_per_group); break;
-    case 112: hipLaunchKernelGGL(cached_attn_join_kernel<112>, grid, dim3(256), 0, s, a, rows_per_group); break;
-    default: hipLaunchKernelGGL(cached_attn_join_kernel<128>, grid, dim3(256), 0, s, a, rows_per_group); break;
+    case 16: launch_join<16>(a, rows_per_group, s); break;
+    case 32: launch_join<32>(a, rows_per_group, s); break;
+    case 48: launch_join<48>(a, rows_per_group, s); break;
+    case 64: launch_join<64>(a, rows_per_group, s); break;
+    case 80: launch_join<80>(a, rows_per_group, s); break;
+    case 96: launch_join<96>(a, rows_per_group, s); break;
+    case 112: launch_join<112>(a, rows_per_group, s); break;
+    default: launch_join<128>(a, rows_per_group, s); break;
   }
   const hipError_t e = hipGetLastError();
   profile_end(mk, "cached_attn_join", s);
@@ -36,32 +52,33 @@ fc_status bad(const char* who, const char* what, fc_status code = FC_ERR_INVALID
 }
 bool off(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; }
 
-constexpr int kLeastTiles = 8;      // of a slot: two per wave
-constexpr int kSlotsPerLaunch = 1024;  // four workgroups per CU
+constexpr int kSlots = 512;       // workgroups: two on each of 256 CUs, which their registers allow
+constexpr int kLeastTiles = 12;   // of a share: a sequence's beginning and a tile for each wave
+constexpr int kWholeTiles = 24;   // up to which a sequence is not shared: 17 tiles 10.4 us, in parts 11.5 and the join's 2.3
 
 // The sizes of a call that follow from its descriptor alone (not from the lengths,
 // which lie on the device).
 struct Plan {
-  int row_blocks, groups, share, items;
-  bool parts;          // a sequence may have several slots
+  int row_blocks, groups, shares;
   size_t o_bytes, s_bytes;
 };
 
 Plan plan_of(const CacheGeom& g, int H, int N, int left) {
   Plan p;
   const int rows = H / g.Hkv * N;
-  const int most = g.type == FC_CACHE_BF16 && g.D > 64 ? 2 : 4;
-  p.row_blocks = rows <= 16 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
+  // Two blocks of sixteen rows read the keys once for both: 16 sequences of 4000 int8 keys
+  // with 32 rows and 8 KV heads in 32 us for 38.  Where bf16 rows of more than 64 values leave too few registers
+  // for that (62 us for 48) it is worth it from the third block on only (64 rows: 69 us for 81).
+  const bool spills = g.type == FC_CACHE_BF16 && g.D > 64;
+  p.row_blocks = rows > (spills ? 32 : 16) ? 2 : 1;
   p.groups = (rows + 16 * p.row_blocks - 1) / (16 * p.row_blocks);
-  p.share = std::max(1, std::min(1024, kSlotsPerLaunch / (g.Hkv * p.groups)));
-  // A sequence's tiles, at most: one slot holds them all where these are few.
+  // A sequence's tiles, at most.
   const int64_t span = std::min<int64_t>(g.capacity, (int64_t)left + N + kTileKeys);
-  p.parts = (span + kTileKeys - 1) / kTileKeys + 1 > kLeastTiles;
-  p.items = p.parts ? p.share + g.B : g.B;
-  if (!p.parts) p.share = 1;
-  const int64_t slots = p.parts ? (int64_t)g.Hkv * p.groups * p.items * 16 * p.row_blocks : 0;
-  p.o_bytes = (size_t)slots * g.D * 4;
-  p.s_bytes = (size_t)slots * sizeof(float2);
+  const bool parts = (span + kTileKeys - 1) / kTileKeys > kWholeTiles;
+  p.shares = parts ? std::max(1, kSlots / (g.Hkv * p.groups)) : 0;
+  const int64_t rows_kept = (int64_t)g.Hkv * p.groups * 2 * p.shares * 16 * p.row_blocks;
+  p.o_bytes = (size_t)rows_kept * g.D * 4;
+  p.s_bytes = (size_t)rows_kept * sizeof(float2);
   return p;
 }
 
@@ -126,7 +143,7 @@ fc_status fc_cached_attn(const fc_cache_desc* desc, const fc_cache* cache, const
   a.part_s = reinterpret_cast<float2*>(static_cast<char*>(workspace) + fc::round256(p.o_bytes));
   a.H = options->H, a.N = options->N, a.G = options->H / desc->Hkv, a.rows = a.G * a.N;
   a.left = left, a.tree = options->tree;
-  a.groups = p.groups, a.items = p.items, a.share = p.share, a.least = p.parts ? fc::kLeastTiles : 1 << 30;
+  a.groups = p.groups, a.shares = p.shares, a.least = fc::kLeastTiles;
   const double scale = 1.0 / std::sqrt((double)desc->D);
   a.scale_log2 = (float)(1.4426950408889634 * scale);
   if (options->softcap > 0.0f) {
@@ -137,7 +154,7 @@ fc_status fc_cached_attn(const fc_cache_desc* desc, const fc_cache* cache, const
   hipError_t e = desc->type == FC_CACHE_BF16 ? fc::launch_cached_attn<FC_CACHE_BF16>(a, p.row_blocks, s)
                  : desc->type == FC_CACHE_I8 ? fc::launch_cached_attn<FC_CACHE_I8>(a, p.row_blocks, s)
                                              : fc::launch_cached_attn<FC_CACHE_F8>(a, p.row_blocks, s);
-  if (e == hipSuccess && p.parts) e = fc::launch_cached_attn_join(a, 16 * p.row_blocks, s);
+  if (e == hipSuccess && p.shares > 0) e = fc::launch_cached_attn_join(a, 16 * p.row_blocks, s);
   if (e != hipSuccess) return fc::bad(who, hipGetErrorString(e), FC_ERR_HIP);
   fc::clear_error();
   return FC_OK;

@@ -59,7 +59,7 @@ static void rows() {
 // Slots: all tiles of all sequences are in exactly one, and there are at most share + B.
 static void slots() {
   for (int round = 0; round < 2000; ++round) {
-    const int B = 1 + rng() % 80, share = 1 + rng() % 300, least = any({1, 8, 16, 1 << 30}), N = 1 + rng() % 64;
+    const int B = 1 + rng() % 80, shares = 1 + rng() % 300, least = any({fc::kBegin + 1, 12, 16, 1 << 30}), N = 1 + rng() % 64;
     const int capacity = 16 * (1 + rng() % any({3, 100, 5000})), left = any({0, 1, 31, 512, INT_MAX / 2});
     int64_t total = 0;
     std::vector<fc::Span> spans;
@@ -76,16 +76,38 @@ static void slots() {
         CHECK(s.first * (int64_t)fc::kTileKeys <= s.length);
         if (s.length > left) CHECK(s.first * fc::kTileKeys <= s.length - left);
       }
-      total += s.tiles;
+      total += s.tiles + fc::kBegin;
     }
-    const int tiles = fc::slot_tiles(total, share, least);
-    CHECK(tiles >= 4 && tiles % 4 == 0);
-    int64_t n = 0;
-    for (const auto& s : spans) n += (s.tiles + tiles - 1) / tiles;
-    CHECK(n <= share + B && n >= B);
-    for (const auto& s : spans) CHECK((s.tiles + tiles - 1) / tiles <= share || least == 1 << 30);
+    // The line: every tile of every sequence is in one share, a share has at most two parts of
+    // sequences that it does not hold whole, and no two parts share a slot.
+    const int64_t each = fc::share_of(total, shares, least);
+    CHECK(each >= least && each * shares >= total);
+    std::vector<int> slots(2 * (size_t)shares, 0);
+    int64_t start = 0;
+    for (const auto& s : spans) {
+      int upto = 0;
+      for (int64_t x = start / each; x * each < start + s.tiles + fc::kBegin; ++x) {
+        CHECK(x < shares);
+        const fc::Stretch st = fc::stretch_of(start, s.tiles, x, each);
+        CHECK(st.first <= st.last && (st.first == upto || st.last == 0));
+        if (st.first >= st.last) {  // the room in front alone, in the first share that has any of it
+          CHECK(x == start / each && upto == 0);
+          continue;
+        }
+        upto = st.last;
+        if (st.first == 0 && st.last == s.tiles) continue;
+        const int64_t slot = fc::part_slot(start, x, each);
+        CHECK(slot >= 0 && slot < 2 * shares && ++slots[slot] == 1);
+      }
+      CHECK(upto == s.tiles);
+      // The shares beside it hold nothing of it.
+      const fc::Stretch before = fc::stretch_of(start, s.tiles, start / each - 1, each);
+      const fc::Stretch behind = fc::stretch_of(start, s.tiles, (start + s.tiles + fc::kBegin - 1) / each + 1, each);
+      CHECK(before.last == 0 && behind.first == s.tiles);
+      start += s.tiles + fc::kBegin;
+    }
   }
-  CHECK(fc::slot_tiles((int64_t)65535 << 23, 1, 8) > 0);
+  CHECK(fc::share_of((int64_t)1 << 50, 1, 12) == (int64_t)1 << 50);
 }
 
 // The mask of 32 keys against key by key.

@@ -222,10 +222,14 @@ def test_long_sequences_in_parts(gpu, kind, N, H, Hkv, D):
 
 
 def test_many_sequences(gpu):
-    """More sequences than a wave has lanes."""
+    """More sequences than a wave has lanes: each with a workgroup of its own, in parts, and
+    several to a share."""
     rng = np.random.default_rng(8)
     lengths = rng.integers(0, 700, 150)
     _compare(gpu, rng, "int8", lengths, rng.integers(0, 3, 150), 2, 2, 1, 64, 768, 64, tree="run")
+    _compare(gpu, rng, "fp8", rng.integers(0, 1500, 150), rng.integers(0, 3, 150), 2, 2, 1, 64, 1600, 64, tree="run")
+    lengths = np.where(rng.integers(0, 20, 150) > 0, rng.integers(0, 40, 150), 1500)
+    _compare(gpu, rng, "bf16", lengths, rng.integers(0, 4, 150), 3, 64, 8, 32, 1600, 16, tree="each")
 
 
 def test_scores_that_grow_along_the_keys(gpu):
@@ -243,14 +247,15 @@ def test_scores_that_grow_along_the_keys(gpu):
         assert np.abs(O[0].double().cpu().numpy() - want).max() < 2.0 ** -8 * np.abs(want).max() + 30 * O_ROOM * np.abs(V).max()
 
 
+@pytest.mark.parametrize("H,n,capacity", [(4, 90, 128), (12, 90, 128), (12, 1100, 1600)])
 @pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
-def test_what_a_node_does_not_see_does_not_reach_it(gpu, value):
+def test_what_a_node_does_not_see_does_not_reach_it(gpu, value, H, n, capacity):
     """Keys and values that are no numbers at siblings, before the window and behind the sequence."""
     rng = np.random.default_rng(10)
-    N, H, Hkv, D, n = 6, 4, 2, 64, 90
+    N, Hkv, D = 6, 2, 64
     parents = np.array([-1, 0, 0, 1, 2, 4], np.int32)
     for kind, left in (("bf16", -1), ("bf16", 20), ("int8", -1), ("fp8", 20)):
-        cache, K, V = _filled(gpu, rng, kind, [n], [N], N, Hkv, D, 128, 16)
+        cache, K, V = _filled(gpu, rng, kind, [n], [N], N, Hkv, D, capacity, 16)
         Kb, Vb = (_values(rng, 1, n + N, Hkv, D).float() for _ in range(2))
         Kb[0, n + 3, 0, 5], Vb[0, n + 3, :, 7] = value, value  # node 3: only its own row sees it
         if left > 0:
@@ -265,8 +270,9 @@ def test_what_a_node_does_not_see_does_not_reach_it(gpu, value):
         _check(O[others], want[others], clean_v)
         assert not torch.isfinite(O[3, :, 7]).any()
         if kind == "bf16":  # KV head 1's keys are numbers: its queries' other columns are too, and the column is what was put there
-            assert torch.isfinite(O[3, 2:, :7]).all()
-            assert torch.equal(O[3, 2:, 7].float().cpu(), torch.full((2,), value)) or (np.isnan(value) and torch.isnan(O[3, 2:, 7]).all())
+            assert torch.isfinite(O[3, H // 2:, :7]).all()
+            assert torch.equal(O[3, H // 2:, 7].float().cpu(), torch.full((H // 2,), value)) or (
+                np.isnan(value) and torch.isnan(O[3, H // 2:, 7]).all())
 
 
 def test_nodes_that_are_no_trees_and_lie_beyond_the_capacity(gpu):
@@ -313,7 +319,7 @@ def test_rows_of_a_cache_past_32_bits(gpu):
 
 def test_types_streams_and_workspaces(gpu):
     rng = np.random.default_rng(13)
-    cache, K, V = _filled(gpu, rng, "int8", [700, 50], [2, 2], 2, 2, 64, 768, 64)
+    cache, K, V = _filled(gpu, rng, "int8", [700, 50], [2, 2], 2, 2, 64, 1600, 64)
     n = _dev(gpu, np.array([700, 50], np.int32))
     Q = (2.0 * torch.from_numpy(rng.standard_normal((2, 2, 4, 64), dtype=np.float32))).bfloat16().to(gpu)
     O = F.cached_attention(Q, cache, n)
