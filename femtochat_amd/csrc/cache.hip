@@ -186,16 +186,19 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(CacheArgs a) 
   }
 }
 
-// A thread moves one 16-byte piece of every kept token of one head, of k or v
-// (piece < pieces), and of one head's scales (the last piece).  dst j <= path[j] and
-// the path increases, so the sources behind a batch of four lie behind its
-// destinations: no thread overwrites what it (or, its pieces being its own, another)
-// still has to read.
+// A workgroup moves up to kKeepPieces pieces of every kept token: 16 bytes of a head's k or v, or
+// one of its scales.  Its threads take as many tokens at a time as they are, four times over,
+// and read them all before they write any: dst j <= path[j] and the path increases, so what
+// is written then lies before all that is read later.  The tokens' places are looked up 64
+// at a time.  (a thread that moves its piece of one token after another waits for the path, the
+// page and the bytes of each four: 20 layers, 32 sequences, 3 tokens on average, 29 us for 5)
+constexpr int kKeepPieces = 64, kKeepTokens = 64;
 __global__ __launch_bounds__(kCacheThreads) void cache_keep_kernel(CacheArgs a, int pieces, int row_bytes) {
-  const int b = blockIdx.y, layer = blockIdx.z;
-  const int per_head = 2 * pieces + (a.k_scale != nullptr ? 2 : 0);
-  const int i = blockIdx.x * kCacheThreads + threadIdx.x;
-  if (i >= per_head * a.g.Hkv) return;
+  __shared__ int64_t from_row[kKeepTokens], to_row[kKeepTokens];  // of head 0; -1: nothing to move
+  const int b = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x;
+  const int per_head = 2 * pieces + (a.k_scale != nullptr ? 2 : 0), first = blockIdx.x * kKeepPieces;
+  const int here = min(per_head * a.g.Hkv - first, kKeepPieces), at_once = kCacheThreads / here;
+  const int token = tid / here, i = first + tid - token * here;
   const int h = i / per_head, part = i - h * per_head;
   const int n = a.counts == nullptr ? a.T : min(max(a.counts[b], 0), a.T);
   const int length = a.from[b];
@@ -203,32 +206,43 @@ __global__ __launch_bounds__(kCacheThreads) void cache_keep_kernel(CacheArgs a, 
   const int of = scale ? part - 2 * pieces : part / pieces;  // 0: k, 1: v
   char* data = scale ? reinterpret_cast<char*>(of == 0 ? a.k_scale : a.v_scale) : static_cast<char*>(of == 0 ? a.k : a.v);
   const int64_t stride = scale ? 4 : row_bytes;
-  data += scale ? 0 : 16 * (part % pieces);
-  const auto row = [&](int t) {
-    const int64_t r = cache_row(a.g, a.table, layer, b, h, behind(a.g, length, t));
-    return r < 0 ? nullptr : data + r * stride;
-  };
-  for (int j = 0; j < n; j += 4) {
-    char *src[4], *dst[4];
-    uint4 x[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int from = j + e < n ? a.path[(int64_t)b * a.T + j + e] : -1;
-      src[e] = from >= 0 && from < a.T && from != j + e ? row(from) : nullptr;
-      dst[e] = src[e] != nullptr ? row(j + e) : nullptr;
+  data += (int64_t)h * a.g.page_size * stride + (scale ? 0 : 16 * (part % pieces));
+  for (int j0 = 0; j0 < n; j0 += kKeepTokens) {
+    if (tid < kKeepTokens) {
+      const int j = j0 + tid, from = j < n ? a.path[(int64_t)b * a.T + j] : -1;
+      const bool moves = from >= 0 && from < a.T && from != j;
+      const int64_t src = moves ? cache_row(a.g, a.table, layer, b, 0, behind(a.g, length, from)) : -1;
+      const int64_t dst = moves ? cache_row(a.g, a.table, layer, b, 0, behind(a.g, length, j)) : -1;
+      from_row[tid] = dst < 0 ? -1 : src;
+      to_row[tid] = dst;
     }
+    __syncthreads();
+    const int m = min(n - j0, kKeepTokens);
+    for (int j = 0; j < m; j += 4 * at_once) {
+      uint4 x[4];
+      int64_t src[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (dst[e] == nullptr) continue;
-      if (scale) x[e].x = *reinterpret_cast<const uint32_t*>(src[e]);
-      else x[e] = *reinterpret_cast<const uint4*>(src[e]);
-    }
+      for (int e = 0; e < 4; ++e) {
+        const int t = j + e * at_once + token;
+        src[e] = token < at_once && t < m ? from_row[t] : -1;
+        x[e] = make_uint4(0, 0, 0, 0);
+        if (src[e] < 0) continue;
+        if (scale) x[e].x = *reinterpret_cast<const uint32_t*>(data + src[e] * stride);
+        else x[e] = *reinterpret_cast<const uint4*>(data + src[e] * stride);
+      }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (dst[e] == nullptr) continue;
-      if (scale) *reinterpret_cast<uint32_t*>(dst[e]) = x[e].x;
-      else *reinterpret_cast<uint4*>(dst[e]) = x[e];
+      for (int e = 0; e < 4; ++e)  // (the bytes are there before the barrier)
+        asm volatile("" : "+v"(x[e].x), "+v"(x[e].y), "+v"(x[e].z), "+v"(x[e].w));
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (src[e] < 0) continue;
+        char* dst = data + to_row[j + e * at_once + token] * stride;
+        if (scale) *reinterpret_cast<uint32_t*>(dst) = x[e].x;
+        else *reinterpret_cast<uint4*>(dst) = x[e];
+      }
     }
+    __syncthreads();
   }
 }
 
@@ -350,9 +364,9 @@ fc_status fc_cache_keep(const fc_cache_desc* desc, const fc_cache* cache, int32_
   a.path = path;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int row_bytes = desc->D * fc::cache_value_bytes(desc->type), pieces = row_bytes / 16;
-  const int threads = desc->Hkv * (2 * pieces + (a.k_scale != nullptr ? 2 : 0));
+  const int all = desc->Hkv * (2 * pieces + (a.k_scale != nullptr ? 2 : 0));
   const fc::ProfileMark mk = fc::profile_begin(s);
-  hipLaunchKernelGGL(fc::cache_keep_kernel, dim3((unsigned)((threads + fc::kCacheThreads - 1) / fc::kCacheThreads), (unsigned)desc->B, (unsigned)desc->layers),
+  hipLaunchKernelGGL(fc::cache_keep_kernel, dim3((unsigned)((all + fc::kKeepPieces - 1) / fc::kKeepPieces), (unsigned)desc->B, (unsigned)desc->layers),
                      dim3(fc::kCacheThreads), 0, s, a, pieces, row_bytes);
   const hipError_t e = hipGetLastError();
   fc::profile_end(mk, "cache_keep", s);
