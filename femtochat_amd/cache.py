@@ -52,6 +52,8 @@ __all__ = [
 _TYPES = {torch.bfloat16: _lib.FC_CACHE_BF16, torch.int8: _lib.FC_CACHE_I8, torch.float8_e4m3fn: _lib.FC_CACHE_F8}
 _VALUES = (torch.float32, torch.bfloat16)
 _I32 = (torch.int32,)
+_F32 = (torch.float32,)
+_BF16 = (torch.bfloat16,)
 
 
 class KVCache(NamedTuple):
@@ -105,38 +107,55 @@ def kv_cache(sequences: int, capacity: int, n_kv_head: int, head_dim: int, dtype
     return KVCache(k, v, torch.zeros(shape, device=device), torch.zeros(shape, device=device), table)
 
 
-class _Buffers:
-    """A checked cache: its descriptor, pointers, device and sizes."""
+class _Layout:
+    """What follows from a cache's shapes alone, once for each of them: a call on a few
+    tokens is shorter than its preparation."""
 
-    __slots__ = ("desc", "pointers", "device", "lead", "B", "Hkv", "D")
+    __slots__ = ("desc", "ref", "shape", "scales", "pages", "lead", "B", "Hkv", "D", "types", "bytes")
+
+    def __init__(self, shape, dtype, pages, B: int):
+        if len(shape) not in (4, 5) or dtype not in _TYPES:
+            raise ValueError("a cache's k must be a ([layers,] pages, Hkv, page, D) tensor of bfloat16, int8 or float8_e4m3fn")
+        if pages is not None and (len(pages) != 2 or pages[1] == 0):
+            raise ValueError("a cache's pages must be a (B, M) int32 tensor")
+        self.shape, self.types, self.lead, self.B = shape, (dtype,), tuple(shape[:-4]), B
+        self.scales = None if dtype is torch.bfloat16 else shape[:-1]
+        self.pages = None if pages is None else (B, pages[1])
+        P, self.Hkv, S, self.D = shape[-4:]
+        self.desc = _lib.CacheDesc(self.D, self.Hkv, B, self.lead[0] if self.lead else 1, P, S, 0 if pages is None else pages[1], _TYPES[dtype])
+        self.ref = ctypes.byref(self.desc)
+        self.bytes = {}  # of attention's workspace, by what a call adds
+
+
+_layout = lru_cache(maxsize=256)(_Layout)
+
+
+class _Buffers:
+    """A checked cache: its layout, pointers and device."""
+
+    __slots__ = ("layout", "pointers", "device")
 
     def __init__(self, cache: KVCache, B: int):
         k, v, ks, vs, pages = cache
-        if not isinstance(k, torch.Tensor) or k.dim() not in (4, 5) or k.dtype not in _TYPES:
+        if not isinstance(k, torch.Tensor):
             raise ValueError("a cache's k must be a ([layers,] pages, Hkv, page, D) tensor of bfloat16, int8 or float8_e4m3fn")
+        if pages is not None and not isinstance(pages, torch.Tensor):
+            raise ValueError("a cache's pages must be a (B, M) int32 tensor")
+        layout = _layout(k.shape, k.dtype, None if pages is None else pages.shape, B)
         device = k.device
         if device.type != "cuda":
             raise ValueError("the MI355X cache kernels need tensors on a HIP device (torch 'cuda'); there is no CPU path")
-        shape = k.shape
-        _check_tensor("k", k, shape, (k.dtype,), device)
-        _check_tensor("v", v, shape, (k.dtype,), device)
-        if k.dtype is torch.bfloat16:
-            if ks is not None or vs is not None:
-                raise ValueError("a bfloat16 cache has no scales")
-        else:
-            _check_tensor("k_scale", ks, shape[:-1], (torch.float32,), device)
-            _check_tensor("v_scale", vs, shape[:-1], (torch.float32,), device)
-        M = 0
+        _check_tensor("k", k, layout.shape, layout.types, device)
+        _check_tensor("v", v, layout.shape, layout.types, device)
+        if layout.scales is not None:
+            _check_tensor("k_scale", ks, layout.scales, _F32, device)
+            _check_tensor("v_scale", vs, layout.scales, _F32, device)
+        elif ks is not None or vs is not None:
+            raise ValueError("a bfloat16 cache has no scales")
         if pages is not None:
-            if not isinstance(pages, torch.Tensor) or pages.dim() != 2 or pages.shape[1] == 0:
-                raise ValueError("a cache's pages must be a (B, M) int32 tensor")
-            M = pages.shape[1]
-            _check_tensor("pages", pages, (B, M), _I32, device)
-        lead = tuple(shape[:-4])
-        P, Hkv, S, D = shape[-4:]
-        self.desc = _lib.CacheDesc(D, Hkv, B, lead[0] if lead else 1, P, S, M, _TYPES[k.dtype])
+            _check_tensor("pages", pages, layout.pages, _I32, device)
+        self.layout, self.device = layout, device
         self.pointers = _lib.Cache(k.data_ptr(), v.data_ptr(), _ptr(ks), _ptr(vs), _ptr(pages))
-        self.device, self.lead, self.B, self.Hkv, self.D = device, lead, B, Hkv, D
 
 
 def _batch(cache: KVCache, like) -> int:
@@ -147,10 +166,11 @@ def _batch(cache: KVCache, like) -> int:
 
 
 def _check_counts(c: _Buffers, lengths, counts, name: str = "lengths") -> None:
+    B = (c.layout.B,)
     if lengths is not None:
-        _check_tensor(name, lengths, (c.B,), _I32, c.device)
+        _check_tensor(name, lengths, B, _I32, c.device)
     if counts is not None:
-        _check_tensor("counts", counts, (c.B,), _I32, c.device)
+        _check_tensor("counts", counts, B, _I32, c.device)
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -164,21 +184,22 @@ def cache_write_(cache: KVCache, K: torch.Tensor, V: torch.Tensor, lengths: torc
     tokens ``lengths[b]`` to ``lengths[b] + counts[b] - 1`` (T of them without ``counts``),
     quantised to the cache's type.  Tokens beyond the capacity are not written."""
     c = _Buffers(cache, _batch(cache, lengths))
-    T = _check_values(c, K, V, None)
-    _check_tensor("lengths", lengths, (c.B,), _I32, c.device)
+    T = _check_values(c, K, V)
+    _check_tensor("lengths", lengths, (c.layout.B,), _I32, c.device)
     _check_counts(c, None, counts)
     if T == 0:
         return
     K, V = _aligned(K), _aligned(V)
-    _call(c.device, _lib.lib().fc_cache_write, ctypes.byref(c.desc), ctypes.byref(c.pointers), K.data_ptr(), V.data_ptr(),
+    _call(c.device, _lib.lib().fc_cache_write, c.layout.ref, ctypes.byref(c.pointers), K.data_ptr(), V.data_ptr(),
           _dtype_code(K.dtype), T, lengths.data_ptr(), _ptr(counts))
 
 
-def _check_values(c: _Buffers, K, V, T: Optional[int]) -> int:
-    if not isinstance(K, torch.Tensor) or K.dim() != len(c.lead) + 4:
+def _check_values(c: _Buffers, K, V) -> int:
+    layout = c.layout
+    if not isinstance(K, torch.Tensor) or K.dim() != len(layout.shape):
         raise ValueError("K and V must be ([layers,] B, T, Hkv, D) tensors, with layers where the cache has them")
-    T = K.shape[-3] if T is None else T
-    shape = c.lead + (c.B, T, c.Hkv, c.D)
+    T = K.shape[-3]
+    shape = layout.lead + (layout.B, T, layout.Hkv, layout.D)
     _check_tensor("K", K, shape, _VALUES, c.device)
     _check_tensor("V", V, shape, (K.dtype,), c.device)
     return T
@@ -188,13 +209,13 @@ def cache_read_(K: torch.Tensor, V: torch.Tensor, cache: KVCache, starts: Option
                 counts: Optional[torch.Tensor] = None) -> None:
     """``cache_read`` into the caller's K and V."""
     c = _Buffers(cache, _batch(cache, starts if starts is not None else counts))
-    T = _check_values(c, K, V, None)
+    T = _check_values(c, K, V)
     _check_counts(c, starts, counts, "starts")
     if T == 0:
         return
     if (K.data_ptr() | V.data_ptr()) % 16:
         raise ValueError("K and V must start on a 16-byte boundary")
-    _call(c.device, _lib.lib().fc_cache_read, ctypes.byref(c.desc), ctypes.byref(c.pointers), K.data_ptr(), V.data_ptr(),
+    _call(c.device, _lib.lib().fc_cache_read, c.layout.ref, ctypes.byref(c.pointers), K.data_ptr(), V.data_ptr(),
           _dtype_code(K.dtype), T, _ptr(starts), _ptr(counts))
 
 
@@ -213,7 +234,8 @@ def cache_read(cache: KVCache, starts: Optional[torch.Tensor], T: int, counts: O
         raise ValueError("a cache's k must be a ([layers,] pages, Hkv, page, D) tensor of bfloat16, int8 or float8_e4m3fn")
     B = _batch(cache, starts if starts is not None else counts)
     shape = tuple(k.shape[:-4]) + (B, T, k.shape[-3], k.shape[-1])
-    K, V = torch.empty(shape, dtype=dtype, device=k.device), torch.empty(shape, dtype=dtype, device=k.device)
+    K = torch.empty(shape, dtype=dtype, device=k.device)
+    V = torch.empty_like(K)
     cache_read_(K, V, cache, starts, counts)
     return K, V
 
@@ -226,22 +248,14 @@ def cache_keep_(cache: KVCache, lengths: torch.Tensor, path: torch.Tensor, count
     if not isinstance(path, torch.Tensor) or path.dim() != 2:
         raise ValueError("path must be a (B, N) int32 tensor")
     N = path.shape[1]
-    _check_tensor("path", path, (c.B, N), _I32, c.device)
-    _check_tensor("lengths", lengths, (c.B,), _I32, c.device)
-    _check_tensor("counts", counts, (c.B,), _I32, c.device)
+    B = c.layout.B
+    _check_tensor("path", path, (B, N), _I32, c.device)
+    _check_tensor("lengths", lengths, (B,), _I32, c.device)
+    _check_tensor("counts", counts, (B,), _I32, c.device)
     if N == 0:
         return
-    _call(c.device, _lib.lib().fc_cache_keep, ctypes.byref(c.desc), ctypes.byref(c.pointers), N, lengths.data_ptr(),
+    _call(c.device, _lib.lib().fc_cache_keep, c.layout.ref, ctypes.byref(c.pointers), N, lengths.data_ptr(),
           path.data_ptr(), counts.data_ptr())
-
-
-@lru_cache(maxsize=256)
-def _workspace_bytes(D, Hkv, B, P, S, M, kind, H, N, left) -> int:
-    n = ctypes.c_size_t(0)
-    _lib.check(_lib.lib().fc_cached_attn_workspace_bytes(
-        ctypes.byref(_lib.CacheDesc(D, Hkv, B, 1, P, S, M, kind)),
-        ctypes.byref(_lib.CachedAttnOptions(H, N, left, 0, 0.0, None)), ctypes.byref(n)))
-    return n.value
 
 
 def _left(window) -> int:
@@ -255,15 +269,23 @@ def _options(c: _Buffers, N: int, H: int, window, parents, softcap, slopes) -> _
     tree = 0
     if parents is not None:
         tree = 2 if isinstance(parents, torch.Tensor) and parents.dim() == 2 else 1
-        _check_tensor("parents", parents, (c.B, N) if tree == 2 else (N,), _I32, c.device)
+        _check_tensor("parents", parents, (c.layout.B, N) if tree == 2 else (N,), _I32, c.device)
     if slopes is not None:
-        _check_tensor("slopes", slopes, (H,), (torch.float32,), c.device)
+        _check_tensor("slopes", slopes, (H,), _F32, c.device)
     return _lib.CachedAttnOptions(H, N, _left(window), tree, float(softcap), _ptr(slopes))
 
 
-def _bytes(c: _Buffers, o: _lib.CachedAttnOptions) -> int:
-    d = c.desc
-    return _workspace_bytes(d.D, d.Hkv, d.B, d.pages, d.page_size, d.max_pages, d.type, o.H, o.N, o.left)
+def _bytes(layout: _Layout, H: int, N: int, left: int) -> int:
+    key = (H, N, left)
+    known = layout.bytes.get(key)
+    if known is None:
+        n = ctypes.c_size_t(0)
+        _lib.check(_lib.lib().fc_cached_attn_workspace_bytes(
+            layout.ref, ctypes.byref(_lib.CachedAttnOptions(H, N, left, 0, 0.0, None)), ctypes.byref(n)))
+        if len(layout.bytes) >= 256:  # (windows and batches without end)
+            layout.bytes.clear()
+        known = layout.bytes[key] = n.value
+    return known
 
 
 def cached_attention_workspace_bytes(Q: torch.Tensor, cache: KVCache, window=(-1, 0)) -> int:
@@ -272,7 +294,7 @@ def cached_attention_workspace_bytes(Q: torch.Tensor, cache: KVCache, window=(-1
     if not isinstance(Q, torch.Tensor) or Q.dim() != 4:
         raise ValueError("Q must have shape (B, N, H, D)")
     c = _Buffers(cache, Q.shape[0])
-    n = _bytes(c, _lib.CachedAttnOptions(Q.shape[2], Q.shape[1], _left(window), 0, 0.0, None))
+    n = _bytes(c.layout, Q.shape[2], Q.shape[1], _left(window))
     return n + 256 if n > 0 else 0
 
 
@@ -285,15 +307,15 @@ def cached_attention_(O: torch.Tensor, Q: torch.Tensor, cache: KVCache, lengths:
         raise ValueError("Q must have shape (B, N, H, D)")
     B, N, H, D = Q.shape
     c = _Buffers(cache, B)
-    shape = (B, N, H, c.D)
-    _check_tensor("Q", Q, shape, (torch.bfloat16,), c.device)
-    _check_tensor("O", O, shape, (torch.bfloat16,), c.device)
+    shape = (B, N, H, c.layout.D)
+    _check_tensor("Q", Q, shape, _BF16, c.device)
+    _check_tensor("O", O, shape, _BF16, c.device)
     _check_tensor("lengths", lengths, (B,), _I32, c.device)
     _check_counts(c, None, counts)
     if O.data_ptr() % 16:
         raise ValueError("O must start on a 16-byte boundary")
     o = _options(c, N, H, window, parents, softcap, slopes)
-    nbytes = _bytes(c, o)
+    nbytes = _bytes(c.layout, H, N, o.left)
     at = None
     if nbytes > 0:
         if workspace is None:  # freed to this stream's pool on return, so later work on the stream comes after the kernels
@@ -302,7 +324,7 @@ def cached_attention_(O: torch.Tensor, Q: torch.Tensor, cache: KVCache, lengths:
             _check_workspace(workspace, nbytes + 256, c.device)
         at = (workspace.data_ptr() + 255) & ~255
     Q = _aligned(Q)
-    _call(c.device, _lib.lib().fc_cached_attn, ctypes.byref(c.desc), ctypes.byref(c.pointers), ctypes.byref(o), Q.data_ptr(),
+    _call(c.device, _lib.lib().fc_cached_attn, c.layout.ref, ctypes.byref(c.pointers), ctypes.byref(o), Q.data_ptr(),
           O.data_ptr(), lengths.data_ptr(), _ptr(counts), _ptr(parents), at, nbytes)
 
 

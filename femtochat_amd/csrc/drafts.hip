@@ -799,7 +799,7 @@ Layout layout_of(const fc_verify_desc* d) {
   l.both = l.walks + (draws ? round256(B * sizeof(Walk)) : 0);
   l.sums = l.both + (draws ? round256(B * parts * sizeof(double2)) : 0);
   l.arrived = l.sums + round256(B * parts * sizeof(double));
-  l.total = l.arrived + round256(B * sizeof(int32_t));
+  l.total = d->V <= kSmallValues ? 0 : l.arrived + round256(B * sizeof(int32_t));
   return l;
 }
 
@@ -878,8 +878,8 @@ fc_status fc_verify_drafts(const fc_verify_desc* desc, const void* logits, const
       fc::off(path, 4) || fc::off(kept, 4) || fc::off(next, 4))
     return fc::bad(who, "tokens, u and integer buffers must be aligned to their element size");
   const fc::Layout l = fc::layout_of(desc);
-  if (workspace == nullptr || workspace_bytes < l.total) return fc::bad(who, "the workspace is missing or too small", FC_ERR_WORKSPACE);
-  if (fc::off(workspace, 256)) return fc::bad(who, "the workspace must be 256-byte aligned", FC_ERR_WORKSPACE);
+  if (l.total > 0 && (workspace == nullptr || workspace_bytes < l.total)) return fc::bad(who, "the workspace is missing or too small", FC_ERR_WORKSPACE);
+  if (l.total > 0 && fc::off(workspace, 256)) return fc::bad(who, "the workspace must be 256-byte aligned", FC_ERR_WORKSPACE);
   fc::DraftArgs a{};
   a.logits = logits, a.draft = draft ? draft_logits : nullptr, a.tokens = tokens, a.u = u;
   a.parents = parents, a.counts = counts, a.path = path, a.kept = kept, a.next = next;

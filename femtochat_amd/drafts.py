@@ -72,8 +72,9 @@ def _checked(logits, tokens, uniforms, draft_logits, parents, counts, temperatur
 
 def verify_drafts_workspace_bytes(logits, tokens, uniforms, *, draft_logits=None, parents=None, counts=None,
                                   temperature: float = 1.0) -> int:
-    """Bytes of the caller-owned workspace that a call with these arguments accepts."""
-    return _checked(logits, tokens, uniforms, draft_logits, parents, counts, temperature)[2] + 256
+    """Bytes of the caller-owned workspace that a call with these arguments accepts (0 when it needs none)."""
+    n = _checked(logits, tokens, uniforms, draft_logits, parents, counts, temperature)[2]
+    return n + 256 if n > 0 else 0
 
 
 def verify_drafts_(path: torch.Tensor, kept: torch.Tensor, token: torch.Tensor, logits: torch.Tensor, tokens: torch.Tensor,
@@ -86,13 +87,16 @@ def verify_drafts_(path: torch.Tensor, kept: torch.Tensor, token: torch.Tensor, 
     _check_tensor("path", path, (B, N), _I32, device)
     _check_tensor("kept", kept, (B,), _I32, device)
     _check_tensor("token", token, (B,), _I32, device)
-    if workspace is None:  # freed to this stream's pool on return, so later work on the stream comes after the kernels
-        workspace = torch.empty(nbytes + 256, dtype=torch.uint8, device=device)
-    else:
-        _check_workspace(workspace, nbytes + 256, device)
+    at = None
+    if nbytes > 0:
+        if workspace is None:  # freed to this stream's pool on return, so later work on the stream comes after the kernels
+            workspace = torch.empty(nbytes + 256, dtype=torch.uint8, device=device)
+        else:
+            _check_workspace(workspace, nbytes + 256, device)
+        at = (workspace.data_ptr() + 255) & ~255
     _call(device, _lib.lib().fc_verify_drafts, ctypes.byref(d), logits.data_ptr(), _ptr(draft_logits), tokens.data_ptr(),
           _ptr(uniforms), _ptr(parents), _ptr(counts), path.data_ptr(), kept.data_ptr(), token.data_ptr(),
-          (workspace.data_ptr() + 255) & ~255, nbytes)
+          at, nbytes)
 
 
 def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: Optional[torch.Tensor], *,
@@ -112,8 +116,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: Optional
         raise ValueError("tokens must be a (B, N) tensor")
     B, N = tokens.shape
     path = torch.empty((B, N), dtype=torch.int32, device=tokens.device)
-    ends = torch.empty((2, B), dtype=torch.int32, device=tokens.device)
-    kept, token = ends[0], ends[1]
+    kept, token = torch.empty((2, B), dtype=torch.int32, device=tokens.device).unbind(0)
     verify_drafts_(path, kept, token, logits, tokens, uniforms, draft_logits=draft_logits, parents=parents, counts=counts,
                    temperature=temperature, workspace=workspace)
     return path, kept, token
