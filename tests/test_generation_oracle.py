@@ -242,7 +242,9 @@ def test_bad_verifications_are_refused(kw, what):
 
 
 def test_verification_pointers_and_workspace():
-    lib, d, n = L.lib(), _verify_desc(), ctypes.c_size_t(0)
+    lib, d, n = L.lib(), _verify_desc(V=2048), ctypes.c_size_t(0)
+    assert lib.fc_verify_workspace_bytes(d, ctypes.byref(n)) == L.FC_OK and n.value == 0
+    d = _verify_desc(V=2049)
     assert lib.fc_verify_workspace_bytes(d, ctypes.byref(n)) == L.FC_OK and n.value > 0
     ok = [FAKE, FAKE, FAKE, FAKE, None, None, FAKE, FAKE, FAKE, FAKE, n.value, None]
     for at in (0, 1, 2, 3, 6, 7, 8):
