@@ -145,17 +145,21 @@ class _Buffers:
         device = k.device
         if device.type != "cuda":
             raise ValueError("the MI355X cache kernels need tensors on a HIP device (torch 'cuda'); there is no CPU path")
-        _check_tensor("k", k, layout.shape, layout.types, device)
-        _check_tensor("v", v, layout.shape, layout.types, device)
+        if not (k.is_contiguous() and isinstance(v, torch.Tensor) and v.shape == layout.shape and v.dtype is layout.types[0]
+                and v.device == device and v.is_contiguous()):
+            _check_tensor("k", k, layout.shape, layout.types, device)
+            _check_tensor("v", v, layout.shape, layout.types, device)
+        k_scale = v_scale = None
         if layout.scales is not None:
             _check_tensor("k_scale", ks, layout.scales, _F32, device)
             _check_tensor("v_scale", vs, layout.scales, _F32, device)
+            k_scale, v_scale = ks.data_ptr(), vs.data_ptr()
         elif ks is not None or vs is not None:
             raise ValueError("a bfloat16 cache has no scales")
         if pages is not None:
             _check_tensor("pages", pages, layout.pages, _I32, device)
         self.layout, self.device = layout, device
-        self.pointers = _lib.Cache(k.data_ptr(), v.data_ptr(), _ptr(ks), _ptr(vs), _ptr(pages))
+        self.pointers = _lib.Cache(k.data_ptr(), v.data_ptr(), k_scale, v_scale, _ptr(pages))
 
 
 def _batch(cache: KVCache, like) -> int:
