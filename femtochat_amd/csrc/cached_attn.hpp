@@ -62,6 +62,7 @@ struct CachedAttnArgs {
   const float* slopes;
   float* part_o;   // [KV head, row group][2 shares][16 R][D]
   float2* part_s;  // [KV head, row group][2 shares][16 R] (reference, sum)
+  int4* parts;     // of a sequence: how many, the first's slot, the second's, its tokens
   int H, N, G, rows;      // rows = G N
   int left;               // INT_MAX / 2: all
   int tree;               // 0 a run, 1 one tree, 2 a tree per sequence
@@ -108,9 +109,8 @@ struct Line {
   int b;          // which, B past the end
   Chunk chunk;    // from or around it
 };
-// The first sequence of share x, or (x < 0) sequence of_b.  Every lane of a wave calls it
-// and gets the same.
-__device__ inline Line find_on_line(const CachedAttnArgs& a, int x, int of_b) {
+// The first sequence of share x.  Every lane of a wave calls it and gets the same.
+__device__ inline Line find_on_line(const CachedAttnArgs& a, int x) {
   const int lane = threadIdx.x & 63;
   const auto cost = [&](const Chunk& c) { return c.b0 + lane < a.g.B ? c.mine(a).tiles + kBegin : 0; };
   Line l;
@@ -135,7 +135,7 @@ __device__ inline Line find_on_line(const CachedAttnArgs& a, int x, int of_b) {
       const int64_t v = __shfl_up(upto, o);
       if (lane >= o) upto += v;
     }
-    const uint64_t hit = __ballot(n > 0 && (x >= 0 ? at < before + upto : b0 + lane == of_b));
+    const uint64_t hit = __ballot(n > 0 && at < before + upto);
     if (hit != 0) {
       const int i = __ffsll((long long)hit) - 1;
       l.b = b0 + i;
@@ -597,11 +597,12 @@ struct LaneOffsets {
 };
 
 // The stretches of a workgroup, sequence by sequence: body(b, length, count, first tile, last tile, whole, slot).
+// Where `tells`, it leaves for each sequence that begins in it what the join asks.
 template <typename Body>
-__device__ inline void for_each_stretch(const CachedAttnArgs& a, int x, Body body) {
+__device__ inline void for_each_stretch(const CachedAttnArgs& a, int x, bool tells, Body body) {
   Line line{0, 0, x, {}};
   if (a.shares > 0)
-    line = find_on_line(a, x, -1);
+    line = find_on_line(a, x);
   else
     line.chunk.load(a, x);
   bool again = false;
@@ -617,6 +618,10 @@ __device__ inline void for_each_stretch(const CachedAttnArgs& a, int x, Body bod
     }
     if (again) __syncthreads();  // the last sequence's LDS is read
     again = true;
+    if (a.shares > 0 && st.first == 0 && tells && threadIdx.x == 0) {
+      const int64_t last = (start + span.tiles + kBegin - 1) / line.share;
+      a.parts[b] = make_int4((int)(last - x) + 1, (int)part_slot(start, x, line.share), (int)part_slot(start, x + 1, line.share), span.count);
+    }
     body(b, span.length, span.count, span.first + st.first, span.first + st.last, st.first == 0 && st.last == span.tiles,
          part_slot(start, x, line.share));
     if (a.shares == 0) break;
@@ -720,7 +725,7 @@ __global__ __launch_bounds__(256, 2) void cached_attn_kernel(CachedAttnArgs a) {
   const Place at = place_of(a);
   if (at.h >= a.g.Hkv) return;
   const CallScores call = scores_of(a);
-  for_each_stretch(a, at.x, [&](int b, int length, int count, int tile0, int tile1, bool whole, int64_t slot) {
+  for_each_stretch(a, at.x, at.h == 0 && at.group == 0, [&](int b, int length, int count, int tile0, int tile1, bool whole, int64_t slot) {
     const int end = min(length + count, a.g.capacity), first_row = at.group * 16 * kR;
     if (count == 0) tile1 = tile0;  // (nothing to read)
     Raw<8 * C::kEsz> k[2][C::kSteps];
@@ -837,17 +842,12 @@ __global__ __launch_bounds__(256) void cached_attn_join_kernel(CachedAttnArgs a,
   const int row_id = blockIdx.x * (4 / kWaves) + wave / kWaves;  // (b, node, head)
   if (kWaves == 1 && row_id >= a.g.B * a.N * a.H) return;
   const int head = row_id % a.H, bn = row_id / a.H, b = bn / a.N, node = bn - b * a.N;
-  Line line = find_on_line(a, -1, b);
-  const Span span = line.chunk.of(a, b);
-  // The shares that hold some of its tiles; the first may hold only the room in front.
-  int64_t x0 = line.start / line.share;
-  const int64_t x1 = (line.start + span.tiles + kBegin - 1) / line.share;
-  if (stretch_of(line.start, span.tiles, x0, line.share).last == 0) ++x0;
-  if (x0 >= x1) return;
+  const int4 of_b = a.parts[b];
+  const int parts = of_b.x;
+  if (parts < 2) return;
   const int h = head / a.G, row = node * a.G + head - h * a.G, rg = row / rows_per_group, rr = row - rg * rows_per_group;
   const int64_t slots = ((int64_t)h * a.groups + rg) * 2 * a.shares;
-  const auto place = [&](int i) { return (slots + part_slot(line.start, x0 + i, line.share)) * rows_per_group + rr; };
-  const int parts = (int)(x1 - x0) + 1;
+  const auto place = [&](int i) { return (slots + (i == 0 ? of_b.y : of_b.z + 2 * (i - 1))) * rows_per_group + rr; };
   float2 st = lane < parts ? a.part_s[place(lane)] : make_float2(-INFINITY, 0.0f);
   float m = st.x, l = st.y;
   for (int i = lane + 64; i < parts; i += 64) {
@@ -884,7 +884,7 @@ __global__ __launch_bounds__(256) void cached_attn_join_kernel(CachedAttnArgs a,
     for (int w = 1; w < kWaves; ++w) of_wave += sums[w][min(lane, kCols - 1)];
   }
   if (lane < kCols) {
-    v = node < span.count ? of_wave * (1.0f / l) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    v = node < of_b.w ? of_wave * (1.0f / l) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     bf16* O = static_cast<bf16*>(a.O) + (int64_t)row_id * kD;
     *reinterpret_cast<uint2*>(O + d) = make_uint2(pair(v[0], v[1]), pair(v[2], v[3]));
   }

@@ -50,6 +50,7 @@ fc_status bad(const char* who, const char* what, fc_status code = FC_ERR_INVALID
   snprintf(msg, sizeof(msg), "%s: %s", who, what);
   return set_error(code, msg);
 }
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 bool off(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; }
 
 constexpr int kSlots = 512;       // workgroups: two on each of 256 CUs, which their registers allow
@@ -60,7 +61,7 @@ constexpr int kWholeTiles = 24;   // up to which a sequence is not shared: 17 ti
 // which lie on the device).
 struct Plan {
   int row_blocks, groups, shares;
-  size_t o_bytes, s_bytes;
+  size_t s_at, parts_at, bytes;  // in the workspace, behind the parts of O
 };
 
 Plan plan_of(const CacheGeom& g, int H, int N, int left) {
@@ -77,8 +78,9 @@ Plan plan_of(const CacheGeom& g, int H, int N, int left) {
   const bool parts = (span + kTileKeys - 1) / kTileKeys > kWholeTiles;
   p.shares = parts ? std::max(1, kSlots / (g.Hkv * p.groups)) : 0;
   const int64_t rows_kept = (int64_t)g.Hkv * p.groups * 2 * p.shares * 16 * p.row_blocks;
-  p.o_bytes = (size_t)rows_kept * g.D * 4;
-  p.s_bytes = (size_t)rows_kept * sizeof(float2);
+  p.s_at = round256((size_t)rows_kept * g.D * 4);
+  p.parts_at = p.s_at + round256((size_t)rows_kept * sizeof(float2));
+  p.bytes = p.shares > 0 ? p.parts_at + round256((size_t)g.B * sizeof(int4)) : 0;
   return p;
 }
 
@@ -97,7 +99,6 @@ fc_status options_of(const char* who, const CacheGeom& g, const fc_cached_attn_o
   return FC_OK;
 }
 int left_of(const fc_cached_attn_options* o) { return o->left < 0 ? INT_MAX / 2 : std::min(o->left, INT_MAX / 2); }
-size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace
 
@@ -114,7 +115,7 @@ fc_status fc_cached_attn_workspace_bytes(const fc_cache_desc* desc, const fc_cac
   if ((st = fc::options_of(who, g, options)) != FC_OK) return st;
   if (bytes == nullptr) return fc::bad(who, "bytes is null");
   const fc::Plan p = fc::plan_of(g, options->H, options->N, fc::left_of(options));
-  *bytes = fc::round256(p.o_bytes) + fc::round256(p.s_bytes);
+  *bytes = p.bytes;
   fc::clear_error();
   return FC_OK;
 }
@@ -133,14 +134,15 @@ fc_status fc_cached_attn(const fc_cache_desc* desc, const fc_cache* cache, const
   if (fc::off(lengths, 4) || fc::off(counts, 4) || fc::off(parents, 4)) return fc::bad(who, "integer buffers must be 4-byte aligned");
   const int left = fc::left_of(options);
   const fc::Plan p = fc::plan_of(a.g, options->H, options->N, left);
-  const size_t need = fc::round256(p.o_bytes) + fc::round256(p.s_bytes);
+  const size_t need = p.bytes;
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return fc::bad(who, "the workspace is missing or too small", FC_ERR_WORKSPACE);
   if (need > 0 && fc::off(workspace, 256)) return fc::bad(who, "the workspace must be 256-byte aligned", FC_ERR_WORKSPACE);
   a.k = cache->k, a.v = cache->v, a.k_scale = cache->k_scale, a.v_scale = cache->v_scale;
   a.table = desc->max_pages > 0 ? cache->table : nullptr;
   a.Q = Q, a.O = O, a.lengths = lengths, a.counts = counts, a.parents = parents, a.slopes = options->slopes;
   a.part_o = reinterpret_cast<float*>(workspace);
-  a.part_s = reinterpret_cast<float2*>(static_cast<char*>(workspace) + fc::round256(p.o_bytes));
+  a.part_s = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.s_at);
+  a.parts = reinterpret_cast<int4*>(static_cast<char*>(workspace) + p.parts_at);
   a.H = options->H, a.N = options->N, a.G = options->H / desc->Hkv, a.rows = a.G * a.N;
   a.left = left, a.tree = options->tree;
   a.groups = p.groups, a.shares = p.shares, a.least = fc::kLeastTiles;

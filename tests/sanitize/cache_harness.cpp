@@ -98,6 +98,7 @@ static void slots() {
         if (st.first == 0 && st.last == s.tiles) continue;
         const int64_t slot = fc::part_slot(start, x, each);
         CHECK(slot >= 0 && slot < 2 * shares && ++slots[slot] == 1);
+        if (st.first > 0) CHECK(slot == 2 * x);  // (behind the first part, every second slot)
       }
       CHECK(upto == s.tiles);
       // The shares beside it hold nothing of it.
