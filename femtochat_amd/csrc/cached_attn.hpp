@@ -26,7 +26,7 @@
 // Each wave reads keys of its own for sixteen or 32 rows, with neither LDS (but for the queries)
 // nor barriers in the loop: its operands are used twice at most, and eight waves that shared
 // them through LDS in steps of 128 keys waited for each other longer than for the bytes
-// (16 sequences of 4096 int8 keys, 64 rows, 8 KV heads: 75 us for 61).
+// (16 sequences of up to 8192 int8 keys, 64 rows, 8 KV heads: 75 us for 61).
 //
 // The lengths lie on the device, so the launch is the same whatever they are: as many
 // workgroups as the GPU holds at once, each of which finds its equal share of all
@@ -36,7 +36,7 @@
 // Measured, codes of 8 bits, heads of 128, the kernel alone: 64 sequences of up to 4096 keys,
 // 5 KV heads, one token each, 40 us (192 MB, 4.8 TB/s; a copy reaches 5.1); one of 131072 keys,
 // 8 KV heads, 50 us (277 MB; part of it stays in the 256 MB cache between calls); 16 of up to
-// 8192 keys, 8 KV heads, 32 nodes of two heads each, 61 us (168 MB, 2.8 TB/s), where the vector
+// 8192 keys, 8 KV heads, 32 nodes of two heads each, 58 us (168 MB, 2.9 TB/s), where the vector
 // units are busy for four fifths: a third of it turns codes into numbers and a fourth makes
 // two numbers of each probability.
 //
@@ -782,6 +782,15 @@ __global__ __launch_bounds__(256, 2) void cached_attn_kernel(CachedAttnArgs a) {
     rows.begin(a, nodes, b, at.h, first_row, length, count);
     for (; tile < tile1; tile += 4) {
       const int key0 = tile * kTileKeys, next = key0 + 4 * kTileKeys;
+      if (kR == 2) {
+        // Of a CU's two workgroups the one that is behind goes first; the older one would be done at two
+        // thirds of the time and leave half the CU idle (16 sequences, 32 nodes: 61 us for 58).
+        const int left = 4 * (tile1 - tile), all = tile1 - tile0;
+        if (left > 3 * all) __builtin_amdgcn_s_setprio(3);
+        else if (left > 2 * all) __builtin_amdgcn_s_setprio(2);
+        else if (left > all) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
+      }
       i = (i + 1) & 63;
       if (i == 0) fetch(next);
       // (each operand's next bytes are requested as soon as these have left their registers)
