@@ -115,12 +115,13 @@ __device__ inline Line find_on_line(const CachedAttnArgs& a, int x) {
   const auto cost = [&](const Chunk& c) { return c.b0 + lane < a.g.B ? c.mine(a).tiles + kBegin : 0; };
   Line l;
   l.chunk.load(a, 0);
-  int64_t total = wave_sum(cost(l.chunk));
+  int64_t total = cost(l.chunk);
   for (int b0 = 64; b0 < a.g.B; b0 += 64) {
     Chunk c;
     c.load(a, b0);
-    total += wave_sum(cost(c));
+    total += cost(c);
   }
+  total = wave_sum(total);
   l.share = share_of(total, a.shares, a.least);
   l.b = a.g.B;
   l.start = total;
@@ -240,6 +241,9 @@ struct CachedCfg {
   static constexpr int kRow = kD * kEsz;          // bytes
 };
 
+// A row's reference before its first key: no score but -infinity is below it.
+constexpr float kNoReference = -0x1.fffffep127f;
+
 // What a call needs beside the sequence, the same for every row.
 struct CallScores {
   float factor;  // of a product before its key's scale: log2(e) / sqrt(D), or what the cap takes
@@ -322,7 +326,7 @@ struct Rows {
       any_sees |= sees[rb];
       any_low = min(any_low, low[rb]);
       all_low = max(all_low, there && !broken[rb] ? low[rb] : 0);  // (rows that are not there, or broken, may take whatever comes)
-      ref[rb] = -1e30f;
+      ref[rb] = kNoReference;
       sum[rb] = 0.0f;
 #pragma unroll
       for (int c = 0; c < C::kC; ++c) acc[rb][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -402,7 +406,7 @@ struct Rows {
       for (int rb = 0; rb < kR; ++rb) {
         const uint32_t seen = seen_keys(key0 + g4, low[rb], sees[rb], length);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)  // P = 0: no reference is below -1e30
+        for (int j = 0; j < 8; ++j)  // P = 0, whatever the reference
           s[rb][j >> 2][j & 3] = (seen >> (16 * (j >> 2) + (j & 3)) & 1) != 0 ? s[rb][j >> 2][j & 3] : -INFINITY;
       }
     }

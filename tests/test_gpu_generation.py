@@ -247,6 +247,20 @@ def test_scores_that_grow_along_the_keys(gpu):
         assert np.abs(O[0].double().cpu().numpy() - want).max() < 2.0 ** -8 * np.abs(want).max() + 30 * O_ROOM * np.abs(V).max()
 
 
+@pytest.mark.parametrize("N,H", [(1, 2), (3, 12)])
+def test_scores_far_below_zero(gpu, N, H):
+    """Every score of a row near -4e32: equal ones share, and a smaller one has nothing."""
+    D, n = 16, 900
+    cache = F.kv_cache(1, 1024, 1, D, torch.bfloat16, device=gpu)
+    K, V = torch.full((1, n + N, 1, D), 1e16), torch.randn(1, n + N, 1, D)
+    K[0, :n // 2] = 2e16
+    F.cache_write_(cache, K.to(gpu), V.to(gpu), torch.zeros(1, dtype=torch.int32, device=gpu))
+    Q = torch.full((1, N, H, D), -1e16, dtype=torch.bfloat16, device=gpu)
+    O = F.cached_attention(Q, cache, _dev(gpu, np.array([n], np.int32)))[0]
+    Kh, Vh = G.held(K.numpy(), "bf16")[0], G.held(V.numpy(), "bf16")[0]
+    _check(O, G.attend(Q[0].double().cpu().numpy(), Kh, Vh, n, N), Vh)
+
+
 @pytest.mark.parametrize("H,n,capacity", [(4, 90, 128), (12, 90, 128), (12, 1100, 1600)])
 @pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
 def test_what_a_node_does_not_see_does_not_reach_it(gpu, value, H, n, capacity):
