@@ -111,7 +111,7 @@ class _Layout:
     """What follows from a cache's shapes alone, once for each of them: a call on a few
     tokens is shorter than its preparation."""
 
-    __slots__ = ("desc", "ref", "shape", "scales", "pages", "lead", "B", "Hkv", "D", "types", "bytes")
+    __slots__ = ("desc", "ref", "shape", "scales", "pages", "lead", "batch", "B", "Hkv", "D", "types", "bytes")
 
     def __init__(self, shape, dtype, pages, B: int):
         if len(shape) not in (4, 5) or dtype not in _TYPES:
@@ -120,6 +120,7 @@ class _Layout:
             raise ValueError("a cache's pages must be a (B, M) int32 tensor")
         self.shape, self.types, self.lead, self.B = shape, (dtype,), tuple(shape[:-4]), B
         self.scales = None if dtype is torch.bfloat16 else shape[:-1]
+        self.batch = (B,)
         self.pages = None if pages is None else (B, pages[1])
         P, self.Hkv, S, self.D = shape[-4:]
         self.desc = _lib.CacheDesc(self.D, self.Hkv, B, self.lead[0] if self.lead else 1, P, S, 0 if pages is None else pages[1], _TYPES[dtype])
@@ -130,36 +131,42 @@ class _Layout:
 _layout = lru_cache(maxsize=256)(_Layout)
 
 
-class _Buffers:
+class _Buffers(NamedTuple):
     """A checked cache: its layout, pointers and device."""
 
-    __slots__ = ("layout", "pointers", "device")
+    layout: _Layout
+    pointers: _lib.Cache
+    device: torch.device
 
-    def __init__(self, cache: KVCache, B: int):
-        k, v, ks, vs, pages = cache
-        if not isinstance(k, torch.Tensor):
-            raise ValueError("a cache's k must be a ([layers,] pages, Hkv, page, D) tensor of bfloat16, int8 or float8_e4m3fn")
-        if pages is not None and not isinstance(pages, torch.Tensor):
-            raise ValueError("a cache's pages must be a (B, M) int32 tensor")
-        layout = _layout(k.shape, k.dtype, None if pages is None else pages.shape, B)
-        device = k.device
-        if device.type != "cuda":
-            raise ValueError("the MI355X cache kernels need tensors on a HIP device (torch 'cuda'); there is no CPU path")
-        if not (k.is_contiguous() and isinstance(v, torch.Tensor) and v.shape == layout.shape and v.dtype is layout.types[0]
-                and v.device == device and v.is_contiguous()):
-            _check_tensor("k", k, layout.shape, layout.types, device)
-            _check_tensor("v", v, layout.shape, layout.types, device)
-        k_scale = v_scale = None
-        if layout.scales is not None:
+
+def _buffers(cache: KVCache, B: int) -> _Buffers:
+    k, v, ks, vs, pages = cache
+    if not isinstance(k, torch.Tensor):
+        raise ValueError("a cache's k must be a ([layers,] pages, Hkv, page, D) tensor of bfloat16, int8 or float8_e4m3fn")
+    if pages is not None and not isinstance(pages, torch.Tensor):
+        raise ValueError("a cache's pages must be a (B, M) int32 tensor")
+    layout = _layout(k.shape, k.dtype, None if pages is None else pages.shape, B)
+    device = k.device
+    if device.type != "cuda":
+        raise ValueError("the MI355X cache kernels need tensors on a HIP device (torch 'cuda'); there is no CPU path")
+    if not (k.is_contiguous() and isinstance(v, torch.Tensor) and v.shape == layout.shape and v.dtype is layout.types[0]
+            and v.device == device and v.is_contiguous()):
+        _check_tensor("k", k, layout.shape, layout.types, device)
+        _check_tensor("v", v, layout.shape, layout.types, device)
+    k_scale = v_scale = table = None
+    if layout.scales is not None:
+        if not (isinstance(ks, torch.Tensor) and isinstance(vs, torch.Tensor) and ks.shape == layout.scales and vs.shape == layout.scales
+                and ks.dtype is torch.float32 and vs.dtype is torch.float32 and ks.device == device and vs.device == device
+                and ks.is_contiguous() and vs.is_contiguous()):
             _check_tensor("k_scale", ks, layout.scales, _F32, device)
             _check_tensor("v_scale", vs, layout.scales, _F32, device)
-            k_scale, v_scale = ks.data_ptr(), vs.data_ptr()
-        elif ks is not None or vs is not None:
-            raise ValueError("a bfloat16 cache has no scales")
-        if pages is not None:
-            _check_tensor("pages", pages, layout.pages, _I32, device)
-        self.layout, self.device = layout, device
-        self.pointers = _lib.Cache(k.data_ptr(), v.data_ptr(), k_scale, v_scale, _ptr(pages))
+        k_scale, v_scale = ks.data_ptr(), vs.data_ptr()
+    elif ks is not None or vs is not None:
+        raise ValueError("a bfloat16 cache has no scales")
+    if pages is not None:
+        _check_tensor("pages", pages, layout.pages, _I32, device)
+        table = pages.data_ptr()
+    return _Buffers(layout, _lib.Cache(k.data_ptr(), v.data_ptr(), k_scale, v_scale, table), device)
 
 
 def _batch(cache: KVCache, like) -> int:
@@ -169,12 +176,13 @@ def _batch(cache: KVCache, like) -> int:
     return cache.k.shape[-4] if cache.pages is None else cache.pages.shape[0]
 
 
-def _check_counts(c: _Buffers, lengths, counts, name: str = "lengths") -> None:
-    B = (c.layout.B,)
-    if lengths is not None:
-        _check_tensor(name, lengths, B, _I32, c.device)
+def _check_counts(c: _Buffers, lengths, counts, name: str = "lengths", required: bool = False) -> None:
+    B, device = c.layout.batch, c.device
+    if (lengths is not None or required) and not (isinstance(lengths, torch.Tensor) and lengths.shape == B and lengths.dtype is torch.int32
+                                                  and lengths.device == device and lengths.is_contiguous()):
+        _check_tensor(name, lengths, B, _I32, device)
     if counts is not None:
-        _check_tensor("counts", counts, B, _I32, c.device)
+        _check_tensor("counts", counts, B, _I32, device)
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -187,10 +195,9 @@ def cache_write_(cache: KVCache, K: torch.Tensor, V: torch.Tensor, lengths: torc
     """Writes K and V ([layers,] B, T, Hkv, D), float32 or bfloat16, as each sequence's
     tokens ``lengths[b]`` to ``lengths[b] + counts[b] - 1`` (T of them without ``counts``),
     quantised to the cache's type.  Tokens beyond the capacity are not written."""
-    c = _Buffers(cache, _batch(cache, lengths))
+    c = _buffers(cache, _batch(cache, lengths))
     T = _check_values(c, K, V)
-    _check_tensor("lengths", lengths, (c.layout.B,), _I32, c.device)
-    _check_counts(c, None, counts)
+    _check_counts(c, lengths, counts, required=True)
     if T == 0:
         return
     K, V = _aligned(K), _aligned(V)
@@ -199,20 +206,23 @@ def cache_write_(cache: KVCache, K: torch.Tensor, V: torch.Tensor, lengths: torc
 
 
 def _check_values(c: _Buffers, K, V) -> int:
-    layout = c.layout
+    layout, device = c.layout, c.device
     if not isinstance(K, torch.Tensor) or K.dim() != len(layout.shape):
         raise ValueError("K and V must be ([layers,] B, T, Hkv, D) tensors, with layers where the cache has them")
-    T = K.shape[-3]
-    shape = layout.lead + (layout.B, T, layout.Hkv, layout.D)
-    _check_tensor("K", K, shape, _VALUES, c.device)
-    _check_tensor("V", V, shape, (K.dtype,), c.device)
+    shape = K.shape
+    T = shape[-3]
+    want = layout.lead + (layout.B, T, layout.Hkv, layout.D)
+    if not (shape == want and K.dtype in _VALUES and K.device == device and K.is_contiguous() and isinstance(V, torch.Tensor)
+            and V.shape == shape and V.dtype is K.dtype and V.device == device and V.is_contiguous()):
+        _check_tensor("K", K, want, _VALUES, device)
+        _check_tensor("V", V, want, (K.dtype,), device)
     return T
 
 
 def cache_read_(K: torch.Tensor, V: torch.Tensor, cache: KVCache, starts: Optional[torch.Tensor] = None,
                 counts: Optional[torch.Tensor] = None) -> None:
     """``cache_read`` into the caller's K and V."""
-    c = _Buffers(cache, _batch(cache, starts if starts is not None else counts))
+    c = _buffers(cache, _batch(cache, starts if starts is not None else counts))
     T = _check_values(c, K, V)
     _check_counts(c, starts, counts, "starts")
     if T == 0:
@@ -238,7 +248,7 @@ def cache_read(cache: KVCache, starts: Optional[torch.Tensor], T: int, counts: O
         raise ValueError("a cache's k must be a ([layers,] pages, Hkv, page, D) tensor of bfloat16, int8 or float8_e4m3fn")
     B = _batch(cache, starts if starts is not None else counts)
     shape = tuple(k.shape[:-4]) + (B, T, k.shape[-3], k.shape[-1])
-    K = torch.empty(shape, dtype=dtype, device=k.device)
+    K = torch.empty(*shape, dtype=dtype, device=k.device)
     V = torch.empty_like(K)
     cache_read_(K, V, cache, starts, counts)
     return K, V
@@ -248,14 +258,14 @@ def cache_keep_(cache: KVCache, lengths: torch.Tensor, path: torch.Tensor, count
     """Keeps a path of the tokens behind ``lengths``: token ``lengths[b] + path[b, j]`` moves to
     ``lengths[b] + j`` for j < counts[b], in every layer that the cache holds.  ``path`` (B, N)
     int32 increases along a row, as ``verify_drafts`` gives it."""
-    c = _Buffers(cache, _batch(cache, lengths))
+    c = _buffers(cache, _batch(cache, lengths))
     if not isinstance(path, torch.Tensor) or path.dim() != 2:
         raise ValueError("path must be a (B, N) int32 tensor")
     N = path.shape[1]
     B = c.layout.B
     _check_tensor("path", path, (B, N), _I32, c.device)
-    _check_tensor("lengths", lengths, (B,), _I32, c.device)
     _check_tensor("counts", counts, (B,), _I32, c.device)
+    _check_counts(c, lengths, None, required=True)
     if N == 0:
         return
     _call(c.device, _lib.lib().fc_cache_keep, c.layout.ref, ctypes.byref(c.pointers), N, lengths.data_ptr(),
@@ -297,7 +307,7 @@ def cached_attention_workspace_bytes(Q: torch.Tensor, cache: KVCache, window=(-1
     library's requirement plus 256 bytes of alignment slack; 0 when the problem needs none)."""
     if not isinstance(Q, torch.Tensor) or Q.dim() != 4:
         raise ValueError("Q must have shape (B, N, H, D)")
-    c = _Buffers(cache, Q.shape[0])
+    c = _buffers(cache, Q.shape[0])
     n = _bytes(c.layout, Q.shape[2], Q.shape[1], _left(window))
     return n + 256 if n > 0 else 0
 
@@ -310,26 +320,29 @@ def cached_attention_(O: torch.Tensor, Q: torch.Tensor, cache: KVCache, lengths:
     if not isinstance(Q, torch.Tensor) or Q.dim() != 4:
         raise ValueError("Q must have shape (B, N, H, D)")
     B, N, H, D = Q.shape
-    c = _Buffers(cache, B)
-    shape = (B, N, H, c.layout.D)
-    _check_tensor("Q", Q, shape, _BF16, c.device)
-    _check_tensor("O", O, shape, _BF16, c.device)
-    _check_tensor("lengths", lengths, (B,), _I32, c.device)
-    _check_counts(c, None, counts)
-    if O.data_ptr() % 16:
+    c = _buffers(cache, B)
+    layout, device = c.layout, c.device
+    if not (D == layout.D and Q.dtype is torch.bfloat16 and Q.device == device and Q.is_contiguous() and isinstance(O, torch.Tensor)
+            and O.shape == Q.shape and O.dtype is torch.bfloat16 and O.device == device and O.is_contiguous()):
+        shape = (B, N, H, layout.D)
+        _check_tensor("Q", Q, shape, _BF16, device)
+        _check_tensor("O", O, shape, _BF16, device)
+    _check_counts(c, lengths, counts, required=True)
+    at = O.data_ptr()
+    if at % 16:
         raise ValueError("O must start on a 16-byte boundary")
     o = _options(c, N, H, window, parents, softcap, slopes)
-    nbytes = _bytes(c.layout, H, N, o.left)
-    at = None
+    nbytes = _bytes(layout, H, N, o.left)
+    ws = None
     if nbytes > 0:
         if workspace is None:  # freed to this stream's pool on return, so later work on the stream comes after the kernels
-            workspace = torch.empty(nbytes + 256, dtype=torch.uint8, device=c.device)
+            workspace = torch.empty(nbytes + 256, dtype=torch.uint8, device=device)
         else:
-            _check_workspace(workspace, nbytes + 256, c.device)
-        at = (workspace.data_ptr() + 255) & ~255
+            _check_workspace(workspace, nbytes + 256, device)
+        ws = (workspace.data_ptr() + 255) & ~255
     Q = _aligned(Q)
-    _call(c.device, _lib.lib().fc_cached_attn, c.layout.ref, ctypes.byref(c.pointers), ctypes.byref(o), Q.data_ptr(),
-          O.data_ptr(), lengths.data_ptr(), _ptr(counts), _ptr(parents), at, nbytes)
+    _call(device, _lib.lib().fc_cached_attn, layout.ref, ctypes.byref(c.pointers), ctypes.byref(o), Q.data_ptr(), at,
+          lengths.data_ptr(), _ptr(counts), _ptr(parents), ws, nbytes)
 
 
 def cached_attention(Q: torch.Tensor, cache: KVCache, lengths: torch.Tensor, window: Tuple[int, int] = (-1, 0), *,
@@ -352,6 +365,5 @@ def cached_attention(Q: torch.Tensor, cache: KVCache, lengths: torch.Tensor, win
                           workspace=workspace)
         return O.to(Q.dtype)
     O = torch.empty_like(Q)
-    cached_attention_(O, Q, cache, lengths, window, counts=counts, parents=parents, softcap=softcap, slopes=slopes,
-                      workspace=workspace)
+    cached_attention_(O, Q, cache, lengths, window, counts=counts, parents=parents, softcap=softcap, slopes=slopes, workspace=workspace)
     return O

@@ -115,8 +115,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: Optional
     if not isinstance(tokens, torch.Tensor) or tokens.dim() != 2:
         raise ValueError("tokens must be a (B, N) tensor")
     B, N = tokens.shape
-    path = torch.empty((B, N), dtype=torch.int32, device=tokens.device)
-    kept, token = torch.empty((2, B), dtype=torch.int32, device=tokens.device).unbind(0)
+    path = torch.empty(B, N, dtype=torch.int32, device=tokens.device)
+    kept, token = torch.empty(2, B, dtype=torch.int32, device=tokens.device).unbind(0)
     verify_drafts_(path, kept, token, logits, tokens, uniforms, draft_logits=draft_logits, parents=parents, counts=counts,
                    temperature=temperature, workspace=workspace)
     return path, kept, token
