@@ -493,6 +493,7 @@ __global__ __launch_bounds__(kDraftThreads) void draft_pick_kernel(DraftArgs a) 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int b = blockIdx.x / a.groups, group = blockIdx.x - b * a.groups;
   const int parts = a.groups * kWaves4;
+  const double u = (double)fminf(fmaxf(a.u[(int64_t)b * a.N], 0.0f), 0x1.fffffep-1f);  // (used at the end of a chain of reads: read here)
   if (!kDraws) {
     if (tid < 64) {
       int best;
@@ -548,15 +549,23 @@ __global__ __launch_bounds__(kDraftThreads) void draft_pick_kernel(DraftArgs a) 
   const auto part_at = [&](int i) {
     return i < parts ? __hip_atomic_load(&sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
   };
-  double total = 0.0;
-  for (int i0 = 0; i0 < parts; i0 += 64) total += part_at(i0 + lane);
+  constexpr int kHeld = 4;  // parts of a lane that stay in registers between the sum and the search
+  double held[kHeld], total = 0.0;
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) held[k] = part_at(64 * k + lane);
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) total += held[k];
+  for (int i0 = 64 * kHeld; i0 < parts; i0 += 64) total += part_at(i0 + lane);
   total = wave_sum(total);
-  const double u = (double)fminf(fmaxf(a.u[(int64_t)b * a.N], 0.0f), 0x1.fffffep-1f);
   double before = 0.0, target = u * total;
   int part = parts - 1;
   if (total > 0.0) {
     for (int i0 = 0; i0 < parts; i0 += 64) {
-      const double upto = before + wave_scan(part_at(i0 + lane));
+      double of_lane = held[0];
+#pragma unroll
+      for (int k = 1; k < kHeld; ++k) of_lane = i0 == 64 * k ? held[k] : of_lane;
+      if (i0 >= 64 * kHeld) of_lane = part_at(i0 + lane);
+      const double upto = before + wave_scan(of_lane);
       const uint64_t hit = __ballot(upto > target);
       if (hit != 0) {
         const int at = __ffsll((long long)hit) - 1;
