@@ -475,6 +475,20 @@ def test_trees_of_candidates_against_the_oracle(gpu, V, dtype, N, temperature):
         _agree(got, logits, tokens, u, None, up, c, temperature)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_row_of_many_parts(gpu, dtype):
+    """More parts of the drawn row than the last workgroup's registers hold, and draws from all over it."""
+    rng = np.random.default_rng(31)
+    B, N, V = 8, 3, 199999
+    logits = torch.from_numpy(0.5 * rng.standard_normal((B, N, V), dtype=np.float32)).to(dtype)
+    draft = torch.from_numpy(0.5 * rng.standard_normal((B, N - 1, V), dtype=np.float32)).to(dtype)
+    tokens = rng.integers(0, V, (B, N))
+    u = rng.random((B, N)).astype(np.float32)
+    u[:, 0] = np.linspace(0.02, 0.98, B)
+    for d in (draft, None):
+        _agree(_verified(gpu, logits, tokens, u, d), logits, tokens, u, d, None, None, 1.0)
+
+
 @pytest.mark.parametrize("off", [1, 2, 3])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_logits_off_a_16_byte_boundary(gpu, dtype, off):
