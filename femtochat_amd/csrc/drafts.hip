@@ -11,13 +11,14 @@
 //
 //  * draft_stats_kernel reads every row of logits (target and draft) once: each
 //    workgroup leaves a chunk's maximum and the sum of its exponentials.
-//  * draft_pick_kernel, a workgroup per sequence and chunk: one wave takes a node per
+//  * draft_sums_kernel, a workgroup per sequence and chunk: one wave takes a node per
 //    lane, tests all of them at once and follows the accepted ones from the root; the
-//    workgroup sums the weights of its chunk of the row where the walk ended; and the last
-//    one of a sequence to get there (the first kernel zeroed their counter) finds the part
-//    that u's share falls into and the token in it.
+//    workgroup sums the weights of its chunk of the row where the walk ended.
+//  * draft_pick_kernel, a wave per sequence, finds the part that u's share falls into and
+//    the token in it.  In small calls the last workgroup of a sequence to leave its sums does
+//    that instead (the first kernel zeroed their counter).
 //  * With the drafts' distributions a weight is p - q, whose two sums have to be there
-//    first: draft_walk_kernel, before the pick, walks and forms them.
+//    first: draft_walk_kernel, before the sums, walks and forms them.
 //  * Vocabularies of up to 2048 run whole in draft_small_kernel, a workgroup per sequence.
 #include "attn_device.hpp"
 #include "attn_launch.hpp"
@@ -68,7 +69,7 @@ struct DraftArgs {
   Walk* walks;       // [B] (draws)
   double2* both;     // [B][groups][kWaves4]: sums of the two exponentials (draws)
   double* sums;      // [B][groups][kWaves4], of the weights
-  int32_t* arrived;  // [B]: workgroups of the pick that left their sums
+  int32_t* arrived;  // [B]: workgroups that left their sums
   int B, N, V, chunks;
   int groups;        // workgroups of a sequence in the walk and the pick, a part to each of their waves
   int index64, tree;
@@ -481,75 +482,39 @@ __global__ __launch_bounds__(kDraftThreads) void draft_walk_kernel(DraftArgs a) 
   if (lane == 0) a.both[((int64_t)b * a.groups + group) * kWaves4 + wave] = make_double2(sp, sq);
 }
 
-// kDraws: the walk is done.
-template <typename E, bool kDraws, int kPart>
-__global__ __launch_bounds__(kDraftThreads) void draft_pick_kernel(DraftArgs a) {
-  constexpr int P = kPiece<E>;
-  constexpr int kMine = kPart / 64, kPieces = kMine / P;  // the pick: values of a lane
-  static_assert(kMine % P == 0, "a lane's values are whole pieces");
-  __shared__ Walk walk;
-  __shared__ uint32_t bits[kWaves4 * kPart / 32];
-  __shared__ int is_last;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const int b = blockIdx.x / a.groups, group = blockIdx.x - b * a.groups;
-  const int parts = a.groups * kWaves4;
-  const double u = (double)fminf(fmaxf(a.u[(int64_t)b * a.N], 0.0f), 0x1.fffffep-1f);  // (used at the end of a chain of reads: read here)
-  if (!kDraws) {
-    if (tid < 64) {
-      int best;
-      RowStat p, q;
-      node_stats<false>(a, b, &best, &p, &q);
-      const Walk w = walk_nodes<E, false>(a, b, group == 0, best, p, q);
-      if (tid == 0) walk = w;
-    }
-    __syncthreads();
-  }
-  // (draws: the sums come with the walk, whether it needs them or not)
+// The weights of the row where sequence b's walk ended, as they are after a residual's two sums: false
+// where a row has a NaN or +infinity, or only -infinities, and so no sum.
+template <typename E, bool kDraws>
+__device__ inline bool drawn_row(const DraftArgs& a, int b, const Walk& w, int parts, Weights<E>* ws) {
+  const int lane = threadIdx.x & 63;
   double sp = 0.0, sq = 0.0;
-  if (kDraws) {
+  if (kDraws) {  // (they come with the walk, whether it needs them or not)
     for (int i0 = 0; i0 < parts; i0 += 64) {
       const double2 s = i0 + lane < parts ? a.both[(int64_t)b * parts + i0 + lane] : make_double2(0.0, 0.0);
       sp += s.x;
       sq += s.y;
     }
   }
-  const Walk w = kDraws ? a.walks[b] : walk;
-  // (a row with a NaN or +infinity, or of -infinities, has no sum)
-  if (w.last < 0 || !(w.p.sum > 0.0 && w.p.sum < 1e300) || (w.residual != 0 && !(w.q.sum > 0.0 && w.q.sum < 1e300))) {
-    if (group == 0 && tid == 0) a.next[b] = -1;
-    return;
-  }
-  Weights<E> ws = weights_of<E>(a, w, b);
-  const int head = row_head(ws.row);
+  if (w.last < 0 || !(w.p.sum > 0.0 && w.p.sum < 1e300) || (w.residual != 0 && !(w.q.sum > 0.0 && w.q.sum < 1e300))) return false;
+  *ws = weights_of<E>(a, w, b);
   if (kDraws && w.residual != 0) {
-    ws.ip = 1.0 / wave_sum(sp);
-    ws.iq = 1.0 / wave_sum(sq);
+    ws->ip = 1.0 / wave_sum(sp);
+    ws->iq = 1.0 / wave_sum(sq);
   }
-  double* sums = a.sums + (int64_t)b * parts;
-  const uint32_t* strikes = nullptr;
-  {
-    const int first = group * kWaves4 * kPart - head;
-    if (w.struck != 0) {
-      strike<kWaves4 * kPart, kDraftThreads>(bits, a, b, w.struck, first);
-      strikes = bits + wave * (kPart / 32);
-    }
-    const double s = part_sum<E, kPart>(ws, strikes, first + wave * kPart);
-    // What the last workgroup reads is written and read at the agent's scope, past the
-    // XCDs' own caches; the wave waits for its store before the barrier, and the counter
-    // moves behind that.  (A release at that scope would write the whole L2 back: 20 us.)
-    if (lane == 0) __hip_atomic_store(&sums[group * kWaves4 + wave], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  }
-  __syncthreads();
-  if (tid == 0)
-    is_last = __hip_atomic_fetch_add(&a.arrived[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.groups - 1;
-  __syncthreads();
-  if (is_last == 0 || wave != 0) return;
-  // The last one's first wave: the part that u's share falls into.
-  const auto part_at = [&](int i) {
-    return i < parts ? __hip_atomic_load(&sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
-  };
-  constexpr int kHeld = 4;  // parts of a lane that stay in registers between the sum and the search
+  return true;
+}
+
+// The part that u's share falls into, and the token in it, by one wave.  part_at(i) is part i's sum; bits:
+// kPart / 32 words of LDS.
+template <typename E, int kPart, typename Part>
+__device__ inline void pick_token(const DraftArgs& a, int b, const Walk& w, Weights<E> ws, int parts, double u, uint32_t* bits, Part part_at) {
+  constexpr int P = kPiece<E>;
+  constexpr int kMine = kPart / 64, kPieces = kMine / P;  // values of a lane
+  constexpr int kHeld = 4;                                // parts of a lane that stay in registers between the sum and the search
+  static_assert(kMine % P == 0, "a lane's values are whole pieces");
+  const int lane = threadIdx.x & 63;
+  const int head = row_head(ws.row);
+  uint64_t struck = w.struck;
   double held[kHeld], total = 0.0;
 #pragma unroll
   for (int k = 0; k < kHeld; ++k) held[k] = part_at(64 * k + lane);
@@ -576,7 +541,8 @@ __global__ __launch_bounds__(kDraftThreads) void draft_pick_kernel(DraftArgs a) 
       before = __shfl(upto, 63);
     }
   } else {  // nothing is left of p (it was rounded away): p itself
-    ws.draft = nullptr, strikes = nullptr;
+    ws.draft = nullptr;
+    struck = 0;
     for (int i = 0; i < parts; ++i) total += part_sum<E, kPart>(ws, nullptr, i * kPart - head);
     target = u * total;
     for (part = 0; part < parts - 1; ++part) {
@@ -588,8 +554,9 @@ __global__ __launch_bounds__(kDraftThreads) void draft_pick_kernel(DraftArgs a) 
   target -= before;
   // The token in it.  A lane's values are neighbours here: the order of the sum is theirs.
   const int first = part * kPart - head;
-  if (strikes != nullptr) {
-    strike<kPart, 64>(bits, a, b, w.struck, first);
+  const uint32_t* strikes = nullptr;
+  if (struck != 0) {
+    strike<kPart, 64>(bits, a, b, struck, first);
     strikes = bits;
   }
   double v[kPieces][P];
@@ -621,6 +588,84 @@ __global__ __launch_bounds__(kDraftThreads) void draft_pick_kernel(DraftArgs a) 
       if (open && v[k][i] > 0.0 && c > target) at = e0 + k * P + i, open = false;
     }
   a.next[b] = at;
+}
+
+// u of the next token.
+__device__ inline double next_uniform(const DraftArgs& a, int b) {
+  return (double)fminf(fmaxf(a.u[(int64_t)b * a.N], 0.0f), 0x1.fffffep-1f);
+}
+
+// The sums of the weights, part by part.  kDraws: the walk is done.  kPicks: the last workgroup of a
+// sequence to get there picks the token, instead of draft_pick_kernel.
+template <typename E, bool kDraws, int kPart, bool kPicks>
+__global__ __launch_bounds__(kDraftThreads) void draft_sums_kernel(DraftArgs a) {
+  __shared__ Walk walk;
+  __shared__ uint32_t bits[kWaves4 * kPart / 32];
+  __shared__ int is_last;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int b = blockIdx.x / a.groups, group = blockIdx.x - b * a.groups;
+  const int parts = a.groups * kWaves4;
+  const double u = kPicks ? next_uniform(a, b) : 0.0;  // (used at the end of a chain of reads: read here)
+  if (!kDraws) {
+    if (tid < 64) {
+      int best;
+      RowStat p, q;
+      node_stats<false>(a, b, &best, &p, &q);
+      const Walk w = walk_nodes<E, false>(a, b, group == 0, best, p, q);
+      if (tid == 0) {
+        walk = w;
+        if (!kPicks && group == 0) a.walks[b] = w;
+      }
+    }
+    __syncthreads();
+  }
+  const Walk w = kDraws ? a.walks[b] : walk;
+  Weights<E> ws;
+  if (!drawn_row<E, kDraws>(a, b, w, parts, &ws)) {
+    if (kPicks && group == 0 && tid == 0) a.next[b] = -1;
+    return;
+  }
+  const int first = group * kWaves4 * kPart - row_head(ws.row);
+  const uint32_t* strikes = nullptr;
+  if (w.struck != 0) {
+    strike<kWaves4 * kPart, kDraftThreads>(bits, a, b, w.struck, first);
+    strikes = bits + wave * (kPart / 32);
+  }
+  const double s = part_sum<E, kPart>(ws, strikes, first + wave * kPart);
+  double* sums = a.sums + (int64_t)b * parts;
+  if constexpr (!kPicks) {
+    if (lane == 0) sums[group * kWaves4 + wave] = s;
+  } else {
+    // What the last workgroup reads is written and read at the agent's scope, past the
+    // XCDs' own caches; the wave waits for its store before the barrier, and the counter
+    // moves behind that.  (A release at that scope would write the whole L2 back: 20 us.)
+    if (lane == 0) __hip_atomic_store(&sums[group * kWaves4 + wave], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0)
+      is_last = __hip_atomic_fetch_add(&a.arrived[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.groups - 1;
+    __syncthreads();
+    if (is_last == 0 || wave != 0) return;
+    pick_token<E, kPart>(a, b, w, ws, parts, u, bits, [&](int i) {
+      return i < parts ? __hip_atomic_load(&sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+    });
+  }
+}
+
+// The next token from the parts' sums: a wave per sequence.
+template <typename E, bool kDraws, int kPart>
+__global__ __launch_bounds__(64) void draft_pick_kernel(DraftArgs a) {
+  __shared__ uint32_t bits[kPart / 32];
+  const int b = blockIdx.x, parts = a.groups * kWaves4;
+  const double* sums = a.sums + (int64_t)b * parts;
+  const double u = next_uniform(a, b);
+  const Walk w = a.walks[b];
+  Weights<E> ws;
+  if (!drawn_row<E, kDraws>(a, b, w, parts, &ws)) {
+    if (threadIdx.x == 0) a.next[b] = -1;
+    return;
+  }
+  pick_token<E, kPart>(a, b, w, ws, parts, u, bits, [&](int i) { return i < parts ? sums[i] : 0.0; });
 }
 
 template <typename E>
@@ -805,12 +850,17 @@ Layout layout_of(const fc_verify_desc* d) {
   const bool draws = rows_of(d) > (int64_t)d->B * d->N;
   l.stats = 0;
   l.walks = round256((size_t)rows_of(d) * chunks * sizeof(ChunkStat));
-  l.both = l.walks + (draws ? round256(B * sizeof(Walk)) : 0);
+  l.both = l.walks + round256(B * sizeof(Walk));
   l.sums = l.both + (draws ? round256(B * parts * sizeof(double2)) : 0);
   l.arrived = l.sums + round256(B * parts * sizeof(double));
   l.total = d->V <= kSmallValues ? 0 : l.arrived + round256(B * sizeof(int32_t));
   return l;
 }
+
+// From this many logits on the pick is a launch of its own: the arrival it saves is 4 us of the GPU's time, the
+// launch 2 to 3 of the host's, which is the longer below it (verify_drafts, 5 nodes, candidates and draws:
+// 8 x 131072 18.0 and 27.8 us for 20.5 and 29.9, 64 x 8192 17.4 and 21.5 for 14.9 and 20.5).
+constexpr int64_t kPickLogits = (int64_t)1 << 22;
 
 template <typename E, int kPart>
 hipError_t launch_ends(const DraftArgs& a, hipStream_t s) {
@@ -822,10 +872,19 @@ hipError_t launch_ends(const DraftArgs& a, hipStream_t s) {
     profile_end(mk, "draft_walk", s);
     if (e != hipSuccess) return e;
   }
-  const ProfileMark mk = profile_begin(s);
-  if (a.draft != nullptr) hipLaunchKernelGGL((draft_pick_kernel<E, true, kPart>), ends, dim3(kDraftThreads), 0, s, a);
-  else hipLaunchKernelGGL((draft_pick_kernel<E, false, kPart>), ends, dim3(kDraftThreads), 0, s, a);
-  const hipError_t e = hipGetLastError();
+  const bool draws = a.draft != nullptr, picks = (int64_t)a.B * a.N * a.V < kPickLogits;
+  ProfileMark mk = profile_begin(s);
+  if (draws && picks) hipLaunchKernelGGL((draft_sums_kernel<E, true, kPart, true>), ends, dim3(kDraftThreads), 0, s, a);
+  else if (draws) hipLaunchKernelGGL((draft_sums_kernel<E, true, kPart, false>), ends, dim3(kDraftThreads), 0, s, a);
+  else if (picks) hipLaunchKernelGGL((draft_sums_kernel<E, false, kPart, true>), ends, dim3(kDraftThreads), 0, s, a);
+  else hipLaunchKernelGGL((draft_sums_kernel<E, false, kPart, false>), ends, dim3(kDraftThreads), 0, s, a);
+  hipError_t e = hipGetLastError();
+  profile_end(mk, "draft_sums", s);
+  if (e != hipSuccess || picks) return e;
+  mk = profile_begin(s);
+  if (draws) hipLaunchKernelGGL((draft_pick_kernel<E, true, kPart>), dim3((unsigned)a.B), dim3(64), 0, s, a);
+  else hipLaunchKernelGGL((draft_pick_kernel<E, false, kPart>), dim3((unsigned)a.B), dim3(64), 0, s, a);
+  e = hipGetLastError();
   profile_end(mk, "draft_pick", s);
   return e;
 }

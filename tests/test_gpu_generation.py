@@ -475,11 +475,13 @@ def test_trees_of_candidates_against_the_oracle(gpu, V, dtype, N, temperature):
         _agree(got, logits, tokens, u, None, up, c, temperature)
 
 
+@pytest.mark.parametrize("B", [2, 8])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_a_row_of_many_parts(gpu, dtype):
-    """More parts of the drawn row than the last workgroup's registers hold, and draws from all over it."""
+def test_a_row_of_many_parts(gpu, dtype, B):
+    """More parts of the drawn row than a wave's registers hold, and draws from all over it, by the
+    last workgroup to arrive and in a launch of its own."""
     rng = np.random.default_rng(31)
-    B, N, V = 8, 3, 199999
+    N, V = 3, 199999
     logits = torch.from_numpy(0.5 * rng.standard_normal((B, N, V), dtype=np.float32)).to(dtype)
     draft = torch.from_numpy(0.5 * rng.standard_normal((B, N - 1, V), dtype=np.float32)).to(dtype)
     tokens = rng.integers(0, V, (B, N))
