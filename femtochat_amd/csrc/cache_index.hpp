@@ -1,5 +1,5 @@
 // Where a cache's tokens lie, and the checks of its descriptor: host and device
-// code, also built alone by the host harness (tests/sanitize/harness.cpp).
+// code, also built alone by the host harness (tests/sanitize/cache_harness.cpp).
 #pragma once
 
 #include <stddef.h>
