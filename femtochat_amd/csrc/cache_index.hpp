@@ -63,13 +63,18 @@ FC_HD inline Span span_of(int length, int count, int N, int left, int capacity) 
   return s;
 }
 // A batch's work is shared out as one line, each sequence's tiles behind the ones before,
-// with room in front for what beginning a sequence costs (in tiles): workgroup x takes the
-// x-th stretch of the line.  One share, and with it one workgroup, may end a sequence,
-// hold others whole and begin another.
+// in fours, as a workgroup's four waves take them, and with room in front for what beginning a
+// sequence costs (in tiles): workgroup x takes the x-th stretch of the line.  One share, and with
+// it one workgroup, may end a sequence, hold others whole and begin another.
 constexpr int kBegin = 8;
 
+FC_HD inline int line_length(int tiles) { return kBegin + (tiles + 3) / 4 * 4; }
+// (a 64-bit quotient is some 150 instructions)
+FC_HD inline int64_t line_quotient(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
 FC_HD inline int64_t share_of(int64_t total, int shares, int least) {
-  const int64_t s = (total + shares - 1) / shares;
+  const int64_t s = line_quotient(total + shares - 1, shares);
   return s > least ? s : least;
 }
 // The tiles (first, last: counted from the sequence's first) of a sequence at `start` of the

@@ -74,17 +74,6 @@ struct CachedAttnArgs {
 
 // ---- which keys a workgroup takes ---------------------------------------------
 
-__device__ inline int64_t wave_sum(int64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-
-__device__ inline int64_t of_lane(int64_t v, int lane) {
-  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, lane), hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)v >> 32), lane);
-  return (int64_t)((uint64_t)hi << 32 | lo);
-}
-
 // The lengths and counts of 64 sequences, one to each lane.
 struct Chunk {
   int b0, length, count;
@@ -109,45 +98,49 @@ struct Line {
   int b;          // which, B past the end
   Chunk chunk;    // from or around it
 };
+// The sum of a wave's values up to each lane, in the vector unit (shuffles through LDS take 130 cycles each).
+__device__ inline int sum_upto(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1, of each sixteen lanes
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15, to the second and fourth
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31, to the last two
+  return v;
+}
 // The first sequence of share x.  Every lane of a wave calls it and gets the same.
 __device__ inline Line find_on_line(const CachedAttnArgs& a, int x) {
   const int lane = threadIdx.x & 63;
-  const auto cost = [&](const Chunk& c) { return c.b0 + lane < a.g.B ? c.mine(a).tiles + kBegin : 0; };
+  const auto length = [&](const Chunk& c) { return c.b0 + lane < a.g.B ? line_length(c.mine(a).tiles) : 0; };
   Line l;
   l.chunk.load(a, 0);
-  int64_t total = cost(l.chunk);
+  int n = length(l.chunk), upto = sum_upto(n);  // with the sequences up to this lane's
+  int64_t total = __builtin_amdgcn_readlane(upto, 63);
   for (int b0 = 64; b0 < a.g.B; b0 += 64) {
     Chunk c;
     c.load(a, b0);
-    total += cost(c);
+    total += __builtin_amdgcn_readlane(sum_upto(length(c)), 63);
   }
-  total = wave_sum(total);
   l.share = share_of(total, a.shares, a.least);
   l.b = a.g.B;
   l.start = total;
   const int64_t at = x * l.share;
   int64_t before = 0;
   for (int b0 = 0; b0 < a.g.B; b0 += 64) {
-    if (b0 > 0) l.chunk.load(a, b0);
-    const int n = cost(l.chunk);
-    int64_t upto = n;  // with the sequences up to this lane's
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t v = __shfl_up(upto, o);
-      if (lane >= o) upto += v;
+    if (b0 > 0) {
+      l.chunk.load(a, b0);
+      n = length(l.chunk);
+      upto = sum_upto(n);
     }
     const uint64_t hit = __ballot(n > 0 && at < before + upto);
     if (hit != 0) {
       const int i = __ffsll((long long)hit) - 1;
       l.b = b0 + i;
-      l.start = before + of_lane(upto - n, i);
+      l.start = before + __builtin_amdgcn_readlane(upto - n, i);
       break;
     }
-    before += of_lane(upto, 63);
+    before += __builtin_amdgcn_readlane(upto, 63);
   }
-  l.share = of_lane(l.share, 0);
-  l.start = of_lane(l.start, 0);
-  l.b = __builtin_amdgcn_readfirstlane(l.b);
   return l;
 }
 
@@ -616,14 +609,14 @@ __device__ inline void for_each_stretch(const CachedAttnArgs& a, int x, bool tel
     const Span span = line.chunk.of(a, b);
     Stretch st{0, span.tiles};
     if (a.shares > 0) {
-      line.start += span.tiles + kBegin;
+      line.start += line_length(span.tiles);
       st = stretch_of(start, span.tiles, x, line.share);
       if (st.first >= st.last) continue;
     }
     if (again) __syncthreads();  // the last sequence's LDS is read
     again = true;
     if (a.shares > 0 && st.first == 0 && tells && threadIdx.x == 0) {
-      const int64_t last = (start + span.tiles + kBegin - 1) / line.share;
+      const int64_t last = line_quotient(start + span.tiles + kBegin - 1, line.share);
       a.parts[b] = make_int4((int)(last - x) + 1, (int)part_slot(start, x, line.share), (int)part_slot(start, x + 1, line.share), span.count);
     }
     body(b, span.length, span.count, span.first + st.first, span.first + st.last, st.first == 0 && st.last == span.tiles,
@@ -679,7 +672,7 @@ __device__ inline void finish(const CachedAttnArgs& a, const Rows<kType, kD, kR>
   // Sixteen threads to a row, four columns each at a time.
   const int of16 = tid >> 4;
   const int64_t out = (((int64_t)h * a.groups + group) * 2 * a.shares + slot) * kRows;
-#pragma unroll 1
+#pragma unroll
   for (int rb = 0; rb < kR; ++rb) {
     const int row = group * kRows + 16 * rb + of16, node = row / a.G, head = h * a.G + row - node * a.G;
     if (row >= a.rows) break;
@@ -695,7 +688,10 @@ __device__ inline void finish(const CachedAttnArgs& a, const Rows<kType, kD, kR>
     if (!whole && (tid & 15) == 0) a.part_s[out + 16 * rb + of16] = make_float2(m, sum);
     const float inv = 1.0f / sum;
     bf16* O = static_cast<bf16*>(a.O) + (((int64_t)b * a.N + node) * a.H + head) * kD;
-    for (int d = 4 * (tid & 15); d < kD; d += 64) {
+#pragma unroll
+    for (int of64 = 0; of64 < (kD + 63) / 64; ++of64) {
+      const int d = 64 * of64 + 4 * (tid & 15);
+      if (kD % 64 != 0 && d >= kD) break;
       f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(x.acc[rb][w] + of16 * kPad + d) * by[w];

@@ -76,7 +76,7 @@ static void slots() {
         CHECK(s.first * (int64_t)fc::kTileKeys <= s.length);
         if (s.length > left) CHECK(s.first * fc::kTileKeys <= s.length - left);
       }
-      total += s.tiles + fc::kBegin;
+      total += fc::line_length(s.tiles);
     }
     // The line: every tile of every sequence is in one share, a share has at most two parts of
     // sequences that it does not hold whole, and no two parts share a slot.
@@ -86,12 +86,13 @@ static void slots() {
     int64_t start = 0;
     for (const auto& s : spans) {
       int upto = 0;
-      for (int64_t x = start / each; x * each < start + s.tiles + fc::kBegin; ++x) {
+      for (int64_t x = start / each; x * each < start + fc::line_length(s.tiles); ++x) {
         CHECK(x < shares);
         const fc::Stretch st = fc::stretch_of(start, s.tiles, x, each);
         CHECK(st.first <= st.last && (st.first == upto || st.last == 0));
-        if (st.first >= st.last) {  // the room in front alone, in the first share that has any of it
-          CHECK(x == start / each && upto == 0);
+        CHECK(fc::line_quotient(start, each) == start / each);
+        if (st.first >= st.last) {  // the room in front alone, in the first share that has any of it, or what fills the last four
+          CHECK((x == start / each && upto == 0) || (upto == s.tiles && x * each >= start + s.tiles + fc::kBegin));
           continue;
         }
         upto = st.last;
@@ -105,7 +106,7 @@ static void slots() {
       const fc::Stretch before = fc::stretch_of(start, s.tiles, start / each - 1, each);
       const fc::Stretch behind = fc::stretch_of(start, s.tiles, (start + s.tiles + fc::kBegin - 1) / each + 1, each);
       CHECK(before.last == 0 && behind.first == s.tiles);
-      start += s.tiles + fc::kBegin;
+      start += fc::line_length(s.tiles);
     }
   }
   CHECK(fc::share_of((int64_t)1 << 50, 1, 12) == (int64_t)1 << 50);
