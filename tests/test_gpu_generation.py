@@ -232,6 +232,23 @@ def test_many_sequences(gpu):
     _compare(gpu, rng, "bf16", lengths, rng.integers(0, 4, 150), 3, 64, 8, 32, 1600, 16, tree="each")
 
 
+def test_thousands_of_sequences(gpu):
+    """A line far longer than the shares' least, whose beginning takes many chunks of lengths."""
+    rng = np.random.default_rng(40)
+    B, Hkv, H, D, capacity = 5000, 1, 3, 16, 1024
+    cache = F.kv_cache(B, capacity, Hkv, D, torch.int8, device=gpu)
+    lengths = torch.from_numpy(np.where(rng.integers(0, 50, B) > 0, rng.integers(0, 60, B), 1023).astype(np.int32))
+    K, V = (1.2 * torch.randn(B, capacity, Hkv, D, generator=torch.Generator().manual_seed(i)) for i in (1, 2))
+    F.cache_write_(cache, K.to(gpu), V.to(gpu), torch.zeros(B, dtype=torch.int32, device=gpu))
+    Q = (2.0 * torch.from_numpy(rng.standard_normal((B, 1, H, D), dtype=np.float32))).bfloat16()
+    O = F.cached_attention(Q.to(gpu), cache, lengths.to(gpu))
+    assert torch.isfinite(O).all()
+    for b in [0, 63, 64, B - 1] + rng.integers(0, B, 20).tolist() + torch.nonzero(lengths == 1023)[:20, 0].tolist():
+        n = int(lengths[b])
+        Kh, Vh = (G.held(x[b:b + 1, :n + 1].numpy(), "int8")[0] for x in (K, V))
+        _check(O[b], G.attend(Q[b].double().numpy(), Kh, Vh, n, 1), Vh)
+
+
 def test_scores_that_grow_along_the_keys(gpu):
     """References move, upwards by far, and a first key may be all there is."""
     rng = np.random.default_rng(9)
