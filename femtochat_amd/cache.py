@@ -173,7 +173,11 @@ def _batch(cache: KVCache, like) -> int:
     """The sequences of a call: those of ``like`` (B, ...), or of the cache's table."""
     if isinstance(like, torch.Tensor) and like.dim() >= 1:
         return like.shape[0]
-    return cache.k.shape[-4] if cache.pages is None else cache.pages.shape[0]
+    rows = cache.k if cache.pages is None else cache.pages
+    at = -4 if cache.pages is None else 0
+    if not isinstance(rows, torch.Tensor) or rows.dim() < (4 if cache.pages is None else 1):
+        raise ValueError("a cache is ([layers,] pages, Hkv, page, D) tensors and a (B, M) int32 table, or None for it")
+    return rows.shape[at]
 
 
 def _check_counts(c: _Buffers, lengths, counts, name: str = "lengths", required: bool = False) -> None:
@@ -223,12 +227,17 @@ def cache_read_(K: torch.Tensor, V: torch.Tensor, cache: KVCache, starts: Option
                 counts: Optional[torch.Tensor] = None) -> None:
     """``cache_read`` into the caller's K and V."""
     c = _buffers(cache, _batch(cache, starts if starts is not None else counts))
-    T = _check_values(c, K, V)
+    _check_values(c, K, V)
+    if K.shape[-3] != 0 and (K.data_ptr() | V.data_ptr()) % 16:
+        raise ValueError("K and V must start on a 16-byte boundary")
+    _read(c, K, V, starts, counts)
+
+
+def _read(c: _Buffers, K, V, starts, counts) -> None:
     _check_counts(c, starts, counts, "starts")
+    T = K.shape[-3]
     if T == 0:
         return
-    if (K.data_ptr() | V.data_ptr()) % 16:
-        raise ValueError("K and V must start on a 16-byte boundary")
     _call(c.device, _lib.lib().fc_cache_read, c.layout.ref, ctypes.byref(c.pointers), K.data_ptr(), V.data_ptr(),
           _dtype_code(K.dtype), T, _ptr(starts), _ptr(counts))
 
@@ -243,14 +252,11 @@ def cache_read(cache: KVCache, starts: Optional[torch.Tensor], T: int, counts: O
         raise TypeError(f"unsupported dtype {dtype}; a cache reads back as float32 or bfloat16")
     if T < 0:
         raise ValueError("T must not be negative")
-    k = cache.k
-    if not isinstance(k, torch.Tensor) or k.dim() not in (4, 5):
-        raise ValueError("a cache's k must be a ([layers,] pages, Hkv, page, D) tensor of bfloat16, int8 or float8_e4m3fn")
-    B = _batch(cache, starts if starts is not None else counts)
-    shape = tuple(k.shape[:-4]) + (B, T, k.shape[-3], k.shape[-1])
-    K = torch.empty(*shape, dtype=dtype, device=k.device)
+    c = _buffers(cache, _batch(cache, starts if starts is not None else counts))
+    layout = c.layout
+    K = torch.empty(*layout.lead, layout.B, T, layout.Hkv, layout.D, dtype=dtype, device=c.device)
     V = torch.empty_like(K)
-    cache_read_(K, V, cache, starts, counts)
+    _read(c, K, V, starts, counts)
     return K, V
 
 

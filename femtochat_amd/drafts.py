@@ -82,11 +82,16 @@ def verify_drafts_(path: torch.Tensor, kept: torch.Tensor, token: torch.Tensor, 
                    parents: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
                    temperature: float = 1.0, workspace: Optional[torch.Tensor] = None) -> None:
     """``verify_drafts`` into the caller's path (B, N), kept (B,) and token (B,), int32."""
-    device, d, nbytes = _checked(logits, tokens, uniforms, draft_logits, parents, counts, temperature)
+    checked = _checked(logits, tokens, uniforms, draft_logits, parents, counts, temperature)
     B, N = tokens.shape
-    _check_tensor("path", path, (B, N), _I32, device)
-    _check_tensor("kept", kept, (B,), _I32, device)
-    _check_tensor("token", token, (B,), _I32, device)
+    _check_tensor("path", path, (B, N), _I32, checked[0])
+    _check_tensor("kept", kept, (B,), _I32, checked[0])
+    _check_tensor("token", token, (B,), _I32, checked[0])
+    _verify(checked, path, kept, token, logits, tokens, uniforms, draft_logits, parents, counts, workspace)
+
+
+def _verify(checked, path, kept, token, logits, tokens, uniforms, draft_logits, parents, counts, workspace) -> None:
+    device, d, nbytes = checked
     at = None
     if nbytes > 0:
         if workspace is None:  # freed to this stream's pool on return, so later work on the stream comes after the kernels
@@ -114,9 +119,9 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniforms: Optional
     token -1; a sequence of no nodes (counts 0) keeps none."""
     if not isinstance(tokens, torch.Tensor) or tokens.dim() != 2:
         raise ValueError("tokens must be a (B, N) tensor")
-    B, N = tokens.shape
-    path = torch.empty(B, N, dtype=torch.int32, device=tokens.device)
-    kept, token = torch.empty(2, B, dtype=torch.int32, device=tokens.device).unbind(0)
-    verify_drafts_(path, kept, token, logits, tokens, uniforms, draft_logits=draft_logits, parents=parents, counts=counts,
-                   temperature=temperature, workspace=workspace)
+    checked = _checked(logits, tokens, uniforms, draft_logits, parents, counts, temperature)
+    device = checked[0]
+    path = torch.empty_like(tokens, dtype=torch.int32)
+    kept, token = torch.empty(2, tokens.shape[0], dtype=torch.int32, device=device).unbind(0)
+    _verify(checked, path, kept, token, logits, tokens, uniforms, draft_logits, parents, counts, workspace)
     return path, kept, token
