@@ -235,10 +235,10 @@ def test_many_sequences(gpu):
 def test_thousands_of_sequences(gpu):
     """A line far longer than the shares' least, whose beginning takes many chunks of lengths."""
     rng = np.random.default_rng(40)
-    B, Hkv, H, D, capacity = 5000, 1, 3, 16, 1024
-    cache = F.kv_cache(B, capacity, Hkv, D, torch.int8, device=gpu)
+    B, Hkv, H, D, T = 5000, 1, 3, 16, 1024
+    cache = F.kv_cache(B, 1600, Hkv, D, torch.int8, device=gpu)
     lengths = torch.from_numpy(np.where(rng.integers(0, 50, B) > 0, rng.integers(0, 60, B), 1023).astype(np.int32))
-    K, V = (1.2 * torch.randn(B, capacity, Hkv, D, generator=torch.Generator().manual_seed(i)) for i in (1, 2))
+    K, V = (1.2 * torch.randn(B, T, Hkv, D, generator=torch.Generator().manual_seed(i)) for i in (1, 2))
     F.cache_write_(cache, K.to(gpu), V.to(gpu), torch.zeros(B, dtype=torch.int32, device=gpu))
     Q = (2.0 * torch.from_numpy(rng.standard_normal((B, 1, H, D), dtype=np.float32))).bfloat16()
     O = F.cached_attention(Q.to(gpu), cache, lengths.to(gpu))
@@ -268,7 +268,7 @@ def test_scores_that_grow_along_the_keys(gpu):
 def test_scores_far_below_zero(gpu, N, H):
     """Every score of a row near -4e32: equal ones share, and a smaller one has nothing."""
     D, n = 16, 900
-    cache = F.kv_cache(1, 1024, 1, D, torch.bfloat16, device=gpu)
+    cache = F.kv_cache(1, 1600, 1, D, torch.bfloat16, device=gpu)
     K, V = torch.full((1, n + N, 1, D), 1e16), torch.randn(1, n + N, 1, D)
     K[0, :n // 2] = 2e16
     F.cache_write_(cache, K.to(gpu), V.to(gpu), torch.zeros(1, dtype=torch.int32, device=gpu))
