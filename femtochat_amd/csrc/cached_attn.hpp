@@ -263,26 +263,33 @@ struct Queries {
   using C = CachedCfg<kType, kD>;
   bf16x8 unit[kR][C::kSteps][64];
 
-  // All 256 threads, sixteen to a row: load, then store, which waits for the values.  Returns
-  // which there are; the others, of which any may be read, are stored as zeros.
-  __device__ static inline uint32_t load(bf16x8 (&to)[kR], const CachedAttnArgs& a, int b, int h, int first_row, int count) {
+  // All of kW waves, sixteen threads to a row and kEach rows each: load, then store, which waits for the
+  // values.  Returns which there are; the others, of which any may be read, are stored as zeros.
+  template <int kW>
+  static constexpr int kEach = (16 * kR + 4 * kW - 1) / (4 * kW);
+  template <int kW>
+  __device__ static inline uint32_t load(bf16x8 (&to)[kEach<kW>], const CachedAttnArgs& a, int b, int h, int first_row, int count) {
     uint32_t there = 0;
 #pragma unroll
-    for (int rb = 0; rb < kR; ++rb) {
-      const int row = first_row + 16 * rb + (int)(threadIdx.x >> 4), node = row / a.G, u = threadIdx.x & 15;
-      const bool mine = node < count && u < C::kU;
+    for (int i = 0; i < kEach<kW>; ++i) {
+      const int of = 4 * kW * i + (int)(threadIdx.x >> 4), row = first_row + of, node = row / a.G, u = threadIdx.x & 15;
+      const bool mine = of < 16 * kR && node < count && u < C::kU;
       const bf16* src = static_cast<const bf16*>(a.Q);
       src += mine ? (((int64_t)b * a.N + node) * a.H + h * a.G + row - node * a.G) * kD + 8 * u : 0;
-      to[rb] = *reinterpret_cast<const bf16x8*>(src);
-      there |= mine ? 1u << rb : 0;
+      to[i] = *reinterpret_cast<const bf16x8*>(src);
+      there |= mine ? 1u << i : 0;
     }
     return there;
   }
-  __device__ inline void store(const bf16x8 (&from)[kR], uint32_t there) {
-    const int n = threadIdx.x >> 4, u = threadIdx.x & 15;
+  template <int kW>
+  __device__ inline void store(const bf16x8 (&from)[kEach<kW>], uint32_t there) {
+    const int u = threadIdx.x & 15;
 #pragma unroll
-    for (int rb = 0; rb < kR; ++rb)
-      if (u < 4 * C::kSteps) unit[rb][u % C::kSteps][n + 16 * (u / C::kSteps)] = (there >> rb & 1) != 0 ? from[rb] : Mma<bf16>::zero();
+    for (int i = 0; i < kEach<kW>; ++i) {
+      const int of = 4 * kW * i + (int)(threadIdx.x >> 4);
+      if (of < 16 * kR && u < 4 * C::kSteps)
+        unit[of / 16][u % C::kSteps][of % 16 + 16 * (u / C::kSteps)] = (there >> i & 1) != 0 ? from[i] : Mma<bf16>::zero();
+    }
   }
 };
 
@@ -640,18 +647,18 @@ __device__ inline Place place_of(const CachedAttnArgs& a) {
   return p;
 }
 
-// A stretch's end: each of four waves holds sums of the workgroup's rows over some of its keys.
-template <int kD, int kR>
+// A stretch's end: each of kW waves holds sums of the workgroup's rows over some of its keys.
+template <int kD, int kR, int kW>
 struct Exchange {
   static constexpr int kPad = kD + 4;  // floats of a row: the lanes' stores spread over the banks
-  float acc[kR][4][16 * kPad];
-  float2 stats[kR][4][16];
+  float acc[kR][kW][16 * kPad];
+  float2 stats[kR][kW][16];
 };
-template <int kType, int kD, int kR>
-__device__ inline void finish(const CachedAttnArgs& a, const Rows<kType, kD, kR>& rows, Exchange<kD, kR>& x, int b, int h, int group,
+template <int kType, int kD, int kR, int kW>
+__device__ inline void finish(const CachedAttnArgs& a, const Rows<kType, kD, kR>& rows, Exchange<kD, kR, kW>& x, int b, int h, int group,
                               int count, bool whole, int64_t slot) {
   using C = CachedCfg<kType, kD>;
-  constexpr int kPad = Exchange<kD, kR>::kPad, kRows = 16 * kR;
+  constexpr int kPad = Exchange<kD, kR, kW>::kPad, kRows = 16 * kR;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int rb = 0; rb < kR; ++rb) {
@@ -670,22 +677,22 @@ __device__ inline void finish(const CachedAttnArgs& a, const Rows<kType, kD, kR>
   }
   __syncthreads();
   // Sixteen threads to a row, four columns each at a time.
-  const int of16 = tid >> 4;
   const int64_t out = (((int64_t)h * a.groups + group) * 2 * a.shares + slot) * kRows;
 #pragma unroll
-  for (int rb = 0; rb < kR; ++rb) {
-    const int row = group * kRows + 16 * rb + of16, node = row / a.G, head = h * a.G + row - node * a.G;
-    if (row >= a.rows) break;
-    float by[4], m = -INFINITY, sum = 0.0f;
+  for (int i = 0; i < (kRows + 4 * kW - 1) / (4 * kW); ++i) {
+    const int of = 4 * kW * i + (tid >> 4), rb = of / 16, of16 = of % 16;
+    const int row = group * kRows + of, node = row / a.G, head = h * a.G + row - node * a.G;
+    if (of >= kRows || row >= a.rows) break;
+    float by[kW], m = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) m = fmaxf(m, x.stats[rb][w][of16].x);
+    for (int w = 0; w < kW; ++w) m = fmaxf(m, x.stats[rb][w][of16].x);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < kW; ++w) {
       const float2 st = x.stats[rb][w][of16];
       by[w] = __builtin_amdgcn_exp2f(st.x - m);
       sum += st.y * by[w];
     }
-    if (!whole && (tid & 15) == 0) a.part_s[out + 16 * rb + of16] = make_float2(m, sum);
+    if (!whole && (tid & 15) == 0) a.part_s[out + of] = make_float2(m, sum);
     const float inv = 1.0f / sum;
     bf16* O = static_cast<bf16*>(a.O) + (((int64_t)b * a.N + node) * a.H + head) * kD;
 #pragma unroll
@@ -694,12 +701,12 @@ __device__ inline void finish(const CachedAttnArgs& a, const Rows<kType, kD, kR>
       if (kD % 64 != 0 && d >= kD) break;
       f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(x.acc[rb][w] + of16 * kPad + d) * by[w];
+      for (int w = 0; w < kW; ++w) v += *reinterpret_cast<const f32x4*>(x.acc[rb][w] + of16 * kPad + d) * by[w];
       if (whole) {
         v = node < count ? v * inv : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         *reinterpret_cast<uint2*>(O + d) = make_uint2(pair(v[0], v[1]), pair(v[2], v[3]));
       } else {
-        *reinterpret_cast<f32x4*>(a.part_o + (out + 16 * rb + of16) * kD + d) = v;
+        *reinterpret_cast<f32x4*>(a.part_o + (out + of) * kD + d) = v;
       }
     }
   }
@@ -712,15 +719,16 @@ __device__ inline const int32_t* parents_of(const CachedAttnArgs& a, int b) {
   return a.parents == nullptr ? nullptr : a.parents + (a.tree == 2 ? (int64_t)b * a.N : 0);
 }
 
-// Four waves take every fourth tile of 32 keys, each straight from memory through its
-// registers, for the 16 kR rows of their workgroup.
-template <int kType, int kD, int kR>
-__global__ __launch_bounds__(256, 2) void cached_attn_kernel(CachedAttnArgs a) {
+// kW waves take every kW-th tile of 32 keys, each straight from memory through its
+// registers, for the 16 kR rows of their workgroup: four, or eight where a workgroup has a CU to
+// itself.
+template <int kType, int kD, int kR, int kW>
+__global__ __launch_bounds__(64 * kW, 2) void cached_attn_kernel(CachedAttnArgs a) {
   using C = CachedCfg<kType, kD>;
   constexpr bool k8 = kType != FC_CACHE_BF16;
   __shared__ Nodes nodes;
   __shared__ __attribute__((aligned(16))) Queries<kType, kD, kR> queries;
-  __shared__ __attribute__((aligned(16))) Exchange<kD, kR> exchange;
+  __shared__ __attribute__((aligned(16))) Exchange<kD, kR, kW> exchange;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = (threadIdx.x & 63) >> 4;
   const Place at = place_of(a);
   if (at.h >= a.g.Hkv) return;
@@ -763,26 +771,26 @@ __global__ __launch_bounds__(256, 2) void cached_attn_kernel(CachedAttnArgs a) {
     };
     // What a stretch begins with is requested before any of it is waited for.
     const auto fetch = [&](int key) {
-      blocks[0].fetch(a, b, key, 4 * kTileKeys, end);
-      blocks[1].fetch(a, b, key + 16, 4 * kTileKeys, end);
+      blocks[0].fetch(a, b, key, kW * kTileKeys, end);
+      blocks[1].fetch(a, b, key + 16, kW * kTileKeys, end);
     };
     int tile = tile0 + wave, i = 0;
     fetch(tile * kTileKeys);
-    bf16x8 q[kR];
-    const uint32_t asked = queries.load(q, a, b, at.h, first_row, count);
+    bf16x8 q[Queries<kType, kD, kR>::template kEach<kW>];
+    const uint32_t asked = queries.template load<kW>(q, a, b, at.h, first_row, count);
     const int32_t* parents = parents_of(a, b);
     const int up = parents != nullptr && (int)threadIdx.x < a.N ? parents[threadIdx.x] : -1;
     locate(0, tile * kTileKeys, tile < tile1);
     load_k();
     load_v();
-    queries.store(q, asked);
+    queries.template store<kW>(q, asked);
     if (wave == 0) trace_nodes(&nodes, parents != nullptr, up, a.N, a.left);
     __syncthreads();
     Rows<kType, kD, kR> rows;
     rows.begin(a, nodes, b, at.h, first_row, length, count);
-    for (; tile < tile1; tile += 4) {
-      const int key0 = tile * kTileKeys, next = key0 + 4 * kTileKeys;
-      if (kR == 2) {
+    for (; tile < tile1; tile += kW) {
+      const int key0 = tile * kTileKeys, next = key0 + kW * kTileKeys;
+      if (kR == 2 && kW == 4) {
         // Of a CU's two workgroups the one that is behind goes first; the older one would be done at two
         // thirds of the time and leave half the CU idle (16 sequences, 32 nodes: 61 us for 58).
         const int left = 4 * (tile1 - tile), all = tile1 - tile0;
@@ -811,7 +819,7 @@ __global__ __launch_bounds__(256, 2) void cached_attn_kernel(CachedAttnArgs a) {
           return k8 ? __builtin_bit_cast(f32x4, scales[kb]) * f : f32x4{f, f, f, f};
         }
         __device__ inline void used() const { request(i, next, more); }
-      } keys{k, ks, page, g, request_k, i, next, tile + 4 < tile1};
+      } keys{k, ks, page, g, request_k, i, next, tile + kW < tile1};
       struct {
         decltype(v)& bytes;
         decltype(vs)& scales;
@@ -836,7 +844,7 @@ __global__ __launch_bounds__(256, 2) void cached_attn_kernel(CachedAttnArgs a) {
       rows.tile(call, queries, nodes, a.N, key0, length, keys, values);
       load_v();
     }
-    finish<kType, kD, kR>(a, rows, exchange, b, at.h, at.group, count, whole, slot);
+    finish<kType, kD, kR, kW>(a, rows, exchange, b, at.h, at.group, count, whole, slot);
   });
 }
 
@@ -900,7 +908,7 @@ __global__ __launch_bounds__(256) void cached_attn_join_kernel(CachedAttnArgs a,
 }
 
 // What a variant of row blocks needs (cached_attn.hip instantiates them by type and head dim).
-template <int kType> hipError_t launch_cached_attn(const CachedAttnArgs& a, int row_blocks, hipStream_t s);
+template <int kType> hipError_t launch_cached_attn(const CachedAttnArgs& a, int row_blocks, int waves, hipStream_t s);
 hipError_t launch_cached_attn_join(const CachedAttnArgs& a, int rows_per_group, hipStream_t s);
 
 }  // namespace fc

@@ -62,7 +62,7 @@ constexpr int kWholeTiles = 32;
 // The sizes of a call that follow from its descriptor alone (not from the lengths,
 // which lie on the device).
 struct Plan {
-  int row_blocks, groups, shares;
+  int row_blocks, groups, shares, waves;
   size_t s_at, parts_at, bytes;  // in the workspace, behind the parts of O
 };
 
@@ -77,8 +77,13 @@ Plan plan_of(const CacheGeom& g, int H, int N, int left) {
   p.groups = (rows + 16 * p.row_blocks - 1) / (16 * p.row_blocks);
   // A sequence's tiles, at most.
   const int64_t span = std::min<int64_t>(g.capacity, (int64_t)left + N + kTileKeys);
-  const bool parts = (span + kTileKeys - 1) / kTileKeys > kWholeTiles;
-  p.shares = parts ? std::max(1, kSlots / (g.Hkv * p.groups)) : 0;
+  const int64_t tiles = (span + kTileKeys - 1) / kTileKeys;
+  p.shares = tiles > kWholeTiles ? std::max(1, kSlots / (g.Hkv * p.groups)) : 0;
+  // Eight waves where each workgroup has a CU to itself and a tile for more than four: 4 x 13 nodes, 8 heads of 64 with
+  // capped and biased scores over 512 keys, 13.0 us with four, 11.8 with eight; 16 x 16 nodes of two heads over 1000 keys 15.2
+  // and 13.7; single tokens the same.
+  const bool few = (int64_t)g.B * g.Hkv * p.groups <= kSlots / 2;
+  p.waves = p.shares == 0 && few && tiles > 4 ? 8 : 4;
   const int64_t rows_kept = (int64_t)g.Hkv * p.groups * 2 * p.shares * 16 * p.row_blocks;
   p.s_at = round256((size_t)rows_kept * g.D * 4);
   p.parts_at = p.s_at + round256((size_t)rows_kept * sizeof(float2));
@@ -155,9 +160,9 @@ fc_status fc_cached_attn(const fc_cache_desc* desc, const fc_cache* cache, const
     a.cap_out = (float)(1.4426950408889634 * options->softcap);
   }
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  hipError_t e = desc->type == FC_CACHE_BF16 ? fc::launch_cached_attn<FC_CACHE_BF16>(a, p.row_blocks, s)
-                 : desc->type == FC_CACHE_I8 ? fc::launch_cached_attn<FC_CACHE_I8>(a, p.row_blocks, s)
-                                             : fc::launch_cached_attn<FC_CACHE_F8>(a, p.row_blocks, s);
+  hipError_t e = desc->type == FC_CACHE_BF16 ? fc::launch_cached_attn<FC_CACHE_BF16>(a, p.row_blocks, p.waves, s)
+                 : desc->type == FC_CACHE_I8 ? fc::launch_cached_attn<FC_CACHE_I8>(a, p.row_blocks, p.waves, s)
+                                             : fc::launch_cached_attn<FC_CACHE_F8>(a, p.row_blocks, p.waves, s);
   if (e == hipSuccess && p.shares > 0) e = fc::launch_cached_attn_join(a, 16 * p.row_blocks, s);
   if (e != hipSuccess) return fc::bad(who, hipGetErrorString(e), FC_ERR_HIP);
   fc::clear_error();

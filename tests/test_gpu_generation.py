@@ -228,6 +228,7 @@ def test_many_sequences(gpu):
     lengths = rng.integers(0, 700, 150)
     _compare(gpu, rng, "int8", lengths, rng.integers(0, 3, 150), 2, 2, 1, 64, 768, 64, tree="run")
     _compare(gpu, rng, "fp8", rng.integers(0, 1500, 150), rng.integers(0, 3, 150), 2, 2, 1, 64, 1600, 64, tree="run")
+    _compare(gpu, rng, "int8", rng.integers(0, 90, 300), rng.integers(0, 3, 300), 2, 20, 2, 32, 768, 64, tree="run")  # (more than a CU has room for)
     lengths = np.where(rng.integers(0, 20, 150) > 0, rng.integers(0, 40, 150), 1500)
     _compare(gpu, rng, "bf16", lengths, rng.integers(0, 4, 150), 3, 64, 8, 32, 1600, 16, tree="each")
 
