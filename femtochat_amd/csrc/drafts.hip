@@ -81,19 +81,23 @@ constexpr int kWaves4 = kDraftThreads / 64;
 
 // exp((x - most) / temperature) for x <= most.  2^t = 2^n 2^f, n the nearest whole number
 // (its bits come from adding 1.5 2^52) and f in [-1/2, 1/2]: a polynomial of degree 10 through
-// the Chebyshev points, within 2^-51 (v_exp_f32 has 2^-22); 17 instructions.
+// the Chebyshev points, within 2^-51 (v_exp_f32 has 2^-22); 20 instructions.  t comes from the
+// difference in float64, of which t = 0 at the largest logit whatever its size.
 struct Exponent {
-  double to_log2, most2;  // log2(e) / temperature, most times that
-  float low;              // logits below it have no weight: 2^-1000
+  double most, to_log2;  // log2(e) / temperature
+  double least;          // of a difference with a weight: 2^-1000
+  float most32, cut;     // both in float32: a difference's rounding moves that end by 2^-23 of itself, however large the logits
 };
 __device__ inline Exponent exponent_of(float most, double to_log2) {
-  return Exponent{to_log2, (double)most * to_log2, (float)((double)most - 1000.0 / to_log2)};
+  const double least = -1000.0 / to_log2;
+  return Exponent{(double)most, to_log2, least, most, (float)least};
 }
 __device__ inline float nan_max(float x, float y) { return __builtin_elementwise_maximum(x, y); }
+__device__ inline bool weightless(float x, const Exponent& e) { return x - e.most32 <= e.cut; }
 // A logit without weight has 2^-1000, which a sum does not notice (weight_of: 0).
 __device__ inline double term_of(float x, const Exponent& e) {
-  const double t = __builtin_fma((double)nan_max(x, e.low), e.to_log2, -e.most2);
-  const double s = t + 0x1.8p52, f = t - (s - 0x1.8p52);
+  const double d = weightless(x, e) ? e.least : (double)x - e.most;
+  const double s = __builtin_fma(d, e.to_log2, 0x1.8p52), f = __builtin_fma(d, e.to_log2, -(s - 0x1.8p52));
   double v = 0x1.e6064532b85cep-28;
   v = __builtin_fma(v, f, 0x1.b675bd731322bp-24);
   v = __builtin_fma(v, f, 0x1.62bfd472702f4p-20);
@@ -112,7 +116,7 @@ __device__ inline double term_of(float x, const Exponent& e) {
 }
 __device__ inline double weight_of(float x, const Exponent& e) {
   const double v = term_of(x, e);
-  return x <= e.low ? 0.0 : v;
+  return weightless(x, e) ? 0.0 : v;
 }
 
 // The values of the row from element e on, as many as 16 bytes hold; -infinity outside
