@@ -52,7 +52,7 @@ struct RowStat {
 // Where a sequence's walk ended.
 struct Walk {
   int last;         // node, -1: nothing is kept
-  int residual;     // draws: weights max(p - q, 0)
+  int residual;     // draws: a draft was refused there, weights max(p - q, 0)
   int next;         // temperature 0
   uint64_t struck;  // candidates: the nodes whose tokens were tried there
   RowStat p, q;
@@ -301,6 +301,7 @@ __device__ inline Walk walk_nodes(const DraftArgs& a, int b, bool write, int bes
   w.struck = 0;
   int kept = count > 0 ? 1 : 0, mine = -1;  // path[lane]
   if (i == 0 && count > 0) mine = 0;
+  w.residual = 0;
   while (w.last >= 0) {
     const uint64_t children = __ballot(known && up == w.last);
     uint64_t hit = kGreedy || a.draft != nullptr ? __ballot(chosen) & children : 0;
@@ -321,12 +322,14 @@ __device__ inline Walk walk_nodes(const DraftArgs& a, int b, bool write, int bes
       }
       w.struck = hit == 0 ? children : 0;
     }
-    if (hit == 0) break;
+    if (hit == 0) {
+      w.residual = a.draft != nullptr && children != 0;  // (a token outside the vocabulary was not drawn from q, and is not refused)
+      break;
+    }
     w.last = __ffsll((long long)hit) - 1;
     if (i == kept) mine = w.last;
     ++kept;
   }
-  w.residual = a.draft != nullptr && kept < count;
   w.next = -1;
   w.p = w.q = RowStat{-INFINITY, 0.0};
   if (w.last >= 0) {

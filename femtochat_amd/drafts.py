@@ -13,7 +13,8 @@ softmax at ``temperature``::
                 order: accepted if u[i] (1 - what those before it have of p) < p(x); the
                 next token is drawn from p without those tried
 
-Either way the text is distributed as the model's own samples are.  The next token of
+Either way the text is distributed as the model's own samples are.  A token outside the
+vocabulary counts as no node: the run ends before it.  The next token of
 a draw is the first whose cumulative weight is above u[0] of the whole.  At temperature 0
 the largest logit (the first of several) is accepted and drawn.  The reference has no
 counterpart.

@@ -112,6 +112,8 @@ fc_status fc_cached_attn(const fc_cache_desc* desc, const fc_cache* cache, const
    Candidates (no draft_logits): a node's children are tried in order; x is accepted
      if u[i] (1 - what those before it have of p) < p(x), and a token tried before is
      not; the next token is drawn from p without the tried ones.
+   A token outside the vocabulary is neither accepted nor refused: as if there were
+     no node, the next token is drawn from p without the tried ones.
    A draw takes the first token whose cumulative weight is above u[0] of the whole.
    At temperature 0 a child that is the largest logit (the first of several) is
    accepted, and the next token is the largest; draft_logits and u are not read.
