@@ -363,7 +363,8 @@ def cached_attention(Q: torch.Tensor, cache: KVCache, lengths: torch.Tensor, win
     it follows the sequence itself.  ``window`` (left, 0), ``softcap`` and ``slopes`` are those of
     ``attention``, over positions in the text (a node's is ``lengths[b]`` plus its ancestors).
     Nodes from ``counts[b]`` on get zeros; one beyond the cache's capacity, or whose
-    parents are no tree's, gets NaN."""
+    parents are no tree's, gets NaN.  A value that is not finite is the result in its column
+    for the nodes that see it, and reaches no other."""
     if isinstance(Q, torch.Tensor) and Q.dtype in (torch.float32, torch.float16):
         x = Q.to(torch.bfloat16)
         O = torch.empty_like(x)

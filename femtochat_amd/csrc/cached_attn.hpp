@@ -40,9 +40,11 @@
 // a SIMD have an instruction under way for 94% of the time, two thirds of it vector ones, of
 // which 190 of 450 a tile turn codes into numbers and 90 make two numbers of each probability.
 //
-// Rows that do not see a key have P = 0 there, but 0 * infinity is not 0: in tiles
-// that some row sees only in part, values that no row sees are taken as zeros,
-// and those that are not finite are left out of the product and put where they are seen.
+// Rows that do not see a key have P = 0 there, but 0 * infinity is not 0, nor has a P of two numbers one
+// sign.  Values that no row sees are taken as zeros.  Where a wave's sums of bf16 values turn out not to be
+// finite, it goes through its keys again, with values that are not as zeros, and puts those where they are
+// seen at the end.  A NaN of float8 (a caller's own codes) is one to all rows that see it; in tiles that
+// some row sees only in part it is taken out and put in likewise, without a second pass.
 #pragma once
 
 #include "attn_fast.hpp"
@@ -237,6 +239,14 @@ struct CachedCfg {
 // A row's reference before its first key: no score but -infinity is below it.
 constexpr float kNoReference = -0x1.fffffep127f;
 
+// Sums under another reference: by may be 0, which leaves an infinity what it is.
+__device__ inline f32x4 scaled(f32x4 v, float by) {
+  f32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = __builtin_isinf(v[i]) ? v[i] : v[i] * by;
+  return r;
+}
+
 // What a call needs beside the sequence, the same for every row.
 struct CallScores {
   float factor;  // of a product before its key's scale: log2(e) / sqrt(D), or what the cap takes
@@ -307,12 +317,14 @@ struct Rows {
   bool broken[kR];              // NaN
   f32x4 acc[kR][C::kC];         // column C (4 g + r) + c of lane n's row
   float ref[kR], sum[kR];
+  uint32_t odd;                 // not 0: a NaN code was taken out
 
   __device__ inline void begin(const CachedAttnArgs& a, const Nodes& nodes, int b, int h, int first_row, int length, int count) {
     const int n = threadIdx.x & 15;
     any_sees = 0;
     any_low = INT_MAX;
     all_low = 0;
+    odd = 0;
 #pragma unroll
     for (int rb = 0; rb < kR; ++rb) {
       const int row = first_row + 16 * rb + n, node = row / a.G, head = h * a.G + row - node * a.G;
@@ -337,6 +349,18 @@ struct Rows {
     all_low = __builtin_amdgcn_readfirstlane((int)reduce16((uint32_t)all_low, [](uint32_t x, uint32_t y) { return max(x, y); }));
   }
 
+  // Whether all the wave's sums are finite.
+  __device__ inline bool all_finite() const {
+    float zero = 0.0f;
+#pragma unroll
+    for (int rb = 0; rb < kR; ++rb)
+#pragma unroll
+      for (int c = 0; c < C::kC; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) zero = __builtin_fmaf(acc[rb][c][r], 0.0f, zero);
+    return __ballot(zero != zero) == 0;
+  }
+
   // Which of a lane's eight keys are set in a mask of 32 from key 4 g on, as halves of
   // the operands' words: keys 2 i and 2 i + 1.
   __device__ static inline u32x4 halves(uint32_t keys) {
@@ -351,13 +375,13 @@ struct Rows {
 
   // Keys key0 .. key0 + 31.  Of `keys`: frag(kb, step), scale(kb) of keys 4 g + r, used() once
   // both are; of `values`: frag(c), scale(kb), and for keys of which some row may be blind
-  // keep(mask: which of the 32 keys from 4 g on any row sees), finite() (non-finite values
-  // become zeros).
+  // keep(mask: which of the 32 keys from 4 g on any row sees) and finite() (values that are not
+  // become zeros; whether any was).  finite: of bf16 in all tiles.
   template <typename Keys, typename Values>
-  __device__ inline void tile(const CallScores& call, const Queries<kType, kD, kR>& queries, const Nodes& nodes, int N, int key0, int length, Keys& keys, Values& values) {
+  __device__ inline void tile(const CallScores& call, bool finite, const Queries<kType, kD, kR>& queries, const Nodes& nodes, int N, int key0, int length, Keys& keys, Values& values) {
     const int g = (threadIdx.x & 63) >> 4;
     // Every row sees every key of a tile before the nodes and behind all rows' first keys.
-    const bool masked = key0 < all_low || key0 + kTileKeys > length;
+    const bool masked = finite || key0 < all_low || key0 + kTileKeys > length;
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));  // (the queries would be kept in registers from tile to tile)
     f32x4 s[kR][2];
@@ -455,47 +479,14 @@ struct Rows {
     }
     if (masked) {
       values.keep(seen_keys(key0 + g4, any_low, any_sees, length));
-      if (k8) {  // (an unseen key's scale may be NaN; codes are finite)
+      if (kType == FC_CACHE_F8) odd |= values.finite();
+      if (finite) values.finite();
+      if (k8) {  // (an unseen key's scale may be NaN)
 #pragma unroll
         for (int rb = 0; rb < kR; ++rb) {
           const u32x4 mine = halves(seen_keys(key0 + g4, low[rb], sees[rb], length));
           ph[rb] &= mine;
           pl[rb] &= mine;
-        }
-      } else {
-        bool odd = false;  // a value that is not finite where some row sees it
-#pragma unroll
-        for (int c = 0; c < C::kC; ++c) {
-          const u32x4 v = __builtin_bit_cast(u32x4, values.frag(c));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) odd |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
-        }
-        if (__ballot(odd) != 0) {
-          // Rare.  Which rows see +infinity, -infinity or NaN in which columns: a product of
-          // ones; such a value is added to those rows alone and is 0 in the others' product.
-#pragma unroll 1
-          for (int kind = 0; kind < 3; ++kind) {
-            const auto is = [&](uint32_t half) {
-              return kind == 0 ? half == 0x7f80u : kind == 1 ? half == 0xff80u : (half & 0x7fffu) > 0x7f80u;
-            };
-            const float what = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN;
-#pragma unroll
-            for (int c = 0; c < C::kC; ++c) {
-              const u32x4 v = __builtin_bit_cast(u32x4, values.frag(c));
-              u32x4 flags;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) flags[i] = (is(v[i] & 0xffffu) ? 0x3f80u : 0) | (is(v[i] >> 16) ? 0x3f800000u : 0);
-#pragma unroll
-              for (int rb = 0; rb < kR; ++rb) {
-                const bf16x8 ones = __builtin_bit_cast(bf16x8, halves(seen_keys(key0 + g4, low[rb], sees[rb], length)) & 0x3f803f80u);
-                const f32x4 found =
-                    __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, flags), ones, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) acc[rb][c][r] += found[r] > 0.0f ? what : 0.0f;
-              }
-            }
-          }
-          values.finite();
         }
       }
     }
@@ -509,9 +500,13 @@ struct Rows {
     }
   }
 };
-// A word's halves that are no finite bf16, as zeros.
-__device__ inline uint32_t finite_halves(uint32_t w) {
-  return w & ((w & 0x7f80u) == 0x7f80u ? 0xffff0000u : ~0u) & ((w & 0x7f800000u) == 0x7f800000u ? 0xffffu : ~0u);
+// A word's values that are not finite, all bits of them: halves of bf16, NaN codes of float8.
+template <int kType>
+__device__ inline uint32_t odd_bits(uint32_t w) {
+  if constexpr (kType == FC_CACHE_BF16)
+    return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+  const uint32_t top = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // (a code's 7 bits and 1)
+  return top | (top - (top >> 7));
 }
 
 // The K operand of 8 neighbouring values, and the V operands of eight keys' C columns.
@@ -647,18 +642,74 @@ __device__ inline Place place_of(const CachedAttnArgs& a) {
   return p;
 }
 
+// The kinds of kC values that are not finite, two bits each: 1 +infinity, 2 -infinity, 3 NaN.
+template <int kType, int kC>
+__device__ inline uint32_t odd_values(const uint32_t* w) {
+  uint32_t kinds = 0;
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    if constexpr (kType == FC_CACHE_BF16) {
+      const uint32_t v = w[c / 2] >> 16 * (c % 2) & 0xffffu;
+      kinds |= (v == 0x7f80u ? 1u : v == 0xff80u ? 2u : (v & 0x7fffu) > 0x7f80u ? 3u : 0u) << 2 * c;
+    } else {
+      kinds |= (w[c / 4] >> 8 * (c % 4) & 0x7fu) == 0x7fu ? 3u << 2 * c : 0u;
+    }
+  }
+  return kinds;
+}
+// What marks of the three kinds (bits 1, 2 and 3) add to a sum.
+__device__ inline float marked_value(uint32_t marks) {
+  return marks == 0 ? 0.0f : marks == 2 ? INFINITY : marks == 4 ? -INFINITY : NAN;
+}
+
 // A stretch's end: each of kW waves holds sums of the workgroup's rows over some of its keys.
-template <int kD, int kR, int kW>
+template <int kType, int kD, int kR, int kW>
 struct Exchange {
+  using C = CachedCfg<kType, kD>;
   static constexpr int kPad = kD + 4;  // floats of a row: the lanes' stores spread over the banks
-  float acc[kR][kW][16 * kPad];
+  float acc[kR][kW][16 * kPad];        // before that, marks of values that are not finite
   float2 stats[kR][kW][16];
+
+  // A wave's own part; all of its lanes call them.
+  __device__ inline void clear(int wave) {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+#pragma unroll 1
+    for (int rb = 0; rb < kR; ++rb)
+#pragma unroll 1
+      for (int i = lane; i < 16 * kPad; i += 64) acc[rb][wave][i] = 0.0f;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  // kinds: of the lane's columns of key key0 + 16 kb + 4 g + r.
+  __device__ inline void mark(int wave, const Rows<kType, kD, kR>& rows, uint32_t kinds, int key0, int kb, int r, int length) {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));  // (what follows from it would be kept in registers all the time)
+    const int n = lane & 15, g = lane >> 4;
+    if (n >= C::kLanes) kinds = 0;  // (another lane's columns)
+    if (__builtin_expect(__ballot(kinds != 0) == 0, 1)) return;
+#pragma unroll
+    for (int rb = 0; rb < kR; ++rb)
+#pragma unroll 1
+      for (int row = 0; row < 16; ++row) {
+        const uint64_t sees = (uint64_t)(uint32_t)__shfl((int)(rows.sees[rb] >> 32), row) << 32 | (uint32_t)__shfl((int)rows.sees[rb], row);
+        const uint32_t seen = seen_keys(key0 + 4 * g, __shfl(rows.low[rb], row), sees, length);
+        if ((seen >> (16 * kb + r) & 1) == 0) continue;
+        uint32_t* marks = reinterpret_cast<uint32_t*>(acc[rb][wave]) + row * kPad + C::kC * n;
+#pragma unroll 1
+        for (uint32_t left = kinds; left != 0;) {
+          const int c = (__ffs(left) - 1) / 2;
+          atomicOr(&marks[c], 1u << (left >> 2 * c & 3));
+          left &= ~(3u << 2 * c);
+        }
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
 };
 template <int kType, int kD, int kR, int kW>
-__device__ inline void finish(const CachedAttnArgs& a, const Rows<kType, kD, kR>& rows, Exchange<kD, kR, kW>& x, int b, int h, int group,
-                              int count, bool whole, int64_t slot) {
+__device__ inline void finish(const CachedAttnArgs& a, const Rows<kType, kD, kR>& rows, Exchange<kType, kD, kR, kW>& x, bool marked, int b, int h,
+                              int group, int count, bool whole, int64_t slot) {
   using C = CachedCfg<kType, kD>;
-  constexpr int kPad = Exchange<kD, kR, kW>::kPad, kRows = 16 * kR;
+  constexpr int kPad = Exchange<kType, kD, kR, kW>::kPad, kRows = 16 * kR;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int rb = 0; rb < kR; ++rb) {
@@ -672,7 +723,8 @@ __device__ inline void finish(const CachedAttnArgs& a, const Rows<kType, kD, kR>
       const int d = C::kC * (4 * g + r);
       if (C::kLanes != 16 && d >= kD) continue;
 #pragma unroll
-      for (int c = 0; c < C::kC; ++c) to[d + c] = rows.acc[rb][c][r];
+      for (int c = 0; c < C::kC; ++c)
+        to[d + c] = marked ? rows.acc[rb][c][r] + marked_value(__float_as_uint(to[d + c])) : rows.acc[rb][c][r];
     }
   }
   __syncthreads();
@@ -701,7 +753,10 @@ __device__ inline void finish(const CachedAttnArgs& a, const Rows<kType, kD, kR>
       if (kD % 64 != 0 && d >= kD) break;
       f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int w = 0; w < kW; ++w) v += *reinterpret_cast<const f32x4*>(x.acc[rb][w] + of16 * kPad + d) * by[w];
+      for (int w = 0; w < kW; ++w) {
+        const f32x4 of_wave = *reinterpret_cast<const f32x4*>(x.acc[rb][w] + of16 * kPad + d);
+        v += kType == FC_CACHE_BF16 ? scaled(of_wave, by[w]) : of_wave * by[w];
+      }
       if (whole) {
         v = node < count ? v * inv : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         *reinterpret_cast<uint2*>(O + d) = make_uint2(pair(v[0], v[1]), pair(v[2], v[3]));
@@ -728,7 +783,7 @@ __global__ __launch_bounds__(64 * kW, 2) void cached_attn_kernel(CachedAttnArgs 
   constexpr bool k8 = kType != FC_CACHE_BF16;
   __shared__ Nodes nodes;
   __shared__ __attribute__((aligned(16))) Queries<kType, kD, kR> queries;
-  __shared__ __attribute__((aligned(16))) Exchange<kD, kR, kW> exchange;
+  __shared__ __attribute__((aligned(16))) Exchange<kType, kD, kR, kW> exchange;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = (threadIdx.x & 63) >> 4;
   const Place at = place_of(a);
   if (at.h >= a.g.Hkv) return;
@@ -788,69 +843,111 @@ __global__ __launch_bounds__(64 * kW, 2) void cached_attn_kernel(CachedAttnArgs 
     __syncthreads();
     Rows<kType, kD, kR> rows;
     rows.begin(a, nodes, b, at.h, first_row, length, count);
-    for (; tile < tile1; tile += kW) {
-      const int key0 = tile * kTileKeys, next = key0 + kW * kTileKeys;
-      if (kR == 2 && kW == 4) {
-        // Of a CU's two workgroups the one that is behind goes first; the older one would be done at two
-        // thirds of the time and leave half the CU idle (16 sequences, 32 nodes: 61 us for 58).
-        const int left = 4 * (tile1 - tile), all = tile1 - tile0;
-        if (left > 3 * all) __builtin_amdgcn_s_setprio(3);
-        else if (left > 2 * all) __builtin_amdgcn_s_setprio(2);
-        else if (left > all) __builtin_amdgcn_s_setprio(1);
-        else __builtin_amdgcn_s_setprio(0);
+    // Marks what is not finite where it is seen.
+    const auto mark = [&] {
+      exchange.clear(wave);
+      i = 0;
+      for (tile = tile0 + wave; tile < tile1; tile += kW) {
+        const int key0 = tile * kTileKeys;
+        if (i == 0) fetch(key0);
+        locate(i, key0, true);
+        i = (i + 1) & 63;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll 1
+          for (int r = 0; r < 4; ++r) {
+            Raw<C::kC * C::kEsz> value;
+            value.load(bytes[kb].v, off.v + r * C::kRow);
+            exchange.mark(wave, rows, odd_values<kType, C::kC>(value.w), key0, kb, r, length);
+          }
       }
-      i = (i + 1) & 63;
-      if (i == 0) fetch(next);
-      // (each operand's next bytes are requested as soon as these have left their registers)
-      struct {
-        decltype(k)& bytes;
-        decltype(ks)& scales;
-        const int (&page)[2];
-        const int g;
-        decltype(request_k)& request;
-        const int i, next;
-        const bool more;
-        __device__ inline bf16x8 frag(int kb, int st) const {
-          const bf16x8 f = key_operand<kType>(bytes[kb][st].w);
-          return 4 * C::kSteps != C::kU && g * C::kSteps + st >= C::kU ? Mma<bf16>::zero() : f;
+    };
+    bool again = false;  // (values that are not finite are zeros)
+    while (true) {
+      for (; tile < tile1; tile += kW) {
+        const int key0 = tile * kTileKeys, next = key0 + kW * kTileKeys;
+        if (kR == 2 && kW == 4) {
+          // Of a CU's two workgroups the one that is behind goes first; the older one would be done at two
+          // thirds of the time and leave half the CU idle (16 sequences, 32 nodes: 61 us for 58).
+          const int left = 4 * (tile1 - tile), all = tile1 - tile0;
+          if (left > 3 * all) __builtin_amdgcn_s_setprio(3);
+          else if (left > 2 * all) __builtin_amdgcn_s_setprio(2);
+          else if (left > all) __builtin_amdgcn_s_setprio(1);
+          else __builtin_amdgcn_s_setprio(0);
         }
-        __device__ inline f32x4 scale(int kb, float by) const {
-          const float f = page[kb] >= 0 ? by : NAN;  // a page that is none
-          return k8 ? __builtin_bit_cast(f32x4, scales[kb]) * f : f32x4{f, f, f, f};
-        }
-        __device__ inline void used() const { request(i, next, more); }
-      } keys{k, ks, page, g, request_k, i, next, tile + kW < tile1};
-      struct {
-        decltype(v)& bytes;
-        decltype(vs)& scales;
-        __device__ inline bf16x8 frag(int c) const {
-          return as_bf16x8(make_uint4(two_keys<kType>(bytes[0].w, bytes[1].w, c), two_keys<kType>(bytes[2].w, bytes[3].w, c),
-                                      two_keys<kType>(bytes[4].w, bytes[5].w, c), two_keys<kType>(bytes[6].w, bytes[7].w, c)));
-        }
-        __device__ inline f32x4 scale(int kb) const { return __builtin_bit_cast(f32x4, scales[kb]); }
-        __device__ inline void keep(uint32_t mask) const {
+        i = (i + 1) & 63;
+        if (i == 0) fetch(next);
+        // (each operand's next bytes are requested as soon as these have left their registers)
+        struct {
+          decltype(k)& bytes;
+          decltype(ks)& scales;
+          const int (&page)[2];
+          const int g;
+          decltype(request_k)& request;
+          const int i, next;
+          const bool more;
+          __device__ inline bf16x8 frag(int kb, int st) const {
+            const bf16x8 f = key_operand<kType>(bytes[kb][st].w);
+            return 4 * C::kSteps != C::kU && g * C::kSteps + st >= C::kU ? Mma<bf16>::zero() : f;
+          }
+          __device__ inline f32x4 scale(int kb, float by) const {
+            const float f = page[kb] >= 0 ? by : NAN;  // a page that is none
+            return k8 ? __builtin_bit_cast(f32x4, scales[kb]) * f : f32x4{f, f, f, f};
+          }
+          __device__ inline void used() const { request(i, next, more); }
+        } keys{k, ks, page, g, request_k, i, next, tile + kW < tile1};
+        struct {
+          decltype(v)& bytes;
+          decltype(vs)& scales;
+          __device__ inline bf16x8 frag(int c) const {
+            return as_bf16x8(make_uint4(two_keys<kType>(bytes[0].w, bytes[1].w, c), two_keys<kType>(bytes[2].w, bytes[3].w, c),
+                                        two_keys<kType>(bytes[4].w, bytes[5].w, c), two_keys<kType>(bytes[6].w, bytes[7].w, c)));
+          }
+          __device__ inline f32x4 scale(int kb) const { return __builtin_bit_cast(f32x4, scales[kb]); }
+          __device__ inline void keep(uint32_t mask) const {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (uint32_t& w : bytes[j].w) w = (mask >> (16 * (j >> 2) + (j & 3)) & 1) != 0 ? w : 0;
-        }
-        __device__ inline void finite() const {
+              for (uint32_t& w : bytes[j].w) w = (mask >> (16 * (j >> 2) + (j & 3)) & 1) != 0 ? w : 0;
+          }
+          __device__ inline uint32_t finite() const {
+            uint32_t any = 0;
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (uint32_t& w : bytes[j].w) w = finite_halves(w);
-        }
-      } values{v, vs};
-      rows.tile(call, queries, nodes, a.N, key0, length, keys, values);
+              for (uint32_t& w : bytes[j].w) {
+                const uint32_t odd = odd_bits<kType>(w);
+                w &= ~odd;
+                any |= odd;
+              }
+            return any;
+          }
+        } values{v, vs};
+        rows.tile(call, kType == FC_CACHE_BF16 && again, queries, nodes, a.N, key0, length, keys, values);
+        load_v();
+      }
+      if (__builtin_expect(kType != FC_CACHE_BF16 || again || rows.all_finite(), 1)) break;
+      again = true;
+      mark();
+      rows.begin(a, nodes, b, at.h, first_row, length, count);
+      tile = tile0 + wave, i = 0;
+      fetch(tile * kTileKeys);
+      locate(0, tile * kTileKeys, tile < tile1);
+      load_k();
       load_v();
     }
-    finish<kType, kD, kR, kW>(a, rows, exchange, b, at.h, at.group, count, whole, slot);
+    bool marked = again;
+    if (kType == FC_CACHE_F8 && __builtin_expect(__ballot(rows.odd != 0) != 0, 0)) {
+      marked = true;
+      mark();
+    }
+    finish<kType, kD, kR, kW>(a, rows, exchange, marked, b, at.h, at.group, count, whole, slot);
   });
 }
 
 // The parts of a row's sequence, where there are several: kWaves waves to a row, of a workgroup's
-// four.
-template <int kD, int kWaves>
+// four.  kInfinite: a part may be infinite (bf16).
+template <int kD, int kWaves, bool kInfinite>
 __global__ __launch_bounds__(256) void cached_attn_join_kernel(CachedAttnArgs a, int rows_per_group) {
   constexpr int kCols = kD / 4;         // threads of a part, four columns each
   constexpr int kAtOnce = 64 / kCols;   // parts of a wave at a time
@@ -885,7 +982,9 @@ __global__ __launch_bounds__(256) void cached_attn_join_kernel(CachedAttnArgs a,
 #pragma unroll 4
     for (int i = wave % kWaves * kAtOnce + q; i < parts; i += kWaves * kAtOnce) {
       const int64_t at = place(i);
-      v += *reinterpret_cast<const f32x4*>(a.part_o + at * kD + d) * __builtin_amdgcn_exp2f(a.part_s[at].x - all);
+      const f32x4 part = *reinterpret_cast<const f32x4*>(a.part_o + at * kD + d);
+      const float by = __builtin_amdgcn_exp2f(a.part_s[at].x - all);
+      v += kInfinite ? scaled(part, by) : part * by;
     }
   }
   f32x4 of_wave = v;

@@ -15,13 +15,18 @@ constexpr int kJoinRows = 2048;
 
 namespace {
 
-template <int kD>
+template <int kD, bool kInfinite>
 void launch_join(const CachedAttnArgs& a, int rows_per_group, hipStream_t s) {
   const int rows = a.g.B * a.N * a.H;
   if (rows <= kJoinRows)
-    hipLaunchKernelGGL((cached_attn_join_kernel<kD, 4>), dim3(rows), dim3(256), 0, s, a, rows_per_group);
+    hipLaunchKernelGGL((cached_attn_join_kernel<kD, 4, kInfinite>), dim3(rows), dim3(256), 0, s, a, rows_per_group);
   else
-    hipLaunchKernelGGL((cached_attn_join_kernel<kD, 1>), dim3((rows + 3) / 4), dim3(256), 0, s, a, rows_per_group);
+    hipLaunchKernelGGL((cached_attn_join_kernel<kD, 1, kInfinite>), dim3((rows + 3) / 4), dim3(256), 0, s, a, rows_per_group);
+}
+template <int kD>
+void launch_join(const CachedAttnArgs& a, int rows_per_group, hipStream_t s) {
+  if (a.g.type == FC_CACHE_BF16) launch_join<kD, true>(a, rows_per_group, s);
+  else launch_join<kD, false>(a, rows_per_group, s);
 }
 
 }  // namespace
@@ -71,7 +76,8 @@ Plan plan_of(const CacheGeom& g, int H, int N, int left) {
   const int rows = H / g.Hkv * N;
   // Two blocks of sixteen rows read the keys once for both: 16 sequences of 4000 int8 keys
   // with 32 rows and 8 KV heads in 32 us for 38.  Where bf16 rows of more than 64 values leave too few registers
-  // for that (62 us for 48) it is worth it from the third block on only (64 rows: 69 us for 81).
+  // for that (16 sequences of up to 4000 keys: 42 us for 38) it is worth it from the third block on only (64
+  // rows: 49 us for 60).
   const bool spills = g.type == FC_CACHE_BF16 && g.D > 64;
   p.row_blocks = rows > (spills ? 32 : 16) ? 2 : 1;
   p.groups = (rows + 16 * p.row_blocks - 1) / (16 * p.row_blocks);

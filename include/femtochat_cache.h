@@ -94,7 +94,9 @@ typedef struct {
    a node sees the sequence, its ancestors and itself, and its position in the text
    (for the window and slopes) is lengths[b] plus the number of its ancestors.
    O is 0 for nodes from counts[b] on and NaN for a node whose parents are not so,
-   or that lies beyond the capacity.  workspace:
+   or that lies beyond the capacity.  A value in the cache that is not finite (bf16,
+   or a NaN among a caller's own float8 codes) is what O has in its column at the
+   nodes that see it, and reaches no other.  workspace:
    fc_cached_attn_workspace_bytes (0 is possible), 256-byte aligned. */
 fc_status fc_cached_attn_workspace_bytes(const fc_cache_desc* desc, const fc_cached_attn_options* options, size_t* bytes);
 fc_status fc_cached_attn(const fc_cache_desc* desc, const fc_cache* cache, const fc_cached_attn_options* options,
