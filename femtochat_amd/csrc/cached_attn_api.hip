@@ -111,6 +111,11 @@ fc_status options_of(const char* who, const CacheGeom& g, const fc_cached_attn_o
   if ((int64_t)g.B * o->N * o->H > (int64_t)1 << 24) return bad(who, "at most 2^24 rows (sequences times new tokens times heads)", FC_ERR_UNSUPPORTED);
   return FC_OK;
 }
+// A launch holds fewer than 2^32 threads (launch_d's grid; eight waves are for few workgroups only).
+fc_status launch_fits(const char* who, const CacheGeom& g, const Plan& p) {
+  const int64_t slots = ((int64_t)(p.shares > 0 ? p.shares : g.B) * g.Hkv + 7) / 8 * 8;
+  return slots * p.groups * 256 < (int64_t)1 << 32 ? FC_OK : bad(who, "fewer than 2^24 workgroups (sequences times KV heads)", FC_ERR_UNSUPPORTED);
+}
 int left_of(const fc_cached_attn_options* o) { return o->left < 0 ? INT_MAX / 2 : std::min(o->left, INT_MAX / 2); }
 
 }  // namespace
@@ -128,6 +133,7 @@ fc_status fc_cached_attn_workspace_bytes(const fc_cache_desc* desc, const fc_cac
   if ((st = fc::options_of(who, g, options)) != FC_OK) return st;
   if (bytes == nullptr) return fc::bad(who, "bytes is null");
   const fc::Plan p = fc::plan_of(g, options->H, options->N, fc::left_of(options));
+  if ((st = fc::launch_fits(who, g, p)) != FC_OK) return st;
   *bytes = p.bytes;
   fc::clear_error();
   return FC_OK;
@@ -147,6 +153,7 @@ fc_status fc_cached_attn(const fc_cache_desc* desc, const fc_cache* cache, const
   if (fc::off(lengths, 4) || fc::off(counts, 4) || fc::off(parents, 4)) return fc::bad(who, "integer buffers must be 4-byte aligned");
   const int left = fc::left_of(options);
   const fc::Plan p = fc::plan_of(a.g, options->H, options->N, left);
+  if ((st = fc::launch_fits(who, a.g, p)) != FC_OK) return st;
   const size_t need = p.bytes;
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return fc::bad(who, "the workspace is missing or too small", FC_ERR_WORKSPACE);
   if (need > 0 && fc::off(workspace, 256)) return fc::bad(who, "the workspace must be 256-byte aligned", FC_ERR_WORKSPACE);

@@ -834,6 +834,8 @@ fc_status check(const char* who, const fc_verify_desc* d) {
   if (!(d->temperature == 0.0 || (d->temperature >= 0x1p-10 && d->temperature <= 0x1p10)))
     return bad(who, "temperature must be 0 or from 2^-10 to 2^10");
   // A launch holds fewer than 2^32 threads.
+  if (d->V <= kSmallValues && (int64_t)d->B * kSmallThreads >= (int64_t)1 << 32)
+    return bad(who, "fewer than 2^22 sequences of a small vocabulary", FC_ERR_UNSUPPORTED);
   if (2 * (int64_t)d->B * d->N * chunks_of(d) >= (int64_t)1 << 24) return bad(who, "too many logits: at most 2^23 chunks of 8192", FC_ERR_UNSUPPORTED);
   return FC_OK;
 }
