@@ -17,7 +17,8 @@ or, with a leading dimension, those of all layers (``cache.layer(i)`` is one).  
 8-bit value is code * scale, with scale = max |x| / 127 (int8) or / 448 (float8) over a
 token's head.  ``lengths`` (B,) int32 are the tokens that the cache holds before a
 call; the call's own tokens lie behind them, ``counts`` (B,) int32 of them where a
-batch is ragged.  A step of generation with drafted tokens is::
+batch is ragged.  None of the calls has a gradient.  A step of generation with drafted
+tokens is::
 
     for i in range(layers):                       # nodes: the last token and the drafts
         cache_write_(cache.layer(i), K, V, lengths, counts)
@@ -198,7 +199,8 @@ def cache_write_(cache: KVCache, K: torch.Tensor, V: torch.Tensor, lengths: torc
                  counts: Optional[torch.Tensor] = None) -> None:
     """Writes K and V ([layers,] B, T, Hkv, D), float32 or bfloat16, as each sequence's
     tokens ``lengths[b]`` to ``lengths[b] + counts[b] - 1`` (T of them without ``counts``),
-    quantised to the cache's type.  Tokens beyond the capacity are not written."""
+    quantised to the cache's type.  Tokens beyond the capacity are not written; ``lengths``
+    is the caller's to move on, once all layers are written."""
     c = _buffers(cache, _batch(cache, lengths))
     T = _check_values(c, K, V)
     _check_counts(c, lengths, counts, required=True)

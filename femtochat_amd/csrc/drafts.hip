@@ -4,10 +4,13 @@
 // The next token is the place of u's share among the vocabulary's cumulative weights,
 // of which one in V lies next to any u: those are exponentials and sums in float64 (in
 // float32 another token would be drawn about once in a hundred rows of 2^15).  An
-// acceptance is one comparison of u with a ratio of two probabilities, for which
-// float32 exponentials summed in float64 (1e-7) are enough.  float64 operations are what
-// costs here, not the bytes (22 us of them for 704 rows of 2^15 bf16 logits that
-// are read in 10), so they are kept for the row where a sequence's walk ends.
+// acceptance is one comparison of u with a ratio of two probabilities, for which a
+// denominator of float32 exponentials is enough, summed by eight in float32 and then in
+// float64: within 2^-17 of itself (an exponent's three roundings of 2^-24, times 26 log 2
+// where 2^26 values at 2^-26 make up the sum; then v_exp_f32's 2^-22 and the eights' sums).
+// float64 operations are what costs here, not the bytes (22 us of them for 704 rows of
+// 2^15 bf16 logits that are read in 10), so they are kept for the row where a sequence's
+// walk ends.
 //
 //  * draft_stats_kernel reads every row of logits (target and draft) once: each
 //    workgroup leaves a chunk's maximum and the sum of its exponentials.

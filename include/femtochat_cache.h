@@ -122,9 +122,10 @@ fc_status fc_cached_attn(const fc_cache_desc* desc, const fc_cache* cache, const
    Out: path (B, N) the accepted nodes from node 0 on, -1 behind them; kept (B)
    their number; next (B) the next token.  A row of logits with a NaN or +infinity,
    or without a finite value, accepts nothing and has the next token -1; so has a
-   sequence with counts[b] = 0, which keeps nothing.  Sums and exponentials are
-   float64.  workspace: fc_verify_workspace_bytes (0 for a small
-   vocabulary), 256-byte aligned. */
+   sequence with counts[b] = 0, which keeps nothing.  The next token's weights and
+   their sums are float64.  So is an acceptance's p(x) but for its denominator, which
+   beyond 2048 tokens is a sum of float32 exponentials (within 2^-17 of itself).  workspace: fc_verify_workspace_bytes (0 for a small vocabulary),
+   256-byte aligned. */
 typedef struct {
   int32_t B, N, V;      /* sequences, nodes (1 to 64), vocabulary */
   int32_t dtype;        /* FC_F32 or FC_BF16: logits and draft_logits */
