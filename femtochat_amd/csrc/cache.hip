@@ -118,20 +118,18 @@ __device__ inline void read_unit(const void* rows, const float* scales, int64_t 
   for (int i = 0; i < 8; ++i) x[i] *= s;
 }
 
-// Token t of sequence b and its head of this thread's vector; false past the end.
+// Token t of sequence b and its head of this thread's vector; i lies within the sequence's tokens.
 struct Vector {
   int layer, b, t, h, u;
-  bool within;
 };
 template <int U>
 __device__ inline Vector vector_of(const CacheArgs& a, int64_t i) {
   constexpr int L = vector_lanes(U);
-  const int64_t n = i / L;
+  const int n = (int)(i / L);
   Vector v;
   v.u = (int)(i % L);
-  v.within = n < (int64_t)a.T * a.g.Hkv;
-  v.t = v.within ? (int)divide((uint32_t)n, a.by_Hkv) : 0;
-  v.h = v.within ? (int)n - v.t * a.g.Hkv : 0;
+  v.t = (int)divide((uint32_t)n, a.by_Hkv);
+  v.h = n - v.t * a.g.Hkv;
   v.b = blockIdx.y;
   v.layer = blockIdx.z;
   return v;
