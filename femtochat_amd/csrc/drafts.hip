@@ -20,7 +20,7 @@
 //  * draft_pick_kernel, a wave per sequence, finds the part that u's share falls into and
 //    the token in it.  In small calls the last workgroup of a sequence to leave its sums does
 //    that instead (the first kernel zeroed their counter).
-//  * With the drafts' distributions a weight is p - q, whose two sums have to be there
+//  * With the drafts' distributions a weight is p - q (p where that leaves nothing), whose two sums have to be there
 //    first: draft_walk_kernel, before the sums, walks and forms them.
 //  * Vocabularies of up to 2048 run whole in draft_small_kernel, a workgroup per sequence.
 #include "attn_device.hpp"
@@ -514,6 +514,10 @@ __device__ inline bool drawn_row(const DraftArgs& a, int b, const Walk& w, int p
   return true;
 }
 
+// Above which a row's weights are something to draw from.  A residual (in units of p) of less than 2^-40
+// is the roundings of equal p and q, or rarer than a draft's refusal ever is seen.
+__device__ inline double least_left(const Walk& w) { return w.residual != 0 ? 0x1p-40 : 0.0; }
+
 // The part that u's share falls into, and the token in it, by one wave.  part_at(i) is part i's sum; bits:
 // kPart / 32 words of LDS.
 template <typename E, int kPart, typename Part>
@@ -534,7 +538,7 @@ __device__ inline void pick_token(const DraftArgs& a, int b, const Walk& w, Weig
   total = wave_sum(total);
   double before = 0.0, target = u * total;
   int part = parts - 1;
-  if (total > 0.0) {
+  if (total > least_left(w)) {
     for (int i0 = 0; i0 < parts; i0 += 64) {
       double of_lane = held[0];
 #pragma unroll
@@ -550,7 +554,7 @@ __device__ inline void pick_token(const DraftArgs& a, int b, const Walk& w, Weig
       }
       before = __shfl(upto, 63);
     }
-  } else {  // nothing is left of p (it was rounded away): p itself
+  } else {  // nothing is left of p: p itself
     ws.draft = nullptr;
     struck = 0;
     for (int i = 0; i < parts; ++i) total += part_sum<E, kPart>(ws, nullptr, i * kPart - head);
@@ -779,7 +783,7 @@ __global__ __launch_bounds__(kSmallThreads) void draft_small_kernel(DraftArgs a)
     }
   }
   double total = 0.0, upto = 0.0;
-  for (int round = 0; round < 2; ++round) {  // a second one where nothing is left of p (it was rounded away): p itself
+  for (int round = 0; round < 2; ++round) {  // a second one where nothing is left of p: p itself
     upto = wave_scan(v[0] + v[1]);
     if (lane == 63) sums[round][wave] = upto;
     __syncthreads();
@@ -788,7 +792,7 @@ __global__ __launch_bounds__(kSmallThreads) void draft_small_kernel(DraftArgs a)
       if (i == wave) upto += total;
       total += sums[round][i];
     }
-    if (total > 0.0) break;
+    if (total > least_left(w)) break;
     v[0] = p[0], v[1] = p[1];
   }
   const double u = (double)fminf(fmaxf(a.u[(int64_t)b * a.N], 0.0f), 0x1.fffffep-1f), target = u * total;

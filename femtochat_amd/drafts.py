@@ -8,7 +8,8 @@ softmax at ``temperature``::
 
     draws       node i was drawn from q, the softmax of draft_logits (B, N - 1, V) at i - 1:
                 accepted if u[i] q(x) < p(x); the first refusal ends the run, and the
-                next token is drawn from max(p - q, 0)
+                next token is drawn from max(p - q, 0), or where that leaves nothing
+                (less than 2^-40) from p
     candidates  no draft_logits: a node's children (a run's next node) are tried in
                 order: accepted if u[i] (1 - what those before it have of p) < p(x); the
                 next token is drawn from p without those tried

@@ -110,7 +110,8 @@ fc_status fc_cached_attn(const fc_cache_desc* desc, const fc_cache* cache, const
    Draws (draft_logits, without parents): node i was drawn from q, the softmax of
      draft_logits (B, N - 1, V) at i - 1.  It is accepted if u[i] q(x) < p(x), p at
      its parent; the first that is not ends the run, and the next token is drawn
-     from max(p - q, 0), or from p behind the last node.
+     from max(p - q, 0), or from p behind the last node or where less than 2^-40 is
+     left.
    Candidates (no draft_logits): a node's children are tried in order; x is accepted
      if u[i] (1 - what those before it have of p) < p(x), and a token tried before is
      not; the next token is drawn from p without the tried ones.
@@ -123,7 +124,7 @@ fc_status fc_cached_attn(const fc_cache_desc* desc, const fc_cache* cache, const
    their number; next (B) the next token.  A row of logits with a NaN or +infinity,
    or without a finite value, accepts nothing and has the next token -1; so has a
    sequence with counts[b] = 0, which keeps nothing.  The next token's weights and
-   their sums are float64.  So is an acceptance's p(x) but for its denominator, which
+   their sums are float64; one of less than 2^-1000 of the row's largest is none.  So is an acceptance's p(x) but for its denominator, which
    beyond 2048 tokens is a sum of float32 exponentials (within 2^-17 of itself).  workspace: fc_verify_workspace_bytes (0 for a small vocabulary),
    256-byte aligned. */
 typedef struct {

@@ -129,7 +129,7 @@ def verify(logits, tokens, u, draft_logits=None, parents=None, count=None, tempe
                     taken = i
                 else:
                     rest = np.maximum(p - q, 0.0)
-                    return path, draw(rest if rest.sum() > 0 else p, float(u[0]))
+                    return path, draw(rest if rest.sum() > 2.0 ** -40 else p, float(u[0]))  # (less is roundings)
             elif x not in tried:
                 if u[i] * left < p[x]:
                     taken = i
