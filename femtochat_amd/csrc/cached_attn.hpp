@@ -33,11 +33,11 @@
 // sequences' tiles (cache_index.hpp).  A sequence in several shares is joined by a
 // second, small kernel.
 //
-// Measured, codes of 8 bits, heads of 128, the kernel alone: 64 sequences of up to 4096 keys,
-// 5 KV heads, one token each, 40 us (192 MB, 4.8 TB/s; a copy reaches 5.1); one of 131072 keys,
-// 8 KV heads, 50 us (277 MB; part of it stays in the 256 MB cache between calls); 16 of up to
-// 8192 keys, 8 KV heads, 32 nodes of two heads each, 56 us (168 MB, 3.0 TB/s): the two waves of
-// a SIMD have an instruction under way for 94% of the time, two thirds of it vector ones, of
+// Measured, codes of 8 bits, heads of 128, a captured call with its join: 64 sequences of up to
+// 4096 keys, 5 KV heads, one token each, 45 us (192 MB; the kernel 41, 4.7 TB/s, and a copy reaches
+// 5.1); one of 131072 keys, 8 KV heads, 56 us (277 MB; part of it stays in the 256 MB cache between
+// calls); 16 of up to 8192 keys, 8 KV heads, 32 nodes of two heads each, 62 us (168 MB, 2.7 TB/s): the two
+// waves of a SIMD have an instruction under way for 94% of the time, two thirds of it vector ones, of
 // which 190 of 450 a tile turn codes into numbers and 90 make two numbers of each probability.
 //
 // Rows that do not see a key have P = 0 there, but 0 * infinity is not 0, nor has a P of two numbers one

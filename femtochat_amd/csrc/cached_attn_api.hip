@@ -61,7 +61,9 @@ bool off(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & 
 constexpr int kSlots = 512;       // workgroups: two on each of 256 CUs, which their registers allow
 constexpr int kLeastTiles = 12;   // of a share: a sequence's beginning and a tile for each wave
 // Up to which a sequence is not shared: the join and its launch cost as much as a longer chain (16 int8 sequences,
-// 8 KV heads of 128, one token: 32 tiles 13.6 us whole and 15.6 in parts, 40 15.5 and 16.0, 48 17.2 and 16.1).
+// 8 KV heads of 128, one token: 32 tiles 13.6 us whole and 15.6 in parts, 40 15.5 and 16.0, 48 17.2 and 16.1;
+// 32 tiles of four sequences with two KV heads 12.6 and 14.1, bf16 15.0 and 16.1).  One sequence of one KV head is
+// the exception, 12.4 for 11.6 us, bf16 14.8 for 12.0.
 constexpr int kWholeTiles = 32;
 
 // The sizes of a call that follow from its descriptor alone (not from the lengths,

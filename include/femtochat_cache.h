@@ -96,7 +96,8 @@ typedef struct {
    O is 0 for nodes from counts[b] on and NaN for a node whose parents are not so,
    or that lies beyond the capacity.  A value in the cache that is not finite (bf16,
    or a NaN among a caller's own float8 codes) is what O has in its column at the
-   nodes that see it, and reaches no other.  workspace:
+   nodes that see it, and reaches no other.  Sums are float32 (of values beyond 2^120
+   over the number of keys they may overflow).  workspace:
    fc_cached_attn_workspace_bytes (0 is possible), 256-byte aligned. */
 fc_status fc_cached_attn_workspace_bytes(const fc_cache_desc* desc, const fc_cached_attn_options* options, size_t* bytes);
 fc_status fc_cached_attn(const fc_cache_desc* desc, const fc_cache* cache, const fc_cached_attn_options* options,
@@ -110,8 +111,8 @@ fc_status fc_cached_attn(const fc_cache_desc* desc, const fc_cache* cache, const
    Draws (draft_logits, without parents): node i was drawn from q, the softmax of
      draft_logits (B, N - 1, V) at i - 1.  It is accepted if u[i] q(x) < p(x), p at
      its parent; the first that is not ends the run, and the next token is drawn
-     from max(p - q, 0), or from p behind the last node or where less than 2^-40 is
-     left.
+     from max(p - q, 0), or from p behind the last node and where less than 2^-40
+     of that is left.
    Candidates (no draft_logits): a node's children are tried in order; x is accepted
      if u[i] (1 - what those before it have of p) < p(x), and a token tried before is
      not; the next token is drawn from p without the tried ones.
@@ -123,10 +124,11 @@ fc_status fc_cached_attn(const fc_cache_desc* desc, const fc_cache* cache, const
    Out: path (B, N) the accepted nodes from node 0 on, -1 behind them; kept (B)
    their number; next (B) the next token.  A row of logits with a NaN or +infinity,
    or without a finite value, accepts nothing and has the next token -1; so has a
-   sequence with counts[b] = 0, which keeps nothing.  The next token's weights and
-   their sums are float64; one of less than 2^-1000 of the row's largest is none.  So is an acceptance's p(x) but for its denominator, which
-   beyond 2048 tokens is a sum of float32 exponentials (within 2^-17 of itself).  workspace: fc_verify_workspace_bytes (0 for a small vocabulary),
-   256-byte aligned. */
+   sequence with counts[b] = 0, which keeps nothing.  Weights and their sums are
+   float64, but for the denominator of an acceptance's p(x) and q(x), which beyond 2048
+   tokens is a sum of float32 exponentials (within 2^-17 of itself); a weight of less
+   than 2^-1000 of the row's largest is none.  workspace: fc_verify_workspace_bytes
+   (0 for a small vocabulary), 256-byte aligned. */
 typedef struct {
   int32_t B, N, V;      /* sequences, nodes (1 to 64), vocabulary */
   int32_t dtype;        /* FC_F32 or FC_BF16: logits and draft_logits */
